@@ -98,8 +98,9 @@ TT_ATTN_API int tt_attn_device_supported(void);
 
 /* Reads (and, when clear != 0, resets) the current device's kernel status bits:
  * bit 0 = a bounded wait inside a kernel ran out (returns TT_ATTN_TIMEOUT);
- * bit 1 = tt_rope_append_bf16 met a device-held position outside the cache or the table and
- * skipped those rows (returns TT_ATTN_BAD_ARG). Synchronises the device. */
+ * bit 1 = tt_rope_append_bf16 met a device-held position outside the cache or the table, or
+ * tt_attn_tree_commit_bf16 a row or path entry outside its buffer, and skipped those rows
+ * (returns TT_ATTN_BAD_ARG). Synchronises the device. */
 TT_ATTN_API tt_attn_status tt_attn_device_status(unsigned* flags, int clear);
 
 /*
@@ -237,6 +238,105 @@ TT_ATTN_API tt_attn_status tt_attn_decode_bf16_noalloc(
     const void* v, const int64_t* v_strides,
     int64_t batch, int64_t heads, int64_t kv_len, const int32_t* kv_lens,
     void* out, float* lse, void* stream);
+
+/* ------------------------------------------------------------------ speculative decoding
+ * Three operators around one step of speculative decoding. A draft proposes a tree of `nodes`
+ * tokens per sequence; the target runs once over all of them (attention by
+ * tt_attn_tree_forward_bf16, each node seeing the cached prefix and its own branch), the walk
+ * through the tree is decided by tt_attn_tree_verify_f32, and the accepted path's K/V rows are
+ * appended to the caches by tt_attn_tree_commit_bf16. The drafted tokens' K/V rows stay outside
+ * the cache until then. No counterpart in the reference, which generates one token at a time
+ * (tiny_transformer/generate.py).
+ *
+ * A tree is given by `parents`: int32 device [nodes] (parents_stride 0, one tree for the batch)
+ * or [batch, nodes] rows parents_stride elements apart. parents[n] is a lower index, or -1 for a
+ * root. A node whose chain of parents does not reach -1 over strictly lower indices is not in use
+ * (padding of a smaller tree): nobody sees it, and its own output is empty.
+ */
+#define TT_ATTN_TREE_MAX_NODES 256
+#define TT_ATTN_TREE_MAX_VOCAB 4194304
+
+/*
+ * Attention of the tree's nodes: node n of sequence b attends to cache rows [0, cache_lens[b]) and
+ * to the tree rows of its chain (itself, its parent, ... up to the root). Scale 1/8, FP32 softmax.
+ *
+ *   q          [batch, q_heads, nodes, 64] bf16; q_heads a multiple of kv_heads: query head h
+ *              reads K/V head h / (q_heads / kv_heads)
+ *   tree_k/v   [batch, kv_heads, nodes, 64] bf16, the drafted tokens' own rows
+ *   cache_k/v  [batch, kv_heads, capacity, 64] bf16
+ *   cache_lens optional device int32[batch], clamped to [0, capacity]; NULL: the whole capacity
+ *   out        contiguous [batch, q_heads, nodes, 64] bf16, 16-byte aligned
+ *   lse        optional contiguous [batch, q_heads, nodes] fp32, natural log
+ *   workspace  tt_attn_tree_workspace_size() bytes, 16-byte aligned (may be NULL when that is 0)
+ *
+ * Nodes not in use get O = 0, LSE = -inf. What a node does not see does not change its output,
+ * whatever it holds (NaN and infinities included). 1 <= nodes <= TT_ATTN_TREE_MAX_NODES. Layout
+ * rules of q and all K/V tensors as for tt_attn_forward_bf16 (TT_ATTN_UNSUPPORTED otherwise).
+ */
+TT_ATTN_API tt_attn_status tt_attn_tree_forward_bf16(
+    const void* q, const int64_t* q_strides, const void* tree_k, const int64_t* tk_strides,
+    const void* tree_v, const int64_t* tv_strides, const void* cache_k, const int64_t* ck_strides,
+    const void* cache_v, const int64_t* cv_strides, int64_t batch, int64_t q_heads,
+    int64_t kv_heads, int64_t nodes, int64_t capacity, int64_t head_dim, const int32_t* parents,
+    int64_t parents_stride, const int32_t* cache_lens, void* out, float* lse, void* workspace,
+    size_t workspace_bytes, void* stream);
+
+/* Scratch bytes tt_attn_tree_forward_bf16 needs for this shape; 0 for invalid shapes too. */
+TT_ATTN_API size_t tt_attn_tree_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                               int64_t nodes, int64_t capacity);
+
+/*
+ * Walk of the tree with given random numbers (speculative sampling). From node 0 the children of
+ * the current node are tried in index order: a child with token t is accepted with probability
+ * min(1, p(t) / q(t)), otherwise p becomes max(p - q, 0), renormalised, for the next child; when
+ * no child is accepted, the next token is drawn from what is left of p.
+ *
+ *   tokens        int64 device [batch, nodes] contiguous: token of each node (node 0's is not read
+ *                 as a candidate). A token outside [0, vocab) is never accepted.
+ *   target_probs  fp32 device [batch, nodes, vocab], unit last stride, element strides tp_sb, tp_sn:
+ *                 row n is the target's distribution of the token after node n
+ *   draft_probs   fp32 likewise (dp_sb, dp_sn): the distribution that n's children were drawn from.
+ *                 NULL: children were chosen, not drawn (q = 1 at the child's token)
+ *   uniforms      fp32 device [batch, nodes] contiguous in [0, 1): entry n decides node n, entry 0
+ *                 draws the next token
+ *   path          int32 [batch, nodes]: the accepted nodes from the root (node 0) on, then -1
+ *   counts        int32 [batch]: accepted nodes, the root included (0 when node 0 is not a root)
+ *   next_tokens   int64 [batch]: the token after the path (-1 where counts is 0, or where no token
+ *                 has any weight)
+ *
+ * Weights are whole numbers (probabilities times 2^36, rounded down), so results do not depend on
+ * the order of any sum; the exact definition is at the kernel. Probabilities are taken into
+ * [0, 2], NaN as 0. 1 <= nodes <= TT_ATTN_TREE_MAX_NODES, vocab <= TT_ATTN_TREE_MAX_VOCAB.
+ */
+TT_ATTN_API tt_attn_status tt_attn_tree_verify_f32(
+    const int64_t* tokens, const int32_t* parents, int64_t parents_stride,
+    const float* target_probs, int64_t tp_sb, int64_t tp_sn, const float* draft_probs,
+    int64_t dp_sb, int64_t dp_sn, const float* uniforms, int64_t batch, int64_t nodes,
+    int64_t vocab, int32_t* path, int32_t* counts, int64_t* next_tokens, void* stream);
+
+/*
+ * Append of the accepted path to the caches of `layers` layers: row i < counts[b] of sequence b
+ * goes from tree row path[b, i] to cache row cache_lens[b] + i, keys and values, all layers.
+ *
+ *   cache_k/v, tree_k/v  host arrays of `layers` device pointers; every layer has the same shape and
+ *                        strides: caches [batch, kv_heads, capacity, 64], trees [batch, kv_heads,
+ *                        nodes, 64] bf16, last stride 1, other strides multiples of 8, 16-byte
+ *                        aligned bases (TT_ATTN_UNSUPPORTED otherwise)
+ *   path                 int32 device [batch, path_len] contiguous
+ *   counts, cache_lens   int32 device [batch]
+ *   new_lens             int32 device [batch]: cache_lens[b] + the rows that fit. A buffer
+ *                        of its own: the kernel's blocks read cache_lens while it is written
+ *
+ * Rows that do not fit the capacity and path entries outside [0, nodes) are skipped and set bit 1
+ * of the device status (tt_attn_device_status). The caches must not overlap the trees.
+ */
+TT_ATTN_API tt_attn_status tt_attn_tree_commit_bf16(
+    void* const* cache_k, const int64_t* ck_strides, void* const* cache_v,
+    const int64_t* cv_strides, const void* const* tree_k, const int64_t* tk_strides,
+    const void* const* tree_v, const int64_t* tv_strides, int64_t layers, int64_t batch,
+    int64_t kv_heads, int64_t nodes, int64_t capacity, int64_t head_dim, const int32_t* path,
+    int64_t path_len, const int32_t* counts, const int32_t* cache_lens, int32_t* new_lens,
+    void* stream);
 
 #ifdef __cplusplus
 }

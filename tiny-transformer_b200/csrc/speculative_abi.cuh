@@ -1,0 +1,316 @@
+// C-ABI implementation of the speculative-decoding operators (include/tt_attention.h): argument
+// validation, variant choice and launches. Part of tt_attention_abi.cu, whose helpers (fail,
+// prepare_device, encode_map, ...) and device status word it uses.
+#pragma once
+
+namespace {
+
+// Query rows per CTA tile of the tree attention: 16 or 32 (tree_attention_kernel<1 or 2>).
+int tree_row_tiles(int64_t rows) { return rows <= 16 ? 1 : 2; }
+
+struct TreePlan {
+  int rt = 1;             // 16-row tiles per CTA
+  int64_t row_tiles = 1;  // CTA tiles of one (batch, K/V head)
+  int splits = 1;         // CTAs per cluster
+};
+
+TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t nodes, int64_t capacity,
+                   int sms) {
+  TreePlan pl;
+  pl.rt = tree_row_tiles(rows);
+  pl.row_tiles = (rows + pl.rt * 16 - 1) / (pl.rt * 16);
+  const int64_t units = batch * kv_heads * pl.row_tiles;
+  const int64_t tiles = (nodes + tt::tree::KEYS - 1) / tt::tree::KEYS +
+                        (capacity + tt::tree::KEYS - 1) / tt::tree::KEYS;
+  pl.splits = static_cast<int>(std::max<int64_t>(
+      1, std::min<int64_t>({tt::tree::MAX_SPLITS, tiles, 3 * static_cast<int64_t>(sms) / units})));
+  return pl;
+}
+
+tt_attn_status set_tree_attributes() {
+  static std::mutex mu;
+  static bool done[kMaxDevices] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(mu);
+  if (e == cudaSuccess && !done[dev]) {
+    e = cudaFuncSetAttribute(tt::tree::tree_attention_kernel<1>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(tt::tree::smem_bytes<1>()));
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(tt::tree::tree_attention_kernel<2>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(tt::tree::smem_bytes<2>()));
+    if (e == cudaSuccess) done[dev] = true;
+  }
+  if (e != cudaSuccess)
+    return fail(TT_ATTN_LAUNCH_FAIL, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
+  return TT_ATTN_OK;
+}
+
+void cluster_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, int64_t blocks, int threads,
+                    size_t smem, int cluster, cudaStream_t stream) {
+  *cfg = cudaLaunchConfig_t{};
+  cfg->gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
+  cfg->blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+  cfg->dynamicSmemBytes = smem;
+  cfg->stream = stream;
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr->val.clusterDim.y = 1;
+  attr->val.clusterDim.z = 1;
+  cfg->attrs = attr;
+  cfg->numAttrs = 1;
+}
+
+// [batch, heads, rows, 64] operand of the speculative operators: readable in place?
+bool operand_ok(const void* p, const Shape4& s) { return aligned16(p) && strides_ok(s.stride); }
+
+}  // namespace
+
+extern "C" {
+
+TT_ATTN_API size_t tt_attn_tree_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                               int64_t nodes, int64_t capacity) {
+  (void)batch; (void)q_heads; (void)kv_heads; (void)nodes; (void)capacity;
+  return 0;
+}
+
+TT_ATTN_API tt_attn_status tt_attn_tree_forward_bf16(
+    const void* q, const int64_t* q_strides, const void* tree_k, const int64_t* tk_strides,
+    const void* tree_v, const int64_t* tv_strides, const void* cache_k, const int64_t* ck_strides,
+    const void* cache_v, const int64_t* cv_strides, int64_t batch, int64_t q_heads,
+    int64_t kv_heads, int64_t nodes, int64_t capacity, int64_t head_dim, const int32_t* parents,
+    int64_t parents_stride, const int32_t* cache_lens, void* out, float* lse, void* workspace,
+    size_t workspace_bytes, void* stream) {
+  namespace tr = tt::tree;
+  // ---- validation: everything is checked before any CUDA call
+  if (!q || !tree_k || !tree_v || !cache_k || !cache_v || !parents || !out || !q_strides ||
+      !tk_strides || !tv_strides || !ck_strides || !cv_strides)
+    return fail(TT_ATTN_BAD_ARG, "tree_attention: q, the tree's and the cache's K/V, parents, out "
+                                 "and the stride arrays must not be NULL");
+  if (head_dim != TT_ATTN_HEAD_DIM)
+    return fail(TT_ATTN_BAD_ARG, "tree_attention currently supports only head_dim=64");
+  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || nodes <= 0 || capacity <= 0)
+    return fail(TT_ATTN_BAD_ARG,
+                "tree_attention: batch, heads, nodes and cache capacity must be positive");
+  if (q_heads % kv_heads != 0)
+    return fail(TT_ATTN_BAD_ARG, "tree_attention: q heads must be a multiple of the K/V heads");
+  if (nodes > TT_ATTN_TREE_MAX_NODES)
+    return fail(TT_ATTN_BAD_ARG, "tree_attention: at most 256 nodes per tree");
+  if (capacity > INT32_MAX - tr::KEYS)
+    return fail(TT_ATTN_BAD_ARG, "tree_attention: the cache capacity must fit int32");
+  if (parents_stride != 0 && parents_stride < nodes)
+    return fail(TT_ATTN_BAD_ARG, "tree_attention: parents_stride must be 0 or at least nodes");
+  const int64_t max_rows = INT32_MAX / (TT_ATTN_TREE_MAX_NODES * tr::MAX_SPLITS);
+  if (batch > max_rows || q_heads > max_rows || batch > max_rows / q_heads)
+    return fail(TT_ATTN_BAD_ARG, "tree_attention: shape exceeds the supported CUDA grid limits");
+  const Shape4 qs = canonical(batch, q_heads, nodes, q_strides);
+  const Shape4 tks = canonical(batch, kv_heads, nodes, tk_strides);
+  const Shape4 tvs = canonical(batch, kv_heads, nodes, tv_strides);
+  const Shape4 cks = canonical(batch, kv_heads, capacity, ck_strides);
+  const Shape4 cvs = canonical(batch, kv_heads, capacity, cv_strides);
+  if (!operand_ok(q, qs) || !operand_ok(tree_k, tks) || !operand_ok(tree_v, tvs) ||
+      !operand_ok(cache_k, cks) || !operand_ok(cache_v, cvs))
+    return fail(TT_ATTN_UNSUPPORTED,
+                "tree_attention: q and the K/V tensors need a unit last stride, other strides in "
+                "multiples of 8 elements and 16-byte aligned bases; copy to aligned contiguous "
+                "storage first");
+  if (!aligned16(out)) return fail(TT_ATTN_BAD_ARG, "tree_attention: out must be 16-byte aligned");
+  for (const void* ptr : {static_cast<const void*>(parents), static_cast<const void*>(cache_lens),
+                          static_cast<const void*>(lse)})
+    if (reinterpret_cast<uintptr_t>(ptr) % 4 != 0)
+      return fail(TT_ATTN_BAD_ARG, "tree_attention: parents, cache_lens and lse must be 4-byte aligned");
+  const size_t need = tt_attn_tree_workspace_size(batch, q_heads, kv_heads, nodes, capacity);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
+    return fail(TT_ATTN_BAD_ARG, "tree_attention: workspace is smaller than "
+                                 "tt_attn_tree_workspace_size() or not 16-byte aligned");
+
+  int dev = 0, sm_count = 0;
+  tt_attn_status st = prepare_device(&dev, &sm_count);
+  if (st != TT_ATTN_OK) return st;
+  if ((st = set_tree_attributes()) != TT_ATTN_OK) return st;
+  CUtensorMap tmk, tmv, tmtk, tmtv;
+  std::string err;
+  if (!encode_map(&tmk, cache_k, cks, &err, tr::KEYS) ||
+      !encode_map(&tmv, cache_v, cvs, &err, tr::KEYS) ||
+      !encode_map(&tmtk, tree_k, tks, &err, tr::KEYS) ||
+      !encode_map(&tmtv, tree_v, tvs, &err, tr::KEYS))
+    return fail(TT_ATTN_UNSUPPORTED, err);
+  const int64_t group = q_heads / kv_heads;
+  const TreePlan pl = tree_plan(batch, kv_heads, group * nodes, nodes, capacity,
+                                sm_count > 0 ? sm_count : 148);
+  tr::Params p{};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_sb = qs.stride[0];
+  p.q_sh = qs.stride[1];
+  p.q_sn = qs.stride[2];
+  p.parents = parents;
+  p.parents_sb = parents_stride;
+  p.lens = cache_lens;
+  p.B = static_cast<int>(batch);
+  p.Hkv = static_cast<int>(kv_heads);
+  p.G = static_cast<int>(group);
+  p.N = static_cast<int>(nodes);
+  p.C = static_cast<int>(capacity);
+  p.row_tiles = static_cast<int>(pl.row_tiles);
+  p.splits = pl.splits;
+  p.o = static_cast<__nv_bfloat16*>(out);
+  p.lse = lse;
+  p.scale_log2 = kScaleLog2;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[1];
+  cluster_config(&cfg, attr, batch * kv_heads * pl.row_tiles * pl.splits, tr::THREADS,
+                 pl.rt == 1 ? tr::smem_bytes<1>() : tr::smem_bytes<2>(), pl.splits,
+                 static_cast<cudaStream_t>(stream));
+  const cudaError_t le =
+      pl.rt == 1 ? cudaLaunchKernelEx(&cfg, tr::tree_attention_kernel<1>, tmk, tmv, tmtk, tmtv, p)
+                 : cudaLaunchKernelEx(&cfg, tr::tree_attention_kernel<2>, tmk, tmv, tmtk, tmtv, p);
+  if (le != cudaSuccess)
+    return fail(TT_ATTN_LAUNCH_FAIL,
+                std::string("tree_attention_kernel launch: ") + cudaGetErrorString(le));
+  return check_launch("tree_attention_kernel launch");
+}
+
+TT_ATTN_API tt_attn_status tt_attn_tree_verify_f32(
+    const int64_t* tokens, const int32_t* parents, int64_t parents_stride,
+    const float* target_probs, int64_t tp_sb, int64_t tp_sn, const float* draft_probs,
+    int64_t dp_sb, int64_t dp_sn, const float* uniforms, int64_t batch, int64_t nodes,
+    int64_t vocab, int32_t* path, int32_t* counts, int64_t* next_tokens, void* stream) {
+  namespace vf = tt::verify;
+  if (!tokens || !parents || !target_probs || !uniforms || !path || !counts || !next_tokens)
+    return fail(TT_ATTN_BAD_ARG, "tree_verify: tokens, parents, target_probs, uniforms and the "
+                                 "outputs must not be NULL");
+  if (batch <= 0 || nodes <= 0 || vocab <= 0)
+    return fail(TT_ATTN_BAD_ARG, "tree_verify: batch, nodes and vocabulary must be positive");
+  if (nodes > TT_ATTN_TREE_MAX_NODES)
+    return fail(TT_ATTN_BAD_ARG, "tree_verify: at most 256 nodes per tree");
+  if (vocab > TT_ATTN_TREE_MAX_VOCAB)
+    return fail(TT_ATTN_BAD_ARG, "tree_verify: at most 4194304 tokens in the vocabulary");
+  if (batch > INT32_MAX / vf::MAX_CLUSTER)
+    return fail(TT_ATTN_BAD_ARG, "tree_verify: shape exceeds the supported CUDA grid limits");
+  if (parents_stride != 0 && parents_stride < nodes)
+    return fail(TT_ATTN_BAD_ARG, "tree_verify: parents_stride must be 0 or at least nodes");
+  if (tp_sb < 0 || tp_sn < 0 || dp_sb < 0 || dp_sn < 0)
+    return fail(TT_ATTN_BAD_ARG, "tree_verify: probability strides must not be negative");
+  for (const void* ptr : {static_cast<const void*>(parents), static_cast<const void*>(target_probs),
+                          static_cast<const void*>(draft_probs), static_cast<const void*>(uniforms),
+                          static_cast<const void*>(path), static_cast<const void*>(counts)})
+    if (reinterpret_cast<uintptr_t>(ptr) % 4 != 0)
+      return fail(TT_ATTN_BAD_ARG, "tree_verify: pointers must be 4-byte aligned");
+  for (const void* ptr : {static_cast<const void*>(tokens), static_cast<const void*>(next_tokens)})
+    if (reinterpret_cast<uintptr_t>(ptr) % 8 != 0)
+      return fail(TT_ATTN_BAD_ARG, "tree_verify: tokens and next_tokens must be 8-byte aligned");
+  int dev = 0;
+  const tt_attn_status st = prepare_device(&dev);
+  if (st != TT_ATTN_OK) return st;
+  vf::Params p{};
+  p.tokens = tokens;
+  p.parents = parents;
+  p.parents_sb = parents_stride;
+  p.p = target_probs;
+  p.p_sb = tp_sb;
+  p.p_sn = tp_sn;
+  p.q = draft_probs;
+  p.q_sb = dp_sb;
+  p.q_sn = dp_sn;
+  p.u = uniforms;
+  p.B = static_cast<int>(batch);
+  p.N = static_cast<int>(nodes);
+  p.V = static_cast<int>(vocab);
+  const int64_t windows = (vocab + vf::WINDOW - 1) / vf::WINDOW;
+  p.cluster = static_cast<int>(std::min<int64_t>(vf::MAX_CLUSTER, (windows + vf::WARPS - 1) / vf::WARPS));
+  p.windows = static_cast<int>((windows + p.cluster - 1) / p.cluster);
+  p.path = path;
+  p.counts = counts;
+  p.next = next_tokens;
+  // 16-byte loads where every row starts on a 16-byte boundary.
+  bool vec = vocab % 4 == 0 && tp_sb % 4 == 0 && tp_sn % 4 == 0 && aligned16(target_probs);
+  if (draft_probs != nullptr)
+    vec = vec && dp_sb % 4 == 0 && dp_sn % 4 == 0 && aligned16(draft_probs);
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[1];
+  cluster_config(&cfg, attr, batch * p.cluster, vf::THREADS, 0, p.cluster,
+                 static_cast<cudaStream_t>(stream));
+  cudaError_t le;
+  if (draft_probs != nullptr)
+    le = vec ? cudaLaunchKernelEx(&cfg, vf::tree_verify_kernel<true, true>, p)
+             : cudaLaunchKernelEx(&cfg, vf::tree_verify_kernel<true, false>, p);
+  else
+    le = vec ? cudaLaunchKernelEx(&cfg, vf::tree_verify_kernel<false, true>, p)
+             : cudaLaunchKernelEx(&cfg, vf::tree_verify_kernel<false, false>, p);
+  if (le != cudaSuccess)
+    return fail(TT_ATTN_LAUNCH_FAIL,
+                std::string("tree_verify_kernel launch: ") + cudaGetErrorString(le));
+  return check_launch("tree_verify_kernel launch");
+}
+
+TT_ATTN_API tt_attn_status tt_attn_tree_commit_bf16(
+    void* const* cache_k, const int64_t* ck_strides, void* const* cache_v,
+    const int64_t* cv_strides, const void* const* tree_k, const int64_t* tk_strides,
+    const void* const* tree_v, const int64_t* tv_strides, int64_t layers, int64_t batch,
+    int64_t kv_heads, int64_t nodes, int64_t capacity, int64_t head_dim, const int32_t* path,
+    int64_t path_len, const int32_t* counts, const int32_t* cache_lens, int32_t* new_lens,
+    void* stream) {
+  namespace cm = tt::commit;
+  if (!cache_k || !cache_v || !tree_k || !tree_v || !ck_strides || !cv_strides || !tk_strides ||
+      !tv_strides || !path || !counts || !cache_lens || !new_lens)
+    return fail(TT_ATTN_BAD_ARG, "tree_commit: pointers must not be NULL");
+  if (head_dim != TT_ATTN_HEAD_DIM)
+    return fail(TT_ATTN_BAD_ARG, "tree_commit currently supports only head_dim=64");
+  if (layers <= 0 || batch <= 0 || kv_heads <= 0 || nodes <= 0 || capacity <= 0 || path_len <= 0)
+    return fail(TT_ATTN_BAD_ARG, "tree_commit: sizes must be positive");
+  if (batch > INT32_MAX / (2 * cm::MAX_LAYERS) || nodes > INT32_MAX || capacity > INT32_MAX ||
+      path_len > INT32_MAX / kv_heads || new_lens == cache_lens)
+    return fail(TT_ATTN_BAD_ARG, new_lens == cache_lens
+                                     ? "tree_commit: new_lens needs a buffer of its own"
+                                     : "tree_commit: shape exceeds the supported CUDA grid limits");
+  const Shape4 ck = canonical(batch, kv_heads, capacity, ck_strides);
+  const Shape4 cv = canonical(batch, kv_heads, capacity, cv_strides);
+  const Shape4 tk = canonical(batch, kv_heads, nodes, tk_strides);
+  const Shape4 tv = canonical(batch, kv_heads, nodes, tv_strides);
+  for (int64_t l = 0; l < layers; ++l) {
+    if (!cache_k[l] || !cache_v[l] || !tree_k[l] || !tree_v[l])
+      return fail(TT_ATTN_BAD_ARG, "tree_commit: pointers must not be NULL");
+    if (!operand_ok(cache_k[l], ck) || !operand_ok(cache_v[l], cv) || !operand_ok(tree_k[l], tk) ||
+        !operand_ok(tree_v[l], tv))
+      return fail(TT_ATTN_UNSUPPORTED,
+                  "tree_commit: caches and trees need a unit last stride, other strides in "
+                  "multiples of 8 elements and 16-byte aligned bases");
+  }
+  for (const int32_t* ptr : {path, counts, cache_lens, static_cast<const int32_t*>(new_lens)})
+    if (reinterpret_cast<uintptr_t>(ptr) % 4 != 0)
+      return fail(TT_ATTN_BAD_ARG, "tree_commit: path, counts and lengths must be 4-byte aligned");
+  int dev = 0;
+  tt_attn_status st = prepare_device(&dev);
+  if (st != TT_ATTN_OK) return st;
+  for (int64_t first = 0; first < layers; first += cm::MAX_LAYERS) {
+    cm::Params p{};
+    p.layers = static_cast<int>(std::min<int64_t>(cm::MAX_LAYERS, layers - first));
+    for (int l = 0; l < p.layers; ++l) {
+      p.cache[0][l] = static_cast<__nv_bfloat16*>(cache_k[first + l]);
+      p.cache[1][l] = static_cast<__nv_bfloat16*>(cache_v[first + l]);
+      p.tree[0][l] = static_cast<const __nv_bfloat16*>(tree_k[first + l]);
+      p.tree[1][l] = static_cast<const __nv_bfloat16*>(tree_v[first + l]);
+    }
+    p.c_sb[0] = ck.stride[0]; p.c_sh[0] = ck.stride[1]; p.c_st[0] = ck.stride[2];
+    p.c_sb[1] = cv.stride[0]; p.c_sh[1] = cv.stride[1]; p.c_st[1] = cv.stride[2];
+    p.t_sb[0] = tk.stride[0]; p.t_sh[0] = tk.stride[1]; p.t_st[0] = tk.stride[2];
+    p.t_sb[1] = tv.stride[0]; p.t_sh[1] = tv.stride[1]; p.t_st[1] = tv.stride[2];
+    p.path = path;
+    p.counts = counts;
+    p.lens = cache_lens;
+    p.new_lens = first == 0 ? new_lens : nullptr;
+    p.B = static_cast<int>(batch);
+    p.H = static_cast<int>(kv_heads);
+    p.N = static_cast<int>(nodes);
+    p.C = static_cast<int>(capacity);
+    p.P = static_cast<int>(path_len);
+    tt::commit::tree_commit_kernel<<<static_cast<unsigned>(batch * p.layers * 2), cm::THREADS, 0,
+                                     static_cast<cudaStream_t>(stream)>>>(p);
+    if ((st = check_launch("tree_commit_kernel launch")) != TT_ATTN_OK) return st;
+  }
+  return TT_ATTN_OK;
+}
+
+}  // extern "C"

@@ -16,6 +16,7 @@
 #include <limits>
 #include <optional>
 #include <tuple>
+#include <vector>
 
 #include "tt_attention.h"
 
@@ -329,6 +330,239 @@ torch::Tensor qkv_rope_append(const torch::Tensor& hidden, const torch::Tensor& 
   return q_out;
 }
 
+// ------------------------------------------------------------------ speculative decoding
+// int32 copy of an index tensor where it is not one already; int64 values are clamped into int32,
+// so that none wraps into a valid index.
+torch::Tensor index32(const torch::Tensor& x, const torch::Tensor& like, const char* what) {
+  TORCH_CHECK(x.defined() && x.is_cuda() && x.device() == like.device(), what,
+              " must be a CUDA tensor on the same device as the other inputs");
+  TORCH_CHECK(x.scalar_type() == at::kInt || x.scalar_type() == at::kLong, what,
+              " must be int32 or int64");
+  if (x.scalar_type() == at::kInt) return x.contiguous();
+  return x.clamp(std::numeric_limits<int32_t>::min(), std::numeric_limits<int32_t>::max())
+      .to(at::kInt)
+      .contiguous();
+}
+
+// [N] (one tree) or [B, N] parents as int32; returns the row stride the C ABI takes.
+torch::Tensor tree_parents(const torch::Tensor& parents, const torch::Tensor& like, int64_t B,
+                           int64_t N, int64_t* stride) {
+  torch::Tensor p = index32(parents, like, "parents");
+  TORCH_CHECK((p.dim() == 1 && p.size(0) == N) ||
+                  (p.dim() == 2 && p.size(0) == B && p.size(1) == N),
+              "parents must have shape [N] or [B, N]");
+  *stride = p.dim() == 2 ? N : 0;
+  return p;
+}
+
+void check_sm100(const torch::Tensor& x) {
+  const auto* props = at::cuda::getDeviceProperties(x.get_device());
+  TORCH_CHECK(props->major == 10,
+              "the bf16 attention kernels require an sm_100 GPU (compute capability 10.x); "
+              "found SM", props->major, props->minor);
+}
+
+struct Strides {
+  int64_t s[4];
+  explicit Strides(const torch::Tensor& x) : s{x.stride(0), x.stride(1), x.stride(2), x.stride(3)} {}
+};
+
+// Attention of a tree of drafted tokens over a cache (tt_attn_tree_forward_bf16).
+std::tuple<torch::Tensor, torch::Tensor> tree_attention(
+    torch::Tensor q, torch::Tensor tree_k, torch::Tensor tree_v, torch::Tensor cache_k,
+    torch::Tensor cache_v, torch::Tensor parents, std::optional<torch::Tensor> cache_lens,
+    bool with_lse) {
+  for (const torch::Tensor* t : {&q, &tree_k, &tree_v, &cache_k, &cache_v}) {
+    TORCH_CHECK(t->defined() && t->is_cuda(), "tree_attention: all inputs must be CUDA tensors");
+    TORCH_CHECK(t->device() == q.device(),
+                "tree_attention: all inputs must be on the same device");
+    TORCH_CHECK(t->scalar_type() == at::kBFloat16,
+                "tree_attention: q, the tree's K/V and the caches must be bf16");
+    TORCH_CHECK(t->layout() == at::kStrided && t->dim() == 4,
+                "tree_attention: q, the tree's K/V and the caches must be strided 4D tensors");
+    TORCH_CHECK(t->size(3) == TT_ATTN_HEAD_DIM,
+                "tree_attention currently supports only head_dim=64");
+    TORCH_CHECK(t->size(0) == q.size(0), "tree_attention: all inputs must have the same batch size");
+  }
+  TORCH_CHECK(!(at::GradMode::is_enabled() &&
+                (q.requires_grad() || tree_k.requires_grad() || tree_v.requires_grad() ||
+                 cache_k.requires_grad() || cache_v.requires_grad())),
+              "tree_attention has no backward; call it under no_grad");
+  const int64_t B = q.size(0), Hq = q.size(1), N = q.size(2), Hkv = cache_k.size(1),
+                C = cache_k.size(2);
+  TORCH_CHECK(B > 0 && Hq > 0 && N > 0 && Hkv > 0 && C > 0,
+              "tree_attention: batch, heads, nodes and cache capacity must be positive");
+  TORCH_CHECK(Hq % Hkv == 0, "tree_attention: q heads must be a multiple of the K/V heads");
+  TORCH_CHECK(N <= TT_ATTN_TREE_MAX_NODES, "tree_attention: at most 256 nodes per tree");
+  TORCH_CHECK(cache_v.sizes() == cache_k.sizes(),
+              "tree_attention: the K and V caches must have the same shape");
+  TORCH_CHECK(tree_k.size(1) == Hkv && tree_k.size(2) == N && tree_v.sizes() == tree_k.sizes(),
+              "tree_attention: the tree's K and V must have shape [B, kv_heads, N, 64]");
+  if (cache_lens.has_value())
+    TORCH_CHECK(cache_lens->defined() && cache_lens->dim() == 1 && cache_lens->size(0) == B,
+                "tree_attention: cache_lens must have shape [B]");
+  const c10::cuda::CUDAGuard device_guard(q.device());
+  check_sm100(q);
+  int64_t parents_stride = 0;
+  parents = tree_parents(parents, q, B, N, &parents_stride);
+  torch::Tensor lens;
+  if (cache_lens.has_value()) lens = index32(*cache_lens, q, "cache_lens");
+  auto stream = c10::cuda::getCurrentCUDAStream(q.get_device());
+  q = aligned_contiguous(q);
+  tree_k = aligned_contiguous(tree_k);
+  tree_v = aligned_contiguous(tree_v);
+  cache_k = aligned_contiguous(cache_k);
+  cache_v = aligned_contiguous(cache_v);
+  auto o = torch::empty({B, Hq, N, TT_ATTN_HEAD_DIM}, q.options());
+  torch::Tensor lse;
+  if (with_lse) lse = torch::empty({B, Hq, N}, q.options().dtype(at::kFloat));
+  const size_t ws_bytes = tt_attn_tree_workspace_size(B, Hq, Hkv, N, C);
+  torch::Tensor ws;
+  if (ws_bytes > 0)
+    ws = torch::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(at::kByte));
+  const Strides qs(q), tks(tree_k), tvs(tree_v), cks(cache_k), cvs(cache_v);
+  const tt_attn_status st = tt_attn_tree_forward_bf16(
+      q.data_ptr(), qs.s, tree_k.data_ptr(), tks.s, tree_v.data_ptr(), tvs.s, cache_k.data_ptr(),
+      cks.s, cache_v.data_ptr(), cvs.s, B, Hq, Hkv, N, C, TT_ATTN_HEAD_DIM,
+      parents.data_ptr<int32_t>(), parents_stride,
+      lens.defined() ? lens.data_ptr<int32_t>() : nullptr, o.data_ptr(),
+      with_lse ? lse.data_ptr<float>() : nullptr, ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes,
+      static_cast<void*>(stream.stream()));
+  TORCH_CHECK(st == TT_ATTN_OK, "tt_attn_tree_forward_bf16 failed: ", tt_attn_status_string(st),
+              ": ", tt_attn_last_error());
+  return {o, lse};
+}
+
+// Walk of a token tree with given random numbers (tt_attn_tree_verify_f32).
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> tree_verify(
+    torch::Tensor tokens, torch::Tensor parents, torch::Tensor target_probs,
+    torch::Tensor uniforms, std::optional<torch::Tensor> draft_probs) {
+  TORCH_CHECK(target_probs.defined() && target_probs.is_cuda(),
+              "verify_tree: all inputs must be CUDA tensors");
+  TORCH_CHECK(target_probs.scalar_type() == at::kFloat && target_probs.dim() == 3,
+              "verify_tree: target_probs must be a float32 [B, N, V] tensor");
+  const int64_t B = target_probs.size(0), N = target_probs.size(1), V = target_probs.size(2);
+  TORCH_CHECK(B > 0 && N > 0 && V > 0, "verify_tree: batch, nodes and vocabulary must be positive");
+  TORCH_CHECK(N <= TT_ATTN_TREE_MAX_NODES, "verify_tree: at most 256 nodes per tree");
+  TORCH_CHECK(V <= TT_ATTN_TREE_MAX_VOCAB,
+              "verify_tree: at most ", TT_ATTN_TREE_MAX_VOCAB, " tokens in the vocabulary");
+  for (const torch::Tensor* t : {&tokens, &uniforms})
+    TORCH_CHECK(t->defined() && t->is_cuda() && t->device() == target_probs.device(),
+                "verify_tree: all inputs must be CUDA tensors on the same device");
+  TORCH_CHECK(tokens.dim() == 2 && tokens.size(0) == B && tokens.size(1) == N &&
+                  (tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt),
+              "verify_tree: tokens must be an int64 or int32 [B, N] tensor");
+  TORCH_CHECK(uniforms.dim() == 2 && uniforms.size(0) == B && uniforms.size(1) == N &&
+                  uniforms.scalar_type() == at::kFloat,
+              "verify_tree: uniforms must be a float32 [B, N] tensor");
+  const bool dense = draft_probs.has_value();
+  if (dense)
+    TORCH_CHECK(draft_probs->defined() && draft_probs->is_cuda() &&
+                    draft_probs->device() == target_probs.device() &&
+                    draft_probs->scalar_type() == at::kFloat &&
+                    draft_probs->sizes() == target_probs.sizes(),
+                "verify_tree: draft_probs must be a float32 [B, N, V] tensor on the same device");
+  const c10::cuda::CUDAGuard device_guard(target_probs.device());
+  check_sm100(target_probs);
+  int64_t parents_stride = 0;
+  parents = tree_parents(parents, target_probs, B, N, &parents_stride);
+  tokens = tokens.to(at::kLong).contiguous();
+  uniforms = uniforms.contiguous();
+  // Rows are read in place when their values are adjacent; other views are copied.
+  if (V > 1 && target_probs.stride(2) != 1) target_probs = target_probs.contiguous();
+  torch::Tensor dp;
+  if (dense)
+    dp = V > 1 && draft_probs->stride(2) != 1 ? draft_probs->contiguous() : *draft_probs;
+  auto path = torch::empty({B, N}, target_probs.options().dtype(at::kInt));
+  auto counts = torch::empty({B}, target_probs.options().dtype(at::kInt));
+  auto next = torch::empty({B}, target_probs.options().dtype(at::kLong));
+  auto stream = c10::cuda::getCurrentCUDAStream(target_probs.get_device());
+  const tt_attn_status st = tt_attn_tree_verify_f32(
+      tokens.data_ptr<int64_t>(), parents.data_ptr<int32_t>(), parents_stride,
+      target_probs.data_ptr<float>(), target_probs.stride(0), target_probs.stride(1),
+      dense ? dp.data_ptr<float>() : nullptr, dense ? dp.stride(0) : 0, dense ? dp.stride(1) : 0,
+      uniforms.data_ptr<float>(), B, N, V, path.data_ptr<int32_t>(), counts.data_ptr<int32_t>(),
+      next.data_ptr<int64_t>(), static_cast<void*>(stream.stream()));
+  TORCH_CHECK(st == TT_ATTN_OK, "tt_attn_tree_verify_f32 failed: ", tt_attn_status_string(st), ": ",
+              tt_attn_last_error());
+  return {path, counts, next};
+}
+
+// Append of the accepted path to the caches of all layers (tt_attn_tree_commit_bf16).
+torch::Tensor tree_commit(std::vector<torch::Tensor> cache_k, std::vector<torch::Tensor> cache_v,
+                          std::vector<torch::Tensor> tree_k, std::vector<torch::Tensor> tree_v,
+                          torch::Tensor path, torch::Tensor counts, torch::Tensor cache_lens) {
+  const size_t L = cache_k.size();
+  TORCH_CHECK(L > 0 && cache_v.size() == L && tree_k.size() == L && tree_v.size() == L,
+              "commit_path: the caches and the trees must have the same, positive number of layers");
+  for (auto* list : {&cache_k, &cache_v, &tree_k, &tree_v})
+    for (const torch::Tensor& t : *list) {
+      TORCH_CHECK(t.defined() && t.is_cuda(), "commit_path: all inputs must be CUDA tensors");
+      TORCH_CHECK(t.device() == cache_k[0].device(),
+                  "commit_path: all inputs must be on the same device");
+      TORCH_CHECK(t.scalar_type() == at::kBFloat16 && t.layout() == at::kStrided && t.dim() == 4,
+                  "commit_path: caches and trees must be strided 4D bf16 tensors");
+      TORCH_CHECK(t.size(3) == TT_ATTN_HEAD_DIM, "commit_path currently supports only head_dim=64");
+      TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()),
+                  "commit_path writes the caches in place and has no backward; call it under no_grad");
+    }
+  const int64_t B = cache_k[0].size(0), H = cache_k[0].size(1), C = cache_k[0].size(2),
+                N = tree_k[0].size(2);
+  TORCH_CHECK(B > 0 && H > 0 && C > 0 && N > 0, "commit_path: sizes must be positive");
+  auto strides_differ = [](const std::vector<torch::Tensor>& list) {
+    for (const torch::Tensor& t : list) {
+      if (!readable_in_place(t)) return true;
+      for (int64_t d = 0; d < 4; ++d)
+        if (t.size(d) > 1 && t.stride(d) != list[0].stride(d)) return true;
+    }
+    return false;
+  };
+  for (auto* list : {&cache_k, &cache_v}) {
+    for (const torch::Tensor& t : *list)
+      TORCH_CHECK(t.sizes() == cache_k[0].sizes(),
+                  "commit_path: all caches must have the same shape");
+    TORCH_CHECK(!strides_differ(*list),
+                "commit_path: the caches need equal strides, a unit last stride, other strides in "
+                "multiples of 8 elements and 16-byte aligned bases (they are written in place)");
+  }
+  for (auto* list : {&tree_k, &tree_v})
+    for (const torch::Tensor& t : *list)
+      TORCH_CHECK(t.size(0) == B && t.size(1) == H && t.size(2) == N,
+                  "commit_path: the trees must have shape [B, kv_heads, N, 64]");
+  TORCH_CHECK(path.defined() && path.dim() == 2 && path.size(0) == B && path.size(1) > 0,
+              "commit_path: path must have shape [B, P]");
+  TORCH_CHECK(counts.defined() && counts.dim() == 1 && counts.size(0) == B && cache_lens.defined() &&
+                  cache_lens.dim() == 1 && cache_lens.size(0) == B,
+              "commit_path: counts and cache_lens must have shape [B]");
+  const c10::cuda::CUDAGuard device_guard(cache_k[0].device());
+  check_sm100(cache_k[0]);
+  path = index32(path, cache_k[0], "path");
+  counts = index32(counts, cache_k[0], "counts");
+  cache_lens = index32(cache_lens, cache_k[0], "cache_lens");
+  for (auto* list : {&tree_k, &tree_v})
+    if (strides_differ(*list))
+      for (torch::Tensor& t : *list) t = t.clone(at::MemoryFormat::Contiguous);
+  auto new_lens = torch::empty({B}, cache_lens.options());
+  std::vector<void*> ck(L), cv(L);
+  std::vector<const void*> tk(L), tv(L);
+  for (size_t l = 0; l < L; ++l) {
+    ck[l] = cache_k[l].data_ptr();
+    cv[l] = cache_v[l].data_ptr();
+    tk[l] = tree_k[l].data_ptr();
+    tv[l] = tree_v[l].data_ptr();
+  }
+  const Strides cks(cache_k[0]), cvs(cache_v[0]), tks(tree_k[0]), tvs(tree_v[0]);
+  auto stream = c10::cuda::getCurrentCUDAStream(cache_k[0].get_device());
+  const tt_attn_status st = tt_attn_tree_commit_bf16(
+      ck.data(), cks.s, cv.data(), cvs.s, tk.data(), tks.s, tv.data(), tvs.s,
+      static_cast<int64_t>(L), B, H, N, C, TT_ATTN_HEAD_DIM, path.data_ptr<int32_t>(), path.size(1),
+      counts.data_ptr<int32_t>(), cache_lens.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(),
+      static_cast<void*>(stream.stream()));
+  TORCH_CHECK(st == TT_ATTN_OK, "tt_attn_tree_commit_bf16 failed: ", tt_attn_status_string(st), ": ",
+              tt_attn_last_error());
+  return new_lens;
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attention_forward", &attention_forward,
         "BF16 causal attention forward on sm_100a (returns O and natural-log FP32 LSE)",
@@ -349,6 +583,20 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("hidden"), pybind11::arg("w_qkv"), pybind11::arg("cos"),
         pybind11::arg("sin"), pybind11::arg("position"), pybind11::arg("cache_k"),
         pybind11::arg("cache_v"));
+  m.def("tree_attention", &tree_attention,
+        "Attention of a tree of drafted tokens over a KV cache; returns O and (with_lse) LSE",
+        pybind11::arg("q"), pybind11::arg("tree_k"), pybind11::arg("tree_v"),
+        pybind11::arg("cache_k"), pybind11::arg("cache_v"), pybind11::arg("parents"),
+        pybind11::arg("cache_lens") = pybind11::none(), pybind11::arg("with_lse") = true);
+  m.def("tree_verify", &tree_verify,
+        "Walk of a drafted token tree with given random numbers; returns path, counts, next tokens",
+        pybind11::arg("tokens"), pybind11::arg("parents"), pybind11::arg("target_probs"),
+        pybind11::arg("uniforms"), pybind11::arg("draft_probs") = pybind11::none());
+  m.def("tree_commit", &tree_commit,
+        "Append of the accepted path's K/V rows to the caches of all layers; returns new lengths",
+        pybind11::arg("cache_k"), pybind11::arg("cache_v"), pybind11::arg("tree_k"),
+        pybind11::arg("tree_v"), pybind11::arg("path"), pybind11::arg("counts"),
+        pybind11::arg("cache_lens"));
   m.attr("HEAD_DIM") = TT_ATTN_HEAD_DIM;
   m.attr("ABI_VERSION") = TT_ATTN_ABI_VERSION;
 }

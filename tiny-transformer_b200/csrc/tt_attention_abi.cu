@@ -26,6 +26,9 @@
 #include "qkv_rope_sm100.cuh"
 #include "backward_sm100.cuh"
 #include "backward_det_sm100.cuh"
+#include "tree_attention_sm100.cuh"
+#include "tree_verify_sm100.cuh"
+#include "tree_commit_sm100.cuh"
 
 namespace {
 
@@ -1294,3 +1297,6 @@ TT_ATTN_API tt_attn_status tt_attn_decode_bf16_noalloc(
 }
 
 }  // extern "C"
+
+// ------------------------------------------------------------------ speculative decoding
+#include "speculative_abi.cuh"

@@ -74,6 +74,26 @@ def load_c_abi() -> ctypes.CDLL:
         ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, i64p, ctypes.c_void_p, i64p,
         ctypes.c_int64, ctypes.c_void_p]
+    lib.tt_attn_tree_forward_bf16.restype = ctypes.c_int
+    lib.tt_attn_tree_forward_bf16.argtypes = [
+        ctypes.c_void_p, i64p, ctypes.c_void_p, i64p, ctypes.c_void_p, i64p, ctypes.c_void_p, i64p,
+        ctypes.c_void_p, i64p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+        ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+    lib.tt_attn_tree_workspace_size.restype = ctypes.c_size_t
+    lib.tt_attn_tree_workspace_size.argtypes = [ctypes.c_int64] * 5
+    lib.tt_attn_tree_verify_f32.restype = ctypes.c_int
+    lib.tt_attn_tree_verify_f32.argtypes = [
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
+        ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
+        ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
+        ctypes.c_void_p, ctypes.c_void_p]
+    voidpp = ctypes.POINTER(ctypes.c_void_p)
+    lib.tt_attn_tree_commit_bf16.restype = ctypes.c_int
+    lib.tt_attn_tree_commit_bf16.argtypes = [
+        voidpp, i64p, voidpp, i64p, voidpp, i64p, voidpp, i64p, ctypes.c_int64, ctypes.c_int64,
+        ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
+        ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
     lib.tt_attn_selftest_wait_timeout.restype = ctypes.c_int
     lib.tt_attn_selftest_wait_timeout.argtypes = [ctypes.c_int64, ctypes.c_void_p]
     lib.tt_attn_status_string.restype = ctypes.c_char_p
