@@ -5,26 +5,59 @@
 
 namespace {
 
-// Query rows per CTA tile of the tree attention: 16 or 32 (tree_attention_kernel<1 or 2>).
-int tree_row_tiles(int64_t rows) { return rows <= 16 ? 1 : 2; }
-
+// Variant and split of one tree-attention call (sizes only: the workspace does not depend on the
+// device).
 struct TreePlan {
-  int rt = 1;             // 16-row tiles per CTA
-  int64_t row_tiles = 1;  // CTA tiles of one (batch, K/V head)
-  int splits = 1;         // CTAs per cluster
+  bool persistent = false;
+  int64_t rows = 0;       // query rows of a CTA's tile
+  int64_t row_tiles = 1;  // tiles of one (batch, K/V head)
+  int rt = 1;             // cluster kernel: 16-row tiles per CTA
+  int splits = 1;         // cluster kernel: CTAs per cluster
+  int dup = 1;            // persistent kernel: copies of the rows in a 128-row tile
+  int64_t grid = 0;       // persistent kernel: CTAs
 };
 
-TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t nodes, int64_t capacity,
-                   int sms) {
+TreePlan tree_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nodes,
+                   int64_t capacity) {
   TreePlan pl;
-  pl.rt = tree_row_tiles(rows);
-  pl.row_tiles = (rows + pl.rt * 16 - 1) / (pl.rt * 16);
+  const int64_t rows = q_heads / kv_heads * nodes;
+  const int64_t tree_tiles = (nodes + tt::tree::KEYS - 1) / tt::tree::KEYS;
+  const int64_t tiles = tree_tiles + (capacity + tt::tree::KEYS - 1) / tt::tree::KEYS;
+  // More than 16 stacked query rows take the persistent kernel: measured 68 against 130 us for 64
+  // rows (B = 32, H = 12, 1024-4096 cached) and 31 against 77 us for 111 rows of 4 shared heads
+  // (9000-20001 cached); with 16 rows or fewer the cluster kernel's lighter start and end win
+  // (151 against 165 us for 16 rows at 1024-8192 cached, 14 against 16 at 256-512).
+  pl.persistent = rows > 16;
+  if (pl.persistent) {
+    constexpr int64_t bm = tt::tree::persist::BM;
+    pl.row_tiles = (rows + bm - 1) / bm;
+    pl.rows = (rows + pl.row_tiles - 1) / pl.row_tiles;
+    pl.dup = pl.rows <= bm / 4 ? 4 : pl.rows <= bm / 2 ? 2 : 1;
+    pl.grid = std::min<int64_t>(kPlanSms, batch * kv_heads * pl.row_tiles * tiles);
+    return pl;
+  }
+  pl.rt = rows <= 16 ? 1 : 2;
+  pl.rows = pl.rt * 16;
+  pl.row_tiles = (rows + pl.rows - 1) / pl.rows;
   const int64_t units = batch * kv_heads * pl.row_tiles;
-  const int64_t tiles = (nodes + tt::tree::KEYS - 1) / tt::tree::KEYS +
-                        (capacity + tt::tree::KEYS - 1) / tt::tree::KEYS;
   pl.splits = static_cast<int>(std::max<int64_t>(
-      1, std::min<int64_t>({tt::tree::MAX_SPLITS, tiles, 3 * static_cast<int64_t>(sms) / units})));
+      1, std::min<int64_t>({tt::tree::MAX_SPLITS, tiles, 3 * kPlanSms / units})));
   return pl;
+}
+
+size_t tree_starts_bytes(const TreePlan& pl) {
+  return (static_cast<size_t>(pl.grid) * sizeof(tt::tree::persist::Start) + 255) & ~size_t(255);
+}
+
+bool tree_shape_ok(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nodes,
+                   int64_t capacity) {
+  const int64_t max_rows = INT32_MAX / (TT_ATTN_TREE_MAX_NODES * tt::tree::MAX_SPLITS);
+  return batch > 0 && q_heads > 0 && kv_heads > 0 && nodes > 0 && capacity > 0 &&
+         q_heads % kv_heads == 0 && nodes <= TT_ATTN_TREE_MAX_NODES &&
+         capacity <= INT32_MAX - tt::tree::KEYS && batch <= max_rows && q_heads <= max_rows &&
+         batch <= max_rows / q_heads &&
+         // key tiles of all (batch, q head, 128-row tile): the persistent kernel counts them in 32 bits
+         (capacity / tt::tree::KEYS + 4) * 2 <= INT32_MAX / (batch * q_heads);
 }
 
 tt_attn_status set_tree_attributes() {
@@ -41,6 +74,12 @@ tt_attn_status set_tree_attributes() {
       e = cudaFuncSetAttribute(tt::tree::tree_attention_kernel<2>,
                                cudaFuncAttributeMaxDynamicSharedMemorySize,
                                static_cast<int>(tt::tree::smem_bytes<2>()));
+    for (auto fn : {tt::tree::persist::tree_persistent_kernel<1>,
+                    tt::tree::persist::tree_persistent_kernel<2>,
+                    tt::tree::persist::tree_persistent_kernel<4>})
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(tt::tree::persist::kSmemBytes));
     if (e == cudaSuccess) done[dev] = true;
   }
   if (e != cudaSuccess)
@@ -63,6 +102,50 @@ void cluster_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, int64_t 
   cfg->numAttrs = 1;
 }
 
+tt_attn_status launch_tree_persistent(const TreePlan& pl, const tt::tree::Params& tp,
+                                      const void* tree_v, const Shape4& tvs, void* workspace,
+                                      int sm_count, const CUtensorMap& tmk, const CUtensorMap& tmv,
+                                      const CUtensorMap& tmtk, const CUtensorMap& tmtv,
+                                      cudaStream_t stream) {
+  namespace ps = tt::tree::persist;
+  ps::Params p{};
+  p.t = tp;
+  p.tree_v = static_cast<const __nv_bfloat16*>(tree_v);
+  p.tv_sb = tvs.stride[0];
+  p.tv_sh = tvs.stride[1];
+  p.tv_sn = tvs.stride[2];
+  p.rows = static_cast<int>(pl.rows);
+  p.units = static_cast<int>(tp.Hkv * pl.row_tiles);
+  p.tree_tiles = (tp.N + tt::tree::KEYS - 1) / tt::tree::KEYS;
+  p.starts = static_cast<ps::Start*>(workspace);
+  p.records = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + tree_starts_bytes(pl));
+  const int grid = static_cast<int>(std::min<int64_t>(pl.grid, sm_count > 0 ? sm_count : kPlanSms));
+  auto kernel = pl.dup == 4 ? ps::tree_persistent_kernel<4>
+                            : pl.dup == 2 ? ps::tree_persistent_kernel<2>
+                                          : ps::tree_persistent_kernel<1>;
+  kernel<<<static_cast<unsigned>(grid), ps::THREADS, ps::kSmemBytes, stream>>>(tmk, tmv, tmtk, tmtv,
+                                                                             p);
+  tt_attn_status st = check_launch("tree_persistent_kernel launch");
+  if (st != TT_ATTN_OK || grid == 1) return st;
+  // The merge may be scheduled while the main kernel runs (programmatic launch); it waits for its
+  // completion on the device.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid - 1),
+                     static_cast<unsigned>((pl.rows + ps::COMBINE_ROWS - 1) / ps::COMBINE_ROWS), 1);
+  cfg.blockDim = dim3(ps::COMBINE_THREADS, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t le = cudaLaunchKernelEx(&cfg, ps::tree_combine_kernel, p, grid);
+  if (le != cudaSuccess)
+    return fail(TT_ATTN_LAUNCH_FAIL,
+                std::string("tree_combine_kernel launch: ") + cudaGetErrorString(le));
+  return check_launch("tree_combine_kernel launch");
+}
+
 // [batch, heads, rows, 64] operand of the speculative operators: readable in place?
 bool operand_ok(const void* p, const Shape4& s) { return aligned16(p) && strides_ok(s.stride); }
 
@@ -72,8 +155,11 @@ extern "C" {
 
 TT_ATTN_API size_t tt_attn_tree_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads,
                                                int64_t nodes, int64_t capacity) {
-  (void)batch; (void)q_heads; (void)kv_heads; (void)nodes; (void)capacity;
-  return 0;
+  if (!tree_shape_ok(batch, q_heads, kv_heads, nodes, capacity)) return 0;
+  const TreePlan pl = tree_plan(batch, q_heads, kv_heads, nodes, capacity);
+  if (!pl.persistent) return 0;
+  return tree_starts_bytes(pl) +
+         static_cast<size_t>(pl.grid) * 2 * pl.rows * tt::tree::REC * sizeof(float);
 }
 
 TT_ATTN_API tt_attn_status tt_attn_tree_forward_bf16(
@@ -102,8 +188,7 @@ TT_ATTN_API tt_attn_status tt_attn_tree_forward_bf16(
     return fail(TT_ATTN_BAD_ARG, "tree_attention: the cache capacity must fit int32");
   if (parents_stride != 0 && parents_stride < nodes)
     return fail(TT_ATTN_BAD_ARG, "tree_attention: parents_stride must be 0 or at least nodes");
-  const int64_t max_rows = INT32_MAX / (TT_ATTN_TREE_MAX_NODES * tr::MAX_SPLITS);
-  if (batch > max_rows || q_heads > max_rows || batch > max_rows / q_heads)
+  if (!tree_shape_ok(batch, q_heads, kv_heads, nodes, capacity))
     return fail(TT_ATTN_BAD_ARG, "tree_attention: shape exceeds the supported CUDA grid limits");
   const Shape4 qs = canonical(batch, q_heads, nodes, q_strides);
   const Shape4 tks = canonical(batch, kv_heads, nodes, tk_strides);
@@ -138,8 +223,7 @@ TT_ATTN_API tt_attn_status tt_attn_tree_forward_bf16(
       !encode_map(&tmtv, tree_v, tvs, &err, tr::KEYS))
     return fail(TT_ATTN_UNSUPPORTED, err);
   const int64_t group = q_heads / kv_heads;
-  const TreePlan pl = tree_plan(batch, kv_heads, group * nodes, nodes, capacity,
-                                sm_count > 0 ? sm_count : 148);
+  const TreePlan pl = tree_plan(batch, q_heads, kv_heads, nodes, capacity);
   tr::Params p{};
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.q_sb = qs.stride[0];
@@ -160,6 +244,9 @@ TT_ATTN_API tt_attn_status tt_attn_tree_forward_bf16(
   p.scale_log2 = kScaleLog2;
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[1];
+  if (pl.persistent)
+    return launch_tree_persistent(pl, p, tree_v, tvs, workspace, sm_count, tmk, tmv, tmtk, tmtv,
+                                  static_cast<cudaStream_t>(stream));
   cluster_config(&cfg, attr, batch * kv_heads * pl.row_tiles * pl.splits, tr::THREADS,
                  pl.rt == 1 ? tr::smem_bytes<1>() : tr::smem_bytes<2>(), pl.splits,
                  static_cast<cudaStream_t>(stream));

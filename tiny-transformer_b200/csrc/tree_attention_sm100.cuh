@@ -70,13 +70,13 @@ struct alignas(1024) Smem {
   };
   float crec[ROWS][REC];                             // the CTA's result, read by the cluster
   uint32_t mask[MAX_NODES][MASK_WORDS];              // bit m of row n: node n sees node m
-  int32_t parent[MAX_NODES];
+  int32_t jump[MAX_NODES];
   uint64_t full[STAGES], empty[STAGES];
   int used[ROWS];                                    // rank 0: rows whose node is in use
   volatile int abort;
 };
 template <int RT>
-constexpr size_t smem_bytes() { return sizeof(Smem<RT>) + 1024; }
+constexpr size_t smem_bytes() { return sizeof(Smem<RT>); }
 
 // Bounded wait that gives up as soon as another warp of the CTA has given up.
 __device__ __forceinline__ bool wait_or_abort(volatile int* abort, uint64_t* bar, uint32_t parity) {
@@ -136,33 +136,51 @@ __device__ __forceinline__ int valid_len(const int32_t* lens, int C, int b) {
   return min(max(__ldg(lens + b), 0), C);
 }
 
-// Ancestor masks of one tree from its parents: thread n climbs from node n and marks its own row.
-// Links go to strictly lower indices (any other link ends the chain as unused), so a climb ends
-// after at most N steps whatever the parents hold. Barrier `sync` is a barrier of `threads`
-// consecutive threads that all call this.
+// Ancestor masks of one tree from its parents, by doubling: mask[n] covers the chain from n up to,
+// and without, jump[n]; a round ORs in the mask at jump[n] and jumps as far as that does, so a
+// chain of any length takes log2(length) rounds. Links go to strictly lower indices (any other
+// link ends the chain as unused, jump -2), so rounds go over blocks of `threads` nodes from the
+// highest down, each reading before it writes, and never meet a node already updated this round.
+// `sync` is a barrier of the `threads` threads that all call this; it returns whether any of them
+// passed true.
 template <typename Sync>
-__device__ __forceinline__ void build_masks(const int32_t* parents, int N, int32_t* parent,
+__device__ __forceinline__ void build_masks(const int32_t* parents, int N, int32_t* jump,
                                             uint32_t (*mask)[MASK_WORDS], int tid, int threads,
                                             Sync sync) {
+  const int words = (N + 31) >> 5;
+  bool more = false;
   for (int n = tid; n < N; n += threads) {
-    parent[n] = __ldg(parents + n);
-#pragma unroll
-    for (int w = 0; w < MASK_WORDS; ++w) mask[n][w] = 0;
+    const int up = __ldg(parents + n);
+    jump[n] = up < n && up >= -1 ? up : -2;
+    more = more || (up < n && up >= 0);
+    for (int w = 0; w < MASK_WORDS; ++w) mask[n][w] = w == n >> 5 ? 1u << (n & 31) : 0u;
   }
-  sync();
-  for (int n = tid; n < N; n += threads) {
-    int m = n;
-    while (m >= 0) {
-      mask[n][m >> 5] |= 1u << (m & 31);
-      const int up = parent[m];
-      m = (up < m && up >= -1) ? up : -2;
-    }
-    if (m != -1) {
+  while (sync(more)) {
+    more = false;
+    for (int base = (N - 1) / threads * threads; base >= 0; base -= threads) {
+      const int n = base + tid;
+      const int j = n < N ? jump[n] : -1;
+      int far = j;
+      uint32_t add[MASK_WORDS];
+      if (j >= 0) {
+        far = jump[j];
 #pragma unroll
+        for (int w = 0; w < MASK_WORDS; ++w) add[w] = w < words ? mask[j][w] : 0u;
+      }
+      sync(false);
+      if (j >= 0) {
+        jump[n] = far;
+#pragma unroll
+        for (int w = 0; w < MASK_WORDS; ++w)
+          if (w < words) mask[n][w] |= add[w];
+        more = more || far >= 0;
+      }
+    }
+  }
+  for (int n = tid; n < N; n += threads)
+    if (jump[n] != -1)
       for (int w = 0; w < MASK_WORDS; ++w) mask[n][w] = 0;
-    }
-  }
-  sync();
+  sync(false);
 }
 
 __device__ __forceinline__ bool node_used(const uint32_t (*mask)[MASK_WORDS], int n) {
@@ -171,6 +189,19 @@ __device__ __forceinline__ bool node_used(const uint32_t (*mask)[MASK_WORDS], in
 
 __device__ __forceinline__ bool has_nonfinite(uint32_t u) {
   return (u & 0x7F80u) == 0x7F80u || (u & 0x7F800000u) == 0x7F800000u;
+}
+
+// Named barrier 1 of `THREADS_` threads; whether any of them passed true.
+template <int THREADS_>
+__device__ __forceinline__ bool barrier_or(bool any) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred.aligned q, 1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r) : "r"(any ? 1u : 0u), "n"(THREADS_) : "memory");
+  return r != 0;
 }
 
 // One warp's state: Q fragments of RT row tiles, and the online softmax of its keys.
@@ -420,9 +451,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_tk,
                       const __grid_constant__ CUtensorMap tm_tv, const Params p) {
   constexpr int ROWS = RT * 16;
-  extern __shared__ uint8_t smem_raw[];
-  Smem<RT>& s = *reinterpret_cast<Smem<RT>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  Smem<RT>& s = *reinterpret_cast<Smem<RT>*>(smem_raw);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
@@ -475,9 +505,9 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tm_k,
     load_q(st, p, b, h, row0, lane);
     reset(st);
     if (first < tree_tiles || rank == 0) {
-      build_masks(p.parents + b * p.parents_sb, p.N, s.parent, s.mask, threadIdx.x,
+      build_masks(p.parents + b * p.parents_sb, p.N, s.jump, s.mask, threadIdx.x,
                   CONSUMER_WARPS * 32,
-                  [] { asm volatile("bar.sync 1, %0;" ::"n"(CONSUMER_WARPS * 32) : "memory"); });
+                  [](bool any) { return barrier_or<CONSUMER_WARPS * 32>(any); });
     }
     if (rank == 0 && threadIdx.x < ROWS) {
       const int r = row0 + static_cast<int>(threadIdx.x);

@@ -27,6 +27,7 @@
 #include "backward_sm100.cuh"
 #include "backward_det_sm100.cuh"
 #include "tree_attention_sm100.cuh"
+#include "tree_persistent_sm100.cuh"
 #include "tree_verify_sm100.cuh"
 #include "tree_commit_sm100.cuh"
 
