@@ -306,7 +306,7 @@ TT_ATTN_API size_t tt_attn_tree_workspace_size(int64_t batch, int64_t q_heads, i
  *
  * Weights are whole numbers (probabilities times 2^36, rounded down), so results do not depend on
  * the order of any sum; the exact definition is at the kernel. Probabilities are taken into
- * [0, 2], NaN as 0. 1 <= nodes <= TT_ATTN_TREE_MAX_NODES, vocab <= TT_ATTN_TREE_MAX_VOCAB.
+ * [0, 1], NaN as 0. 1 <= nodes <= TT_ATTN_TREE_MAX_NODES, vocab <= TT_ATTN_TREE_MAX_VOCAB.
  */
 TT_ATTN_API tt_attn_status tt_attn_tree_verify_f32(
     const int64_t* tokens, const int32_t* parents, int64_t parents_stride,

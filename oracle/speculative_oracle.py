@@ -56,7 +56,7 @@ def verify_tree(tokens, parents, p, u, q=None):
             continue
         cur, taken = 0, [0]
         while True:
-            pc = np.clip(np.nan_to_num(p[b, cur], nan=0.0), 0, 2).astype(np.float64)
+            pc = np.clip(np.nan_to_num(p[b, cur], nan=0.0), 0, 1).astype(np.float64)
             base = np.floor(pc * ONE).astype(np.int64)
             r, S, hit = base.copy(), None, None
             for c in [c for c in range(cur + 1, N) if parents[b, c] == cur]:
@@ -67,7 +67,7 @@ def verify_tree(tokens, parents, p, u, q=None):
                     qc[t if known else slice(0, 0)] = 1.0
                     qt = 1.0
                 else:
-                    qc = np.clip(np.nan_to_num(q[b, cur], nan=0.0), 0, 2).astype(np.float64)
+                    qc = np.clip(np.nan_to_num(q[b, cur], nan=0.0), 0, 1).astype(np.float64)
                     qt = qc[t] if known else 0.0
                 if S is None:
                     ok = known and np.float32(u[b, c]) * np.float32(qt) < np.float32(pc[t])

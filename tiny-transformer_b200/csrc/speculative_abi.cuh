@@ -306,8 +306,14 @@ TT_ATTN_API tt_attn_status tt_attn_tree_verify_f32(
   p.N = static_cast<int>(nodes);
   p.V = static_cast<int>(vocab);
   const int64_t windows = (vocab + vf::WINDOW - 1) / vf::WINDOW;
-  p.cluster = static_cast<int>(std::min<int64_t>(vf::MAX_CLUSTER, (windows + vf::WARPS - 1) / vf::WARPS));
+  // Two CTAs per SM at most, eight windows a CTA at least (4, 8 and 16 measured alike, 32 and 64 up to
+  // 7 us slower on 8192 tokens: a warp then takes its windows one after the other).
+  p.cluster = static_cast<int>(std::max<int64_t>(
+      1, std::min<int64_t>({vf::MAX_CLUSTER, (windows + 7) / 8, 2 * kPlanSms / batch})));
+  p.cluster = std::max(
+      p.cluster, static_cast<int>((windows + vf::MAX_WINDOWS - 1) / vf::MAX_WINDOWS));
   p.windows = static_cast<int>((windows + p.cluster - 1) / p.cluster);
+  const int threads = 32 * std::min(p.windows, vf::MAX_THREADS / 32);
   p.path = path;
   p.counts = counts;
   p.next = next_tokens;
@@ -317,7 +323,7 @@ TT_ATTN_API tt_attn_status tt_attn_tree_verify_f32(
     vec = vec && dp_sb % 4 == 0 && dp_sn % 4 == 0 && aligned16(draft_probs);
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[1];
-  cluster_config(&cfg, attr, batch * p.cluster, vf::THREADS, 0, p.cluster,
+  cluster_config(&cfg, attr, batch * p.cluster, threads, static_cast<size_t>(p.windows) * 8, p.cluster,
                  static_cast<cudaStream_t>(stream));
   cudaError_t le;
   if (draft_probs != nullptr)

@@ -15,9 +15,9 @@
 // holds DUP = 2 or 4 copies of Q, and copy c works on the c-th 128 / DUP keys of every tile only:
 // its other P entries are zero, its running max and sums are its own, and the copies merge at the
 // end of the unit like the CTAs do. So all four softmax warps have work whatever the row count, a
-// thread takes 128 / DUP exponentials a tile, and the tensor work does not change. Of every 8 pairs
-// three take the FMA-pipe exp2 of the prefill kernel; O is rescaled only when a row's max grows by
-// more than 2^8.
+// thread takes 128 / DUP exponentials a tile, and the tensor work does not change. All exponentials
+// are MUFU ones: the FMA-pipe polynomial of the prefill kernel (1e-4) shows in the LSE, and the
+// softmax is not the bound here. O is rescaled only when a row's max grows by more than 2^8.
 //
 // Roles: two softmax warpgroups (warps 0-3 and 4-7, thread = TMEM lane) take the tiles alternately,
 // each with score, P and O columns, a running max and a sum of its own (they merge like the
@@ -208,8 +208,7 @@ struct Walk {
   }
 };
 
-// Maximum that is NaN when an argument is: a row with a NaN score is NaN as a whole (the FMA-pipe
-// exponential would drop one).
+// Maximum that is NaN when an argument is: a row with a NaN score is NaN as a whole.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float d;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -229,20 +228,14 @@ __device__ __forceinline__ float max32(const float (&x)[32]) {
 }
 
 // P = exp2(x * sl2 - m) of 32 scores as bf16x2 to 16 columns at t_p; adds to the FP32 row sums.
-template <int POLY>
 __device__ __forceinline__ void exp_store32(const float (&x)[32], uint64_t sc2, uint64_t nm2,
                                             uint32_t t_p, uint64_t (&acc)[4]) {
   uint32_t pk[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    float t0, t1, p0, p1;
+    float t0, t1;
     f2_unpack(f2_fma(f2_pack(x[2 * i], x[2 * i + 1]), sc2, nm2), t0, t1);
-    if ((i & 7) < POLY) {
-      prefill::exp2_poly2(t0, t1, p0, p1);
-    } else {
-      p0 = ex2_approx(t0);
-      p1 = ex2_approx(t1);
-    }
+    const float p0 = ex2_approx(t0), p1 = ex2_approx(t1);
     acc[i & 3] = f2_add(acc[i & 3], f2_pack(p0, p1));
     pk[i] = pack_bf16x2(p0, p1);
   }
@@ -402,14 +395,13 @@ __device__ __forceinline__ void softmax_role(Smem& s, const Params& p, uint32_t 
           m_run = m_new;
         }
         const float base = m_run == -INFINITY ? 0.f : m_run;
-        constexpr int POLY = DUP == 1 ? prefill::POLY_PAIRS_PER_8 : 0;
         const uint64_t sc2 = f2_pack(sl2, sl2), nm2 = f2_pack(-base, -base);
         uint64_t acc[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
           if (c > 0) load(c);  // chunk 0 is still in x
           if (CHUNKS > 1 && c == CHUNKS - 1) scores_read();
-          exp_store32<POLY>(x, sc2, nm2, t_p + c * 16, acc);
+          exp_store32(x, sc2, nm2, t_p + c * 16, acc);
         }
         acc[0] = f2_add(f2_add(acc[0], acc[1]), f2_add(acc[2], acc[3]));
         float lo, hi;

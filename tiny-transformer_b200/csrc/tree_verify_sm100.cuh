@@ -15,15 +15,17 @@
 //   r_{k+1}(v) = max(r_k(v) - floor(q(v) S_k), 0), S_{k+1} = sum of r_{k+1};
 //   next token: the smallest v whose running sum of r exceeds floor(u_0 * sum of r); r is r_0
 //   again where nothing is left of it.
-// p, q are clamped to [0, 2] (NaN to 0), so that sums of up to 2^22 weights fit 63 bits.
+// p, q are clamped to [0, 1] (NaN to 0), so that sums of up to 2^22 weights fit 63 bits.
 //
-// One thread-block cluster walks one sequence. Every CTA takes the same walk: all accept tests
+// One thread-block cluster walks one sequence, every CTA taking the same walk. All accept tests
 // before a rejection need only p(t) and q(t) of the nodes, gathered once for the whole tree; the
-// rows themselves are read only at a rejection and at the end, each CTA summing its share of the
-// vocabulary in windows of 128 tokens and the cluster adding the shares through distributed
-// shared memory. The rejections at a node are a short list of S_k, so r_k is folded from p and q
-// as they are read (again from L2 after a second rejection) and never stored. The window sums of
-// the last pass locate the next token: one window is read again.
+// rows themselves are read at a rejection and at the end, each CTA summing its share of the
+// vocabulary in windows of 128 tokens, one a warp. A pass is latency, not bandwidth: many warps with
+// four tokens a lane (with 16 a lane the dependent whole-number steps of one warp took 10000 cycles),
+// the next two windows' loads under this one's sums. The rejections at a node are a short list of S_k,
+// so r_k is folded from p and q as they are read and never stored; with chosen children (no q) a
+// rejection changes one weight, so the row is summed once per node. The window sums of the last pass
+// locate the next token: one window is read again.
 #pragma once
 
 #include <cstdint>
@@ -34,9 +36,10 @@ namespace tt {
 namespace verify {
 
 constexpr int MAX_NODES = 256;
-constexpr int THREADS = 256;
-constexpr int WARPS = THREADS / 32;
-constexpr int WINDOW = 128;              // tokens per window: 4 per lane
+constexpr int MAX_THREADS = 512;         // a warp per window, up to 16; two CTAs per SM
+constexpr int LANE_TOKENS = 4;
+constexpr int WINDOW = 128;              // tokens per window: a warp's
+static_assert(WINDOW == 32 * LANE_TOKENS, "a window is what a warp reads at a time");
 constexpr int MAX_CLUSTER = 8;
 constexpr int MAX_WINDOWS = 4096;        // per CTA
 constexpr int64_t MAX_VOCAB = int64_t(1) << 22;  // = MAX_CLUSTER * MAX_WINDOWS * WINDOW
@@ -59,34 +62,83 @@ struct Params {
   int64_t* next;           // [B]
 };
 
+// (The window sums of the last pass are the dynamic shared memory, windows x 8 bytes.)
 struct Smem {
   int32_t parent[MAX_NODES];
   int32_t token[MAX_NODES];     // -1: outside the vocabulary
   float u[MAX_NODES];
   float pt[MAX_NODES], qt[MAX_NODES];  // p and q of the node's token at its parent
   int32_t path[MAX_NODES];
-  double S[MAX_NODES];          // S_k of the rejections at the current node
-  int32_t rejected[MAX_NODES];  // their tokens
-  unsigned long long window[MAX_WINDOWS];
-  unsigned long long part[WARPS];
+  // Rejections at the current node, S_k and token. Every thread writes every entry itself (all the
+  // same), so no barrier is needed to read them; a node's list goes to the other half than the last
+  // one's, which slower threads may still read (each list has a pass and its barrier behind it).
+  unsigned long long S[2][MAX_NODES];
+  long long lost[2][MAX_NODES];  // what r lost at that token (chosen children)
+  int32_t rejected[2][MAX_NODES];
   unsigned long long share[2][MAX_CLUSTER];  // the cluster's sums, by pass parity
 };
 
-__device__ __forceinline__ float clamp_prob(float x) { return fminf(fmaxf(x, 0.f), 2.f); }
+extern __shared__ unsigned long long window_sums[];
 
-// floor(x * S) for 0 <= x <= 2, S a whole number below 2^53.
-__device__ __forceinline__ long long scaled(float x, double S) {
-  return __double2ll_rd(__dmul_rn(static_cast<double>(x), S));
+__device__ __forceinline__ float clamp_prob(float x) { return __saturatef(x); }
+
+// floor(x ONE) for 0 <= x <= 1 as high * 2^16 + low, each a whole number plus MAGIC's bits: 2^23 + y,
+// rounded down, holds floor(y) in its low bits, and what the first sum leaves is exact. Four FP32
+// operations (a conversion to 64 bits runs at 16 a clock and SM; shifting the significand into place
+// took 20 operations a value, and a pass over 16384 tokens 12000 cycles).
+constexpr float MAGIC = 8388608.f;  // 2^23
+struct Fixed {
+  uint32_t high, low;
+};
+__device__ __forceinline__ Fixed fixed_point(float x) {
+  const float h = __fmaf_rd(x, 1048576.f, MAGIC);
+  const float rest = __fmaf_rn(x, 1048576.f, -__fadd_rn(h, -MAGIC));
+  return Fixed{__float_as_uint(h), __float_as_uint(__fmaf_rd(rest, 65536.f, MAGIC))};
+}
+__device__ __forceinline__ long long weight(float x) {
+  const Fixed f = fixed_point(x);
+  const uint32_t magic = __float_as_uint(MAGIC);
+  return (static_cast<long long>(f.high - magic) << 16) + static_cast<long long>(f.low - magic);
 }
 
-// r_K of token v from its p and q, after the K rejections listed in s.
+// floor(fl(x S)) for a whole number S, fl the FP64 rounding.
+__device__ __forceinline__ long long scaled(float x, unsigned long long S) {
+  return __double2ll_rd(__dmul_rn(static_cast<double>(x), static_cast<double>(S)));
+}
+
+// x 2^E for 0 <= x <= 1 by moving x's bits into an FP64 (a zero or subnormal x becomes some number
+// far below 1): conversion instructions run at 16 a clock and SM.
+template <int E>
+__device__ __forceinline__ double to_double(float x) {
+  const uint32_t bits = __float_as_uint(x);
+  return __hiloint2double(static_cast<int>((bits >> 3) + ((896u + E) << 20)),
+                          static_cast<int>(bits << 29));
+}
+
+// max(r_0 - floor(q S_0) - ... - floor(q S_(K-1)), 0), which is r_K (what is taken off is never
+// negative), exact in FP64 below S = 2^51: 2^52 + y, rounded down, is 2^52 + floor(y).
+__device__ __forceinline__ double residual_fp64(float p, float q, int K, const unsigned long long* S) {
+  constexpr double M = 4503599627370496.0;  // 2^52
+  double r = __dadd_rn(__dadd_rd(to_double<36>(p), M), -__dadd_rd(to_double<36>(q), M));
+  const double d = to_double<0>(q);
+  for (int k = 1; k < K; ++k)
+    r = __dadd_rn(r, __dadd_rn(M, -__dadd_rd(__dmul_rn(d, static_cast<double>(S[k])), M)));
+  const int sign = ~(__double2hiint(r) >> 31);  // negative: zero
+  return __hiloint2double(__double2hiint(r) & sign, __double2loint(r) & sign);
+}
+
+// r_K of token v from its p and q, after the K rejections in list `half`.
 template <bool DENSE>
-__device__ __forceinline__ long long residual(const Smem& s, int K, int v, float p, float q) {
-  long long r = scaled(p, ONE);
-  for (int k = 0; k < K; ++k) {
-    const float qk = DENSE ? q : (v == s.rejected[k] ? 1.f : 0.f);
-    const long long left = r - scaled(qk, s.S[k]);
-    r = left > 0 ? left : 0;
+__device__ __forceinline__ long long residual(const Smem& s, int half, int K, int v, float p, float q) {
+  long long r = weight(p);
+  if (K == 0) return r;
+  if (DENSE) {
+    r = max(r - weight(q), 0ll);  // S_0 = ONE
+    for (int k = 1; k < K; ++k) r = max(r - scaled(q, s.S[half][k]), 0ll);
+  } else {
+    for (int k = 0; k < K; ++k)
+      if (v == s.rejected[half][k])
+        r = max(r - static_cast<long long>(s.S[half][k]), 0ll);
   }
   return r;
 }
@@ -101,67 +153,147 @@ __device__ __forceinline__ void st_cluster_u64(uint32_t addr, unsigned long long
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
 
+// p and (after a rejection) q of one lane's 4 tokens of the window at v0, zero past the vocabulary.
+// VEC (rows on 16-byte boundaries, V % 4 == 0): value j is token 4 lane + j of the window, else token
+// 32 j + lane; both keep every load of a warp contiguous.
+template <bool VEC>
+__device__ __forceinline__ int token_of(int lane, int j) {
+  return VEC ? lane * 4 + j : j * 32 + lane;
+}
+template <bool VEC>
+__device__ __forceinline__ void load_lane(const float* row, int v0, int lane, int V,
+                                          float (&x)[LANE_TOKENS]) {
+  if (VEC) {
+    const int v = v0 + lane * 4;
+    const float4 y = v < V ? __ldg(reinterpret_cast<const float4*>(row + v))
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+    x[0] = y.x;
+    x[1] = y.y;
+    x[2] = y.z;
+    x[3] = y.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < LANE_TOKENS; ++j) {
+      const int v = v0 + j * 32 + lane;
+      x[j] = v < V ? __ldg(row + v) : 0.f;
+    }
+  }
+}
+
 // One pass over the rows of node `cur`: this CTA's window sums of r_K, and the sum over all CTAs
 // (whole numbers: the same in every CTA). Every thread of every CTA of the cluster calls it.
 template <bool DENSE, bool VEC>
 __device__ __forceinline__ unsigned long long sum_pass(Smem& s, const Params& a, int b, int cur,
-                                                       int K, int rank, int pass) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+                                                       int half, int K, int rank, int pass) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, par = pass & 1;
   const float* prow = a.p + b * a.p_sb + cur * a.p_sn;
   const float* qrow = DENSE ? a.q + b * a.q_sb + cur * a.q_sn : nullptr;
+  const int step = static_cast<int>(blockDim.x >> 5);
   const bool with_q = DENSE && K > 0;
-  unsigned long long mine = 0;
-  for (int w = warp; w < a.windows; w += WARPS) {
-    const int64_t v0 = (static_cast<int64_t>(rank) * a.windows + w) * WINDOW;
-    long long r = 0;
-    if (VEC) {
-      const int64_t v = v0 + lane * 4;
-      if (v < a.V) {  // V % 4 == 0
-        const float4 x = *reinterpret_cast<const float4*>(prow + v);
-        const float4 y = with_q ? *reinterpret_cast<const float4*>(qrow + v)
-                                : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+  // Products of this size of S keep the FP64 form exact (a row of probabilities has S <= 2^36).
+  const bool fp64_exact = !with_q || K == 1 || s.S[half][1] < (1ull << 51);
+  // Sum of r_K over one lane's tokens of the window at v0.
+  auto lane_sum = [&](const float (&ps)[LANE_TOKENS], const float (&qs)[LANE_TOKENS], int v0) {
+    long long sum = 0;
+    if (with_q && K == 1) {
+      // max(w(p) - w(q), 0) is the difference where p > q (w does not decrease), else zero.
+      int high = 0, low = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          r += residual<DENSE>(s, K, static_cast<int>(v) + i, clamp_prob(xs[i]), clamp_prob(ys[i]));
+      for (int j = 0; j < LANE_TOKENS; ++j) {
+        const float pj = clamp_prob(ps[j]), qj = clamp_prob(qs[j]);
+        const Fixed fp = fixed_point(pj), fq = fixed_point(qj);
+        high += pj > qj ? static_cast<int>(fp.high - fq.high) : 0;
+        low += pj > qj ? static_cast<int>(fp.low - fq.low) : 0;
+      }
+      sum = static_cast<long long>(high) * 65536 + low;
+    } else if (with_q && fp64_exact) {
+      double total = 0.0;
+#pragma unroll
+      for (int j = 0; j < LANE_TOKENS; ++j)
+        total = __dadd_rn(total, residual_fp64(clamp_prob(ps[j]), clamp_prob(qs[j]), K, s.S[half]));
+      sum = __double2ll_rn(total);
+    } else if (with_q) {
+#pragma unroll 1
+      for (int j = 0; j < LANE_TOKENS; ++j) {
+        const float pj = j == 0 ? ps[0] : j == 1 ? ps[1] : j == 2 ? ps[2] : ps[3];
+        const float qj = j == 0 ? qs[0] : j == 1 ? qs[1] : j == 2 ? qs[2] : qs[3];
+        sum += residual<DENSE>(s, half, K, 0, clamp_prob(pj), clamp_prob(qj));
       }
     } else {
-      float xs[4], ys[4];
+      uint32_t high = 0, low = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t v = v0 + i * 32 + lane;
-        xs[i] = v < a.V ? prow[v] : 0.f;
-        ys[i] = with_q && v < a.V ? qrow[v] : 0.f;
+      for (int j = 0; j < LANE_TOKENS; ++j) {
+        const Fixed f = fixed_point(clamp_prob(ps[j]));
+        high += f.high - __float_as_uint(MAGIC);
+        low += f.low - __float_as_uint(MAGIC);
       }
+      sum = (static_cast<long long>(high) << 16) + low;
+      if (!DENSE) {
+        for (int k = 0; k < K; ++k) {
+          // The rejected token's weight, where this lane has it: S_k taken off, down to zero.
+          const int at = s.rejected[half][k] - v0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        r += residual<DENSE>(s, K, static_cast<int>(v0) + i * 32 + lane, clamp_prob(xs[i]),
-                             clamp_prob(ys[i]));
+          for (int j = 0; j < LANE_TOKENS; ++j)
+            if (at == token_of<VEC>(lane, j)) {
+              const float pj = clamp_prob(ps[j]);
+              sum += residual<DENSE>(s, half, k + 1, v0 + at, pj, 0.f) -
+                     residual<DENSE>(s, half, k, v0 + at, pj, 0.f);
+            }
+        }
+      }
     }
-    const unsigned long long sum = warp_sum(static_cast<unsigned long long>(r));
-    if (lane == 0) s.window[w] = sum;
-    mine += sum;
+    return sum;
+  };
+  // Two windows at a time, the next two's loads under their sums.
+  float ps[2][LANE_TOKENS], qs[2][LANE_TOKENS], pn[2][LANE_TOKENS], qn[2][LANE_TOKENS];
+  auto request = [&](int w) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      // A window past this CTA's share is past the row for these loads.
+      const int v0 = w + i * step < a.windows ? (rank * a.windows + w + i * step) * WINDOW : a.V;
+      load_lane<VEC>(prow, v0, lane, a.V, pn[i]);
+      if (with_q) load_lane<VEC>(qrow, v0, lane, a.V, qn[i]);
+    }
+  };
+  request(warp);
+  for (int w = warp; w < a.windows; w += 2 * step) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < LANE_TOKENS; ++j) {
+        ps[i][j] = pn[i][j];
+        qs[i][j] = qn[i][j];
+      }
+    if (w + 2 * step < a.windows) request(w + 2 * step);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = w + i * step;
+      if (at >= a.windows) break;
+      const unsigned long long all = warp_sum(static_cast<unsigned long long>(
+          lane_sum(ps[i], qs[i], (rank * a.windows + at) * WINDOW)));
+      if (lane == 0) window_sums[at] = all;
+    }
   }
-  if (lane == 0) s.part[warp] = mine;
   __syncthreads();
   unsigned long long total = 0;
   if (warp == 0) {
-    total = warp_sum(lane < WARPS ? s.part[lane] : 0ull);
+    for (int w = lane; w < a.windows; w += 32) total += window_sums[w];
+    total = warp_sum(total);
     if (a.cluster == 1) {
-      if (lane == 0) s.share[pass & 1][0] = total;
+      if (lane == 0) s.share[par][0] = total;
     } else if (lane < a.cluster) {
-      st_cluster_u64(map_to_rank(smem_u32(&s.share[pass & 1][rank]), lane), total);
+      st_cluster_u64(map_to_rank(smem_u32(&s.share[par][rank]), lane), total);
     }
   }
   if (a.cluster == 1) __syncthreads();
   else cluster_sync();
   total = 0;
-  for (int c = 0; c < a.cluster; ++c) total += s.share[pass & 1][c];
+  for (int c = 0; c < a.cluster; ++c) total += s.share[par][c];
   return total;
 }
 
 template <bool DENSE, bool VEC>
-__global__ void __launch_bounds__(THREADS) tree_verify_kernel(const Params a) {
+__global__ void __launch_bounds__(MAX_THREADS, 2) tree_verify_kernel(const Params a) {
   __shared__ Smem s;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = static_cast<int>(cluster_ctarank());
@@ -169,7 +301,7 @@ __global__ void __launch_bounds__(THREADS) tree_verify_kernel(const Params a) {
   const int N = a.N;
 
   // The tree, the random numbers, and p(t), q(t) of every node at its parent.
-  for (int n = threadIdx.x; n < N; n += THREADS) {
+  for (int n = threadIdx.x; n < N; n += blockDim.x) {
     const int up = __ldg(a.parents + b * a.parents_sb + n);
     const int64_t t = __ldg(reinterpret_cast<const long long*>(a.tokens) + static_cast<int64_t>(b) * N + n);
     const bool child = up >= 0 && up < n;
@@ -181,6 +313,8 @@ __global__ void __launch_bounds__(THREADS) tree_verify_kernel(const Params a) {
     if (child && known) {
       pt = clamp_prob(__ldg(a.p + b * a.p_sb + up * a.p_sn + t));
       qt = DENSE ? clamp_prob(__ldg(a.q + b * a.q_sb + up * a.q_sn + t)) : 1.f;
+    } else if (!DENSE) {
+      qt = 1.f;
     }
     s.pt[n] = pt;
     s.qt[n] = qt;
@@ -190,7 +324,9 @@ __global__ void __launch_bounds__(THREADS) tree_verify_kernel(const Params a) {
   else cluster_sync();
 
   const bool in_use = s.parent[0] == -1;
-  int cur = 0, count = in_use ? 1 : 0, K = 0, passes = 0;
+  int cur = 0, count = in_use ? 1 : 0, passes = 0;
+  int K = 0, half = 0;       // rejections at this node, and where their list is
+  bool summed = false;       // `total` is the sum of r_K
   unsigned long long total = 0;
   if (threadIdx.x == 0) s.path[0] = 0;
   int at = 0;  // nodes up to here have been tried
@@ -208,11 +344,14 @@ __global__ void __launch_bounds__(THREADS) tree_verify_kernel(const Params a) {
     if (c < 0) break;
     at = c;
     const float pt = s.pt[c], qt = s.qt[c];
+    const int token = s.token[c];
+    long long r = 0;  // r_K of the child's token
     bool take;
     if (K == 0) {
       take = __fmul_rn(s.u[c], qt) < pt;
+      r = weight(pt);
     } else {
-      const long long r = residual<DENSE>(s, K, s.token[c], pt, qt);
+      r = residual<DENSE>(s, half, K, token, pt, qt);
       take = __dmul_rn(__dmul_rn(static_cast<double>(s.u[c]), static_cast<double>(qt)),
                        static_cast<double>(total)) < static_cast<double>(r);
     }
@@ -221,26 +360,34 @@ __global__ void __launch_bounds__(THREADS) tree_verify_kernel(const Params a) {
       if (threadIdx.x == 0) s.path[count] = c;
       ++count;
       K = 0;
+      summed = false;
       continue;
     }
-    __syncthreads();  // every thread has read the list of rejections
-    if (threadIdx.x == 0) {
-      s.S[K] = K == 0 ? ONE : static_cast<double>(total);
-      s.rejected[K] = s.token[c];
-    }
-    __syncthreads();
+    if (K == 0) half ^= 1;
+    const unsigned long long S = K == 0 ? static_cast<unsigned long long>(ONE) : total;
+    s.S[half][K] = S;
+    s.rejected[half][K] = token;
+    __syncwarp();
     ++K;
-    total = sum_pass<DENSE, VEC>(s, a, b, cur, K, rank, passes++);
+    if (DENSE || !summed) {
+      total = sum_pass<DENSE, VEC>(s, a, b, cur, half, K, rank, passes++);
+      summed = true;
+    } else {
+      // One weight has changed, and the sum by as much (the last pass's windows: at the end).
+      const long long lost = r - max(r - static_cast<long long>(S), 0ll);
+      s.lost[half][K - 1] = lost;
+      total -= static_cast<unsigned long long>(lost);
+    }
   }
-  if (in_use && K == 0) total = sum_pass<DENSE, VEC>(s, a, b, cur, 0, rank, passes++);
+  if (in_use && K == 0) total = sum_pass<DENSE, VEC>(s, a, b, cur, half, 0, rank, passes++);
   if (in_use && K > 0 && total == 0) {
     K = 0;
-    total = sum_pass<DENSE, VEC>(s, a, b, cur, 0, rank, passes++);
+    total = sum_pass<DENSE, VEC>(s, a, b, cur, half, 0, rank, passes++);
   }
 
   if (rank == 0) {
     __syncthreads();
-    for (int n = threadIdx.x; n < N; n += THREADS)
+    for (int n = threadIdx.x; n < N; n += blockDim.x)
       a.path[static_cast<int64_t>(b) * N + n] = n < count ? s.path[n] : -1;
     if (threadIdx.x == 0) {
       a.counts[b] = count;
@@ -250,30 +397,50 @@ __global__ void __launch_bounds__(THREADS) tree_verify_kernel(const Params a) {
   if (warp != 0 || total == 0) return;
 
   // The CTA, then the window, then the token in which the running sum passes the goal.
+  const int par = (passes - 1) & 1;
   unsigned long long goal = 0;
   {
     const double x = floor(__dmul_rn(static_cast<double>(s.u[0]), static_cast<double>(total)));
     goal = x > 0.0 ? (x < static_cast<double>(total) ? static_cast<unsigned long long>(x) : total - 1)
                    : 0ull;
   }
+  // Chosen children rejected after the pass at this node: what the sums of their windows lost since.
+  const int later = DENSE ? 0 : K;
+  auto lost_in = [&](int from, int to) {  // windows [from, to) of the row
+    unsigned long long x = 0;
+    for (int k = 1; k < later; ++k) {
+      const int t = s.rejected[half][k];
+      if (t >= from * WINDOW && t < to * WINDOW) x += static_cast<unsigned long long>(s.lost[half][k]);
+    }
+    return x;
+  };
+  __syncwarp();
   unsigned long long before = 0;
-  for (int c = 0; c < rank; ++c) before += s.share[(passes - 1) & 1][c];
-  if (goal < before || goal >= before + s.share[(passes - 1) & 1][rank]) return;
+  for (int c = 0; c < rank; ++c) before += s.share[par][c];
+  before -= lost_in(0, rank * a.windows);
+  const unsigned long long own =
+      s.share[par][rank] - lost_in(rank * a.windows, (rank + 1) * a.windows);
+  if (goal < before || goal >= before + own) return;
   goal -= before;
-  int win = -1;
-  for (int base = 0; base < a.windows; base += 32) {
-    const int w = base + lane;
-    unsigned long long run = w < a.windows ? s.window[w] : 0ull;
+  auto scan = [&](unsigned long long x) {  // running sum over the lanes
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const unsigned long long y = __shfl_up_sync(0xffffffffu, run, off);
-      if (lane >= off) run += y;
+      const unsigned long long y = __shfl_up_sync(0xffffffffu, x, off);
+      if (lane >= off) x += y;
     }
+    return x;
+  };
+  int win = 0;
+  for (int base = 0; base < a.windows; base += 32) {
+    const int w = base + lane;
+    const int at_row = rank * a.windows + w;
+    const unsigned long long x =
+        w < a.windows ? window_sums[w] - lost_in(at_row, at_row + 1) : 0ull;
+    const unsigned long long run = scan(x);
     const unsigned hit = __ballot_sync(0xffffffffu, run > goal);
     if (hit != 0) {
       const int first = __ffs(hit) - 1;
-      const unsigned long long prev = __shfl_sync(0xffffffffu, run, first > 0 ? first - 1 : 0);
-      if (first > 0) goal -= prev;
+      goal -= __shfl_sync(0xffffffffu, run - x, first);
       win = base + first;
       break;
     }
@@ -281,22 +448,40 @@ __global__ void __launch_bounds__(THREADS) tree_verify_kernel(const Params a) {
   }
   const float* prow = a.p + b * a.p_sb + cur * a.p_sn;
   const float* qrow = DENSE ? a.q + b * a.q_sb + cur * a.q_sn : nullptr;
-  const int64_t v0 = (static_cast<int64_t>(rank) * a.windows + win) * WINDOW;
-#pragma unroll 1
-  for (int i = 0; i < 4; ++i) {
-    const int64_t v = v0 + i * 32 + lane;
-    const float x = v < a.V ? clamp_prob(prow[v]) : 0.f;
-    const float y = DENSE && K > 0 && v < a.V ? clamp_prob(qrow[v]) : 0.f;
-    unsigned long long run =
-        static_cast<unsigned long long>(residual<DENSE>(s, K, static_cast<int>(v), x, y));
+  const int v0 = (rank * a.windows + win) * WINDOW;
+  float ps[LANE_TOKENS], qs[LANE_TOKENS];
+  load_lane<VEC>(prow, v0, lane, a.V, ps);
+  if (DENSE && K > 0) {
+    load_lane<VEC>(qrow, v0, lane, a.V, qs);
+  } else {
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const unsigned long long z = __shfl_up_sync(0xffffffffu, run, off);
-      if (lane >= off) run += z;
+    for (int j = 0; j < LANE_TOKENS; ++j) qs[j] = 0.f;
+  }
+  constexpr int GROUP = VEC ? LANE_TOKENS : 1;  // adjacent tokens of a lane
+#pragma unroll
+  for (int i = 0; i < LANE_TOKENS; i += GROUP) {
+    unsigned long long r[GROUP], x = 0;
+#pragma unroll
+    for (int j = 0; j < GROUP; ++j) {
+      r[j] = static_cast<unsigned long long>(
+          residual<DENSE>(s, half, K, v0 + token_of<VEC>(lane, i + j), clamp_prob(ps[i + j]),
+                          clamp_prob(qs[i + j])));
+      x += r[j];
     }
+    const unsigned long long run = scan(x);
     const unsigned hit = __ballot_sync(0xffffffffu, run > goal);
     if (hit != 0) {
-      if (lane == 0) a.next[b] = v0 + i * 32 + __ffs(hit) - 1;
+      if (lane == __ffs(hit) - 1) {
+        unsigned long long left = goal - (run - x);
+        int j = 0;
+#pragma unroll
+        for (int k = 0; k + 1 < GROUP; ++k)
+          if (j == k && left >= r[k]) {
+            left -= r[k];
+            ++j;
+          }
+        a.next[b] = v0 + token_of<VEC>(lane, i + j);
+      }
       return;
     }
     goal -= __shfl_sync(0xffffffffu, run, 31);
