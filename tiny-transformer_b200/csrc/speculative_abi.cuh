@@ -60,13 +60,10 @@ bool tree_shape_ok(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nod
          (capacity / tt::tree::KEYS + 4) * 2 <= INT32_MAX / (batch * q_heads);
 }
 
-tt_attn_status set_tree_attributes() {
-  static std::mutex mu;
-  static bool done[kMaxDevices] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  std::lock_guard<std::mutex> lock(mu);
-  if (e == cudaSuccess && !done[dev]) {
+tt_attn_status set_tree_attributes(int dev) {
+  static std::atomic<bool> done[kMaxDevices] = {};
+  cudaError_t e = cudaSuccess;
+  if (!done[dev].load(std::memory_order_acquire)) {
     e = cudaFuncSetAttribute(tt::tree::tree_attention_kernel<1>,
                              cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(tt::tree::smem_bytes<1>()));
@@ -80,7 +77,7 @@ tt_attn_status set_tree_attributes() {
       if (e == cudaSuccess)
         e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  static_cast<int>(tt::tree::persist::kSmemBytes));
-    if (e == cudaSuccess) done[dev] = true;
+    if (e == cudaSuccess) done[dev].store(true, std::memory_order_release);
   }
   if (e != cudaSuccess)
     return fail(TT_ATTN_LAUNCH_FAIL, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
@@ -214,7 +211,7 @@ TT_ATTN_API tt_attn_status tt_attn_tree_forward_bf16(
   int dev = 0, sm_count = 0;
   tt_attn_status st = prepare_device(&dev, &sm_count);
   if (st != TT_ATTN_OK) return st;
-  if ((st = set_tree_attributes()) != TT_ATTN_OK) return st;
+  if ((st = set_tree_attributes(dev)) != TT_ATTN_OK) return st;
   CUtensorMap tmk, tmv, tmtk, tmtv;
   std::string err;
   if (!encode_map(&tmk, cache_k, cks, &err, tr::KEYS) ||

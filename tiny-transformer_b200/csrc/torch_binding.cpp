@@ -7,6 +7,7 @@
 // through tt_attn_forward_bf16 on the current stream.
 #include <torch/extension.h>
 
+#include <ATen/autocast_mode.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -488,73 +489,90 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> tree_verify(
   return {path, counts, next};
 }
 
+// One list of the commit's per-layer tensors (caches or trees): all checks of a tensor in one pass,
+// since there are four tensors a layer on every step.
+struct LayerTensors {
+  std::vector<torch::Tensor> t;
+  bool in_place = true;  // equal strides, and every tensor can be read (and written) where it is
+};
+
+LayerTensors layer_tensors(const pybind11::list& list, c10::Device* device) {
+  LayerTensors out;
+  out.t.reserve(list.size());
+  const bool grad = at::GradMode::is_enabled();
+  for (const pybind11::handle item : list) {
+    TORCH_CHECK(THPVariable_Check(item.ptr()), "commit_path: caches and trees must be tensors");
+    const torch::Tensor& x = THPVariable_Unpack(item.ptr());
+    TORCH_CHECK(x.is_cuda(), "commit_path: all inputs must be CUDA tensors");
+    if (out.t.empty() && device->is_cpu()) *device = x.device();
+    TORCH_CHECK(x.device() == *device, "commit_path: all inputs must be on the same device");
+    TORCH_CHECK(x.scalar_type() == at::kBFloat16 && x.layout() == at::kStrided && x.dim() == 4,
+                "commit_path: caches and trees must be strided 4D bf16 tensors");
+    TORCH_CHECK(x.size(3) == TT_ATTN_HEAD_DIM, "commit_path currently supports only head_dim=64");
+    TORCH_CHECK_NOT_IMPLEMENTED(
+        !(grad && x.requires_grad()),
+        "commit_path writes the caches in place and has no backward; call it under no_grad");
+    out.t.push_back(x);
+    const torch::Tensor& first = out.t.front();
+    TORCH_CHECK(x.sizes() == first.sizes(),
+                "commit_path: all caches, and all trees, must have the same shape");
+    bool same = readable_in_place(x);
+    for (int64_t d = 0; d < 4; ++d) same = same && (x.size(d) == 1 || x.stride(d) == first.stride(d));
+    out.in_place = out.in_place && same;
+  }
+  return out;
+}
+
 // Append of the accepted path to the caches of all layers (tt_attn_tree_commit_bf16).
-torch::Tensor tree_commit(std::vector<torch::Tensor> cache_k, std::vector<torch::Tensor> cache_v,
-                          std::vector<torch::Tensor> tree_k, std::vector<torch::Tensor> tree_v,
+torch::Tensor tree_commit(const pybind11::list& cache_k, const pybind11::list& cache_v,
+                          const pybind11::list& tree_k, const pybind11::list& tree_v,
                           torch::Tensor path, torch::Tensor counts, torch::Tensor cache_lens) {
   const size_t L = cache_k.size();
   TORCH_CHECK(L > 0 && cache_v.size() == L && tree_k.size() == L && tree_v.size() == L,
               "commit_path: the caches and the trees must have the same, positive number of layers");
-  for (auto* list : {&cache_k, &cache_v, &tree_k, &tree_v})
-    for (const torch::Tensor& t : *list) {
-      TORCH_CHECK(t.defined() && t.is_cuda(), "commit_path: all inputs must be CUDA tensors");
-      TORCH_CHECK(t.device() == cache_k[0].device(),
-                  "commit_path: all inputs must be on the same device");
-      TORCH_CHECK(t.scalar_type() == at::kBFloat16 && t.layout() == at::kStrided && t.dim() == 4,
-                  "commit_path: caches and trees must be strided 4D bf16 tensors");
-      TORCH_CHECK(t.size(3) == TT_ATTN_HEAD_DIM, "commit_path currently supports only head_dim=64");
-      TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()),
-                  "commit_path writes the caches in place and has no backward; call it under no_grad");
-    }
-  const int64_t B = cache_k[0].size(0), H = cache_k[0].size(1), C = cache_k[0].size(2),
-                N = tree_k[0].size(2);
+  TORCH_CHECK(!at::autocast::is_autocast_enabled(at::kCUDA),
+              "commit_path does not support AMP/autocast yet");
+  c10::Device device(at::kCPU);
+  LayerTensors c[2] = {layer_tensors(cache_k, &device), layer_tensors(cache_v, &device)};
+  LayerTensors t[2] = {layer_tensors(tree_k, &device), layer_tensors(tree_v, &device)};
+  const torch::Tensor& first = c[0].t[0];
+  const int64_t B = first.size(0), H = first.size(1), C = first.size(2), N = t[0].t[0].size(2);
   TORCH_CHECK(B > 0 && H > 0 && C > 0 && N > 0, "commit_path: sizes must be positive");
-  auto strides_differ = [](const std::vector<torch::Tensor>& list) {
-    for (const torch::Tensor& t : list) {
-      if (!readable_in_place(t)) return true;
-      for (int64_t d = 0; d < 4; ++d)
-        if (t.size(d) > 1 && t.stride(d) != list[0].stride(d)) return true;
-    }
-    return false;
-  };
-  for (auto* list : {&cache_k, &cache_v}) {
-    for (const torch::Tensor& t : *list)
-      TORCH_CHECK(t.sizes() == cache_k[0].sizes(),
-                  "commit_path: all caches must have the same shape");
-    TORCH_CHECK(!strides_differ(*list),
+  TORCH_CHECK(c[1].t[0].sizes() == first.sizes(),
+              "commit_path: all caches must have the same shape");
+  for (int i = 0; i < 2; ++i) {
+    TORCH_CHECK(c[i].in_place,
                 "commit_path: the caches need equal strides, a unit last stride, other strides in "
                 "multiples of 8 elements and 16-byte aligned bases (they are written in place)");
+    const torch::Tensor& x = t[i].t[0];
+    TORCH_CHECK(x.size(0) == B && x.size(1) == H && x.size(2) == N,
+                "commit_path: the trees must have shape [B, kv_heads, N, 64]");
   }
-  for (auto* list : {&tree_k, &tree_v})
-    for (const torch::Tensor& t : *list)
-      TORCH_CHECK(t.size(0) == B && t.size(1) == H && t.size(2) == N,
-                  "commit_path: the trees must have shape [B, kv_heads, N, 64]");
   TORCH_CHECK(path.defined() && path.dim() == 2 && path.size(0) == B && path.size(1) > 0,
               "commit_path: path must have shape [B, P]");
   TORCH_CHECK(counts.defined() && counts.dim() == 1 && counts.size(0) == B && cache_lens.defined() &&
                   cache_lens.dim() == 1 && cache_lens.size(0) == B,
               "commit_path: counts and cache_lens must have shape [B]");
-  const c10::cuda::CUDAGuard device_guard(cache_k[0].device());
-  check_sm100(cache_k[0]);
-  path = index32(path, cache_k[0], "path");
-  counts = index32(counts, cache_k[0], "counts");
-  cache_lens = index32(cache_lens, cache_k[0], "cache_lens");
-  for (auto* list : {&tree_k, &tree_v})
-    if (strides_differ(*list))
-      for (torch::Tensor& t : *list) t = t.clone(at::MemoryFormat::Contiguous);
+  const c10::cuda::CUDAGuard device_guard(device);
+  check_sm100(first);
+  path = index32(path, first, "path");
+  counts = index32(counts, first, "counts");
+  cache_lens = index32(cache_lens, first, "cache_lens");
+  for (LayerTensors& x : t)
+    if (!x.in_place)
+      for (torch::Tensor& y : x.t) y = y.clone(at::MemoryFormat::Contiguous);
   auto new_lens = torch::empty({B}, cache_lens.options());
-  std::vector<void*> ck(L), cv(L);
-  std::vector<const void*> tk(L), tv(L);
+  std::vector<void*> ptr(4 * L);
   for (size_t l = 0; l < L; ++l) {
-    ck[l] = cache_k[l].data_ptr();
-    cv[l] = cache_v[l].data_ptr();
-    tk[l] = tree_k[l].data_ptr();
-    tv[l] = tree_v[l].data_ptr();
+    ptr[l] = c[0].t[l].data_ptr();
+    ptr[L + l] = c[1].t[l].data_ptr();
+    ptr[2 * L + l] = t[0].t[l].data_ptr();
+    ptr[3 * L + l] = t[1].t[l].data_ptr();
   }
-  const Strides cks(cache_k[0]), cvs(cache_v[0]), tks(tree_k[0]), tvs(tree_v[0]);
-  auto stream = c10::cuda::getCurrentCUDAStream(cache_k[0].get_device());
+  const Strides cks(first), cvs(c[1].t[0]), tks(t[0].t[0]), tvs(t[1].t[0]);
+  auto stream = c10::cuda::getCurrentCUDAStream(device.index());
   const tt_attn_status st = tt_attn_tree_commit_bf16(
-      ck.data(), cks.s, cv.data(), cvs.s, tk.data(), tks.s, tv.data(), tvs.s,
+      ptr.data(), cks.s, ptr.data() + L, cvs.s, ptr.data() + 2 * L, tks.s, ptr.data() + 3 * L, tvs.s,
       static_cast<int64_t>(L), B, H, N, C, TT_ATTN_HEAD_DIM, path.data_ptr<int32_t>(), path.size(1),
       counts.data_ptr<int32_t>(), cache_lens.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(),
       static_cast<void*>(stream.stream()));

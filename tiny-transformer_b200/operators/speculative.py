@@ -21,12 +21,14 @@ from ._extension import load_attention_extension
 
 
 def _guard(name, tensors):
-    if not all(x.is_cuda for x in tensors):
-        raise RuntimeError(f"{name} requires CUDA tensors")
+    grad = torch.is_grad_enabled()
+    for x in tensors:
+        if not x.is_cuda:
+            raise RuntimeError(f"{name} requires CUDA tensors")
+        if grad and x.requires_grad:
+            raise NotImplementedError(f"{name} has no backward; call it under torch.no_grad()")
     if torch.is_autocast_enabled("cuda"):
         raise RuntimeError(f"{name} does not support AMP/autocast yet")
-    if torch.is_grad_enabled() and any(x.requires_grad for x in tensors):
-        raise NotImplementedError(f"{name} has no backward; call it under torch.no_grad()")
 
 
 def tree_attention(q, tree_k, tree_v, cache_k, cache_v, parents, cache_lens=None):
@@ -91,7 +93,7 @@ def commit_path(cache_k, cache_v, tree_k, tree_v, path, counts, cache_lens):
     Returns the new lengths, int32 ``[B]``. Rows past the capacity and path entries outside the
     tree are skipped and set the range bit of the device status (``tt_attn_device_status``).
     """
-    lists = [list(x) if isinstance(x, (list, tuple)) else [x]
+    lists = [x if isinstance(x, list) else list(x) if isinstance(x, tuple) else [x]
              for x in (cache_k, cache_v, tree_k, tree_v)]
-    _guard("commit_path", [t for x in lists for t in x])
+    # Four tensors a layer: device, gradient and shape are checked natively, in one pass.
     return load_attention_extension().tree_commit(*lists, path, counts, cache_lens)
