@@ -11,7 +11,6 @@ struct TreePlan {
   bool persistent = false;
   int64_t rows = 0;       // query rows of a CTA's tile
   int64_t row_tiles = 1;  // tiles of one (batch, K/V head)
-  int rt = 1;             // cluster kernel: 16-row tiles per CTA
   int splits = 1;         // cluster kernel: CTAs per cluster
   int dup = 1;            // persistent kernel: copies of the rows in a 128-row tile
   int64_t grid = 0;       // persistent kernel: CTAs
@@ -27,7 +26,7 @@ TreePlan tree_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nod
   // rows (B = 32, H = 12, 1024-4096 cached) and 31 against 77 us for 111 rows of 4 shared heads
   // (9000-20001 cached); with 16 rows or fewer the cluster kernel's lighter start and end win
   // (151 against 165 us for 16 rows at 1024-8192 cached, 14 against 16 at 256-512).
-  pl.persistent = rows > 16;
+  pl.persistent = rows > tt::tree::ROWS;
   if (pl.persistent) {
     constexpr int64_t bm = tt::tree::persist::BM;
     pl.row_tiles = (rows + bm - 1) / bm;
@@ -36,12 +35,10 @@ TreePlan tree_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nod
     pl.grid = std::min<int64_t>(kPlanSms, batch * kv_heads * pl.row_tiles * tiles);
     return pl;
   }
-  pl.rt = rows <= 16 ? 1 : 2;
-  pl.rows = pl.rt * 16;
-  pl.row_tiles = (rows + pl.rows - 1) / pl.rows;
-  const int64_t units = batch * kv_heads * pl.row_tiles;
+  // Three CTAs fit an SM; a cluster shares a sequence's tiles.
+  const int64_t units = batch * kv_heads;
   pl.splits = static_cast<int>(std::max<int64_t>(
-      1, std::min<int64_t>({tt::tree::MAX_SPLITS, tiles, 3 * kPlanSms / units})));
+      1, std::min<int64_t>({tt::tree::MAX_SPLITS, tiles - tree_tiles, 3 * kPlanSms / units})));
   return pl;
 }
 
@@ -64,13 +61,9 @@ tt_attn_status set_tree_attributes(int dev) {
   static std::atomic<bool> done[kMaxDevices] = {};
   cudaError_t e = cudaSuccess;
   if (!done[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(tt::tree::tree_attention_kernel<1>,
+    e = cudaFuncSetAttribute(tt::tree::tree_attention_kernel,
                              cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(tt::tree::smem_bytes<1>()));
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(tt::tree::tree_attention_kernel<2>,
-                               cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               static_cast<int>(tt::tree::smem_bytes<2>()));
+                             static_cast<int>(tt::tree::kSmemBytes));
     for (auto fn : {tt::tree::persist::tree_persistent_kernel<1>,
                     tt::tree::persist::tree_persistent_kernel<2>,
                     tt::tree::persist::tree_persistent_kernel<4>})
@@ -100,17 +93,13 @@ void cluster_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, int64_t 
 }
 
 tt_attn_status launch_tree_persistent(const TreePlan& pl, const tt::tree::Params& tp,
-                                      const void* tree_v, const Shape4& tvs, void* workspace,
+                                      void* workspace,
                                       int sm_count, const CUtensorMap& tmk, const CUtensorMap& tmv,
                                       const CUtensorMap& tmtk, const CUtensorMap& tmtv,
                                       cudaStream_t stream) {
   namespace ps = tt::tree::persist;
   ps::Params p{};
   p.t = tp;
-  p.tree_v = static_cast<const __nv_bfloat16*>(tree_v);
-  p.tv_sb = tvs.stride[0];
-  p.tv_sh = tvs.stride[1];
-  p.tv_sn = tvs.stride[2];
   p.rows = static_cast<int>(pl.rows);
   p.units = static_cast<int>(tp.Hkv * pl.row_tiles);
   p.tree_tiles = (tp.N + tt::tree::KEYS - 1) / tt::tree::KEYS;
@@ -212,20 +201,28 @@ TT_ATTN_API tt_attn_status tt_attn_tree_forward_bf16(
   tt_attn_status st = prepare_device(&dev, &sm_count);
   if (st != TT_ATTN_OK) return st;
   if ((st = set_tree_attributes(dev)) != TT_ATTN_OK) return st;
+  const int64_t group = q_heads / kv_heads;
+  const TreePlan pl = tree_plan(batch, q_heads, kv_heads, nodes, capacity);
   CUtensorMap tmk, tmv, tmtk, tmtv;
   std::string err;
   if (!encode_map(&tmk, cache_k, cks, &err, tr::KEYS) ||
       !encode_map(&tmv, cache_v, cvs, &err, tr::KEYS) ||
-      !encode_map(&tmtk, tree_k, tks, &err, tr::KEYS) ||
-      !encode_map(&tmtv, tree_v, tvs, &err, tr::KEYS))
+      (pl.persistent && (!encode_map(&tmtk, tree_k, tks, &err, tr::KEYS) ||
+                         !encode_map(&tmtv, tree_v, tvs, &err, tr::KEYS))))
     return fail(TT_ATTN_UNSUPPORTED, err);
-  const int64_t group = q_heads / kv_heads;
-  const TreePlan pl = tree_plan(batch, q_heads, kv_heads, nodes, capacity);
   tr::Params p{};
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.q_sb = qs.stride[0];
   p.q_sh = qs.stride[1];
   p.q_sn = qs.stride[2];
+  p.tk = static_cast<const __nv_bfloat16*>(tree_k);
+  p.tk_sb = tks.stride[0];
+  p.tk_sh = tks.stride[1];
+  p.tk_sn = tks.stride[2];
+  p.tv = static_cast<const __nv_bfloat16*>(tree_v);
+  p.tv_sb = tvs.stride[0];
+  p.tv_sh = tvs.stride[1];
+  p.tv_sn = tvs.stride[2];
   p.parents = parents;
   p.parents_sb = parents_stride;
   p.lens = cache_lens;
@@ -242,14 +239,11 @@ TT_ATTN_API tt_attn_status tt_attn_tree_forward_bf16(
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[1];
   if (pl.persistent)
-    return launch_tree_persistent(pl, p, tree_v, tvs, workspace, sm_count, tmk, tmv, tmtk, tmtv,
+    return launch_tree_persistent(pl, p, workspace, sm_count, tmk, tmv, tmtk, tmtv,
                                   static_cast<cudaStream_t>(stream));
-  cluster_config(&cfg, attr, batch * kv_heads * pl.row_tiles * pl.splits, tr::THREADS,
-                 pl.rt == 1 ? tr::smem_bytes<1>() : tr::smem_bytes<2>(), pl.splits,
+  cluster_config(&cfg, attr, batch * kv_heads * pl.splits, tr::THREADS, tr::kSmemBytes, pl.splits,
                  static_cast<cudaStream_t>(stream));
-  const cudaError_t le =
-      pl.rt == 1 ? cudaLaunchKernelEx(&cfg, tr::tree_attention_kernel<1>, tmk, tmv, tmtk, tmtv, p)
-                 : cudaLaunchKernelEx(&cfg, tr::tree_attention_kernel<2>, tmk, tmv, tmtk, tmtv, p);
+  const cudaError_t le = cudaLaunchKernelEx(&cfg, tr::tree_attention_kernel, tmk, tmv, p);
   if (le != cudaSuccess)
     return fail(TT_ATTN_LAUNCH_FAIL,
                 std::string("tree_attention_kernel launch: ") + cudaGetErrorString(le));

@@ -13,16 +13,18 @@
 // (batch, K/V head), so the cache is read once for all of them. The operator does 2 * G * N
 // products per cached element and is bound by reading the cache for the trees it is made for.
 //
-// tree_attention_kernel<RT>: RT 16-row tiles (16 or 32 query rows) against tiles of 128 keys.
-// One thread-block cluster takes one (batch, K/V head, row tile); its CTAs share the sequence's
-// actual tiles evenly (tree tiles first, so rank 0 holds the mask), whatever the length. A
-// producer warp keeps a ring of 128-key K and V tiles in flight with TMA (128-byte swizzle: 16-
-// byte piece c of row r at piece c ^ (r % 8)); 4 consumer warps take 32 keys of a tile each, so
-// that K and V fragments are read from shared memory once for all rows. Scores and P.V are
-// mma.m16n8k16 on register fragments (Q stays in registers, P goes from the score fragments to
-// the second product's A operand without leaving them); every warp keeps its own online softmax
-// (m, l, O) and the CTA merges its warps at the end, the cluster its CTAs through distributed
-// shared memory, each rank merging its share of the rows.
+// tree_attention_kernel: up to 16 stacked query rows (so at most 16 nodes). One thread-block cluster
+// takes one (batch, K/V head); its CTAs share the sequence's actual 128-key cache tiles evenly,
+// whatever the length. A producer warp keeps a two-stage ring of K and V tiles in flight with TMA
+// (128-byte swizzle: 16-byte piece c of row r at piece c ^ (r % 8)); 4 consumer warps take 32 keys
+// of a tile each, so that K and V fragments are read from shared memory once. Scores and P.V are
+// mma.m16n8k16 on register fragments (Q stays in registers, P goes from the score fragments to the
+// second product's A operand without leaving them). The tree's 16 keys are one step of rank 0's
+// first warp, loaded with plain loads under the first tiles' flight. Every warp keeps its own online
+// softmax (m, l, O); the CTA merges its warps, every CTA pushes each row to the rank that owns it
+// (st.shared::cluster), and after one cluster barrier each rank merges and writes its rows. 70 KiB
+// of shared memory and 128 registers leave room for three CTAs per SM (192 KiB of loads in flight).
+// More rows take tree_persistent_sm100.cuh: 32 rows in registers left one CTA per SM.
 #pragma once
 
 #include <cuda.h>
@@ -50,33 +52,34 @@ constexpr float LN2 = 0.69314718055994530942f;
 struct Params {
   const __nv_bfloat16* q;
   int64_t q_sb, q_sh, q_sn;   // element strides of q [B, G * Hkv, N, 64]
+  const __nv_bfloat16* tk;    // the tree's K and V [B, Hkv, N, 64]
+  const __nv_bfloat16* tv;
+  int64_t tk_sb, tk_sh, tk_sn, tv_sb, tv_sh, tv_sn;
   const int32_t* parents;     // [N] (stride 0) or [B, N]
   int64_t parents_sb;
   const int32_t* lens;        // optional [B]
   int B, Hkv, G, N, C;
-  int row_tiles;              // row tiles of one (batch, K/V head)
-  int splits;                 // CTAs per cluster
+  int row_tiles;              // persistent kernel: row tiles of one (batch, K/V head)
+  int splits;                 // cluster kernel: CTAs per cluster
   __nv_bfloat16* o;           // contiguous [B, G * Hkv, N, 64]
   float* lse;                 // optional [B, G * Hkv, N]
   float scale_log2;
 };
 
-template <int RT>
+constexpr int ROWS = 16;                              // query rows of a unit, nodes of a tree
+constexpr int PUSH_ROWS = 24;                         // splits * ceil(ROWS / splits) at most
+
 struct alignas(1024) Smem {
-  static constexpr int ROWS = RT * 16;
   union {
-    uint8_t ring[STAGES][2][TILE_BYTES];             // K and V tiles
-    float rec[CONSUMER_WARPS][ROWS][REC];            // after the last tile: the warps' results
+    uint8_t ring[STAGES][2][TILE_BYTES];              // K and V tiles
+    float rec[CONSUMER_WARPS][ROWS][REC];             // after the last tile: the warps' results
   };
-  float crec[ROWS][REC];                             // the CTA's result, read by the cluster
-  uint32_t mask[MAX_NODES][MASK_WORDS];              // bit m of row n: node n sees node m
-  int32_t jump[MAX_NODES];
+  float push[PUSH_ROWS][REC];                         // this rank's rows from every CTA
+  uint8_t tree[2][ROWS * ROW_BYTES];                  // rank 0: the tree's K and V rows
   uint64_t full[STAGES], empty[STAGES];
-  int used[ROWS];                                    // rank 0: rows whose node is in use
   volatile int abort;
 };
-template <int RT>
-constexpr size_t smem_bytes() { return sizeof(Smem<RT>); }
+constexpr size_t kSmemBytes = sizeof(Smem);
 
 // Bounded wait that gives up as soon as another warp of the CTA has given up.
 __device__ __forceinline__ bool wait_or_abort(volatile int* abort, uint64_t* bar, uint32_t parity) {
@@ -114,23 +117,6 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
-  int v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-
 __device__ __forceinline__ int valid_len(const int32_t* lens, int C, int b) {
   if (lens == nullptr) return C;
   return min(max(__ldg(lens + b), 0), C);
@@ -204,172 +190,118 @@ __device__ __forceinline__ bool barrier_or(bool any) {
   return r != 0;
 }
 
-// One warp's state: Q fragments of RT row tiles, and the online softmax of its keys.
-template <int RT>
+// One warp's state: Q fragments, and the online softmax of its keys.
 struct WarpState {
-  uint32_t qf[RT][4][4];   // A fragments of Q: 4 k-steps of 16 features
-  float o[RT][8][4];       // O: 8 n-tiles of 8 features
-  float m[RT][2], l[RT][2];
+  uint32_t qf[4][4];   // A fragments of Q: 4 k-steps of 16 features
+  float o[8][4];       // O: 8 n-tiles of 8 features
+  float m[2], l[2];    // rows lane / 4 and lane / 4 + 8
 };
 
-template <int RT>
-__device__ __forceinline__ void reset(WarpState<RT>& st) {
+__device__ __forceinline__ void load_q(WarpState& st, const Params& p, int b, int h, int lane) {
 #pragma unroll
-  for (int t = 0; t < RT; ++t) {
+  for (int half = 0; half < 2; ++half) {
+    const int r = half * 8 + (lane >> 2);
+    const bool in = r < p.G * p.N;
+    const int g = in ? r / p.N : 0, n = in ? r - g * p.N : 0;
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(
+        p.q + b * p.q_sb + static_cast<int64_t>(h * p.G + g) * p.q_sh + n * p.q_sn) + (lane & 3);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) st.o[t][j][e] = 0.f;
-    st.m[t][0] = st.m[t][1] = -INFINITY;
-    st.l[t][0] = st.l[t][1] = 0.f;
-  }
-}
-
-template <int RT>
-__device__ __forceinline__ void load_q(WarpState<RT>& st, const Params& p, int b, int h, int row0,
-                                       int lane) {
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int r = row0 + t * 16 + half * 8 + (lane >> 2);
-      const bool in = r < p.G * p.N;
-      const int g = in ? r / p.N : 0, n = in ? r - g * p.N : 0;
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(
-          p.q + b * p.q_sb + static_cast<int64_t>(h * p.G + g) * p.q_sh + n * p.q_sn) + (lane & 3);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        st.qf[t][k][half] = in ? __ldg(src + k * 8) : 0u;
-        st.qf[t][k][half + 2] = in ? __ldg(src + k * 8 + 4) : 0u;
-      }
+    for (int k = 0; k < 4; ++k) {
+      st.qf[k][half] = in ? __ldg(src + k * 8) : 0u;
+      st.qf[k][half + 2] = in ? __ldg(src + k * 8 + 4) : 0u;
     }
   }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) st.o[j][e] = 0.f;
+  st.m[0] = st.m[1] = -INFINITY;
+  st.l[0] = st.l[1] = 0.f;
 }
 
-// One warp's 32 keys of a tile: ks / vs are the shared addresses of its K and V rows (the first
-// a multiple of 32 rows, so row % 8 is the swizzle phase), n_valid the rows that exist. TREE: the
-// keys are tree nodes key0 .. key0 + 31 under the mask; otherwise every row sees every valid key.
-template <int RT, bool TREE>
-__device__ __forceinline__ void tile_step(WarpState<RT>& st, const Params& p, uint32_t ks,
-                                          uint32_t vs, int n_valid, int lane,
-                                          const uint32_t (*mask)[MASK_WORDS], int key0, int row0) {
-  // V rows that no row may read: zeroed, so that 0 * (whatever they hold) stays 0.
-  uint32_t bad = 0;  // TREE: keys in use whose V row holds an infinity or a NaN
-  if (TREE || n_valid < 32) {
-    bool clear = lane >= n_valid;
-    if (TREE) clear = clear || !node_used(mask, key0 + lane);
-    const uint32_t row = vs + lane * ROW_BYTES;
-    if (clear) {
+// One warp's KEYS_ keys (32 of a cache tile, or the tree's 16): ks / vs are the shared addresses of
+// its K and V rows (the first a multiple of 8 rows, so row % 8 is the swizzle phase). see[half]: the
+// keys that row lane / 4 + 8 half sees. bad: keys whose V row holds infinities or NaN (tree only);
+// their products are added under the mask, and the rows must not reach the matrix product.
+template <int KEYS_>
+__device__ __forceinline__ void tile_step(WarpState& st, float scale_log2, uint32_t ks, uint32_t vs,
+                                          bool masked, const uint32_t (&see)[2], uint32_t bad,
+                                          int lane) {
+  constexpr int NT = KEYS_ / 8;
+  // S = Q K^T: n-tiles of 8 keys. One ldmatrix.x4 holds 8 keys x 32 features (two k-steps).
+  float s[NT][4];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) sts_u4(row + c * 16, 0, 0, 0, 0);
-    } else if (TREE) {
-      bool nf = false;
+  for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const uint4 u = lds_u4(row + c * 16);
-        nf = nf || has_nonfinite(u.x) || has_nonfinite(u.y) || has_nonfinite(u.z) ||
-             has_nonfinite(u.w);
-      }
-      bad = nf ? 1u : 0u;
-    }
-    if (TREE) bad = __ballot_sync(0xffffffffu, bad != 0);
-    __syncwarp();
-  }
-  // S = Q K^T: 4 n-tiles of 8 keys. One ldmatrix.x4 holds 8 keys x 32 features (two k-steps).
-  float s[RT][4][4];
-#pragma unroll
-  for (int t = 0; t < RT; ++t)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[t][j][e] = 0.f;
+    for (int e = 0; e < 4; ++e) s[j][e] = 0.f;
   const uint32_t kr = ks + (lane & 7) * ROW_BYTES;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < NT; ++j) {
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
       uint32_t bfr[4];
       ldmatrix_x4(kr + j * 8 * ROW_BYTES + (((kk * 4 + (lane >> 3)) ^ (lane & 7)) << 4), bfr);
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        mma_16816(s[t][j], st.qf[t][kk * 2], bfr[0], bfr[1]);
-        mma_16816(s[t][j], st.qf[t][kk * 2 + 1], bfr[2], bfr[3]);
-      }
+      mma_16816(s[j], st.qf[kk * 2], bfr[0], bfr[1]);
+      mma_16816(s[j], st.qf[kk * 2 + 1], bfr[2], bfr[3]);
     }
   }
-  // Mask, running max and exponentials. Thread: rows lane / 4 and lane / 4 + 8 of each row tile,
-  // keys 8 j + 2 (lane % 4) + {0, 1}.
-  uint32_t pf[RT][4][2];
+  // Mask, running max and exponentials. Thread: rows lane / 4 and lane / 4 + 8, keys
+  // 8 j + 2 (lane % 4) + {0, 1}.
+  uint32_t pf[NT][2];
 #pragma unroll
-  for (int t = 0; t < RT; ++t) {
+  for (int half = 0; half < 2; ++half) {
+    if (masked) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if (TREE) {
-        const int r = row0 + t * 16 + half * 8 + (lane >> 2);
-        const uint32_t bits = r < p.G * p.N ? mask[r % p.N][key0 >> 5] : 0u;
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int e = 0; e < 2; ++e)
+          if (!((see[half] >> (j * 8 + (lane & 3) * 2 + e)) & 1u)) s[j][half * 2 + e] = -INFINITY;
+    }
+    float mx = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (!((bits >> (j * 8 + (lane & 3) * 2 + e)) & 1u)) s[t][j][half * 2 + e] = -INFINITY;
-      } else if (n_valid < 32) {
+    for (int j = 0; j < NT; ++j) mx = fmaxf(mx, fmaxf(s[j][half * 2], s[j][half * 2 + 1]));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    const float m_new = fmaxf(st.m[half], mx * scale_log2);
+    const float base = m_new == -INFINITY ? 0.f : m_new;  // nothing visible yet: exp2(-inf) = 0
+    const float f = ex2_approx(st.m[half] - base);
+    st.m[half] = m_new;
+    float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < NT; ++j) {
+      const float p0 = ex2_approx(fmaf(s[j][half * 2], scale_log2, -base));
+      const float p1 = ex2_approx(fmaf(s[j][half * 2 + 1], scale_log2, -base));
+      sum += p0 + p1;
+      pf[j][half] = pack_bf16x2(p0, p1);
+    }
+    st.l[half] = st.l[half] * f + sum;
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (j * 8 + (lane & 3) * 2 + e >= n_valid) s[t][j][half * 2 + e] = -INFINITY;
-      }
-      float mx = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) mx = fmaxf(mx, fmaxf(s[t][j][half * 2], s[t][j][half * 2 + 1]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float m_new = fmaxf(st.m[t][half], mx * p.scale_log2);
-      const float base = m_new == -INFINITY ? 0.f : m_new;  // nothing visible yet: exp2(-inf) = 0
-      const float f = ex2_approx(st.m[t][half] - base);
-      st.m[t][half] = m_new;
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float p0 = ex2_approx(fmaf(s[t][j][half * 2], p.scale_log2, -base));
-        const float p1 = ex2_approx(fmaf(s[t][j][half * 2 + 1], p.scale_log2, -base));
-        sum += p0 + p1;
-        pf[t][j][half] = pack_bf16x2(p0, p1);
-      }
-      st.l[t][half] = st.l[t][half] * f + sum;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        st.o[t][j][half * 2] *= f;
-        st.o[t][j][half * 2 + 1] *= f;
-      }
+    for (int j = 0; j < 8; ++j) {
+      st.o[j][half * 2] *= f;
+      st.o[j][half * 2 + 1] *= f;
     }
   }
-  if (TREE && bad != 0) {
+  if (bad != 0) {
     // Visible rows add p * v of these keys one by one; the V rows are then cleared.
     for (uint32_t left = bad; left != 0; left &= left - 1) {
       const int key = __ffs(left) - 1;
       const int src = (lane & ~3) | ((key & 7) >> 1);
       const uint32_t row = vs + key * ROW_BYTES;
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
+      for (int half = 0; half < 2; ++half) {
+        uint32_t pair = 0;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int r = row0 + t * 16 + half * 8 + (lane >> 2);
-          const bool sees = r < p.G * p.N && ((mask[r % p.N][key0 >> 5] >> key) & 1u);
-          uint32_t pair = 0;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t x = __shfl_sync(0xffffffffu, pf[t][j][half], src);
-            if (j == key >> 3) pair = x;
-          }
-          const float pr = (key & 1) ? bf16_hi(pair) : bf16_lo(pair);
+        for (int j = 0; j < NT; ++j) {
+          const uint32_t x = __shfl_sync(0xffffffffu, pf[j][half], src);
+          if (j == key >> 3) pair = x;
+        }
+        const float pr = (key & 1) ? bf16_hi(pair) : bf16_lo(pair);
+        if ((see[half] >> key) & 1u) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const uint32_t v2 = lds_u32(row + ((j ^ (key & 7)) << 4) + (lane & 3) * 4);
-            if (sees) {
-              st.o[t][j][half * 2] = fmaf(pr, bf16_lo(v2), st.o[t][j][half * 2]);
-              st.o[t][j][half * 2 + 1] = fmaf(pr, bf16_hi(v2), st.o[t][j][half * 2 + 1]);
-            }
+            st.o[j][half * 2] = fmaf(pr, bf16_lo(v2), st.o[j][half * 2]);
+            st.o[j][half * 2 + 1] = fmaf(pr, bf16_hi(v2), st.o[j][half * 2 + 1]);
           }
         }
       }
@@ -381,48 +313,35 @@ __device__ __forceinline__ void tile_step(WarpState<RT>& st, const Params& p, ui
     }
     __syncwarp();
   }
-  // O += P V: two k-steps of 16 keys. One transposing ldmatrix.x4 holds 16 keys x 16 features.
+  // O += P V: k-steps of 16 keys. One transposing ldmatrix.x4 holds 16 keys x 16 features.
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < NT / 2; ++k) {
     const int key = k * 16 + (lane & 15);
     const uint32_t vr = vs + key * ROW_BYTES;
+    const uint32_t a[4] = {pf[2 * k][0], pf[2 * k][1], pf[2 * k + 1][0], pf[2 * k + 1][1]};
 #pragma unroll
     for (int jj = 0; jj < 4; ++jj) {
       uint32_t bfr[4];
       ldmatrix_x4_trans(vr + (((jj * 2 + (lane >> 4)) ^ (key & 7)) << 4), bfr);
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        const uint32_t a[4] = {pf[t][2 * k][0], pf[t][2 * k][1], pf[t][2 * k + 1][0],
-                               pf[t][2 * k + 1][1]};
-        mma_16816(st.o[t][jj * 2], a, bfr[0], bfr[1]);
-        mma_16816(st.o[t][jj * 2 + 1], a, bfr[2], bfr[3]);
-      }
+      mma_16816(st.o[jj * 2], a, bfr[0], bfr[1]);
+      mma_16816(st.o[jj * 2 + 1], a, bfr[2], bfr[3]);
     }
   }
-  // Zeroed rows were generic writes; the next TMA write of the stage is an asynchronous one.
-  if (TREE || n_valid < 32) fence_proxy_async_smem();
 }
 
 // The warp's result into its record: O (not normalised), m and the full row sum l.
-template <int RT>
-__device__ __forceinline__ void store_record(WarpState<RT>& st, float (*rec)[REC], int lane) {
+__device__ __forceinline__ void store_record(const WarpState& st, float (*rec)[REC], int lane) {
 #pragma unroll
-  for (int t = 0; t < RT; ++t) {
+  for (int half = 0; half < 2; ++half) {
+    float l = st.l[half];
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    float* row = rec[half * 8 + (lane >> 2)];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      float l = st.l[t][half];
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
-      float* row = rec[t * 16 + half * 8 + (lane >> 2)];
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        *reinterpret_cast<float2*>(row + j * 8 + (lane & 3) * 2) =
-            make_float2(st.o[t][j][half * 2], st.o[t][j][half * 2 + 1]);
-      if ((lane & 3) == 0) {
-        row[HD] = st.m[t][half];
-        row[HD + 1] = l;
-      }
-    }
+    for (int j = 0; j < 8; ++j)
+      *reinterpret_cast<float2*>(row + j * 8 + (lane & 3) * 2) =
+          make_float2(st.o[j][half * 2], st.o[j][half * 2 + 1]);
+    if ((lane & 3) == 0) *reinterpret_cast<float2*>(row + HD) = make_float2(st.m[half], l);
   }
 }
 
@@ -444,86 +363,138 @@ __device__ __forceinline__ void write_out(const Params& p, int64_t out_row, int 
     p.lse[out_row] = (used && den != 0.f) ? (M + log2f(den)) * LN2 : -INFINITY;
 }
 
-template <int RT>
-__global__ void __launch_bounds__(THREADS)
+// The step over the tree's own keys, by one warp: its K and V rows into shared memory (rows that are
+// not in use as zeros), then 16 keys under the ancestor masks. chain: lane n holds node n's mask.
+__device__ __forceinline__ void tree_step(WarpState& st, const Params& p, Smem& s, int b, int h,
+                                          uint32_t chain, uint32_t used, int lane) {
+  const int c = lane & 7;
+  uint4 k[4], v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = i * 4 + (lane >> 3);
+    k[i] = v[i] = make_uint4(0, 0, 0, 0);
+    if (n < p.N && ((used >> n) & 1u)) {
+      k[i] = __ldg(reinterpret_cast<const uint4*>(p.tk + b * p.tk_sb + h * p.tk_sh + n * p.tk_sn) + c);
+      v[i] = __ldg(reinterpret_cast<const uint4*>(p.tv + b * p.tv_sb + h * p.tv_sh + n * p.tv_sn) + c);
+    }
+  }
+  const uint32_t ks = smem_u32(s.tree[0]), vs = smem_u32(s.tree[1]);
+  uint32_t bad = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = i * 4 + (lane >> 3);
+    const uint32_t at = n * ROW_BYTES + ((c ^ (n & 7)) << 4);
+    sts_u4(ks + at, k[i].x, k[i].y, k[i].z, k[i].w);
+    sts_u4(vs + at, v[i].x, v[i].y, v[i].z, v[i].w);
+    const unsigned nf = __ballot_sync(0xffffffffu, has_nonfinite(v[i].x) || has_nonfinite(v[i].y) ||
+                                                       has_nonfinite(v[i].z) || has_nonfinite(v[i].w));
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (nf & (0xFFu << (8 * r))) bad |= 1u << (i * 4 + r);
+  }
+  __syncwarp();
+  uint32_t see[2];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int r = half * 8 + (lane >> 2);
+    const uint32_t bits = __shfl_sync(0xffffffffu, chain, r % p.N);
+    see[half] = r < p.G * p.N ? bits : 0u;
+  }
+  tile_step<16>(st, p.scale_log2, ks, vs, true, see, bad, lane);
+}
+
+__global__ void __launch_bounds__(THREADS, 3)
 tree_attention_kernel(const __grid_constant__ CUtensorMap tm_k,
-                      const __grid_constant__ CUtensorMap tm_v,
-                      const __grid_constant__ CUtensorMap tm_tk,
-                      const __grid_constant__ CUtensorMap tm_tv, const Params p) {
-  constexpr int ROWS = RT * 16;
+                      const __grid_constant__ CUtensorMap tm_v, const Params p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  Smem<RT>& s = *reinterpret_cast<Smem<RT>*>(smem_raw);
+  Smem& s = *reinterpret_cast<Smem*>(smem_raw);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
-  const int unit = static_cast<int>(blockIdx.x) / p.splits;
-  const int bh = unit / p.row_tiles;
-  const int row0 = (unit - bh * p.row_tiles) * ROWS;
+  const int bh = static_cast<int>(blockIdx.x) / p.splits;
   const int b = bh / p.Hkv, h = bh - b * p.Hkv;
+  const int rows = p.G * p.N;
   const int L = valid_len(p.lens, p.C, b);
-  const int tree_tiles = (p.N + KEYS - 1) / KEYS;
-  const int tiles = tree_tiles + (L + KEYS - 1) / KEYS;
+  const int tiles = (L + KEYS - 1) / KEYS;
   const int first = static_cast<int>(static_cast<int64_t>(tiles) * rank / p.splits);
   const int last = static_cast<int>(static_cast<int64_t>(tiles) * (rank + 1) / p.splits);
+  // No CTA writes another's shared memory before that CTA has started (waited for at the end).
+  if (p.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&s.full[i], 1);
-      mbar_init(&s.empty[i], CONSUMER_WARPS);
+  // Producer: tile i into stage i % STAGES once the consumers have released it; the first tiles go
+  // out before the CTA meets. Rows past the capacity read as zero; rows past the length are loaded
+  // and never used.
+  auto issue = [&](int i) {
+    const int st = (i - first) % STAGES;
+    mbar_arrive_expect_tx(&s.full[st], 2 * TILE_BYTES);
+    tma_load_4d(s.ring[st][0], &tm_k, &s.full[st], 0, i * KEYS, h, b);
+    tma_load_4d(s.ring[st][1], &tm_v, &s.full[st], 0, i * KEYS, h, b);
+  };
+  WarpState st;
+  uint32_t chain = 0, used = 0;
+  if (warp == CONSUMER_WARPS) {
+    if (lane == 0) {
+      for (int i = 0; i < STAGES; ++i) {
+        mbar_init(&s.full[i], 1);
+        mbar_init(&s.empty[i], CONSUMER_WARPS);
+      }
+      s.abort = 0;
+      fence_barrier_init();
+      for (int i = first; i < min(last, first + STAGES); ++i) issue(i);
     }
-    s.abort = 0;
-    fence_barrier_init();
+    __syncwarp();
+  } else {
+    load_q(st, p, b, h, lane);
+    // Ancestor mask of node `lane`, by climbing: links go to lower indices, so 16 steps at most.
+    const int32_t* parents = p.parents + b * p.parents_sb;
+    const int up = lane < p.N ? __ldg(parents + lane) : -2;
+    const int link = up < lane && up >= -1 ? up : -2;
+    int at = lane;
+    while (__any_sync(0xffffffffu, at >= 0)) {
+      if (at >= 0) chain |= 1u << at;
+      const int next = __shfl_sync(0xffffffffu, link, at & 31);
+      if (at >= 0) at = next;
+    }
+    if (at != -1) chain = 0;
+    used = __ballot_sync(0xffffffffu, chain != 0);
   }
   __syncthreads();
 
   if (warp == CONSUMER_WARPS) {
-    // Producer: tile i into stage i % STAGES once the consumers have released it. Rows past the
-    // tensor's end read as zero; rows past the length are loaded and never used.
     if (lane == 0) {
-      int issued = 0;
-      for (int i = first; i < last; ++i, ++issued) {
-        const int st = issued % STAGES;
-        if (issued >= STAGES && !wait_or_abort(&s.abort, &s.empty[st], ((issued / STAGES) + 1) & 1))
-          break;
-        mbar_arrive_expect_tx(&s.full[st], 2 * TILE_BYTES);
-        if (i < tree_tiles) {
-          tma_load_4d(s.ring[st][0], &tm_tk, &s.full[st], 0, i * KEYS, h, b);
-          tma_load_4d(s.ring[st][1], &tm_tv, &s.full[st], 0, i * KEYS, h, b);
-        } else {
-          tma_load_4d(s.ring[st][0], &tm_k, &s.full[st], 0, (i - tree_tiles) * KEYS, h, b);
-          tma_load_4d(s.ring[st][1], &tm_v, &s.full[st], 0, (i - tree_tiles) * KEYS, h, b);
-        }
+      int issued = min(last, first + STAGES);
+      for (; issued < last; ++issued) {
+        const int k = issued - first;
+        if (!wait_or_abort(&s.abort, &s.empty[k % STAGES], ((k / STAGES) + 1) & 1)) break;
+        issue(issued);
       }
       // Never leave while a TMA write into this CTA's shared memory is pending.
       if (s.abort)
-        for (int c = max(0, issued - STAGES); c < issued; ++c)
-          mbar_wait(&s.full[c % STAGES], (c / STAGES) & 1);
+        for (int k = max(0, issued - first - STAGES); k < issued - first; ++k)
+          mbar_wait(&s.full[k % STAGES], (k / STAGES) & 1);
     }
     __syncwarp();
   } else {
-    WarpState<RT> st;
-    load_q(st, p, b, h, row0, lane);
-    reset(st);
-    if (first < tree_tiles || rank == 0) {
-      build_masks(p.parents + b * p.parents_sb, p.N, s.jump, s.mask, threadIdx.x,
-                  CONSUMER_WARPS * 32,
-                  [](bool any) { return barrier_or<CONSUMER_WARPS * 32>(any); });
-    }
-    if (rank == 0 && threadIdx.x < ROWS) {
-      const int r = row0 + static_cast<int>(threadIdx.x);
-      s.used[threadIdx.x] = r < p.G * p.N && node_used(s.mask, r % p.N);
-    }
+    if (rank == 0 && warp == 0) tree_step(st, p, s, b, h, chain, used, lane);
     for (int i = first; i < last; ++i) {
       const int c = i - first, sg = c % STAGES;
       if (!warp_wait(&s.abort, &s.full[sg], (c / STAGES) & 1)) break;
-      const bool is_tree = i < tree_tiles;
-      const int key0 = (is_tree ? i : i - tree_tiles) * KEYS + warp * 32;
-      const int n_valid = min(32, (is_tree ? p.N : L) - key0);
+      const int n_valid = min(32, L - i * KEYS - warp * 32);
       if (n_valid > 0) {
         const uint32_t ks = smem_u32(s.ring[sg][0]) + warp * 32 * ROW_BYTES;
         const uint32_t vs = smem_u32(s.ring[sg][1]) + warp * 32 * ROW_BYTES;
-        if (is_tree) tile_step<RT, true>(st, p, ks, vs, n_valid, lane, s.mask, key0, row0);
-        else tile_step<RT, false>(st, p, ks, vs, n_valid, lane, s.mask, key0, row0);
+        const uint32_t all = n_valid < 32 ? (1u << n_valid) - 1u : 0xffffffffu;
+        const uint32_t see[2] = {all, all};
+        if (n_valid < 32) {
+          // V rows past the length: zeroed, so that 0 * (whatever they hold) stays 0.
+          if (lane >= n_valid) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sts_u4(vs + lane * ROW_BYTES + k * 16, 0, 0, 0, 0);
+          }
+          __syncwarp();
+        }
+        tile_step<32>(st, p.scale_log2, ks, vs, n_valid < 32, see, 0u, lane);
+        // (No TMA write follows the generic ones: a partial tile is the sequence's last.)
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.empty[sg]);
@@ -531,59 +502,68 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tm_k,
     // Every tile of this CTA has landed and been read by all warps before the ring is reused.
     asm volatile("bar.sync 1, %0;" ::"n"(CONSUMER_WARPS * 32) : "memory");
     if (!s.abort) store_record(st, s.rec[warp], lane);
+    asm volatile("bar.sync 1, %0;" ::"n"(CONSUMER_WARPS * 32) : "memory");
   }
-  __syncthreads();
 
-  // The CTA's warps: 8 threads a row, 8 features each.
-  const int64_t out0 = static_cast<int64_t>(bh) * p.G * p.N + row0;
-  const int rows = min(ROWS, p.G * p.N - row0);
-  for (int i = threadIdx.x; i < rows * 8; i += THREADS) {
-    const int r = i >> 3, c8 = i & 7;
-    float M = -INFINITY, den = 0.f, n[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < CONSUMER_WARPS; ++w) M = fmaxf(M, s.rec[w][r][HD]);
+  // The CTA's warps: 8 threads a row, 8 features each; then row r goes to rank r % splits.
+  const int r = static_cast<int>(threadIdx.x) >> 3, c8 = threadIdx.x & 7;
+  const bool task = warp < CONSUMER_WARPS && r < rows;
+  float M = -INFINITY, den = 0.f, n[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  auto add = [&](const float* rec, float weight) {
+    const float4 x = reinterpret_cast<const float4*>(rec)[c8 * 2];
+    const float4 y = reinterpret_cast<const float4*>(rec)[c8 * 2 + 1];
+    n[0] = fmaf(weight, x.x, n[0]); n[1] = fmaf(weight, x.y, n[1]);
+    n[2] = fmaf(weight, x.z, n[2]); n[3] = fmaf(weight, x.w, n[3]);
+    n[4] = fmaf(weight, y.x, n[4]); n[5] = fmaf(weight, y.y, n[5]);
+    n[6] = fmaf(weight, y.z, n[6]); n[7] = fmaf(weight, y.w, n[7]);
+  };
+  if (task) {
+    float2 ml[CONSUMER_WARPS];
 #pragma unroll
     for (int w = 0; w < CONSUMER_WARPS; ++w) {
-      const float wt = merge_weight(s.rec[w][r][HD], M);
-      den = fmaf(wt, s.rec[w][r][HD + 1], den);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) n[e] = fmaf(wt, s.rec[w][r][c8 * 8 + e], n[e]);
+      ml[w] = *reinterpret_cast<const float2*>(s.rec[w][r] + HD);
+      M = fmaxf(M, ml[w].x);
     }
-    if (p.splits == 1) {
-      write_out(p, out0 + r, c8, n, M, den, s.used[r] != 0);
-    } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s.crec[r][c8 * 8 + e] = n[e];
-      if (c8 == 0) {
-        s.crec[r][HD] = M;
-        s.crec[r][HD + 1] = den;
-      }
+    for (int w = 0; w < CONSUMER_WARPS; ++w) {
+      const float weight = merge_weight(ml[w].x, M);
+      den = fmaf(weight, ml[w].y, den);
+      add(s.rec[w][r], weight);
     }
   }
-  if (p.splits == 1) return;
+  const int64_t out0 = static_cast<int64_t>(bh) * rows;
+  if (p.splits == 1) {
+    if (task) write_out(p, out0 + r, c8, n, M, den, (used >> (r % p.N)) & 1u);
+    return;
+  }
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  const int each = (ROWS + p.splits - 1) / p.splits;  // rows a rank owns
+  if (task) {
+    const uint32_t dst =
+        map_to_rank(smem_u32(s.push[rank * each + r / p.splits]), static_cast<uint32_t>(r % p.splits));
+    st_cluster_v4(dst + c8 * 32, __float_as_uint(n[0]), __float_as_uint(n[1]), __float_as_uint(n[2]),
+                  __float_as_uint(n[3]));
+    st_cluster_v4(dst + c8 * 32 + 16, __float_as_uint(n[4]), __float_as_uint(n[5]),
+                  __float_as_uint(n[6]), __float_as_uint(n[7]));
+    if (c8 == 0) st_cluster_f32x2(dst + HD * 4, M, den);
+  }
   cluster_sync();
-  // The cluster's CTAs: rank k merges rows k, k + splits, ...
-  for (int i = threadIdx.x; i < rows * 8; i += THREADS) {
-    const int r = (i >> 3) * p.splits + rank, c8 = i & 7;
-    if (r >= rows) break;
-    const uint32_t mine = smem_u32(s.crec[r]);
-    float M = -INFINITY, den = 0.f, n[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int c = 0; c < p.splits; ++c)
-      M = fmaxf(M, ld_cluster_f32(map_to_rank(mine, c) + HD * 4));
-    for (int c = 0; c < p.splits; ++c) {
-      const uint32_t src = map_to_rank(mine, c);
-      const float wt = merge_weight(ld_cluster_f32(src + HD * 4), M);
-      den = fmaf(wt, ld_cluster_f32(src + (HD + 1) * 4), den);
-      const float4 x = ld_cluster_f4(src + c8 * 32), y = ld_cluster_f4(src + c8 * 32 + 16);
-      n[0] = fmaf(wt, x.x, n[0]); n[1] = fmaf(wt, x.y, n[1]);
-      n[2] = fmaf(wt, x.z, n[2]); n[3] = fmaf(wt, x.w, n[3]);
-      n[4] = fmaf(wt, y.x, n[4]); n[5] = fmaf(wt, y.y, n[5]);
-      n[6] = fmaf(wt, y.z, n[6]); n[7] = fmaf(wt, y.w, n[7]);
-    }
-    write_out(p, out0 + r, c8, n, M, den,
-              ld_cluster_s32(map_to_rank(smem_u32(&s.used[r]), 0)) != 0);
+  // The cluster's CTAs, for this rank's rows. Nothing is written to another CTA any more.
+  const int own = r * p.splits + rank;
+  if (warp >= CONSUMER_WARPS || r >= each || own >= rows) return;
+  M = -INFINITY;
+  den = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) n[e] = 0.f;
+  for (int k = 0; k < p.splits; ++k) M = fmaxf(M, s.push[k * each + r][HD]);
+  for (int k = 0; k < p.splits; ++k) {
+    const float* rec = s.push[k * each + r];
+    const float2 ml = *reinterpret_cast<const float2*>(rec + HD);
+    const float weight = merge_weight(ml.x, M);
+    den = fmaf(weight, ml.y, den);
+    add(rec, weight);
   }
-  cluster_sync();  // no CTA leaves while another reads its records
+  write_out(p, out0 + own, c8, n, M, den, (used >> (own % p.N)) & 1u);
 }
 
 }  // namespace tree

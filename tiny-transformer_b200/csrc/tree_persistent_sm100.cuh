@@ -70,8 +70,6 @@ struct Start {
 
 struct Params {
   tree::Params t;
-  const __nv_bfloat16* tree_v;  // for V rows with infinities or NaN
-  int64_t tv_sb, tv_sh, tv_sn;
   int rows;                     // query rows of a unit's tile (the last tile may have fewer)
   int units;                    // units per batch row: Hkv * row_tiles
   int tree_tiles;
@@ -288,8 +286,8 @@ __device__ __forceinline__ void add_nonfinite(const Smem& s, const Params& p, in
   const uint32_t* see = s.mask[qb][row % p.t.N];
   for (int k = 0; k < MASK_WORDS; ++k) {
     for (uint32_t left = s.bad[qb][k] & see[k]; left != 0; left &= left - 1) {
-      const __nv_bfloat16* src = p.tree_v + un.b * p.tv_sb + un.h * p.tv_sh +
-                                 (k * 32 + __ffs(left) - 1) * p.tv_sn + col;
+      const __nv_bfloat16* src = p.t.tv + un.b * p.t.tv_sb + un.h * p.t.tv_sh +
+                                 (k * 32 + __ffs(left) - 1) * p.t.tv_sn + col;
       const uint2 u = *reinterpret_cast<const uint2*>(src);
       if (!isfinite(bf16_lo(u.x))) n.x += bf16_lo(u.x);
       if (!isfinite(bf16_hi(u.x))) n.y += bf16_hi(u.x);
