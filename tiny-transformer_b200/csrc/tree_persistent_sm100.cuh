@@ -57,8 +57,9 @@ constexpr float RESCALE_THRESHOLD = 8.0f;
 constexpr unsigned UNIT_COST = 3;                 // a unit's fixed cost, in tiles
 constexpr int MERGE_COLS = 32;                    // O columns merged at a time
 constexpr uint32_t MERGE_BYTES = (MERGE_COLS + 4) * 4;
-constexpr int COMBINE_ROWS = 32;                  // rows per combine block
-constexpr int COMBINE_THREADS = COMBINE_ROWS * 8;
+constexpr int COMBINE_ROWS = 8;                   // rows per combine block
+constexpr int COMBINE_SHARES = 2;                 // threads that share a row's records
+constexpr int COMBINE_THREADS = COMBINE_ROWS * 8 * COMBINE_SHARES;
 
 // Where a CTA's part of the flat list starts (all counts fit 32 bits: the host checks).
 struct Start {
@@ -811,7 +812,8 @@ tree_persistent_kernel(const __grid_constant__ CUtensorMap tm_k,
 
 // Merge of the units that lie in more than one CTA. Block (c, g) looks at the boundary between
 // CTAs c and c + 1: if it is the first one inside a unit, the block merges that unit's records
-// for rows [32 g, 32 g + 32), 8 threads a row, eight records' loads in flight at a time.
+// for rows [8 g, 8 g + 8), 8 threads a row for the columns and two shares of the records, whose
+// loads are all in flight together (a thread per row and column walking 13 records took 8 us).
 __global__ void __launch_bounds__(COMBINE_THREADS) tree_combine_kernel(const Params p, int grid) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int c = static_cast<int>(blockIdx.x);
@@ -836,22 +838,25 @@ __global__ void __launch_bounds__(COMBINE_THREADS) tree_combine_kernel(const Par
   const int R = p.t.G * p.t.N;
   const int row0 = (unit_u % p.t.row_tiles) * p.rows;
   const int rows = min(p.rows, R - row0);
-  const int r = static_cast<int>(blockIdx.y) * COMBINE_ROWS + static_cast<int>(threadIdx.x >> 3);
+  const int r_in = static_cast<int>(threadIdx.x >> 3) % COMBINE_ROWS;
+  const int share = static_cast<int>(threadIdx.x >> 3) / COMBINE_ROWS;
+  const int r = static_cast<int>(blockIdx.y) * COMBINE_ROWS + r_in;
   const int c8 = threadIdx.x & 7;
-  if (r >= rows) return;
-  const float* first = p.records + (static_cast<int64_t>(c) * 2 * p.rows + r) * REC;
+  const bool in_unit = r < rows;
+  const float* first = p.records + (static_cast<int64_t>(c) * 2 * p.rows + (in_unit ? r : 0)) * REC;
   const int64_t step = static_cast<int64_t>(2) * p.rows * REC;
   float M = -INFINITY, den = 0.f, n[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   float used = 0.f;
   constexpr int BATCH = 8;
-  for (int k0 = 0; k0 < pieces; k0 += BATCH) {
+  for (int k0 = share; k0 < pieces; k0 += BATCH * COMBINE_SHARES) {
     float4 ml[BATCH], x[BATCH], y[BATCH];
 #pragma unroll
     for (int k = 0; k < BATCH; ++k) {
-      const bool in = k0 + k < pieces;
+      const int at = k0 + k * COMBINE_SHARES;
+      const bool in = at < pieces;
       // The first piece is in its CTA's second record, the others in their first.
-      const float4* src = reinterpret_cast<const float4*>(
-          first + (in ? k0 + k : 0) * step + (in && k0 + k > 0 ? 0 : p.rows * REC));
+      const float4* src = reinterpret_cast<const float4*>(first + (in ? at : 0) * step +
+                                                          (in && at > 0 ? 0 : p.rows * REC));
       ml[k] = in ? src[HD / 4] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
       x[k] = in ? src[c8 * 2] : make_float4(0.f, 0.f, 0.f, 0.f);
       y[k] = in ? src[c8 * 2 + 1] : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -874,6 +879,27 @@ __global__ void __launch_bounds__(COMBINE_THREADS) tree_combine_kernel(const Par
       n[4] = fmaf(wt, y[k].x, n[4]); n[5] = fmaf(wt, y[k].y, n[5]);
       n[6] = fmaf(wt, y[k].z, n[6]); n[7] = fmaf(wt, y[k].w, n[7]);
     }
+  }
+  // The second share's result to the first.
+  __shared__ float part[COMBINE_SHARES - 1][COMBINE_ROWS * 8][10];
+  if (share > 0) {
+    float* dst = part[share - 1][r_in * 8 + c8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dst[e] = n[e];
+    dst[8] = M;
+    dst[9] = den;
+  }
+  __syncthreads();
+  if (share > 0 || !in_unit) return;
+#pragma unroll
+  for (int k = 0; k < COMBINE_SHARES - 1; ++k) {
+    const float* src = part[k][r_in * 8 + c8];
+    const float m_new = fmaxf(M, src[8]);
+    const float a = merge_weight(M, m_new), w = merge_weight(src[8], m_new);
+    M = m_new;
+    den = den * a + src[9] * w;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) n[e] = n[e] * a + src[e] * w;
   }
   const int bh = unit_b * p.t.Hkv + unit_u / p.t.row_tiles;
   write_out(p.t, static_cast<int64_t>(bh) * R + row0 + r, c8, n, M, den, used != 0.f);

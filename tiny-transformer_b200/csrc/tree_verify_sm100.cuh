@@ -73,6 +73,7 @@ struct Smem {
   // same), so no barrier is needed to read them; a node's list goes to the other half than the last
   // one's, which slower threads may still read (each list has a pass and its barrier behind it).
   unsigned long long S[2][MAX_NODES];
+  double Sd[2][MAX_NODES];       // the same in FP64
   long long lost[2][MAX_NODES];  // what r lost at that token (chosen children)
   int32_t rejected[2][MAX_NODES];
   unsigned long long share[2][MAX_CLUSTER];  // the cluster's sums, by pass parity
@@ -117,12 +118,14 @@ __device__ __forceinline__ double to_double(float x) {
 
 // max(r_0 - floor(q S_0) - ... - floor(q S_(K-1)), 0), which is r_K (what is taken off is never
 // negative), exact in FP64 below S = 2^51: 2^52 + y, rounded down, is 2^52 + floor(y).
-__device__ __forceinline__ double residual_fp64(float p, float q, int K, const unsigned long long* S) {
+__device__ __forceinline__ double residual_fp64(float p, float q, int K, double S1,
+                                                const double* S) {
   constexpr double M = 4503599627370496.0;  // 2^52
   double r = __dadd_rn(__dadd_rd(to_double<36>(p), M), -__dadd_rd(to_double<36>(q), M));
   const double d = to_double<0>(q);
-  for (int k = 1; k < K; ++k)
-    r = __dadd_rn(r, __dadd_rn(M, -__dadd_rd(__dmul_rn(d, static_cast<double>(S[k])), M)));
+  r = __dadd_rn(r, __dadd_rn(M, -__dadd_rd(__dmul_rn(d, S1), M)));
+  for (int k = 2; k < K; ++k)
+    r = __dadd_rn(r, __dadd_rn(M, -__dadd_rd(__dmul_rn(d, S[k]), M)));
   const int sign = ~(__double2hiint(r) >> 31);  // negative: zero
   return __hiloint2double(__double2hiint(r) & sign, __double2loint(r) & sign);
 }
@@ -192,6 +195,7 @@ __device__ __forceinline__ unsigned long long sum_pass(Smem& s, const Params& a,
   const bool with_q = DENSE && K > 0;
   // Products of this size of S keep the FP64 form exact (a row of probabilities has S <= 2^36).
   const bool fp64_exact = !with_q || K == 1 || s.S[half][1] < (1ull << 51);
+  const double S1 = with_q && K > 1 ? s.Sd[half][1] : 0.0;
   // Sum of r_K over one lane's tokens of the window at v0.
   auto lane_sum = [&](const float (&ps)[LANE_TOKENS], const float (&qs)[LANE_TOKENS], int v0) {
     long long sum = 0;
@@ -210,7 +214,7 @@ __device__ __forceinline__ unsigned long long sum_pass(Smem& s, const Params& a,
       double total = 0.0;
 #pragma unroll
       for (int j = 0; j < LANE_TOKENS; ++j)
-        total = __dadd_rn(total, residual_fp64(clamp_prob(ps[j]), clamp_prob(qs[j]), K, s.S[half]));
+        total = __dadd_rn(total, residual_fp64(clamp_prob(ps[j]), clamp_prob(qs[j]), K, S1, s.Sd[half]));
       sum = __double2ll_rn(total);
     } else if (with_q) {
 #pragma unroll 1
@@ -366,6 +370,7 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) tree_verify_kernel(const Param
     if (K == 0) half ^= 1;
     const unsigned long long S = K == 0 ? static_cast<unsigned long long>(ONE) : total;
     s.S[half][K] = S;
+    s.Sd[half][K] = static_cast<double>(S);
     s.rejected[half][K] = token;
     __syncwarp();
     ++K;
