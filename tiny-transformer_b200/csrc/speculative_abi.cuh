@@ -35,10 +35,13 @@ TreePlan tree_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nod
     pl.grid = std::min<int64_t>(kPlanSms, batch * kv_heads * pl.row_tiles * tiles);
     return pl;
   }
-  // Three CTAs fit an SM; a cluster shares a sequence's tiles.
-  const int64_t units = batch * kv_heads;
-  pl.splits = static_cast<int>(std::max<int64_t>(
-      1, std::min<int64_t>({tt::tree::MAX_SPLITS, tiles - tree_tiles, 3 * kPlanSms / units})));
+  // Three CTAs fit an SM; a cluster shares a sequence's tiles: enough CTAs to fill the SMs once, and
+  // for long caches CTAs of about 16 tiles whatever their number, so that the last ones to run are
+  // short (us at 1, 2, 3, 4 CTAs a sequence: 384 sequences x 64 tiles 87, 83, 81, 82; 768 x 32 tiles
+  // 86, 84, 87, 92; 768 x 8 tiles 30, 37, 47, 54; 96 x 16 tiles 16, 12, 11, 10.4).
+  const int64_t units = batch * kv_heads, cached = tiles - tree_tiles;
+  const int64_t fill = std::min<int64_t>({tt::tree::MAX_SPLITS, cached, 3 * kPlanSms / units});
+  pl.splits = static_cast<int>(std::max<int64_t>({1, fill, std::min<int64_t>(3, cached / 16)}));
   return pl;
 }
 
