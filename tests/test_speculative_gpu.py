@@ -99,6 +99,57 @@ def test_tree_attention_matches_oracle(spec, B, Hq, Hkv, N, C, lens, ragged):
     assert torch.equal(o, again)
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,N,C,lens,ragged", [
+    (2, 4, 4, 24, 70000, [300, 5], True),    # a large capacity: 24 rows in the persistent kernel
+    (2, 8, 2, 8, 140000, [1000, 0], False),  # 32 rows of four shared heads
+    (1, 2, 2, 40, 4100, [4097], False),      # units shared by CTAs, 40 rows
+    (2, 2, 1, 100, 3000, [2999, 10], True),  # 200 rows in two tiles, one short sequence
+    (3, 1, 1, 65, 5000, [0, 4990, 129], True),
+    (1, 4, 4, 33, 130, [130], False),        # whole units
+    (5, 1, 1, 17, 128, [128, 0, 1, 127, 64], True),   # two 16-row tiles, two steps over the tree
+    (1, 16, 1, 32, 260, [259], True),        # 512 rows, 32 tiles of one K/V head
+])
+def test_tree_attention_variants(spec, B, Hq, Hkv, N, C, lens, ragged):
+    """Sizes on both sides of the choices between and within the kernels."""
+    t, parents, _ = _case(B, Hq, Hkv, N, C, 3 * N + C, ragged=ragged)
+    o, lse = _run(spec, t, parents, lens)
+    _check(o, lse, t, parents, lens)
+    o2, lse2 = _run(spec, t, parents, lens)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("N,C", [(24, 70000), (140, 700)])
+def test_masked_places_in_the_persistent_kernel(spec, value, N, C):
+    """As above where the persistent kernel runs; 140 nodes span two key tiles. Unused nodes, cached
+    rows past the length, and the V rows of leaves in both tiles."""
+    lens = [130, 0]
+    t, parents, _ = _case(2, 4, 4, N, C, 13, fan=4)
+    parents[:, N - 3:] = -2
+    want, want_lse = _run(spec, t, parents, lens)
+    x = {k: v.clone() for k, v in t.items()}
+    for b in range(2):
+        x["cache_k"][b, :, lens[b]:] = value
+        x["cache_v"][b, :, lens[b]:] = value
+    for k in ("q", "tree_k", "tree_v"):
+        x[k][:, :, N - 3:] = value
+    leaves = [[n for n in range(1, N - 3) if n not in parents[b]] for b in range(2)]
+    touched = [{leaves[b][0], leaves[b][-1]} for b in range(2)]
+    for b in range(2):
+        for n in touched[b]:
+            x["tree_v"][b, :, n, 5] = value
+    got, lse = _run(spec, x, parents, lens)
+    assert torch.equal(lse, want_lse)
+    for b in range(2):
+        others = [n for n in range(N) if n not in touched[b]]
+        assert torch.equal(got[b, :, others], want[b, :, others])
+        for n in touched[b]:
+            keep = [d for d in range(64) if d != 5]
+            assert not torch.isfinite(got[b, :, n, 5]).any()
+            # The row's other columns see the finite entries of that V row as before.
+            assert torch.equal(got[b, :, n][:, keep], want[b, :, n][:, keep])
+
+
 @pytest.mark.parametrize("kind", ["chain", "star", "forest", "links"])
 def test_tree_shapes(spec, kind):
     """One shared tree [N]: a chain, a star, several roots, and links that end a chain unused."""

@@ -14,6 +14,7 @@ struct TreePlan {
   int splits = 1;         // cluster kernel: CTAs per cluster
   int dup = 1;            // persistent kernel: copies of the rows in a 128-row tile
   int64_t grid = 0;       // persistent kernel: CTAs
+  bool whole = false;     // persistent kernel: no unit is shared by CTAs
 };
 
 TreePlan tree_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nodes,
@@ -22,24 +23,32 @@ TreePlan tree_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nod
   const int64_t rows = q_heads / kv_heads * nodes;
   const int64_t tree_tiles = (nodes + tt::tree::KEYS - 1) / tt::tree::KEYS;
   const int64_t tiles = tree_tiles + (capacity + tt::tree::KEYS - 1) / tt::tree::KEYS;
-  // More than 16 stacked query rows take the persistent kernel: measured 68 against 130 us for 64
-  // rows (B = 32, H = 12, 1024-4096 cached) and 31 against 77 us for 111 rows of 4 shared heads
-  // (9000-20001 cached); with 16 rows or fewer the cluster kernel's lighter start and end win
-  // (151 against 165 us for 16 rows at 1024-8192 cached, 14 against 16 at 256-512).
-  pl.persistent = rows > tt::tree::ROWS;
+  // The cluster kernel reads the cache once per 16 rows, but starts and ends in half the persistent
+  // kernel's time. With one row tile it always wins (142 against 165 us for 16 rows at B = 64, 1024-
+  // 8192 cached); with more, up to about 8192 tile reads (us persistent / cluster: 96 sequences, 32
+  // rows, capacity 2048, 3072 reads 19.6 / 16.8; 384, 32, 1024, 6144 reads 33.6 / 28.8; 96, 24, 8192,
+  // 12288 reads 30.9 / 40.1; 384, 32, 4096, 24576 reads 60 / 71).
+  const int64_t cluster_tiles = (rows + tt::tree::ROWS - 1) / tt::tree::ROWS;
+  const int64_t reads = batch * kv_heads * cluster_tiles * (tiles - tree_tiles);
+  pl.persistent = nodes > tt::tree::CLUSTER_NODES || (cluster_tiles > 1 && reads > 8192);
   if (pl.persistent) {
     constexpr int64_t bm = tt::tree::persist::BM;
     pl.row_tiles = (rows + bm - 1) / bm;
     pl.rows = (rows + pl.row_tiles - 1) / pl.row_tiles;
     pl.dup = pl.rows <= bm / 4 ? 4 : pl.rows <= bm / 2 ? 2 : 1;
-    pl.grid = std::min<int64_t>(kPlanSms, batch * kv_heads * pl.row_tiles * tiles);
+    // Sharing a unit costs a second epilogue and the merge kernel, about eight tiles' time.
+    const int64_t units = batch * kv_heads * pl.row_tiles;
+    pl.whole = tiles <= 9;
+    pl.grid = std::min<int64_t>(kPlanSms, pl.whole ? units : units * tiles);
     return pl;
   }
   // Three CTAs fit an SM; a cluster shares a sequence's tiles: enough CTAs to fill the SMs once, and
   // for long caches CTAs of about 16 tiles whatever their number, so that the last ones to run are
   // short (us at 1, 2, 3, 4 CTAs a sequence: 384 sequences x 64 tiles 87, 83, 81, 82; 768 x 32 tiles
   // 86, 84, 87, 92; 768 x 8 tiles 30, 37, 47, 54; 96 x 16 tiles 16, 12, 11, 10.4).
-  const int64_t units = batch * kv_heads, cached = tiles - tree_tiles;
+  pl.rows = tt::tree::ROWS;
+  pl.row_tiles = cluster_tiles;
+  const int64_t units = batch * kv_heads * pl.row_tiles, cached = tiles - tree_tiles;
   const int64_t fill = std::min<int64_t>({tt::tree::MAX_SPLITS, cached, 3 * kPlanSms / units});
   pl.splits = static_cast<int>(std::max<int64_t>({1, fill, std::min<int64_t>(3, cached / 16)}));
   return pl;
@@ -64,9 +73,10 @@ tt_attn_status set_tree_attributes(int dev) {
   static std::atomic<bool> done[kMaxDevices] = {};
   cudaError_t e = cudaSuccess;
   if (!done[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(tt::tree::tree_attention_kernel,
-                             cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(tt::tree::kSmemBytes));
+    for (auto fn : {tt::tree::tree_attention_kernel<false>, tt::tree::tree_attention_kernel<true>})
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(tt::tree::kSmemBytes));
     for (auto fn : {tt::tree::persist::tree_persistent_kernel<1>,
                     tt::tree::persist::tree_persistent_kernel<2>,
                     tt::tree::persist::tree_persistent_kernel<4>})
@@ -106,6 +116,7 @@ tt_attn_status launch_tree_persistent(const TreePlan& pl, const tt::tree::Params
   p.rows = static_cast<int>(pl.rows);
   p.units = static_cast<int>(tp.Hkv * pl.row_tiles);
   p.tree_tiles = (tp.N + tt::tree::KEYS - 1) / tt::tree::KEYS;
+  p.whole = pl.whole;
   p.starts = static_cast<ps::Start*>(workspace);
   p.records = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + tree_starts_bytes(pl));
   const int grid = static_cast<int>(std::min<int64_t>(pl.grid, sm_count > 0 ? sm_count : kPlanSms));
@@ -115,7 +126,7 @@ tt_attn_status launch_tree_persistent(const TreePlan& pl, const tt::tree::Params
   kernel<<<static_cast<unsigned>(grid), ps::THREADS, ps::kSmemBytes, stream>>>(tmk, tmv, tmtk, tmtv,
                                                                              p);
   tt_attn_status st = check_launch("tree_persistent_kernel launch");
-  if (st != TT_ATTN_OK || grid == 1) return st;
+  if (st != TT_ATTN_OK || grid == 1 || pl.whole) return st;
   // The merge may be scheduled while the main kernel runs (programmatic launch); it waits for its
   // completion on the device.
   cudaLaunchConfig_t cfg{};
@@ -148,7 +159,7 @@ TT_ATTN_API size_t tt_attn_tree_workspace_size(int64_t batch, int64_t q_heads, i
   const TreePlan pl = tree_plan(batch, q_heads, kv_heads, nodes, capacity);
   if (!pl.persistent) return 0;
   return tree_starts_bytes(pl) +
-         static_cast<size_t>(pl.grid) * 2 * pl.rows * tt::tree::REC * sizeof(float);
+         (pl.whole ? 0 : static_cast<size_t>(pl.grid) * 2 * pl.rows * tt::tree::REC * sizeof(float));
 }
 
 TT_ATTN_API tt_attn_status tt_attn_tree_forward_bf16(
@@ -244,9 +255,12 @@ TT_ATTN_API tt_attn_status tt_attn_tree_forward_bf16(
   if (pl.persistent)
     return launch_tree_persistent(pl, p, workspace, sm_count, tmk, tmv, tmtk, tmtv,
                                   static_cast<cudaStream_t>(stream));
-  cluster_config(&cfg, attr, batch * kv_heads * pl.splits, tr::THREADS, tr::kSmemBytes, pl.splits,
+  cluster_config(&cfg, attr, batch * kv_heads * pl.row_tiles * pl.splits, tr::THREADS, tr::kSmemBytes, pl.splits,
                  static_cast<cudaStream_t>(stream));
-  const cudaError_t le = cudaLaunchKernelEx(&cfg, tr::tree_attention_kernel, tmk, tmv, p);
+  const bool multi = pl.row_tiles > 1 || nodes > 16;
+  const cudaError_t le =
+      multi ? cudaLaunchKernelEx(&cfg, tr::tree_attention_kernel<true>, tmk, tmv, p)
+            : cudaLaunchKernelEx(&cfg, tr::tree_attention_kernel<false>, tmk, tmv, p);
   if (le != cudaSuccess)
     return fail(TT_ATTN_LAUNCH_FAIL,
                 std::string("tree_attention_kernel launch: ") + cudaGetErrorString(le));

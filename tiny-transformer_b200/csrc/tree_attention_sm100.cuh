@@ -13,18 +13,19 @@
 // (batch, K/V head), so the cache is read once for all of them. The operator does 2 * G * N
 // products per cached element and is bound by reading the cache for the trees it is made for.
 //
-// tree_attention_kernel: up to 16 stacked query rows (so at most 16 nodes). One thread-block cluster
-// takes one (batch, K/V head); its CTAs share the sequence's actual 128-key cache tiles evenly,
-// whatever the length. A producer warp keeps a two-stage ring of K and V tiles in flight with TMA
+// tree_attention_kernel: trees of at most 32 nodes, 16 stacked query rows at a time. One thread-block
+// cluster takes one (batch, K/V head, 16 rows); its CTAs share the sequence's actual 128-key cache
+// tiles evenly, whatever the length. A producer warp keeps a two-stage ring of K and V tiles in flight with TMA
 // (128-byte swizzle: 16-byte piece c of row r at piece c ^ (r % 8)); 4 consumer warps take 32 keys
 // of a tile each, so that K and V fragments are read from shared memory once. Scores and P.V are
 // mma.m16n8k16 on register fragments (Q stays in registers, P goes from the score fragments to the
-// second product's A operand without leaving them). The tree's 16 keys are one step of rank 0's
-// first warp, loaded with plain loads under the first tiles' flight. Every warp keeps its own online
+// second product's A operand without leaving them). The tree's keys are a step or two of rank 0's
+// first warp, 16 keys each, loaded with plain loads under the first tiles' flight. Every warp keeps its own online
 // softmax (m, l, O); the CTA merges its warps, every CTA pushes each row to the rank that owns it
 // (st.shared::cluster), and after one cluster barrier each rank merges and writes its rows. 70 KiB
 // of shared memory and 128 registers leave room for three CTAs per SM (192 KiB of loads in flight).
-// More rows take tree_persistent_sm100.cuh: 32 rows in registers left one CTA per SM.
+// Larger trees, and more rows over long caches (which would be read once per 16 rows), take
+// tree_persistent_sm100.cuh.
 #pragma once
 
 #include <cuda.h>
@@ -59,14 +60,15 @@ struct Params {
   int64_t parents_sb;
   const int32_t* lens;        // optional [B]
   int B, Hkv, G, N, C;
-  int row_tiles;              // persistent kernel: row tiles of one (batch, K/V head)
+  int row_tiles;              // row tiles of one (batch, K/V head)
   int splits;                 // cluster kernel: CTAs per cluster
   __nv_bfloat16* o;           // contiguous [B, G * Hkv, N, 64]
   float* lse;                 // optional [B, G * Hkv, N]
   float scale_log2;
 };
 
-constexpr int ROWS = 16;                              // query rows of a unit, nodes of a tree
+constexpr int ROWS = 16;                              // query rows of a unit
+constexpr int CLUSTER_NODES = 32;                     // nodes of a tree, cluster kernel
 constexpr int PUSH_ROWS = 24;                         // splits * ceil(ROWS / splits) at most
 
 struct alignas(1024) Smem {
@@ -75,7 +77,7 @@ struct alignas(1024) Smem {
     float rec[CONSUMER_WARPS][ROWS][REC];             // after the last tile: the warps' results
   };
   float push[PUSH_ROWS][REC];                         // this rank's rows from every CTA
-  uint8_t tree[2][ROWS * ROW_BYTES];                  // rank 0: the tree's K and V rows
+  uint8_t tree[2][16 * ROW_BYTES];                    // rank 0: K and V rows of 16 nodes
   uint64_t full[STAGES], empty[STAGES];
   volatile int abort;
 };
@@ -197,10 +199,11 @@ struct WarpState {
   float m[2], l[2];    // rows lane / 4 and lane / 4 + 8
 };
 
-__device__ __forceinline__ void load_q(WarpState& st, const Params& p, int b, int h, int lane) {
+__device__ __forceinline__ void load_q(WarpState& st, const Params& p, int b, int h, int row0,
+                                       int lane) {
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    const int r = half * 8 + (lane >> 2);
+    const int r = row0 + half * 8 + (lane >> 2);
     const bool in = r < p.G * p.N;
     const int g = in ? r / p.N : 0, n = in ? r - g * p.N : 0;
     const uint32_t* src = reinterpret_cast<const uint32_t*>(
@@ -363,15 +366,17 @@ __device__ __forceinline__ void write_out(const Params& p, int64_t out_row, int 
     p.lse[out_row] = (used && den != 0.f) ? (M + log2f(den)) * LN2 : -INFINITY;
 }
 
-// The step over the tree's own keys, by one warp: its K and V rows into shared memory (rows that are
-// not in use as zeros), then 16 keys under the ancestor masks. chain: lane n holds node n's mask.
+// The step over 16 of the tree's own keys, from node `key0` on, by one warp: their K and V rows into
+// shared memory (rows that are not in use as zeros), then the products under the ancestor masks.
+// chain: lane n holds node n's mask.
 __device__ __forceinline__ void tree_step(WarpState& st, const Params& p, Smem& s, int b, int h,
-                                          uint32_t chain, uint32_t used, int lane) {
+                                          int row0, int key0, uint32_t chain, uint32_t used,
+                                          int lane) {
   const int c = lane & 7;
   uint4 k[4], v[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int n = i * 4 + (lane >> 3);
+    const int n = key0 + i * 4 + (lane >> 3);
     k[i] = v[i] = make_uint4(0, 0, 0, 0);
     if (n < p.N && ((used >> n) & 1u)) {
       k[i] = __ldg(reinterpret_cast<const uint4*>(p.tk + b * p.tk_sb + h * p.tk_sh + n * p.tk_sn) + c);
@@ -396,13 +401,17 @@ __device__ __forceinline__ void tree_step(WarpState& st, const Params& p, Smem& 
   uint32_t see[2];
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    const int r = half * 8 + (lane >> 2);
+    const int r = row0 + half * 8 + (lane >> 2);
     const uint32_t bits = __shfl_sync(0xffffffffu, chain, r % p.N);
-    see[half] = r < p.G * p.N ? bits : 0u;
+    see[half] = r < p.G * p.N ? bits >> key0 : 0u;
   }
   tile_step<16>(st, p.scale_log2, ks, vs, true, see, bad, lane);
+  __syncwarp();  // every lane has read the rows before the next step's
 }
 
+// MULTI: several row tiles per K/V head, or more than 16 nodes. (An instantiation of its own: carrying
+// both costs the one-tile kernel 5 % on long caches.)
+template <bool MULTI>
 __global__ void __launch_bounds__(THREADS, 3)
 tree_attention_kernel(const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const Params p) {
@@ -411,9 +420,11 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tm_k,
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
-  const int bh = static_cast<int>(blockIdx.x) / p.splits;
+  const int unit = static_cast<int>(blockIdx.x) / p.splits;
+  const int bh = MULTI ? unit / p.row_tiles : unit;
+  const int row0 = MULTI ? (unit - bh * p.row_tiles) * ROWS : 0;
   const int b = bh / p.Hkv, h = bh - b * p.Hkv;
-  const int rows = p.G * p.N;
+  const int rows = MULTI ? min(ROWS, p.G * p.N - row0) : p.G * p.N;
   const int L = valid_len(p.lens, p.C, b);
   const int tiles = (L + KEYS - 1) / KEYS;
   const int first = static_cast<int>(static_cast<int64_t>(tiles) * rank / p.splits);
@@ -444,8 +455,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tm_k,
     }
     __syncwarp();
   } else {
-    load_q(st, p, b, h, lane);
-    // Ancestor mask of node `lane`, by climbing: links go to lower indices, so 16 steps at most.
+    load_q(st, p, b, h, row0, lane);
+    // Ancestor mask of node `lane`, by climbing: links go to lower indices, so 32 steps at most.
     const int32_t* parents = p.parents + b * p.parents_sb;
     const int up = lane < p.N ? __ldg(parents + lane) : -2;
     const int link = up < lane && up >= -1 ? up : -2;
@@ -475,7 +486,9 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tm_k,
     }
     __syncwarp();
   } else {
-    if (rank == 0 && warp == 0) tree_step(st, p, s, b, h, chain, used, lane);
+    if (rank == 0 && warp == 0)
+      for (int key0 = 0; key0 < (MULTI ? p.N : 1); key0 += 16)
+        tree_step(st, p, s, b, h, row0, key0, chain, used, lane);
     for (int i = first; i < last; ++i) {
       const int c = i - first, sg = c % STAGES;
       if (!warp_wait(&s.abort, &s.full[sg], (c / STAGES) & 1)) break;
@@ -531,9 +544,9 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tm_k,
       add(s.rec[w][r], weight);
     }
   }
-  const int64_t out0 = static_cast<int64_t>(bh) * rows;
+  const int64_t out0 = static_cast<int64_t>(bh) * p.G * p.N + row0;
   if (p.splits == 1) {
-    if (task) write_out(p, out0 + r, c8, n, M, den, (used >> (r % p.N)) & 1u);
+    if (task) write_out(p, out0 + r, c8, n, M, den, (used >> ((row0 + r) % p.N)) & 1u);
     return;
   }
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -563,7 +576,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tm_k,
     den = fmaf(weight, ml.y, den);
     add(rec, weight);
   }
-  write_out(p, out0 + own, c8, n, M, den, (used >> (own % p.N)) & 1u);
+  write_out(p, out0 + own, c8, n, M, den, (used >> ((row0 + own) % p.N)) & 1u);
 }
 
 }  // namespace tree

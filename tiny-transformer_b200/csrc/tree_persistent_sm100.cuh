@@ -74,6 +74,7 @@ struct Params {
   int rows;                     // query rows of a unit's tile (the last tile may have fewer)
   int units;                    // units per batch row: Hkv * row_tiles
   int tree_tiles;
+  bool whole;                   // parts begin and end at units: nothing to merge
   Start* starts;                // [grid]: workspace
   float* records;               // [grid][2][rows][REC]: workspace; 0: unit begun by another CTA
 };
@@ -112,7 +113,8 @@ __device__ __forceinline__ int tiles_of(const Params& p, int b) {
 
 // One warp: the CTA's part [total * i / grid, total * (i + 1) / grid) of the list, in cost. A cost
 // position inside a unit is tile max(0, position - UNIT_COST): a part that ends in a unit's fixed
-// cost ends before the unit, so parts may be empty, but not those that begin inside a unit.
+// cost ends before the unit, so parts may be empty, but not those that begin inside a unit. With
+// p.whole a position moves to the nearer end of its unit.
 __device__ __forceinline__ Start find_start(const Params& p, unsigned cta, unsigned grid, int lane) {
   // The lengths of the first 32 batch rows stay in a register, later ones are read again (L1).
   const unsigned tiles0 = lane < p.t.B ? tiles_of(p, lane) : 0;
@@ -148,9 +150,13 @@ __device__ __forceinline__ Start find_start(const Params& p, unsigned cta, unsig
       const int l = __ffs(hit) - 1;
       const unsigned t = __shfl_sync(0xffffffffu, tiles, l);
       const unsigned in_b = at - before - __shfl_sync(0xffffffffu, run - cost, l);
-      const unsigned unit = in_b / (t + UNIT_COST);
+      unsigned unit = in_b / (t + UNIT_COST);
       const unsigned in_unit = in_b - unit * (t + UNIT_COST);
-      const unsigned tile = in_unit > UNIT_COST ? in_unit - UNIT_COST : 0;
+      unsigned tile = in_unit > UNIT_COST ? in_unit - UNIT_COST : 0;
+      if (p.whole) {
+        tile = 0;
+        if (2 * in_unit >= t + UNIT_COST) ++unit;  // p.units: the next row's first, see below
+      }
       // Tiles before this row: its cost without the fixed parts.
       const unsigned row_tiles_before =
           tiles_before + __shfl_sync(0xffffffffu, run - cost, l) - UNIT_COST * p.units * l;
@@ -162,6 +168,11 @@ __device__ __forceinline__ Start find_start(const Params& p, unsigned cta, unsig
         s.unit = static_cast<int>(unit);
         s.tile = static_cast<int>(tile);
         s.tiles = static_cast<int>(t);
+        if (s.unit == p.units) {
+          s.unit = 0;
+          ++s.b;
+          s.tiles = s.b < p.t.B ? tiles_of(p, s.b) : 0;
+        }
       } else {
         s.count = static_cast<int>(flat - first);
         return s;
