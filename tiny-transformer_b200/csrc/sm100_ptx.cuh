@@ -354,6 +354,14 @@ __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+// ------------------------------------------------------------------ programmatic launch
+// Kernels launched with programmatic stream serialisation may start while the kernel before them in
+// the stream still runs: this waits until it has completed and its writes are visible. Before it a
+// kernel touches its own shared memory and parameters only.
+__device__ __forceinline__ void wait_for_previous_kernel() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // ------------------------------------------------------------------ register budget
 // Warpgroup-wide register re-allocation. The counts a kernel uses must add up to no more than
 // the registers the CTA was launched with (threads x launch registers per thread), or the

@@ -9,6 +9,7 @@
 
 #include <ATen/autocast_mode.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -332,6 +333,12 @@ torch::Tensor qkv_rope_append(const torch::Tensor& hidden, const torch::Tensor& 
 }
 
 // ------------------------------------------------------------------ speculative decoding
+// Uninitialised CUDA tensor without a trip through the dispatcher: these calls are as short as a
+// launch, and every allocation's host time shows.
+torch::Tensor new_cuda(at::IntArrayRef sizes, at::ScalarType dtype, const c10::Device& device) {
+  return at::detail::empty_cuda(sizes, dtype, device, std::nullopt);
+}
+
 // int32 copy of an index tensor where it is not one already; int64 values are clamped into int32,
 // so that none wraps into a valid index.
 torch::Tensor index32(const torch::Tensor& x, const torch::Tensor& like, const char* what) {
@@ -339,7 +346,7 @@ torch::Tensor index32(const torch::Tensor& x, const torch::Tensor& like, const c
               " must be a CUDA tensor on the same device as the other inputs");
   TORCH_CHECK(x.scalar_type() == at::kInt || x.scalar_type() == at::kLong, what,
               " must be int32 or int64");
-  if (x.scalar_type() == at::kInt) return x.contiguous();
+  if (x.scalar_type() == at::kInt) return x.is_contiguous() ? x : x.contiguous();
   return x.clamp(std::numeric_limits<int32_t>::min(), std::numeric_limits<int32_t>::max())
       .to(at::kInt)
       .contiguous();
@@ -414,13 +421,13 @@ std::tuple<torch::Tensor, torch::Tensor> tree_attention(
   tree_v = aligned_contiguous(tree_v);
   cache_k = aligned_contiguous(cache_k);
   cache_v = aligned_contiguous(cache_v);
-  auto o = torch::empty({B, Hq, N, TT_ATTN_HEAD_DIM}, q.options());
+  auto o = new_cuda({B, Hq, N, TT_ATTN_HEAD_DIM}, at::kBFloat16, q.device());
   torch::Tensor lse;
-  if (with_lse) lse = torch::empty({B, Hq, N}, q.options().dtype(at::kFloat));
+  if (with_lse) lse = new_cuda({B, Hq, N}, at::kFloat, q.device());
   const size_t ws_bytes = tt_attn_tree_workspace_size(B, Hq, Hkv, N, C);
   torch::Tensor ws;
   if (ws_bytes > 0)
-    ws = torch::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(at::kByte));
+    ws = new_cuda({static_cast<int64_t>(ws_bytes)}, at::kByte, q.device());
   const Strides qs(q), tks(tree_k), tvs(tree_v), cks(cache_k), cvs(cache_v);
   const tt_attn_status st = tt_attn_tree_forward_bf16(
       q.data_ptr(), qs.s, tree_k.data_ptr(), tks.s, tree_v.data_ptr(), tvs.s, cache_k.data_ptr(),
@@ -467,16 +474,17 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> tree_verify(
   check_sm100(target_probs);
   int64_t parents_stride = 0;
   parents = tree_parents(parents, target_probs, B, N, &parents_stride);
-  tokens = tokens.to(at::kLong).contiguous();
-  uniforms = uniforms.contiguous();
+  if (tokens.scalar_type() != at::kLong) tokens = tokens.to(at::kLong);
+  if (!tokens.is_contiguous()) tokens = tokens.contiguous();
+  if (!uniforms.is_contiguous()) uniforms = uniforms.contiguous();
   // Rows are read in place when their values are adjacent; other views are copied.
   if (V > 1 && target_probs.stride(2) != 1) target_probs = target_probs.contiguous();
   torch::Tensor dp;
   if (dense)
     dp = V > 1 && draft_probs->stride(2) != 1 ? draft_probs->contiguous() : *draft_probs;
-  auto path = torch::empty({B, N}, target_probs.options().dtype(at::kInt));
-  auto counts = torch::empty({B}, target_probs.options().dtype(at::kInt));
-  auto next = torch::empty({B}, target_probs.options().dtype(at::kLong));
+  auto path = new_cuda({B, N}, at::kInt, target_probs.device());
+  auto counts = new_cuda({B}, at::kInt, target_probs.device());
+  auto next = new_cuda({B}, at::kLong, target_probs.device());
   auto stream = c10::cuda::getCurrentCUDAStream(target_probs.get_device());
   const tt_attn_status st = tt_attn_tree_verify_f32(
       tokens.data_ptr<int64_t>(), parents.data_ptr<int32_t>(), parents_stride,
@@ -561,7 +569,7 @@ torch::Tensor tree_commit(const pybind11::list& cache_k, const pybind11::list& c
   for (LayerTensors& x : t)
     if (!x.in_place)
       for (torch::Tensor& y : x.t) y = y.clone(at::MemoryFormat::Contiguous);
-  auto new_lens = torch::empty({B}, cache_lens.options());
+  auto new_lens = new_cuda({B}, at::kInt, device);
   std::vector<void*> ptr(4 * L);
   for (size_t l = 0; l < L; ++l) {
     ptr[l] = c[0].t[l].data_ptr();

@@ -425,6 +425,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tm_k,
   const int row0 = MULTI ? (unit - bh * p.row_tiles) * ROWS : 0;
   const int b = bh / p.Hkv, h = bh - b * p.Hkv;
   const int rows = MULTI ? min(ROWS, p.G * p.N - row0) : p.G * p.N;
+  wait_for_previous_kernel();
   const int L = valid_len(p.lens, p.C, b);
   const int tiles = (L + KEYS - 1) / KEYS;
   const int first = static_cast<int>(static_cast<int64_t>(tiles) * rank / p.splits);

@@ -39,6 +39,7 @@ __global__ void __launch_bounds__(THREADS) tree_commit_kernel(const __grid_const
   const int b = static_cast<int>(blockIdx.x) % p.B;
   const int lk = static_cast<int>(blockIdx.x) / p.B;   // layer * 2 + (keys or values)
   const int kv = lk & 1, layer = lk >> 1;
+  wait_for_previous_kernel();
   const int len = __ldg(p.lens + b);
   const int count = min(max(__ldg(p.counts + b), 0), p.P);
   // Rows that fit: all of them unless the length is negative or the cache is full.

@@ -742,10 +742,11 @@ tree_persistent_kernel(const __grid_constant__ CUtensorMap tm_k,
   Smem& s = *reinterpret_cast<Smem*>(smem_raw);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  // The combine kernel may be scheduled from here on; it waits for this grid to complete.
+  // The next kernel (the merge) may be scheduled from here on; it waits for this grid to complete.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (warp == 0) {
+    wait_for_previous_kernel();
     const Start st = find_start(p, blockIdx.x, gridDim.x, lane);
     if (lane == 0) {
       s.start = st;
@@ -775,6 +776,7 @@ tree_persistent_kernel(const __grid_constant__ CUtensorMap tm_k,
     s.abort = 0;
     fence_barrier_init();
   }
+  if (warp != 0) wait_for_previous_kernel();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -826,7 +828,7 @@ tree_persistent_kernel(const __grid_constant__ CUtensorMap tm_k,
 // for rows [8 g, 8 g + 8), 8 threads a row for the columns and two shares of the records, whose
 // loads are all in flight together (a thread per row and column walking 13 records took 8 us).
 __global__ void __launch_bounds__(COMBINE_THREADS) tree_combine_kernel(const Params p, int grid) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_previous_kernel();
   const int c = static_cast<int>(blockIdx.x);
   const int lane = threadIdx.x & 31;
   // Lane k looks at CTA c + k: the pieces are the CTAs after c that began inside the same unit.

@@ -304,6 +304,7 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) tree_verify_kernel(const Param
   const int b = static_cast<int>(blockIdx.x) / a.cluster;
   const int N = a.N;
 
+  wait_for_previous_kernel();
   // The tree, the random numbers, and p(t), q(t) of every node at its parent.
   for (int n = threadIdx.x; n < N; n += blockDim.x) {
     const int up = __ldg(a.parents + b * a.parents_sb + n);
