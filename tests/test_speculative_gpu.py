@@ -605,3 +605,43 @@ def test_commit_refusals(spec, change, error, match):
     change(a)
     with pytest.raises(error, match=match):
         spec.commit_path(**a)
+
+
+@pytest.mark.parametrize("N", [4, 40])
+def test_back_to_back_calls_see_each_other(spec, N):
+    """Programmatic launches overlap a kernel's start with the end of the one before it: a chain in
+    which every call reads what the last one wrote gives the same with and without waiting between
+    the calls. (4 nodes: the cluster kernel; 40: the persistent one.)"""
+    B, H, C, V = 3, 2, 600, 1000
+    gen = torch.Generator().manual_seed(17)
+    q, tk, tv = (_randn(gen, B, H, N, 64).cuda() for _ in range(3))
+    parents = torch.arange(-1, N - 1, dtype=torch.int32).cuda()
+    p = torch.softmax(torch.randn(B, N, V, generator=gen) * 3, -1).cuda()
+    uniforms = torch.rand(60, B, N, generator=gen).cuda()
+    start = [_randn(gen, B, H, C, 64).cuda() for _ in range(2)]
+
+    def chain(wait):
+        ck, cv = (x.clone() for x in start)
+        lens = torch.zeros(B, dtype=torch.int32, device="cuda")
+        tokens = torch.zeros(B, N, dtype=torch.long, device="cuda")
+        k, v, seen = tk.clone(), tv.clone(), []
+        for step in range(60):
+            o = spec.tree_attention(q, k, v, ck, cv, parents, lens)
+            if wait:
+                torch.cuda.synchronize()
+            path, counts, nxt = spec.verify_tree(tokens, parents, p, uniforms[step], p)
+            if wait:
+                torch.cuda.synchronize()
+            counts = counts.clamp(max=9)
+            lens = spec.commit_path(ck, cv, k, v, path, counts, lens)
+            if wait:
+                torch.cuda.synchronize()
+            k, v = o, o * 0.5 + v * 0.5           # the next step's rows come from this one's output
+            tokens = (tokens + nxt[:, None]) % V
+            seen.append(nxt)
+        return o, lens, ck, cv, torch.stack(seen)
+
+    want = chain(True)
+    for _ in range(5):
+        for a, b in zip(chain(False), want):
+            assert torch.equal(a, b)

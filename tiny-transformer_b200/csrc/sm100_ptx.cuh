@@ -357,7 +357,8 @@ __device__ __forceinline__ void tmem_wait_st() {
 // ------------------------------------------------------------------ programmatic launch
 // Kernels launched with programmatic stream serialisation may start while the kernel before them in
 // the stream still runs: this waits until it has completed and its writes are visible. Before it a
-// kernel touches its own shared memory and parameters only.
+// kernel touches its own shared memory and parameters only, and it reads nothing through the
+// non-coherent path (__ldg): what it reads may have been written after it started.
 __device__ __forceinline__ void wait_for_previous_kernel() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }

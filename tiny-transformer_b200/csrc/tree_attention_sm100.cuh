@@ -127,7 +127,7 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
 }
 __device__ __forceinline__ int valid_len(const int32_t* lens, int C, int b) {
   if (lens == nullptr) return C;
-  return min(max(__ldg(lens + b), 0), C);
+  return min(max(lens[b], 0), C);
 }
 
 // Ancestor masks of one tree from its parents, by doubling: mask[n] covers the chain from n up to,
@@ -144,7 +144,7 @@ __device__ __forceinline__ void build_masks(const int32_t* parents, int N, int32
   const int words = (N + 31) >> 5;
   bool more = false;
   for (int n = tid; n < N; n += threads) {
-    const int up = __ldg(parents + n);
+    const int up = parents[n];
     jump[n] = up < n && up >= -1 ? up : -2;
     more = more || (up < n && up >= 0);
     for (int w = 0; w < MASK_WORDS; ++w) mask[n][w] = w == n >> 5 ? 1u << (n & 31) : 0u;
@@ -216,8 +216,8 @@ __device__ __forceinline__ void load_q(WarpState& st, const Params& p, int b, in
         p.q + b * p.q_sb + static_cast<int64_t>(h * p.G + g) * p.q_sh + n * p.q_sn) + (lane & 3);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      st.qf[k][half] = in ? __ldg(src + k * 8) : 0u;
-      st.qf[k][half + 2] = in ? __ldg(src + k * 8 + 4) : 0u;
+      st.qf[k][half] = in ? src[k * 8] : 0u;
+      st.qf[k][half + 2] = in ? src[k * 8 + 4] : 0u;
     }
   }
 #pragma unroll
@@ -385,8 +385,8 @@ __device__ __forceinline__ void tree_step(WarpState& st, const Params& p, Smem& 
     const int n = key0 + i * 4 + (lane >> 3);
     k[i] = v[i] = make_uint4(0, 0, 0, 0);
     if (n < p.N && ((used >> n) & 1u)) {
-      k[i] = __ldg(reinterpret_cast<const uint4*>(p.tk + b * p.tk_sb + h * p.tk_sh + n * p.tk_sn) + c);
-      v[i] = __ldg(reinterpret_cast<const uint4*>(p.tv + b * p.tv_sb + h * p.tv_sh + n * p.tv_sn) + c);
+      k[i] = reinterpret_cast<const uint4*>(p.tk + b * p.tk_sb + h * p.tk_sh + n * p.tk_sn)[c];
+      v[i] = reinterpret_cast<const uint4*>(p.tv + b * p.tv_sb + h * p.tv_sh + n * p.tv_sn)[c];
     }
   }
   const uint32_t ks = smem_u32(s.tree[0]), vs = smem_u32(s.tree[1]);
@@ -465,7 +465,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tm_k,
     load_q(st, p, b, h, row0, lane);
     // Ancestor mask of node `lane`, by climbing: links go to lower indices, so 32 steps at most.
     const int32_t* parents = p.parents + b * p.parents_sb;
-    const int up = lane < p.N ? __ldg(parents + lane) : -2;
+    const int up = lane < p.N ? parents[lane] : -2;
     const int link = up < lane && up >= -1 ? up : -2;
     int at = lane;
     while (__any_sync(0xffffffffu, at >= 0)) {

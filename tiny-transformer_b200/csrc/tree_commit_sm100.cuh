@@ -42,8 +42,8 @@ __global__ void __launch_bounds__(THREADS) tree_commit_kernel(const __grid_const
   const int lk = static_cast<int>(blockIdx.x) / p.B;   // layer * 2 + (keys or values)
   const int kv = lk & 1, layer = lk >> 1;
   wait_for_previous_kernel();
-  const int len = __ldg(p.lens + b);
-  const int count = min(max(__ldg(p.counts + b), 0), p.P);
+  const int len = p.lens[b];
+  const int count = min(max(p.counts[b], 0), p.P);
   // Rows that fit: all of them unless the length is negative or the cache is full.
   const int room = (len < 0 || len > p.C) ? 0 : p.C - len;
   const int rows = min(count, room);
@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(THREADS) tree_commit_kernel(const __grid_const
   const int piece = threadIdx.x & 7;
   for (int i = threadIdx.x >> 3; i < rows * p.H; i += THREADS / 8) {
     const int h = i / rows, r = i - h * rows;
-    const int n = __ldg(p.path + static_cast<int64_t>(b) * p.P + r);
+    const int n = p.path[static_cast<int64_t>(b) * p.P + r];
     if (n < 0 || n >= p.N) {
       atomicOr(&g_tt_status, TT_ERR_RANGE);
       continue;

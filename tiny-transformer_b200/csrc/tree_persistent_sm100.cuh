@@ -211,7 +211,7 @@ struct Walk {
     prefetch(p);
   }
   __device__ __forceinline__ void prefetch(const Params& p) {
-    next_len = p.t.lens != nullptr && b + 1 < p.t.B ? __ldg(p.t.lens + b + 1) : p.t.C;
+    next_len = p.t.lens != nullptr && b + 1 < p.t.B ? p.t.lens[b + 1] : p.t.C;
   }
   __device__ __forceinline__ void next(const Params& p) {
     left -= n;

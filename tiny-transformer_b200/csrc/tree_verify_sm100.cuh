@@ -174,7 +174,7 @@ __device__ __forceinline__ void load_lane(const float* row, int v0, int lane, in
                                           float (&x)[LANE_TOKENS]) {
   if (VEC) {
     const int v = v0 + lane * 4;
-    const float4 y = v < V ? __ldg(reinterpret_cast<const float4*>(row + v))
+    const float4 y = v < V ? *reinterpret_cast<const float4*>(row + v)
                            : make_float4(0.f, 0.f, 0.f, 0.f);
     x[0] = y.x;
     x[1] = y.y;
@@ -184,7 +184,7 @@ __device__ __forceinline__ void load_lane(const float* row, int v0, int lane, in
 #pragma unroll
     for (int j = 0; j < LANE_TOKENS; ++j) {
       const int v = v0 + j * 32 + lane;
-      x[j] = v < V ? __ldg(row + v) : 0.f;
+      x[j] = v < V ? row[v] : 0.f;
     }
   }
 }
@@ -313,17 +313,17 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) tree_verify_kernel(const Param
   wait_for_previous_kernel();
   // The tree, the random numbers, and p(t), q(t) of every node at its parent.
   for (int n = threadIdx.x; n < N; n += blockDim.x) {
-    const int up = __ldg(a.parents + b * a.parents_sb + n);
-    const int64_t t = __ldg(reinterpret_cast<const long long*>(a.tokens) + static_cast<int64_t>(b) * N + n);
+    const int up = a.parents[b * a.parents_sb + n];
+    const int64_t t = a.tokens[static_cast<int64_t>(b) * N + n];
     const bool child = up >= 0 && up < n;
     const bool known = t >= 0 && t < a.V;
     s.parent[n] = child ? up : (up == -1 ? -1 : -2);
     s.token[n] = known ? static_cast<int32_t>(t) : -1;
-    s.u[n] = __ldg(a.u + static_cast<int64_t>(b) * N + n);
+    s.u[n] = a.u[static_cast<int64_t>(b) * N + n];
     float pt = 0.f, qt = 0.f;
     if (child && known) {
-      pt = clamp_prob(__ldg(a.p + b * a.p_sb + up * a.p_sn + t));
-      qt = DENSE ? clamp_prob(__ldg(a.q + b * a.q_sb + up * a.q_sn + t)) : 1.f;
+      pt = clamp_prob(a.p[b * a.p_sb + up * a.p_sn + t]);
+      qt = DENSE ? clamp_prob(a.q[b * a.q_sb + up * a.q_sn + t]) : 1.f;
     } else if (!DENSE) {
       qt = 1.f;
     }
