@@ -270,7 +270,8 @@ TT_ATTN_API tt_attn_status tt_attn_decode_bf16_noalloc(
  *   workspace  tt_attn_tree_workspace_size() bytes, 16-byte aligned (may be NULL when that is 0)
  *
  * Nodes not in use get O = 0, LSE = -inf. What a node does not see does not change its output,
- * whatever it holds (NaN and infinities included). 1 <= nodes <= TT_ATTN_TREE_MAX_NODES. Layout
+ * whatever it holds (NaN and infinities included); an infinity in a cached V row that is seen makes
+ * that feature of the output infinite or NaN. 1 <= nodes <= TT_ATTN_TREE_MAX_NODES. Layout
  * rules of q and all K/V tensors as for tt_attn_forward_bf16 (TT_ATTN_UNSUPPORTED otherwise).
  */
 TT_ATTN_API tt_attn_status tt_attn_tree_forward_bf16(

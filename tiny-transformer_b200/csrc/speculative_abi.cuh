@@ -65,8 +65,10 @@ bool tree_shape_ok(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nod
          q_heads % kv_heads == 0 && nodes <= TT_ATTN_TREE_MAX_NODES &&
          capacity <= INT32_MAX - tt::tree::KEYS && batch <= max_rows && q_heads <= max_rows &&
          batch <= max_rows / q_heads &&
-         // key tiles of all (batch, q head, 128-row tile): the persistent kernel counts them in 32 bits
-         (capacity / tt::tree::KEYS + 4) * 2 <= INT32_MAX / (batch * q_heads);
+         // cost (key tiles and the fixed part) of all (batch, q head, 128-row tile): the persistent
+         // kernel counts it in 32 bits
+         (capacity / tt::tree::KEYS + 1 + TT_ATTN_TREE_MAX_NODES / tt::tree::KEYS +
+          tt::tree::persist::UNIT_COST) * 2 <= INT32_MAX / (batch * q_heads);
 }
 
 tt_attn_status set_tree_attributes(int dev) {
@@ -358,7 +360,7 @@ TT_ATTN_API tt_attn_status tt_attn_tree_commit_bf16(
   if (layers <= 0 || batch <= 0 || kv_heads <= 0 || nodes <= 0 || capacity <= 0 || path_len <= 0)
     return fail(TT_ATTN_BAD_ARG, "tree_commit: sizes must be positive");
   if (batch > INT32_MAX / (2 * cm::MAX_LAYERS) || nodes > INT32_MAX || capacity > INT32_MAX ||
-      path_len > INT32_MAX / kv_heads || new_lens == cache_lens)
+      path_len > (INT32_MAX - cm::THREADS) / kv_heads || new_lens == cache_lens)
     return fail(TT_ATTN_BAD_ARG, new_lens == cache_lens
                                      ? "tree_commit: new_lens needs a buffer of its own"
                                      : "tree_commit: shape exceeds the supported CUDA grid limits");

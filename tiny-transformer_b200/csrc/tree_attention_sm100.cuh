@@ -134,7 +134,7 @@ __device__ __forceinline__ int valid_len(const int32_t* lens, int C, int b) {
 // and without, jump[n]; a round ORs in the mask at jump[n] and jumps as far as that does, so a
 // chain of any length takes log2(length) rounds. Links go to strictly lower indices (any other
 // link ends the chain as unused, jump -2), so rounds go over blocks of `threads` nodes from the
-// highest down, each reading before it writes, and never meet a node already updated this round.
+// highest down, each reading before it writes, and never meet a node that its round has updated.
 // `sync` is a barrier of the `threads` threads that all call this; it returns whether any of them
 // passed true.
 template <typename Sync>
@@ -556,6 +556,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tm_k,
     if (task) write_out(p, out0 + r, c8, n, M, den, (used >> ((row0 + r) % p.N)) & 1u);
     return;
   }
+  __syncwarp();  // .aligned barriers take whole warps
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   const int each = (ROWS + p.splits - 1) / p.splits;  // rows a rank owns
   if (task) {
@@ -567,6 +568,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tm_k,
                   __float_as_uint(n[6]), __float_as_uint(n[7]));
     if (c8 == 0) st_cluster_f32x2(dst + HD * 4, M, den);
   }
+  __syncwarp();
   cluster_sync();
   // The cluster's CTAs, for this rank's rows. Nothing is written to another CTA any more.
   const int own = r * p.splits + rank;

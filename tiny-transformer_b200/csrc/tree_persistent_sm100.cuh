@@ -44,7 +44,6 @@
 #include <cstdint>
 #include <type_traits>
 
-#include "prefill_sm100.cuh"
 #include "sm100_ptx.cuh"
 #include "tree_attention_sm100.cuh"
 
@@ -735,7 +734,10 @@ __device__ __forceinline__ void q_role(Smem& s, const Params& p, int lane) {
     if (w.seg == 1 && !warp_wait(&s.abort, &s.q_full[0], 0)) break;
     if (w.seg >= 2 && !warp_wait(&s.abort, &s.q_free[qb], ((w.seg >> 1) + 1) & 1)) break;
     load_unit<DUP>(s, p, w, qb, lane, 32, built[qb],
-                   [](bool any) { return __any_sync(0xffffffffu, any) != 0; });
+                   [](bool any) {
+                     __syncwarp();  // a vote alone orders no memory
+                     return __any_sync(0xffffffffu, any) != 0;
+                   });
     __syncwarp();
     if (lane == 0) mbar_arrive(&s.q_full[qb]);
   }

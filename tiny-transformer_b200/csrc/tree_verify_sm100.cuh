@@ -295,6 +295,7 @@ __device__ __forceinline__ unsigned long long sum_pass(Smem& s, const Params& a,
       st_cluster_u64(map_to_rank(smem_u32(&s.share[par][rank]), lane), total);
     }
   }
+  __syncwarp();  // cluster barriers take whole warps
   if (a.cluster == 1) __syncthreads();
   else cluster_sync();
   total = 0;
@@ -331,6 +332,7 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) tree_verify_kernel(const Param
     s.qt[n] = qt;
   }
   // Also: no CTA writes another's shared memory before that CTA has started.
+  __syncwarp();
   if (a.cluster == 1) __syncthreads();
   else cluster_sync();
 
