@@ -143,3 +143,39 @@ def test_speculation_on_the_gpu(temperature, branching):
     _, stats = generate_speculative(model, model, prompt, 24, (1, 1, 1), temperature,
                                     torch.Generator("cuda").manual_seed(3))
     assert stats["accepted"] > 2.5
+
+
+@pytest.mark.parametrize("time,new_tokens,branching", [(5, 10, (1, 1, 1)), (1, 5, (1,)), (6, 7, (2, 2))])
+def test_finished_sequences_stay_inside_the_position_tables_cpu(time, new_tokens, branching):
+    """Sequence 0 accepts a whole branch at every step, the others nothing, so it stands finished for
+    many steps; ``max_seq_len`` is the least that is accepted. No node is ever past the tables, and
+    the tokens are those of the same models with long tables."""
+    tree, starts = TokenTree(branching), []
+    branch = oracle.chains(tree.parents.tolist())[-1][::-1]
+
+    def verify_tree(tokens, parents, p, u, q=None):
+        batch = len(tokens)
+        path = torch.full(tokens.shape, -1, dtype=torch.int32)
+        path[:, 0] = 0
+        path[0, :len(branch)] = torch.tensor(branch, dtype=torch.int32)
+        counts = torch.ones(batch, dtype=torch.int32)
+        counts[0] = len(branch)
+        return path, counts, (tokens.sum(1) * 7 + 3) % SMALL.vocab_size
+
+    def run(max_seq_len):
+        config = DecoderConfig(vocab_size=96, dim=128, n_layers=1, n_heads=2, hidden_dim=128,
+                               max_seq_len=max_seq_len)
+        ops = _cpu_ops()
+        attention = ops.tree_attention
+        ops.tree_attention = lambda *a: (starts.append(int(a[-1].max())), attention(*a))[1]
+        ops.verify_tree = verify_tree
+        return generate_speculative(_model(3, config=config), _model(4, config=config),
+                                    _prompt(3, time), new_tokens, branching, 1.0,
+                                    torch.Generator().manual_seed(2), ops)[0]
+
+    limit = time + new_tokens + len(branching)
+    want = run(128)
+    assert max(starts) + tree.depth < limit
+    assert torch.equal(run(limit), want)
+    with pytest.raises(ValueError, match="max_seq_len"):
+        run(limit - 1)

@@ -59,8 +59,8 @@ def allocate(model: Decoder, cache: KVCache):
 def forward_tree(model: Decoder, ids, tree_parents, depths, cache: KVCache, lens, ops=None):
     """One pass of ``model`` over the drafted tokens ``ids`` ``[B, N]``: logits ``[B, N, V]`` and the
     nodes' K and V rows of every layer, ``[B, H, N, 64]`` each. Node n of sequence b is at position
-    ``lens[b] + depths[n]`` and sees cache rows ``[0, lens[b])`` and its own branch; the cache is not
-    changed."""
+    ``lens[b] + depths[n]``, which has to stay below ``max_seq_len``, and sees cache rows
+    ``[0, lens[b])`` and its own branch; the cache is not changed."""
     ops = ops or _ops()
     cfg = model.config
     batch, nodes = ids.shape
@@ -146,9 +146,9 @@ def generate_speculative(model: Decoder, draft: Decoder, prompt, new_tokens: int
     # The last token of the prompt is the first root: it is in no cache yet.
     lens = torch.full((batch,), time - 1, dtype=torch.int32, device=device)
     root = prompt[:, -1]
-    # One step yields up to depth + 1 tokens past the last needed one.
-    out = torch.zeros(batch, new_tokens + tree.depth + 1, dtype=torch.long, device=device)
-    have = torch.zeros(batch, dtype=torch.long, device=device)
+    # The last column takes what is not kept.
+    out = torch.zeros(batch, new_tokens + 1, dtype=torch.long, device=device)
+    have = torch.zeros(batch, dtype=torch.int32, device=device)
     column = torch.arange(tree.size, device=device)
     steps, yielded = 0, 0
     while True:
@@ -157,18 +157,20 @@ def generate_speculative(model: Decoder, draft: Decoder, prompt, new_tokens: int
         uniforms = torch.rand(batch, tree.size, device=device, generator=generator)
         path, counts, nxt = ops.verify_tree(tokens, tree.parents, _probabilities(logits, temperature),
                                             uniforms, q)
-        counts = torch.where(have >= new_tokens, 0, counts)      # finished sequences stand still
-        ops.commit_path(caches[1].keys, caches[1].values, dk, dv, path, counts, lens)
-        lens = ops.commit_path(caches[0].keys, caches[0].values, tk, tv, path, counts, lens)
+        # Not past the last token that is asked for: a finished sequence stands still while the others
+        # go on, with its length at most time - 1 + new_tokens and its nodes inside the tables.
+        kept = torch.minimum(counts, new_tokens - have)
+        ops.commit_path(caches[1].keys, caches[1].values, dk, dv, path, kept, lens)
+        lens = ops.commit_path(caches[0].keys, caches[0].values, tk, tv, path, kept, lens)
         # The accepted tokens after the root, then the drawn one: counts of them.
         step = tokens.gather(1, path.clamp(min=0).long()).roll(-1, dims=1)
         step = torch.where(column[None] == counts[:, None].long() - 1, nxt[:, None], step)
-        at = torch.where(column[None] < counts[:, None], have[:, None] + column[None], out.shape[1] - 1)
+        at = torch.where(column[None] < kept[:, None], have[:, None] + column[None], new_tokens)
         out.scatter_(1, at, step)
-        have = have + counts
-        root = torch.where(counts > 0, nxt, root)
+        have = have + kept
+        root = torch.where(kept > 0, nxt, root)
         steps += 1
-        done = int(have.clamp(max=new_tokens).sum())
+        done = int(have.sum())
         yielded = done
         if done == batch * new_tokens:
             break
