@@ -179,3 +179,48 @@ def test_finished_sequences_stay_inside_the_position_tables_cpu(time, new_tokens
     assert torch.equal(run(limit), want)
     with pytest.raises(ValueError, match="max_seq_len"):
         run(limit - 1)
+
+
+def _without_finite_logits(config=SMALL):
+    model = _model(3, config=config)
+    with torch.no_grad():
+        model.blocks[0].qkv.fill_(float("nan"))
+    return model
+
+
+def test_a_target_without_probabilities_raises_cpu():
+    """All logits of the target are NaN: the walk draws no token (-1), and none may become a root."""
+    with pytest.raises(RuntimeError, match="no token"):
+        generate_speculative(_without_finite_logits(), _model(4), _prompt(2, 5), 6, (2, 1), 1.0,
+                             torch.Generator().manual_seed(1), _cpu_ops())
+
+
+@pytest.mark.parametrize("finished", [True, False])
+def test_no_token_drawn_matters_to_running_sequences_only_cpu(finished):
+    """Sequence 0 draws no token at the second step. That ends the call unless it needs none: it has
+    finished before, or the accepted tokens are all that were asked for."""
+    calls = []
+
+    def verify_tree(tokens, parents, p, u, q=None):
+        calls.append(None)
+        batch, nodes = tokens.shape
+        path = torch.arange(nodes, dtype=torch.int32).repeat(batch, 1)
+        counts = torch.ones(batch, dtype=torch.int32)
+        counts[0] = nodes
+        nxt = torch.full((batch,), 5)
+        if len(calls) >= 2:
+            nxt[0] = -1
+        return path, counts, nxt
+
+    ops = _cpu_ops()
+    ops.verify_tree = verify_tree
+    # A chain of 3: sequence 0 has 4 tokens after a step, 8 after two.
+    args = (_model(3), _model(4), _prompt(2, 5), 7 if finished else 8, (1, 1, 1), 1.0,
+            torch.Generator().manual_seed(1), ops)
+    if finished:
+        out, _ = generate_speculative(*args)
+        assert ((out >= 0) & (out < SMALL.vocab_size)).all() and len(calls) == 7
+    else:
+        with pytest.raises(RuntimeError, match="no token"):
+            generate_speculative(*args)
+        assert len(calls) == 2

@@ -121,8 +121,9 @@ def generate_speculative(model: Decoder, draft: Decoder, prompt, new_tokens: int
 
     ``branching`` is the tree's shape (children per node at each depth). Returns ``(tokens
     [B, new_tokens], stats)``; ``stats["steps"]`` target passes and ``stats["accepted"]`` the mean
-    number of tokens a pass yielded. ``ops`` replaces the operators (a test runs the host logic on
-    CPU with it).
+    number of tokens a pass yielded. Raises RuntimeError where the target's logits are not finite and
+    no token can be drawn from them. ``ops`` replaces the operators (a test runs the host logic on CPU
+    with it).
     """
     if new_tokens <= 0:
         raise ValueError("new_tokens must be positive")
@@ -168,9 +169,14 @@ def generate_speculative(model: Decoder, draft: Decoder, prompt, new_tokens: int
         at = torch.where(column[None] < kept[:, None], have[:, None] + column[None], new_tokens)
         out.scatter_(1, at, step)
         have = have + kept
-        root = torch.where(kept > 0, nxt, root)
+        # The drawn token of a path kept whole is output, and the next root: -1 (the target's row has no
+        # weight, so its logits are not finite) must not reach the embedding.
+        whole = kept == counts
+        root = torch.where(whole, nxt, root)
         steps += 1
-        done = int(have.sum())
+        done, undrawn = torch.stack([have.sum(), (whole & (nxt < 0)).sum()]).tolist()
+        if undrawn:
+            raise RuntimeError("no token can be drawn: the target's logits are not finite")
         yielded = done
         if done == batch * new_tokens:
             break
