@@ -224,3 +224,16 @@ def test_no_token_drawn_matters_to_running_sequences_only_cpu(finished):
         with pytest.raises(RuntimeError, match="no token"):
             generate_speculative(*args)
         assert len(calls) == 2
+
+
+def test_a_draft_without_probabilities_proposes_uniformly_cpu():
+    """All logits of the draft are NaN: its tokens are drawn uniformly, which is what the walk is told,
+    so the call goes on with the target's own tokens."""
+    seen, ops = [], _cpu_ops()
+    verify = ops.verify_tree
+    ops.verify_tree = lambda *a: (seen.append(a[-1].clone()), verify(*a))[1]
+    out, stats = generate_speculative(_model(3), _without_finite_logits(), _prompt(2, 5), 6, (2, 1), 1.0,
+                                      torch.Generator().manual_seed(1), ops)
+    assert ((out >= 0) & (out < SMALL.vocab_size)).all() and 1 <= stats["accepted"] <= 3
+    inner = TokenTree((2, 1)).levels[-1][0]   # nodes with children
+    assert all(torch.equal(q[:, :inner], torch.full_like(q[:, :inner], 1 / SMALL.vocab_size)) for q in seen)

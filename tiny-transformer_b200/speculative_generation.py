@@ -105,7 +105,9 @@ def propose(draft: Decoder, root, tree: TokenTree, cache: KVCache, lens, tempera
         if temperature == 0:
             children = level.topk(k, dim=-1).indices
         else:
-            rows = _probabilities(level, temperature)
+            # Any distribution may propose as long as the walk is told which: a row without one (logits
+            # that are not finite; sampling from it would be a device-side assertion) becomes uniform.
+            rows = _probabilities(level, temperature).nan_to_num_(nan=1 / vocab)
             q[:, first:last] = rows
             children = torch.multinomial(rows.flatten(0, 1), k, replacement=True, generator=generator)
         tokens[:, nxt:end] = children.reshape(batch, end - nxt)
