@@ -645,3 +645,23 @@ def test_back_to_back_calls_see_each_other(spec, N):
     for _ in range(5):
         for a, b in zip(chain(False), want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dense", [True, False])
+@pytest.mark.parametrize("B,V", [(1, 1 << 22), (99, 920001), (150, 460001)])
+def test_verify_largest_shares_of_the_vocabulary(spec, B, V, dense):
+    """The most windows a CTA takes: the largest vocabulary, and large ones on as few CTAs a sequence as
+    the batch leaves (2 and 1). One row of probabilities for the whole batch, other draws."""
+    rs = np.random.RandomState(V % 1000)
+    gen = torch.Generator().manual_seed(V)
+    logits = torch.randn(1, 2, V, generator=gen) * 2
+    p = torch.softmax(logits, -1)
+    q = torch.softmax(logits + torch.randn(1, 2, V, generator=gen), -1)
+    w = q[0, 0].double().numpy()
+    tokens = np.zeros((B, 2), np.int64)
+    tokens[:, 1] = rs.choice(V, B, p=w / w.sum())
+    u = torch.rand(B, 2, generator=gen)
+    want = _same_walk(spec, tokens, np.tile(np.array([[-1, 0]], np.int32), (B, 1)), p.expand(B, 2, V), u,
+                      q.expand(B, 2, V) if dense else None,
+                      lambda x: x[:1].cuda().expand(B, 2, V))
+    assert (want[2] >= 0).all()

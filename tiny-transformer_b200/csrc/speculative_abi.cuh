@@ -71,7 +71,8 @@ bool tree_shape_ok(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nod
           tt::tree::persist::UNIT_COST) * 2 <= INT32_MAX / (batch * q_heads);
 }
 
-tt_attn_status set_tree_attributes(int dev) {
+// Shared memory beyond the default 48 KiB, for the kernels that may ask for it.
+tt_attn_status set_speculative_attributes(int dev) {
   static std::atomic<bool> done[kMaxDevices] = {};
   cudaError_t e = cudaSuccess;
   if (!done[dev].load(std::memory_order_acquire)) {
@@ -85,6 +86,13 @@ tt_attn_status set_tree_attributes(int dev) {
       if (e == cudaSuccess)
         e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  static_cast<int>(tt::tree::persist::kSmemBytes));
+    for (auto fn : {tt::verify::tree_verify_kernel<false, false>,
+                    tt::verify::tree_verify_kernel<false, true>,
+                    tt::verify::tree_verify_kernel<true, false>,
+                    tt::verify::tree_verify_kernel<true, true>})
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(tt::verify::kMaxDynamicSmem));
     if (e == cudaSuccess) done[dev].store(true, std::memory_order_release);
   }
   if (e != cudaSuccess)
@@ -215,7 +223,7 @@ TT_ATTN_API tt_attn_status tt_attn_tree_forward_bf16(
   int dev = 0, sm_count = 0;
   tt_attn_status st = prepare_device(&dev, &sm_count);
   if (st != TT_ATTN_OK) return st;
-  if ((st = set_tree_attributes(dev)) != TT_ATTN_OK) return st;
+  if ((st = set_speculative_attributes(dev)) != TT_ATTN_OK) return st;
   const int64_t group = q_heads / kv_heads;
   const TreePlan pl = tree_plan(batch, q_heads, kv_heads, nodes, capacity);
   CUtensorMap tmk, tmv, tmtk, tmtv;
@@ -296,8 +304,9 @@ TT_ATTN_API tt_attn_status tt_attn_tree_verify_f32(
     if (reinterpret_cast<uintptr_t>(ptr) % 8 != 0)
       return fail(TT_ATTN_BAD_ARG, "tree_verify: tokens and next_tokens must be 8-byte aligned");
   int dev = 0;
-  const tt_attn_status st = prepare_device(&dev);
+  tt_attn_status st = prepare_device(&dev);
   if (st != TT_ATTN_OK) return st;
+  if ((st = set_speculative_attributes(dev)) != TT_ATTN_OK) return st;
   vf::Params p{};
   p.tokens = tokens;
   p.parents = parents;
@@ -329,7 +338,7 @@ TT_ATTN_API tt_attn_status tt_attn_tree_verify_f32(
   if (draft_probs != nullptr)
     vec = vec && dp_sb % 4 == 0 && dp_sn % 4 == 0 && aligned16(draft_probs);
   const Launch launch(dim3(static_cast<unsigned>(batch * p.cluster)), threads,
-                      static_cast<size_t>(p.windows) * 8, p.cluster,
+                      p.windows * sizeof(unsigned long long), p.cluster,
                       static_cast<cudaStream_t>(stream));
   cudaError_t le;
   if (draft_probs != nullptr)

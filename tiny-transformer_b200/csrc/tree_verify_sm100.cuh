@@ -86,6 +86,10 @@ struct Smem {
 };
 
 extern __shared__ unsigned long long window_sums[];
+// Beside Smem more than the default 48 KiB (from 3569 windows a CTA on): the host opts in. Two CTAs
+// per SM in any case, each with the 1 KiB that the system takes.
+constexpr size_t kMaxDynamicSmem = MAX_WINDOWS * sizeof(unsigned long long);
+static_assert(2 * (sizeof(Smem) + kMaxDynamicSmem + 1024) <= 228 * 1024, "two CTAs per SM");
 
 __device__ __forceinline__ float clamp_prob(float x) { return __saturatef(x); }
 
