@@ -201,3 +201,20 @@ def test_oracle_walk_follows_the_target_distribution():
     first = np.where(counts > 1, np.take_along_axis(tokens, np.maximum(path[:, 1:2], 0), 1)[:, 0], nxt)
     seen = np.bincount(first, minlength=V)
     assert ((seen - p * B) ** 2 / (p * B)).sum() < 35
+
+
+def test_every_cuda_failure_is_reported_by_the_helper_that_clears_it():
+    """A failed launch leaves its error pending in the runtime; a return that does not read it makes the
+    next call report it as its own."""
+    import os
+    import re
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                        "tiny-transformer_b200", "csrc")
+    abi = open(os.path.join(csrc, "tt_attention_abi.cu")).read()
+    text = abi + open(os.path.join(csrc, "speculative_abi.cuh")).read()
+    helper = re.search(r"tt_attn_status cuda_fail\(.*?\n}\n", abi, re.S).group(0)
+    assert "cudaGetLastError()" in helper and "cudaGetErrorString" in helper
+    assert text.count("cudaGetErrorString") == 1
+    # What a launch call returns goes to the check that reads the pending error too.
+    launches = re.findall(r"cudaLaunchKernelEx\(", text)
+    assert len(launches) > 0 and len(re.findall(r"check_launch\(\"[^\"]+\", le\)", text)) == 6

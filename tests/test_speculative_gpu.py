@@ -665,3 +665,74 @@ def test_verify_largest_shares_of_the_vocabulary(spec, B, V, dense):
                       q.expand(B, 2, V) if dense else None,
                       lambda x: x[:1].cuda().expand(B, 2, V))
     assert (want[2] >= 0).all()
+
+
+# ------------------------------------------------------------------------------ errors of launches
+
+class _LegacyStreamClosed:
+    """While a blocking stream is being captured, a launch into the legacy stream is refused by the
+    driver (and ends the capture as invalid): a launch failure that nothing of it reaches the GPU."""
+
+    def __enter__(self):
+        import ctypes
+        self.cuda, self.stream = ctypes.CDLL("libcuda.so.1"), ctypes.c_void_p()
+        assert self.cuda.cuStreamCreate(ctypes.byref(self.stream), 0) == 0
+        assert self.cuda.cuStreamBeginCapture_v2(self.stream, 0) == 0
+
+    def __exit__(self, *_):
+        import ctypes
+        graph = ctypes.c_void_p()
+        self.cuda.cuStreamEndCapture(self.stream, ctypes.byref(graph))
+        assert not graph.value
+        assert self.cuda.cuStreamDestroy_v2(self.stream) == 0
+
+
+@pytest.mark.parametrize("failing", ["tree", "large tree", "verify", "commit", "decode"])
+def test_a_failed_launch_is_reported_once(failing):
+    """By the call that failed, and not again by the next one."""
+    import ctypes
+    from tiny_transformer_b200.operators._extension import load_c_abi
+    lib = load_c_abi()
+    B, H, C, V = 1, 1, 64, 10
+    make = lambda n: torch.zeros(B, H, n, 64, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    cache, rows, out, query = make(C), make(40), make(40), make(1)
+    ints = torch.zeros(2, 40, dtype=torch.int32, device="cuda")
+    parents = torch.arange(-1, 39, dtype=torch.int32, device="cuda")
+    tokens, drawn = (torch.zeros(B, 40, dtype=torch.long, device="cuda") for _ in range(2))
+    probs = torch.full((B, 40, V), 1 / V, device="cuda")
+    u, lse = torch.zeros(B, 40, device="cuda"), torch.zeros(B, H, 40, device="cuda")
+    work = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+    s = lambda x: (ctypes.c_int64 * 4)(*x.stride())  # noqa: E731
+    one = lambda x: (ctypes.c_void_p * 1)(x.data_ptr())  # noqa: E731
+    assert lib.tt_attn_tree_workspace_size(B, H, H, 40, C) <= work.numel()
+
+    def tree(nodes):
+        return lib.tt_attn_tree_forward_bf16(
+            rows.data_ptr(), s(rows), rows.data_ptr(), s(rows), rows.data_ptr(), s(rows),
+            cache.data_ptr(), s(cache), cache.data_ptr(), s(cache), B, H, H, nodes, C, 64,
+            parents.data_ptr(), 0, None, out.data_ptr(), None, work.data_ptr(), work.numel(), None)
+
+    calls = {
+        "tree": lambda: tree(4),
+        "large tree": lambda: tree(40),
+        "verify": lambda: lib.tt_attn_tree_verify_f32(
+            tokens.data_ptr(), parents.data_ptr(), 0, probs.data_ptr(), 40 * V, V, None, 0, 0,
+            u.data_ptr(), B, 40, V, ints.data_ptr(), ints[1].data_ptr(), drawn.data_ptr(), None),
+        "commit": lambda: lib.tt_attn_tree_commit_bf16(
+            one(cache), s(cache), one(cache), s(cache), one(rows), s(rows), one(rows), s(rows), 1, B,
+            H, 40, C, 64, ints.data_ptr(), 40, ints[1].data_ptr(), ints[1, 1:].data_ptr(),
+            ints[1, 2:].data_ptr(), None),
+        "decode": lambda: lib.tt_attn_forward_bf16(
+            query.data_ptr(), s(query), cache.data_ptr(), s(cache), cache.data_ptr(), s(cache), B, H, 1,
+            C, 64, C - 1, None, out.data_ptr(), lse.data_ptr(), None, 0, None),
+    }
+    assert lib.tt_attn_forward_workspace_size(B, H, 1, C) == 0
+    for name, call in calls.items():
+        assert call() == 0, (name, lib.tt_attn_last_error())
+    torch.cuda.synchronize()
+    with _LegacyStreamClosed():
+        status = calls[failing]()
+    assert status != 0 and "launch" in lib.tt_attn_last_error().decode()
+    for name, call in calls.items():
+        assert call() == 0, (name, lib.tt_attn_last_error())
+    torch.cuda.synchronize()

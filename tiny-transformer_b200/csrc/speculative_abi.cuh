@@ -96,7 +96,7 @@ tt_attn_status set_speculative_attributes(int dev) {
     if (e == cudaSuccess) done[dev].store(true, std::memory_order_release);
   }
   if (e != cudaSuccess)
-    return fail(TT_ATTN_LAUNCH_FAIL, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
+    return cuda_fail("cudaFuncSetAttribute", e);
   return TT_ATTN_OK;
 }
 
@@ -149,10 +149,7 @@ tt_attn_status launch_tree_persistent(const TreePlan& pl, const tt::tree::Params
                        ps::COMBINE_THREADS, 0, 1, stream);
     le = cudaLaunchKernelEx(&merge.cfg, ps::tree_combine_kernel, p, grid);
   }
-  if (le != cudaSuccess)
-    return fail(TT_ATTN_LAUNCH_FAIL,
-                std::string("tree_persistent_kernel launch: ") + cudaGetErrorString(le));
-  return check_launch("tree_persistent_kernel launch");
+  return check_launch("tree_persistent_kernel launch", le);
 }
 
 // [batch, heads, rows, 64] operand of the speculative operators: readable in place?
@@ -268,10 +265,7 @@ TT_ATTN_API tt_attn_status tt_attn_tree_forward_bf16(
   const cudaError_t le =
       multi ? cudaLaunchKernelEx(&launch.cfg, tr::tree_attention_kernel<true>, tmk, tmv, p)
             : cudaLaunchKernelEx(&launch.cfg, tr::tree_attention_kernel<false>, tmk, tmv, p);
-  if (le != cudaSuccess)
-    return fail(TT_ATTN_LAUNCH_FAIL,
-                std::string("tree_attention_kernel launch: ") + cudaGetErrorString(le));
-  return check_launch("tree_attention_kernel launch");
+  return check_launch("tree_attention_kernel launch", le);
 }
 
 TT_ATTN_API tt_attn_status tt_attn_tree_verify_f32(
@@ -347,10 +341,7 @@ TT_ATTN_API tt_attn_status tt_attn_tree_verify_f32(
   else
     le = vec ? cudaLaunchKernelEx(&launch.cfg, vf::tree_verify_kernel<false, true>, p)
              : cudaLaunchKernelEx(&launch.cfg, vf::tree_verify_kernel<false, false>, p);
-  if (le != cudaSuccess)
-    return fail(TT_ATTN_LAUNCH_FAIL,
-                std::string("tree_verify_kernel launch: ") + cudaGetErrorString(le));
-  return check_launch("tree_verify_kernel launch");
+  return check_launch("tree_verify_kernel launch", le);
 }
 
 TT_ATTN_API tt_attn_status tt_attn_tree_commit_bf16(
@@ -417,10 +408,7 @@ TT_ATTN_API tt_attn_status tt_attn_tree_commit_bf16(
     const Launch launch(dim3(static_cast<unsigned>(batch * p.layers * 2)), cm::THREADS, 0, 1,
                         static_cast<cudaStream_t>(stream));
     const cudaError_t le = cudaLaunchKernelEx(&launch.cfg, cm::tree_commit_kernel, p);
-    if (le != cudaSuccess)
-      return fail(TT_ATTN_LAUNCH_FAIL,
-                  std::string("tree_commit_kernel launch: ") + cudaGetErrorString(le));
-    if ((st = check_launch("tree_commit_kernel launch")) != TT_ATTN_OK) return st;
+    if ((st = check_launch("tree_commit_kernel launch", le)) != TT_ATTN_OK) return st;
   }
   return TT_ATTN_OK;
 }

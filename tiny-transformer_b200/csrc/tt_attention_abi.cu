@@ -44,6 +44,13 @@ tt_attn_status fail(tt_attn_status st, const std::string& msg) {
   return st;
 }
 
+// Report of a failed CUDA call. The runtime keeps the error of a failed launch until it is read: it is
+// read here, or the next call's check_launch would take it for its own.
+tt_attn_status cuda_fail(const char* what, cudaError_t e) {
+  (void)cudaGetLastError();
+  return fail(TT_ATTN_LAUNCH_FAIL, std::string(what) + ": " + cudaGetErrorString(e));
+}
+
 // ------------------------------------------------------------------ shape helpers
 struct Shape4 {
   int64_t size[4];
@@ -444,13 +451,13 @@ std::mutex g_dev_mu;
 tt_attn_status prepare_device(int* dev_out, int* sm_count = nullptr) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return fail(TT_ATTN_LAUNCH_FAIL, std::string("cudaGetDevice: ") + cudaGetErrorString(e));
+  if (e != cudaSuccess) return cuda_fail("cudaGetDevice", e);
   if (dev < 0 || dev >= kMaxDevices) return fail(TT_ATTN_UNSUPPORTED, "device index out of range");
   // Make the device's primary context current on this thread: a thread that has made no
   // runtime call yet (e.g. an autograd worker) has none, and the driver-API tensor-map
   // encoding that follows needs one.
   e = cudaSetDevice(dev);
-  if (e != cudaSuccess) return fail(TT_ATTN_LAUNCH_FAIL, std::string("cudaSetDevice: ") + cudaGetErrorString(e));
+  if (e != cudaSuccess) return cuda_fail("cudaSetDevice", e);
   *dev_out = dev;
   std::lock_guard<std::mutex> lock(g_dev_mu);
   DeviceState& ds = g_dev[dev];
@@ -459,11 +466,11 @@ tt_attn_status prepare_device(int* dev_out, int* sm_count = nullptr) {
     e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
     if (e != cudaSuccess)
-      return fail(TT_ATTN_LAUNCH_FAIL, std::string("cudaDeviceGetAttribute: ") + cudaGetErrorString(e));
+      return cuda_fail("cudaDeviceGetAttribute", e);
     ds.supported = (major == 10);
     e = cudaDeviceGetAttribute(&ds.sm_count, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess)
-      return fail(TT_ATTN_LAUNCH_FAIL, std::string("cudaDeviceGetAttribute: ") + cudaGetErrorString(e));
+      return cuda_fail("cudaDeviceGetAttribute", e);
     ds.checked = true;
     if (!ds.supported) {
       char buf[160];
@@ -492,8 +499,7 @@ tt_attn_status prepare_device(int* dev_out, int* sm_count = nullptr) {
       cudaFuncAttributes fa{};
       e = cudaFuncGetAttributes(&fa, prefill_fn);
       if (e != cudaSuccess)
-        return fail(TT_ATTN_LAUNCH_FAIL,
-                    std::string("cudaFuncGetAttributes: ") + cudaGetErrorString(e));
+        return cuda_fail("cudaFuncGetAttributes", e);
       if (fa.numRegs != static_cast<int>(launch_regs)) {
         char buf[160];
         std::snprintf(buf, sizeof(buf),
@@ -528,18 +534,18 @@ tt_attn_status prepare_device(int* dev_out, int* sm_count = nullptr) {
                                cudaFuncAttributeMaxDynamicSharedMemorySize,
                                static_cast<int>(tt::backward_det::kSmemKV));
     if (e != cudaSuccess)
-      return fail(TT_ATTN_LAUNCH_FAIL, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
+      return cuda_fail("cudaFuncSetAttribute", e);
     ds.attrs_set = true;
   }
   if (sm_count) *sm_count = ds.sm_count;
   return TT_ATTN_OK;
 }
 
-tt_attn_status check_launch(const char* what) {
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess)
-    return fail(TT_ATTN_LAUNCH_FAIL, std::string(what) + ": " + cudaGetErrorString(e));
-  return TT_ATTN_OK;
+// `launched`: what a launch call returned (a <<<>>> launch returns nothing: its error is pending).
+tt_attn_status check_launch(const char* what, cudaError_t launched = cudaSuccess) {
+  const cudaError_t pending = cudaGetLastError();
+  const cudaError_t e = launched != cudaSuccess ? launched : pending;
+  return e == cudaSuccess ? TT_ATTN_OK : cuda_fail(what, e);
 }
 
 }  // namespace
@@ -593,10 +599,11 @@ TT_ATTN_API size_t tt_attn_forward_workspace_size(int64_t batch, int64_t heads, 
 
 TT_ATTN_API int tt_attn_device_supported(void) {
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
   int major = 0;
-  if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess) return 0;
-  return major == 10 ? 1 : 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  return e == cudaSuccess && major == 10 ? 1 : 0;
 }
 
 TT_ATTN_API tt_attn_status tt_attn_device_status(unsigned* flags, int clear) {
@@ -607,7 +614,7 @@ TT_ATTN_API tt_attn_status tt_attn_device_status(unsigned* flags, int clear) {
     const unsigned zero = 0;
     e = cudaMemcpyToSymbol(tt::g_tt_status, &zero, sizeof(unsigned));
   }
-  if (e != cudaSuccess) return fail(TT_ATTN_LAUNCH_FAIL, std::string("status read: ") + cudaGetErrorString(e));
+  if (e != cudaSuccess) return cuda_fail("status read", e);
   if (*flags & tt::TT_ERR_TIMEOUT) return TT_ATTN_TIMEOUT;
   return (*flags & tt::TT_ERR_RANGE) ? TT_ATTN_BAD_ARG : TT_ATTN_OK;
 }
@@ -733,9 +740,7 @@ TT_ATTN_API tt_attn_status tt_qkv_rope_append_bf16(
   p.m_tiles = static_cast<int>(pl.m_tiles);
   p.red_rows = pl.red_rows;
   const cudaError_t le = launch_qkv_rope(pl, tm_h, tm_w, p, static_cast<cudaStream_t>(stream));
-  if (le != cudaSuccess)
-    return fail(TT_ATTN_LAUNCH_FAIL, std::string("qkv_rope_append launch: ") + cudaGetErrorString(le));
-  return check_launch("qkv_rope_append launch");
+  return check_launch("qkv_rope_append launch", le);
 }
 
 // Backward workspace: -LSE * log2(e) and -D per query row, each [B, H, Tq_pad] FP32 with Tq
@@ -941,8 +946,7 @@ tt_attn_status backward_impl(
                                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                 static_cast<int>(tt::backward::persist::kSmemBytes));
     if (ae != cudaSuccess)
-      return fail(TT_ATTN_LAUNCH_FAIL,
-                  std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(ae));
+      return cuda_fail("cudaFuncSetAttribute", ae);
     tt::backward::persist::bwd_persistent_kernel<<<static_cast<unsigned>(grid),
                                                    tt::backward::persist::THREADS,
                                                    tt::backward::persist::kSmemBytes, cs>>>(
@@ -1123,10 +1127,7 @@ TT_ATTN_API tt_attn_status tt_attn_forward_bf16(
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     const cudaError_t le = cudaLaunchKernelEx(&cfg, dd::decode_direct_kernel, tmk, tmv, p);
-    if (le != cudaSuccess)
-      return fail(TT_ATTN_LAUNCH_FAIL,
-                  std::string("decode_direct_kernel launch: ") + cudaGetErrorString(le));
-    return check_launch("decode_direct_kernel launch");
+    return check_launch("decode_direct_kernel launch", le);
   }
   if (is_decode) {
     tt::decode::Params p{};
@@ -1161,8 +1162,7 @@ TT_ATTN_API tt_attn_status tt_attn_forward_bf16(
         n_chunks > 1 ? tt::decode::kCounterBytes + arrival_bytes : sizeof(unsigned);
     const cudaError_t me = cudaMemsetAsync(ws, 0, clear, cs);
     if (me != cudaSuccess)
-      return fail(TT_ATTN_LAUNCH_FAIL, std::string("cudaMemsetAsync(decode counters): ") +
-                                           cudaGetErrorString(me));
+      return cuda_fail("cudaMemsetAsync(decode counters)", me);
     // Persistent grid: one CTA per SM streams work items; no more CTAs than items.
     const int64_t ctas = std::min<int64_t>(sm_count, grid);
     tt::decode::decode_split_kernel<<<static_cast<unsigned>(ctas), tt::decode::THREADS,
@@ -1283,9 +1283,7 @@ TT_ATTN_API tt_attn_status tt_attn_decode_bf16_noalloc(
       void* ptr = nullptr;
       const cudaError_t se = cudaGetSymbolAddress(&ptr, g_noalloc_scratch);
       if (se != cudaSuccess || ptr == nullptr)
-        return fail(TT_ATTN_LAUNCH_FAIL,
-                    std::string("cudaGetSymbolAddress(no-allocation scratch): ") +
-                        cudaGetErrorString(se));
+        return cuda_fail("cudaGetSymbolAddress(no-allocation scratch)", se);
       slot.ptr = ptr;
       slot.ctx = static_cast<void*>(ctx);
     }
