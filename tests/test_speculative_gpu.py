@@ -736,3 +736,47 @@ def test_a_failed_launch_is_reported_once(failing):
     for name, call in calls.items():
         assert call() == 0, (name, lib.tt_attn_last_error())
     torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------------------ long caches, value by value
+
+def marked_values(rows):
+    """V rows of which each has one entry, 1, at a place that differs within every 64 rows and from one
+    64 rows to the next: a V row that is lost, doubled or out of its place moves weight between features.
+    No entry is negative, so A equals |ref| and the bound of the file is relative: 2^-7 + 2^-11."""
+    j = torch.arange(rows)
+    return torch.nn.functional.one_hot((j + 7 * (j // 64)) % 64, 64).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("Hq,Hkv,N,C,lens", [
+    (2, 2, 3, 9000, [8999, 4097]),      # the cluster kernel, cache shared by its CTAs
+    (3, 1, 8, 9000, [9000, 2500]),      # the same, two row tiles
+    (2, 2, 40, 9000, [8999, 4097]),     # the persistent kernel: two copies of Q
+    (1, 1, 33, 20001, [20001, 64]),     # one long unit shared by many CTAs
+    (3, 1, 37, 9000, [9000, 129]),      # 111 rows: one copy
+    (2, 1, 130, 6000, [5999, 3000]),    # 260 rows in three tiles, two key tiles of the tree
+])
+def test_every_value_of_a_long_cache_has_its_weight(spec, Hq, Hkv, N, C, lens):
+    B = len(lens)
+    t, parents, _ = _case(B, Hq, Hkv, N, C, 17 * N + C)
+    t["cache_v"] = marked_values(C).expand(B, Hkv, C, 64).contiguous()
+    t["tree_v"] = marked_values(N).expand(B, Hkv, N, 64).contiguous()
+    o, lse = _run(spec, t, parents, lens)
+    _check(o, lse, t, parents, lens)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("G,N", [(1, 12), (1, 30), (3, 16), (2, 64)])
+def test_a_leaf_that_is_not_finite_shows_in_its_own_row(spec, value, G, N):
+    """K and V of one leaf: every feature of that node's row, in every head, and no other row."""
+    lens = [130, 0]
+    t, parents, _ = _case(2, 2 * G, 2, N, 300, 11, fan=4)
+    want, want_lse = _run(spec, t, parents, lens)
+    leaf = [n for n in range(N) if n not in parents[0]][-1]
+    t["tree_k"][0, :, leaf] = value
+    t["tree_v"][0, :, leaf] = value
+    got, lse = _run(spec, t, parents, lens)
+    assert not torch.isfinite(got[0, :, leaf]).any() and not torch.isfinite(lse[0, :, leaf]).any()
+    others = [n for n in range(N) if n != leaf]
+    assert torch.equal(got[0][:, others], want[0][:, others]) and torch.equal(got[1], want[1])
+    assert torch.equal(lse[0][:, others], want_lse[0][:, others]) and torch.equal(lse[1], want_lse[1])
