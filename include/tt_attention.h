@@ -306,7 +306,8 @@ TT_ATTN_API size_t tt_attn_tree_workspace_size(int64_t batch, int64_t q_heads, i
  *                 has any weight)
  *
  * Weights are whole numbers (probabilities times 2^36, rounded down), so results do not depend on
- * the order of any sum; the exact definition is at the kernel. Probabilities are taken into
+ * the order of any sum; the exact definition is at the kernel. Uniforms that are 2^-24 apart, as FP32
+ * generators draw them, resolve the next token's probabilities to 2^-24. Probabilities are taken into
  * [0, 1], NaN as 0. 1 <= nodes <= TT_ATTN_TREE_MAX_NODES, vocab <= TT_ATTN_TREE_MAX_VOCAB.
  */
 TT_ATTN_API tt_attn_status tt_attn_tree_verify_f32(
@@ -329,7 +330,9 @@ TT_ATTN_API tt_attn_status tt_attn_tree_verify_f32(
  *                        of its own: the kernel's blocks read cache_lens while it is written
  *
  * Rows that do not fit the capacity and path entries outside [0, nodes) are skipped and set bit 1
- * of the device status (tt_attn_device_status). The caches must not overlap the trees.
+ * of the device status (tt_attn_device_status). The row of such a path entry is not written but
+ * counts in new_lens, as later rows of the path keep their places: after that status the rows
+ * appended to the sequence must not be used. The caches must not overlap the trees.
  */
 TT_ATTN_API tt_attn_status tt_attn_tree_commit_bf16(
     void* const* cache_k, const int64_t* ck_strides, void* const* cache_v,

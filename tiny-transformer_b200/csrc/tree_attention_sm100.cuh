@@ -19,17 +19,22 @@
 // (128-byte swizzle: 16-byte piece c of row r at piece c ^ (r % 8)); 4 consumer warps take 32 keys
 // of a tile each, so that K and V fragments are read from shared memory once. Scores and P.V are
 // mma.m16n8k16 on register fragments (Q stays in registers, P goes from the score fragments to the
-// second product's A operand without leaving them). The tree's keys are a step or two of rank 0's
+// second product's A operand without leaving them). P is rounded to BF16 for that product, the only
+// rounding below 32 bits before the output's: it is what the tensor cores take beside a BF16 V, and what
+// the framework's other attention kernels do. It adds up to 2^-8 of each weight; measured against 64
+// bits, the outputs' relative error is 0.0020-0.0023, of which 0.00165 is the output's own rounding. Sums
+// take P before it is rounded. The tree's keys are a step or two of rank 0's
 // first warp, 16 keys each, loaded with plain loads under the first tiles' flight. Every warp keeps its own online
 // softmax (m, l, O); the CTA merges its warps, every CTA pushes each row to the rank that owns it
-// (st.shared::cluster), and after one cluster barrier each rank merges and writes its rows. 70 KiB
+// (st.shared::cluster), and after one cluster barrier each rank merges and writes its rows. 75 KiB
 // of shared memory and 128 registers leave room for three CTAs per SM (192 KiB of loads in flight).
 // Larger trees, and more rows over long caches (which would be read once per 16 rows), take
 // tree_persistent_sm100.cuh.
 //
 // Measured (B200, 12 heads): 142 us, 6.42 TB/s, for 64 sequences of 1024-8192 cached rows and 16 nodes
-// (99 % of the copy rate; 923 MB of DRAM reads for 909 MB of operands); 18.1 us, 4.2 TB/s, for 32
-// sequences of 512-1024 rows and one node (384 CTAs on 148 SMs: some have three, some two); 6.8 us
+// (99 % of the copy rate; 923 MB of DRAM reads for 911 MB of operands); 18.1 us, 4.2 TB/s, for 32
+// sequences of 512-1024 rows and one node (384 short CTAs on 148 SMs: some SMs have three, some two, a
+// sixth of the time; the rest above the memory's 11.7 us is their start and end); 6.8 us
 // for 8 sequences of 256-512 rows and 16 nodes, 4.6 us for one of 320 rows and 8 nodes (latency: one
 // tile's flight, four warps' step, the merges and one cluster barrier).
 #pragma once
@@ -88,6 +93,9 @@ struct alignas(1024) Smem {
   volatile int abort;
 };
 constexpr size_t kSmemBytes = sizeof(Smem);
+// With the 1 KiB that the system takes of each, three CTAs fill the SM's 228 KiB exactly (two CTAs per
+// SM: 14.2 instead of 7.4 us for 8 sequences of 256-512 rows).
+static_assert(3 * (kSmemBytes + 1024) <= 228 * 1024, "three CTAs per SM");
 
 // Bounded wait that gives up as soon as another warp of the CTA has given up.
 __device__ __forceinline__ bool wait_or_abort(volatile int* abort, uint64_t* bar, uint32_t parity) {
@@ -416,7 +424,7 @@ __device__ __forceinline__ void tree_step(WarpState& st, const Params& p, Smem& 
 }
 
 // MULTI: several row tiles per K/V head, or more than 16 nodes. (An instantiation of its own: carrying
-// both costs the one-tile kernel 5 % on long caches.)
+// both costs the one-tile kernel 5 % on long caches. At 128 registers it spills 32 bytes, the other 4.)
 template <bool MULTI>
 __global__ void __launch_bounds__(THREADS, 3)
 tree_attention_kernel(const __grid_constant__ CUtensorMap tm_k,

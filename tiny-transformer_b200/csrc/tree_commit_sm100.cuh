@@ -3,8 +3,8 @@
 // Row i < counts[b] of sequence b's path: cache[layer][b, h, lens[b] + i] = tree[layer][b, h,
 // path[b, i]], keys and values, every layer in one launch; new_lens[b] = lens[b] + counts[b].
 // A path entry outside [0, N), or a row outside [0, capacity), is skipped and sets the range bit
-// of the device status, as the other appends do; new_lens counts the rows before the first one
-// that does not fit.
+// of the device status, as the other appends do. new_lens counts the rows before the first one
+// that does not fit the capacity; the row of a skipped path entry is among them and holds what it held.
 //
 // 2 * 128 bytes a row: a few hundred kilobytes at most, so latency decides. One block takes one
 // (layer, keys or values, sequence) and copies its heads x rows with 8 threads of 16 bytes a row;

@@ -17,7 +17,8 @@
 // end of the unit like the CTAs do. So all four softmax warps have work whatever the row count, a
 // thread takes 128 / DUP exponentials a tile, and the tensor work does not change. All exponentials
 // are MUFU ones: the FMA-pipe polynomial of the prefill kernel (1e-4) shows in the LSE, and the
-// softmax is not the bound here. O is rescaled only when a row's max grows by more than 2^8.
+// softmax is not the bound here. P is rounded to BF16 (see tree_attention_sm100.cuh), the sums take it
+// before. O is rescaled only when a row's max grows by more than 2^8.
 //
 // Roles: two softmax warpgroups (warps 0-3 and 4-7, thread = TMEM lane) take the tiles alternately,
 // each with score, P and O columns, a running max and a sum of its own (they merge like the
@@ -33,8 +34,10 @@
 // rows and 64 nodes: a tile takes about 1250 cycles of a CTA, what the memory needs to deliver it,
 // but the start (6000 cycles), 3.6 units' epilogues a CTA (4000 each, in which the ring of four
 // tiles fills up) and the merge kernel (6 us) come on top. 31 us for 3 sequences x 4 K/V heads of 9000-
-// 20001 rows, 37 nodes and 3 query heads each (9 tiles a CTA of 1700 cycles, softmax-bound: a thread
-// has 128 exponentials a tile). Tried: one softmax warpgroup 96 us; scores held 64 at a time with
+// 20001 rows, 37 nodes and 3 query heads each (9 tiles a CTA of 1700 cycles: a thread
+// has 128 exponentials a tile, 1024 cycles of the MUFU units, and the kernel with one copy of Q, alone of
+// the three, spills 144 bytes; start, tiles, epilogues and merge add up to 21 of the 31 us, the rest is
+// not accounted for). Tried: one softmax warpgroup 96 us; scores held 64 at a time with
 // spills, with and without handing registers over (setmaxnreg) 94-122; equal tiles instead of equal
 // cost per CTA 74; S and P.V from one thread 115.
 #pragma once

@@ -15,7 +15,10 @@
 //   r_{k+1}(v) = max(r_k(v) - floor(q(v) S_k), 0), S_{k+1} = sum of r_{k+1};
 //   next token: the smallest v whose running sum of r exceeds floor(u_0 * sum of r); r is r_0
 //   again where nothing is left of it.
-// p, q are clamped to [0, 1] (NaN to 0), so that sums of up to 2^22 weights fit 63 bits.
+// p, q are clamped to [0, 1] (NaN to 0), so that sums of up to 2^22 weights fit 63 bits. Rounding the
+// weights moves a probability by less than 2^-36. The random numbers are FP32, 2^-24 apart as generators
+// draw them, which weighs more: the drawn token's probabilities move by less than 2^-24 each (V 2^-24
+// together, 0.8 % at 128000 tokens), and a token below 2^-24 may never be drawn.
 //
 // One thread-block cluster walks one sequence, every CTA taking the same walk. All accept tests
 // before a rejection need only p(t) and q(t) of the nodes, gathered once for the whole tree; the
@@ -29,7 +32,9 @@
 //
 // Measured (B200): 5.6 us for one sequence, 8 nodes, 8192 tokens (a chain of loads: the tree, p and q of
 // its tokens, the row, the window); 11.1 us for 32 sequences of 16 nodes in threes, where some reject
-// three siblings (a pass each); 10.5 us for 5 x 50257 tokens, chosen children; 32 us for 32 x 128000
+// three siblings (a pass each); 10.5 us for 5 x 50257 tokens, chosen children (a pass for each node at
+// which one is rejected, on 40 CTAs, with 4-byte loads; at 64 registers this variant spills 120-136 bytes, the
+// one with draft probabilities 16-28); 32 us for 32 x 128000
 // (39 MB read; up to three passes of 8-10 us, the first from DRAM with 64 KiB a SM in flight, a second
 // rejection's bound by its FP64 and whole-number steps).
 #pragma once

@@ -38,7 +38,8 @@ def tree_attention(q, tree_k, tree_v, cache_k, cache_v, parents, cache_lens=None
     ``cache_k`` / ``cache_v`` ``[B, Hkv, C, 64]``, all BF16; ``Hq`` is a multiple of ``Hkv`` and
     query head h reads K/V head ``h // (Hq // Hkv)``. Node n of sequence b sees cache rows
     ``[0, cache_lens[b])`` (int32/int64 CUDA ``[B]``, clamped to ``[0, C]``; None: all C rows) and
-    its chain of parents, itself included; scale 1/8, FP32 softmax. A node not in use gets O = 0.
+    its chain of parents, itself included; scale 1/8, FP32 softmax, its weights rounded to BF16 for the
+    product with V. A node not in use gets O = 0.
     Rows that a node does not see never change its output, whatever they hold.
 
     Strided views are read in place under the rules of ``student.attention``; others are copied.
@@ -76,7 +77,8 @@ def verify_tree(tokens, parents, target_probs, uniforms, draft_probs=None):
     no token has any weight).
 
     Probabilities are weighed as whole multiples of 2^-36, so the result depends on no order of
-    summation: the same inputs give the same walk on any split of the work.
+    summation: the same inputs give the same walk on any split of the work. Uniforms that are 2^-24
+    apart, as ``torch.rand`` draws them, resolve the next token's probabilities to 2^-24.
     """
     return load_attention_extension().tree_verify(tokens, parents, target_probs, uniforms,
                                                   draft_probs)
@@ -91,7 +93,9 @@ def commit_path(cache_k, cache_v, tree_k, tree_v, path, counts, cache_lens):
     sequence b goes from tree row ``path[b, i]`` to cache row ``cache_lens[b] + i``.
 
     Returns the new lengths, int32 ``[B]``. Rows past the capacity and path entries outside the
-    tree are skipped and set the range bit of the device status (``tt_attn_device_status``).
+    tree are skipped and set the range bit of the device status (``tt_attn_device_status``). The length
+    counts the row of such a path entry although it is not written: after that status the rows appended
+    to the sequence must not be used.
     """
     lists = [x if isinstance(x, list) else list(x) if isinstance(x, tuple) else [x]
              for x in (cache_k, cache_v, tree_k, tree_v)]
