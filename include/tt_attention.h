@@ -342,6 +342,115 @@ TT_ATTN_API tt_attn_status tt_attn_tree_commit_bf16(
     int64_t path_len, const int32_t* counts, const int32_t* cache_lens, int32_t* new_lens,
     void* stream);
 
+/* ------------------------------------------------------------------ query/key norm
+ * RMS norm of every query and key head of a fused QKV projection with the rotary embedding in the same
+ * pass. No counterpart in the reference, whose blocks norm the hidden state only (tiny_transformer/model.py:46-76)
+ * and rotate in operations of their own (reference.py:30-34).
+ *
+ *   qkv        [batch, q_len, q_heads + 2 kv_heads, 64] bf16 (query, key, value heads), features adjacent, element
+ *              strides qkv_strides[3] (batch, token, head) in multiples of 8, 16-byte aligned
+ *              (TT_ATTN_UNSUPPORTED otherwise)
+ *   q_weight, k_weight  [64] bf16, or FP32 with weights_f32 != 0; both NULL: no norm, the rotation alone
+ *   cos, sin   [table_len, 32] FP32, row = position, 16-byte aligned; used in FP32
+ *   position   of token 0 (validated here), or position_dev: token (b, t) is at
+ *              position_dev[b * position_sb + t * position_st], + t where position_st is 0
+ *   q_out      contiguous [batch, q_heads, q_len, 64] bf16; k_out [batch, kv_heads, q_len, 64]
+ *
+ * For a head x of weight w: n = x w / sqrt(mean(x^2) + eps), then adjacent pairs (n_2i, n_2i+1) are turned by the
+ * table row of the position. FP32, rounded to bf16 once. Rows whose device-held position is outside the table are
+ * zero and set status bit 1.
+ */
+TT_ATTN_API tt_attn_status tt_attn_qkv_norm_rope_bf16(
+    const void* qkv, const int64_t* qkv_strides, int64_t batch, int64_t q_len, int64_t q_heads,
+    int64_t kv_heads, const void* q_weight, const void* k_weight, int weights_f32, const float* cos,
+    const float* sin, int64_t table_len, int64_t position, const int64_t* position_dev,
+    int64_t position_sb, int64_t position_st, double eps, void* q_out, void* k_out, void* stream);
+
+/*
+ * Gradients of tt_attn_qkv_norm_rope_bf16: its arguments, then
+ *   dq, dk, dv   [batch, heads, q_len, 64] bf16 with element strides (layout rules of tt_attn_forward_bf16): the
+ *                gradients of q_out, k_out and of the value heads; NULL: zero
+ *   dqkv         contiguous [batch, q_len, q_heads + 2 kv_heads, 64] bf16, dv copied into its value heads
+ *   dq_weight, dk_weight  [64] in the weights' type (not used without weights)
+ *   workspace    tt_attn_qkv_norm_rope_backward_workspace_size() bytes, 16-byte aligned (not used without weights)
+ * The weights' gradients are added in a fixed order: the same inputs give the same bits.
+ */
+TT_ATTN_API tt_attn_status tt_attn_qkv_norm_rope_backward_bf16(
+    const void* qkv, const int64_t* qkv_strides, int64_t batch, int64_t q_len, int64_t q_heads,
+    int64_t kv_heads, const void* q_weight, const void* k_weight, int weights_f32, const float* cos,
+    const float* sin, int64_t table_len, int64_t position, const int64_t* position_dev,
+    int64_t position_sb, int64_t position_st, double eps, const void* dq, const int64_t* dq_strides,
+    const void* dk, const int64_t* dk_strides, const void* dv, const int64_t* dv_strides, void* dqkv,
+    void* dq_weight, void* dk_weight, void* workspace, size_t workspace_bytes, void* stream);
+
+TT_ATTN_API size_t tt_attn_qkv_norm_rope_backward_workspace_size(void);
+
+/* ------------------------------------------------------------------ 4-bit KV cache
+ * A KV cache of 36 bytes a row (128 in bf16): rows are quantised as they are written, read back as bf16, and
+ * attended to without ever being expanded in memory. No counterpart in the reference, whose cache has the model's
+ * type (tiny_transformer/model.py:11-43).
+ *
+ * A cache is [batch, kv_heads, blocks, 576] bytes, byte strides c*_strides[4] (last 1, others multiples of 16),
+ * 16-byte aligned (TT_ATTN_UNSUPPORTED otherwise); its capacity is 16 * blocks rows. A block holds 16 rows:
+ *   bytes 0-511    codes, row r at 32 r: feature 2i in the low half of byte i, 2i + 1 in the high half; a code is e2m1
+ *                  (bit 3 the sign, then 0 0.5 1 1.5 2 3 4 6)
+ *   bytes 512-575  scales, row r at 512 + 4 r, one for 16 features: the upper byte of a half without its sign (5
+ *                  bits of exponent, 3 of mantissa), at most 0xE2 = 10240, or 0xFF = NaN
+ * A value is code x scale. 16 values are quantised with scale = max|x| / 6 rounded to nearest even (at most
+ * 10240), codes rounded to nearest, ties to the even code, saturating. A group with a NaN gets the scale NaN.
+ */
+#define TT_ATTN_CACHE4_BLOCK_ROWS 16
+#define TT_ATTN_CACHE4_BLOCK_BYTES 576
+#define TT_ATTN_CACHE4_MAX_QUERIES 16
+
+/*
+ * tt_attn_qkv_norm_rope_bf16's pass with the cache append in it: q goes to q_out, the keys (as bf16, correctly
+ * rounded) and the values are quantised into rows position + t of the caches. Other rows are left as they are.
+ * position_dev[b * position_sb] + t with a device-held position. Rows outside the cache or the table are not
+ * written, their q is zero, and status bit 1 is set.
+ */
+TT_ATTN_API tt_attn_status tt_attn_cache4_append_bf16(
+    const void* qkv, const int64_t* qkv_strides, int64_t batch, int64_t q_len, int64_t q_heads,
+    int64_t kv_heads, const void* q_weight, const void* k_weight, int weights_f32, const float* cos,
+    const float* sin, int64_t table_len, int64_t position, const int64_t* position_dev,
+    int64_t position_sb, double eps, void* q_out, void* cache_k, const int64_t* ck_strides,
+    void* cache_v, const int64_t* cv_strides, int64_t blocks, void* stream);
+
+/*
+ * Rows start + i, i < rows, of both caches as bf16 (exact): k_out and v_out contiguous [batch, kv_heads, rows, 64].
+ * start is validated here; with start_dev, sequence b starts at start_dev[b * start_sb], and rows outside the
+ * cache read as zero and set status bit 1.
+ */
+TT_ATTN_API tt_attn_status tt_attn_cache4_read_bf16(
+    const void* cache_k, const int64_t* ck_strides, const void* cache_v, const int64_t* cv_strides,
+    int64_t batch, int64_t kv_heads, int64_t blocks, int64_t start, const int64_t* start_dev,
+    int64_t start_sb, int64_t rows, void* k_out, void* v_out, void* stream);
+
+/*
+ * Attention of the last q_len tokens of each sequence, whose rows are in the caches: query t of sequence b sees
+ * rows j < kv_lens[b] - (q_len - 1 - t). Scale 1/8, FP32 softmax.
+ *
+ *   q         [batch, q_heads, q_len, 64] bf16 (layout rules of tt_attn_forward_bf16), 1 <= q_len <=
+ *             TT_ATTN_CACHE4_MAX_QUERIES; q_heads a multiple of kv_heads: query head h reads K/V head
+ *             h / (q_heads / kv_heads)
+ *   kv_lens   optional device int32[batch], clamped to [0, 16 * blocks]; NULL: the whole capacity
+ *   out       contiguous [batch, q_heads, q_len, 64] bf16, 16-byte aligned
+ *   lse       optional contiguous [batch, q_heads, q_len] FP32, natural log
+ *   workspace tt_attn_cache4_workspace_size() bytes, 16-byte aligned (may be NULL when that is 0)
+ *
+ * A query that sees no row gets O = 0, LSE = -inf. Rows that a query does not see never change its output, whatever
+ * they hold.
+ */
+TT_ATTN_API tt_attn_status tt_attn_cache4_forward_bf16(
+    const void* q, const int64_t* q_strides, const void* cache_k, const int64_t* ck_strides,
+    const void* cache_v, const int64_t* cv_strides, int64_t batch, int64_t q_heads, int64_t kv_heads,
+    int64_t q_len, int64_t blocks, int64_t head_dim, const int32_t* kv_lens, void* out, float* lse,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Scratch bytes tt_attn_cache4_forward_bf16 needs for this shape; 0 for invalid shapes too. */
+TT_ATTN_API size_t tt_attn_cache4_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                                 int64_t q_len, int64_t blocks);
+
 #ifdef __cplusplus
 }
 #endif

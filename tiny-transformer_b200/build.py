@@ -35,7 +35,8 @@ KERNEL_HEADERS = ["sm100_ptx.cuh", "prefill_sm100.cuh", "decode_sm100.cuh",
                   "decode_direct_sm100.cuh",
                   "rope_append_sm100.cuh", "qkv_rope_sm100.cuh", "selftest_sm100.cuh", "backward_sm100.cuh",
                   "backward_det_sm100.cuh", "tree_attention_sm100.cuh", "tree_persistent_sm100.cuh",
-                  "tree_verify_sm100.cuh", "tree_commit_sm100.cuh", "speculative_abi.cuh"]
+                  "tree_verify_sm100.cuh", "tree_commit_sm100.cuh", "speculative_abi.cuh",
+                  "norm_rope_sm100.cuh", "cache4_sm100.cuh", "cache4_attention_sm100.cuh", "cache4_abi.cuh"]
 
 
 def _nvcc() -> str:

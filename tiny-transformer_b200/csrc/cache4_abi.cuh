@@ -1,0 +1,422 @@
+// C-ABI implementation of the query/key norm and of the 4-bit KV cache (include/tt_attention.h): argument
+// validation, variant choice and launches. Part of tt_attention_abi.cu, whose helpers (fail, prepare_device,
+// check_launch, Launch, ...) and device status word it uses.
+#pragma once
+
+namespace {
+
+// ------------------------------------------------------------------ query/key norm
+
+struct NormRopeArgs {
+  const void* qkv;
+  const int64_t* strides;
+  int64_t batch, q_len, q_heads, kv_heads;
+  const void *q_weight, *k_weight;
+  int weights_f32;
+  const float *cos, *sin;
+  int64_t table_len, position;
+  const int64_t* position_dev;
+  int64_t pos_sb, pos_st;
+  double eps;
+};
+
+// Checks of what a pass over a projection has in common; `what` names the entry point.
+tt_attn_status norm_rope_common(const std::string& what, const NormRopeArgs& a, tt::norm_rope::Common* c) {
+  if (!a.qkv || !a.strides || !a.cos || !a.sin)
+    return fail(TT_ATTN_BAD_ARG, what + ": qkv, its strides and the cos/sin tables must not be NULL");
+  if (a.batch <= 0 || a.q_len <= 0 || a.q_heads <= 0 || a.kv_heads <= 0 || a.table_len <= 0)
+    return fail(TT_ATTN_BAD_ARG, what + ": sizes must be positive");
+  if ((a.q_weight == nullptr) != (a.k_weight == nullptr))
+    return fail(TT_ATTN_BAD_ARG, what + ": both weights or neither");
+  if (!(a.eps >= 0.0 && a.eps <= 3.0e38))
+    return fail(TT_ATTN_BAD_ARG, what + ": eps must be finite and not negative");
+  // (batch, 4 tokens, head) items, and q_len + position, stay far inside int32 / int64.
+  constexpr int64_t kMax = INT32_MAX / 8;
+  if (a.batch > kMax || a.q_len > kMax || a.q_heads > kMax || a.kv_heads > kMax ||
+      (a.q_len + 3) / 4 > kMax / a.batch || a.q_heads + 2 * a.kv_heads > kMax / (a.batch * ((a.q_len + 3) / 4)))
+    return fail(TT_ATTN_BAD_ARG, what + ": shape exceeds the supported CUDA grid limits");
+  if (a.position_dev == nullptr && (a.position < 0 || a.position > a.table_len - a.q_len))
+    return fail(TT_ATTN_BAD_ARG, what + ": position + q_len exceeds the cos/sin table");
+  if (a.pos_sb < 0 || a.pos_st < 0)
+    return fail(TT_ATTN_BAD_ARG, what + ": position strides must not be negative");
+  if (reinterpret_cast<uintptr_t>(a.position_dev) % 8 != 0)
+    return fail(TT_ATTN_BAD_ARG, what + ": the position must be 8-byte aligned");
+  for (const void* w : {a.q_weight, a.k_weight})
+    if (reinterpret_cast<uintptr_t>(w) % (a.weights_f32 ? 4 : 2) != 0)
+      return fail(TT_ATTN_BAD_ARG, what + ": the weights must be aligned to their type");
+  if (!aligned16(a.cos) || !aligned16(a.sin))
+    return fail(TT_ATTN_BAD_ARG, what + ": the cos/sin tables must be 16-byte aligned");
+  const int64_t size[3] = {a.batch, a.q_len, a.q_heads + 2 * a.kv_heads};
+  for (int d = 0; d < 3; ++d)
+    if (size[d] > 1 && (a.strides[d] <= 0 || a.strides[d] % 8 != 0))
+      return fail(TT_ATTN_UNSUPPORTED, what + ": qkv needs strides in multiples of 8 elements; copy to "
+                                              "contiguous storage first");
+  if (!aligned16(a.qkv))
+    return fail(TT_ATTN_UNSUPPORTED, what + ": qkv must be 16-byte aligned; copy to aligned storage first");
+  c->qkv = static_cast<const __nv_bfloat16*>(a.qkv);
+  c->x_sb = a.strides[0];
+  c->x_st = a.strides[1];
+  c->x_sh = a.strides[2];
+  c->B = static_cast<int>(a.batch);
+  c->T = static_cast<int>(a.q_len);
+  c->Hq = static_cast<int>(a.q_heads);
+  c->Hkv = static_cast<int>(a.kv_heads);
+  c->w[0] = a.q_weight;
+  c->w[1] = a.k_weight;
+  c->w_f32 = a.weights_f32 != 0;
+  c->cos = a.cos;
+  c->sin = a.sin;
+  c->table_len = a.table_len;
+  c->position = a.position;
+  c->position_dev = a.position_dev;
+  c->pos_sb = a.pos_sb;
+  c->pos_st = a.pos_st;
+  c->eps = a.eps;
+  return TT_ATTN_OK;
+}
+
+// Splits the heads of a group of four tokens into warp items: as many heads to an item as leave `warps` items, at
+// most `most`. Returns the items.
+int64_t norm_rope_items(tt::norm_rope::Common* c, int64_t heads, int64_t warps, int64_t most) {
+  const int64_t groups = static_cast<int64_t>(c->B) * ((c->T + tt::norm_rope::ROWS - 1) / tt::norm_rope::ROWS);
+  const int64_t per = std::max<int64_t>(1, std::min<int64_t>({most, heads, groups * heads / warps}));
+  c->items_per_group = static_cast<int>((heads + per - 1) / per);
+  c->heads_per_item = static_cast<int>((heads + c->items_per_group - 1) / c->items_per_group);
+  return groups * c->items_per_group;
+}
+
+unsigned norm_rope_grid(int64_t items) {
+  return static_cast<unsigned>((items + tt::norm_rope::WARPS - 1) / tt::norm_rope::WARPS);
+}
+
+constexpr int64_t kNormBackwardCtas = 6 * kPlanSms;   // also the rows of its workspace
+
+// ------------------------------------------------------------------ 4-bit cache
+
+// Byte strides of a cache [batch, kv_heads, blocks, 576]; those of size-1 dimensions do not matter.
+bool cache4_view(void* base, const int64_t* st, int64_t batch, int64_t kv_heads, int64_t blocks,
+                 tt::cache4::View* v) {
+  constexpr int64_t row = tt::cache4::BLOCK_BYTES;
+  const int64_t size[3] = {batch, kv_heads, blocks};
+  int64_t s[3] = {st[0], st[1], st[2]};
+  for (int d = 0; d < 3; ++d) {
+    if (size[d] == 1) s[d] = row;
+    if (s[d] <= 0 || s[d] % 16 != 0) return false;
+  }
+  if (st[3] != 1) return false;
+  *v = {static_cast<uint8_t*>(base), s[0], s[1], s[2]};
+  return aligned16(base);
+}
+
+const char* const kCache4Layout =
+    ": the caches need a unit last stride, other strides in multiples of 16 bytes and 16-byte aligned bases";
+
+tt_attn_status cache4_sizes(const std::string& what, int64_t batch, int64_t kv_heads, int64_t blocks) {
+  if (batch <= 0 || kv_heads <= 0 || blocks <= 0)
+    return fail(TT_ATTN_BAD_ARG, what + ": sizes must be positive");
+  if (blocks > INT32_MAX / (2 * tt::cache4::BLOCK_ROWS))
+    return fail(TT_ATTN_BAD_ARG, what + ": the cache capacity must fit int32");
+  return TT_ATTN_OK;
+}
+
+// Variant and split of one attention call over a 4-bit cache (sizes only: the workspace does not depend on the
+// device).
+struct Cache4Plan {
+  int nt = 1;             // query rows of a tile, in eights
+  int64_t row_tiles = 1;
+  int cluster = 1;
+  int64_t parts = 1;
+};
+
+Cache4Plan cache4_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t blocks) {
+  namespace at = tt::cache4::attn;
+  Cache4Plan pl;
+  const int64_t rows = q_heads / kv_heads * q_len;
+  pl.nt = rows <= 8 ? 1 : 2;
+  pl.row_tiles = (rows + 8 * pl.nt - 1) / (8 * pl.nt);
+  const int64_t units = batch * kv_heads * pl.row_tiles;
+  const int64_t tiles = (blocks + at::TILE_BLOCKS - 1) / at::TILE_BLOCKS;
+  // CTAs of a unit: enough to fill three to an SM, each warp with a tile at least; for long caches CTAs of about 64
+  // tiles whatever their number, so that uneven lengths leave short ends.
+  const int64_t most = (tiles + at::WARPS - 1) / at::WARPS;
+  const int64_t want = std::min(most, std::max<int64_t>(3 * kPlanSms / units, std::min<int64_t>(4, tiles / 64)));
+  pl.cluster = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, at::MAX_CLUSTER)));
+  pl.parts = std::max<int64_t>(1, want / at::MAX_CLUSTER);
+  return pl;
+}
+
+bool cache4_shape_ok(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t blocks) {
+  constexpr int64_t kMax = INT32_MAX / (tt::cache4::MAX_QUERIES * tt::cache4::attn::MAX_CLUSTER);
+  return batch > 0 && q_heads > 0 && kv_heads > 0 && q_len > 0 && blocks > 0 && q_heads % kv_heads == 0 &&
+         q_len <= tt::cache4::MAX_QUERIES && blocks <= INT32_MAX / (2 * tt::cache4::BLOCK_ROWS) &&
+         batch <= kMax && q_heads <= kMax / batch;
+}
+
+template <int NT>
+cudaError_t launch_cache4(const Cache4Plan& pl, const tt::cache4::attn::Params& p, cudaStream_t stream) {
+  namespace at = tt::cache4::attn;
+  const int64_t grid = static_cast<int64_t>(p.B) * p.Hkv * pl.row_tiles * pl.parts * pl.cluster;
+  const Launch launch(dim3(static_cast<unsigned>(grid)), at::THREADS, sizeof(at::Smem<NT>), pl.cluster, stream);
+  cudaError_t e = cudaLaunchKernelEx(&launch.cfg, at::attention_kernel<NT>, p);
+  if (e == cudaSuccess && pl.parts > 1) {
+    const Launch merge(dim3(static_cast<unsigned>(static_cast<int64_t>(p.B) * p.Hkv * p.G * p.T)),
+                       at::COMBINE_WARPS * 32, 0, 1, stream);
+    e = cudaLaunchKernelEx(&merge.cfg, at::combine_kernel, p, 8 * NT);
+  }
+  return e;
+}
+
+tt_attn_status set_cache4_attributes(int dev) {
+  namespace at = tt::cache4::attn;
+  static std::atomic<bool> done[kMaxDevices] = {};
+  if (done[dev].load(std::memory_order_acquire)) return TT_ATTN_OK;
+  cudaError_t e = cudaFuncSetAttribute(at::attention_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(sizeof(at::Smem<1>)));
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(at::attention_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(sizeof(at::Smem<2>)));
+  if (e != cudaSuccess) return cuda_fail("cudaFuncSetAttribute", e);
+  done[dev].store(true, std::memory_order_release);
+  return TT_ATTN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+TT_ATTN_API tt_attn_status tt_attn_qkv_norm_rope_bf16(
+    const void* qkv, const int64_t* qkv_strides, int64_t batch, int64_t q_len, int64_t q_heads,
+    int64_t kv_heads, const void* q_weight, const void* k_weight, int weights_f32, const float* cos,
+    const float* sin, int64_t table_len, int64_t position, const int64_t* position_dev,
+    int64_t position_sb, int64_t position_st, double eps, void* q_out, void* k_out, void* stream) {
+  namespace nr = tt::norm_rope;
+  nr::ForwardParams p{};
+  tt_attn_status st = norm_rope_common(
+      "qkv_norm_rope",
+      {qkv, qkv_strides, batch, q_len, q_heads, kv_heads, q_weight, k_weight, weights_f32, cos, sin, table_len,
+       position, position_dev, position_sb, position_st, eps},
+      &p.c);
+  if (st != TT_ATTN_OK) return st;
+  if (!q_out || !k_out || !aligned16(q_out) || !aligned16(k_out))
+    return fail(TT_ATTN_BAD_ARG, "qkv_norm_rope: the outputs must not be NULL and be 16-byte aligned");
+  int dev = 0;
+  if ((st = prepare_device(&dev)) != TT_ATTN_OK) return st;
+  p.q_out = static_cast<__nv_bfloat16*>(q_out);
+  p.k_out = static_cast<__nv_bfloat16*>(k_out);
+  const int64_t items = norm_rope_items(&p.c, q_heads + kv_heads, 16 * kPlanSms, 8);
+  const Launch launch(dim3(norm_rope_grid(items)), nr::THREADS, 0, 1, static_cast<cudaStream_t>(stream));
+  const cudaError_t le = q_weight != nullptr ? cudaLaunchKernelEx(&launch.cfg, nr::forward_kernel<true>, p)
+                                             : cudaLaunchKernelEx(&launch.cfg, nr::forward_kernel<false>, p);
+  return check_launch("qkv_norm_rope launch", le);
+}
+
+TT_ATTN_API size_t tt_attn_qkv_norm_rope_backward_workspace_size(void) {
+  return static_cast<size_t>(kNormBackwardCtas) * 2 * TT_ATTN_HEAD_DIM * sizeof(float);
+}
+
+TT_ATTN_API tt_attn_status tt_attn_qkv_norm_rope_backward_bf16(
+    const void* qkv, const int64_t* qkv_strides, int64_t batch, int64_t q_len, int64_t q_heads,
+    int64_t kv_heads, const void* q_weight, const void* k_weight, int weights_f32, const float* cos,
+    const float* sin, int64_t table_len, int64_t position, const int64_t* position_dev,
+    int64_t position_sb, int64_t position_st, double eps, const void* dq, const int64_t* dq_strides,
+    const void* dk, const int64_t* dk_strides, const void* dv, const int64_t* dv_strides, void* dqkv,
+    void* dq_weight, void* dk_weight, void* workspace, size_t workspace_bytes, void* stream) {
+  namespace nr = tt::norm_rope;
+  nr::BackwardParams p{};
+  tt_attn_status st = norm_rope_common(
+      "qkv_norm_rope backward",
+      {qkv, qkv_strides, batch, q_len, q_heads, kv_heads, q_weight, k_weight, weights_f32, cos, sin, table_len,
+       position, position_dev, position_sb, position_st, eps},
+      &p.c);
+  if (st != TT_ATTN_OK) return st;
+  const bool norm = q_weight != nullptr;
+  if (!dqkv || !aligned16(dqkv))
+    return fail(TT_ATTN_BAD_ARG, "qkv_norm_rope backward: dqkv must not be NULL and be 16-byte aligned");
+  if (norm && (!dq_weight || !dk_weight || !workspace || !aligned16(workspace) ||
+               workspace_bytes < tt_attn_qkv_norm_rope_backward_workspace_size()))
+    return fail(TT_ATTN_BAD_ARG, "qkv_norm_rope backward: the weights' gradients must not be NULL, and workspace "
+                                 "tt_attn_qkv_norm_rope_backward_workspace_size() bytes, 16-byte aligned");
+  for (const void* w : {static_cast<const void*>(dq_weight), static_cast<const void*>(dk_weight)})
+    if (norm && reinterpret_cast<uintptr_t>(w) % (weights_f32 ? 4 : 2) != 0)
+      return fail(TT_ATTN_BAD_ARG, "qkv_norm_rope backward: the weights' gradients must be aligned to their type");
+  const void* g[3] = {dq, dk, dv};
+  const int64_t* gs[3] = {dq_strides, dk_strides, dv_strides};
+  for (int i = 0; i < 3; ++i) {
+    if (g[i] == nullptr) continue;
+    if (gs[i] == nullptr)
+      return fail(TT_ATTN_BAD_ARG, "qkv_norm_rope backward: a gradient needs its strides");
+    const Shape4 s = canonical(batch, i == 0 ? q_heads : kv_heads, q_len, gs[i]);
+    if (!aligned16(g[i]) || !strides_ok(s.stride))
+      return fail(TT_ATTN_UNSUPPORTED,
+                  "qkv_norm_rope backward: gradients need a unit last stride, other strides in multiples of 8 "
+                  "elements and 16-byte aligned bases; copy to aligned contiguous storage first");
+    p.g[i] = static_cast<const __nv_bfloat16*>(g[i]);
+    p.g_sb[i] = s.stride[0];
+    p.g_sh[i] = s.stride[1];
+    p.g_st[i] = s.stride[2];
+  }
+  int dev = 0;
+  if ((st = prepare_device(&dev)) != TT_ATTN_OK) return st;
+  p.dx = static_cast<__nv_bfloat16*>(dqkv);
+  p.partial = static_cast<float*>(workspace);
+  p.dw[0] = dq_weight;
+  p.dw[1] = dk_weight;
+  const int64_t items = norm_rope_items(&p.c, q_heads + 2 * kv_heads, 16 * kPlanSms, 8);
+  p.blocks = static_cast<int>(std::min<int64_t>(norm_rope_grid(items), kNormBackwardCtas));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const Launch launch(dim3(static_cast<unsigned>(p.blocks)), nr::THREADS, 0, 1, s);
+  cudaError_t le = norm ? cudaLaunchKernelEx(&launch.cfg, nr::backward_kernel<true>, p)
+                        : cudaLaunchKernelEx(&launch.cfg, nr::backward_kernel<false>, p);
+  if (le == cudaSuccess && norm) {
+    const Launch reduce(dim3(2 * nr::HD / nr::REDUCE_FEATURES), 32 * nr::REDUCE_FEATURES, 0, 1, s);
+    le = cudaLaunchKernelEx(&reduce.cfg, nr::reduce_kernel, p);
+  }
+  return check_launch("qkv_norm_rope backward launch", le);
+}
+
+TT_ATTN_API tt_attn_status tt_attn_cache4_append_bf16(
+    const void* qkv, const int64_t* qkv_strides, int64_t batch, int64_t q_len, int64_t q_heads,
+    int64_t kv_heads, const void* q_weight, const void* k_weight, int weights_f32, const float* cos,
+    const float* sin, int64_t table_len, int64_t position, const int64_t* position_dev,
+    int64_t position_sb, double eps, void* q_out, void* cache_k, const int64_t* ck_strides,
+    void* cache_v, const int64_t* cv_strides, int64_t blocks, void* stream) {
+  namespace nr = tt::norm_rope;
+  namespace c4 = tt::cache4;
+  c4::AppendParams p{};
+  tt_attn_status st = norm_rope_common(
+      "cache4_append",
+      {qkv, qkv_strides, batch, q_len, q_heads, kv_heads, q_weight, k_weight, weights_f32, cos, sin, table_len,
+       position, position_dev, position_sb, 0, eps},
+      &p.c);
+  if (st != TT_ATTN_OK) return st;
+  if ((st = cache4_sizes("cache4_append", batch, kv_heads, blocks)) != TT_ATTN_OK) return st;
+  if (!q_out || !aligned16(q_out) || !cache_k || !cache_v || !ck_strides || !cv_strides)
+    return fail(TT_ATTN_BAD_ARG, "cache4_append: q_out, the caches and their strides must not be NULL, and q_out "
+                                 "16-byte aligned");
+  if (!cache4_view(cache_k, ck_strides, batch, kv_heads, blocks, &p.cache[0]) ||
+      !cache4_view(cache_v, cv_strides, batch, kv_heads, blocks, &p.cache[1]))
+    return fail(TT_ATTN_UNSUPPORTED, std::string("cache4_append") + kCache4Layout);
+  p.capacity = blocks * c4::BLOCK_ROWS;
+  if (position_dev == nullptr && position > p.capacity - q_len)
+    return fail(TT_ATTN_BAD_ARG, "cache4_append: position + q_len exceeds the cache capacity");
+  int dev = 0;
+  if ((st = prepare_device(&dev)) != TT_ATTN_OK) return st;
+  p.q_out = static_cast<__nv_bfloat16*>(q_out);
+  const int64_t items = norm_rope_items(&p.c, q_heads + 2 * kv_heads, 16 * kPlanSms, 8);
+  const Launch launch(dim3(norm_rope_grid(items)), nr::THREADS, 0, 1, static_cast<cudaStream_t>(stream));
+  const cudaError_t le = q_weight != nullptr ? cudaLaunchKernelEx(&launch.cfg, c4::append_kernel<true>, p)
+                                             : cudaLaunchKernelEx(&launch.cfg, c4::append_kernel<false>, p);
+  return check_launch("cache4_append launch", le);
+}
+
+TT_ATTN_API tt_attn_status tt_attn_cache4_read_bf16(
+    const void* cache_k, const int64_t* ck_strides, const void* cache_v, const int64_t* cv_strides,
+    int64_t batch, int64_t kv_heads, int64_t blocks, int64_t start, const int64_t* start_dev,
+    int64_t start_sb, int64_t rows, void* k_out, void* v_out, void* stream) {
+  namespace c4 = tt::cache4;
+  c4::ReadParams p{};
+  tt_attn_status st = cache4_sizes("cache4_read", batch, kv_heads, blocks);
+  if (st != TT_ATTN_OK) return st;
+  if (!cache_k || !cache_v || !ck_strides || !cv_strides || !k_out || !v_out || !aligned16(k_out) ||
+      !aligned16(v_out))
+    return fail(TT_ATTN_BAD_ARG, "cache4_read: the caches, their strides and the outputs must not be NULL, and the "
+                                 "outputs 16-byte aligned");
+  if (rows <= 0) return fail(TT_ATTN_BAD_ARG, "cache4_read: sizes must be positive");
+  constexpr int64_t kMax = INT32_MAX / 8;
+  if (batch > kMax || kv_heads > kMax / batch || rows > INT64_MAX / 2 / (batch * kv_heads) ||
+      batch * kv_heads * rows > kMax * (c4::READ_THREADS / 8) || rows > INT32_MAX)
+    return fail(TT_ATTN_BAD_ARG, "cache4_read: shape exceeds the supported CUDA grid limits");
+  if (start_sb < 0 || reinterpret_cast<uintptr_t>(start_dev) % 8 != 0)
+    return fail(TT_ATTN_BAD_ARG, "cache4_read: the start needs a stride that is not negative and 8-byte alignment");
+  if (!cache4_view(const_cast<void*>(cache_k), ck_strides, batch, kv_heads, blocks, &p.cache[0]) ||
+      !cache4_view(const_cast<void*>(cache_v), cv_strides, batch, kv_heads, blocks, &p.cache[1]))
+    return fail(TT_ATTN_UNSUPPORTED, std::string("cache4_read") + kCache4Layout);
+  p.capacity = blocks * c4::BLOCK_ROWS;
+  if (start_dev == nullptr && (start < 0 || start > p.capacity - rows))
+    return fail(TT_ATTN_BAD_ARG, "cache4_read: start + rows exceeds the cache capacity");
+  int dev = 0;
+  if ((st = prepare_device(&dev)) != TT_ATTN_OK) return st;
+  p.out[0] = static_cast<__nv_bfloat16*>(k_out);
+  p.out[1] = static_cast<__nv_bfloat16*>(v_out);
+  p.B = static_cast<int>(batch);
+  p.Hkv = static_cast<int>(kv_heads);
+  p.rows = static_cast<int>(rows);
+  p.start = start;
+  p.start_dev = start_dev;
+  p.start_sb = start_sb;
+  constexpr int64_t per_block = c4::READ_THREADS / 8 * c4::READ_STEPS;
+  const Launch launch(dim3(static_cast<unsigned>((2 * batch * kv_heads * rows + per_block - 1) / per_block)),
+                      c4::READ_THREADS, 0, 1, static_cast<cudaStream_t>(stream));
+  return check_launch("cache4_read launch", cudaLaunchKernelEx(&launch.cfg, c4::read_kernel, p));
+}
+
+TT_ATTN_API size_t tt_attn_cache4_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                                 int64_t q_len, int64_t blocks) {
+  if (!cache4_shape_ok(batch, q_heads, kv_heads, q_len, blocks)) return 0;
+  const Cache4Plan pl = cache4_plan(batch, q_heads, kv_heads, q_len, blocks);
+  if (pl.parts == 1) return 0;
+  return static_cast<size_t>(batch * kv_heads * pl.row_tiles * pl.parts) * 8 * pl.nt *
+         tt::cache4::attn::REC * sizeof(float);
+}
+
+TT_ATTN_API tt_attn_status tt_attn_cache4_forward_bf16(
+    const void* q, const int64_t* q_strides, const void* cache_k, const int64_t* ck_strides,
+    const void* cache_v, const int64_t* cv_strides, int64_t batch, int64_t q_heads, int64_t kv_heads,
+    int64_t q_len, int64_t blocks, int64_t head_dim, const int32_t* kv_lens, void* out, float* lse,
+    void* workspace, size_t workspace_bytes, void* stream) {
+  namespace at = tt::cache4::attn;
+  if (!q || !q_strides || !cache_k || !ck_strides || !cache_v || !cv_strides || !out)
+    return fail(TT_ATTN_BAD_ARG, "cache4_attention: q, the caches, out and the stride arrays must not be NULL");
+  if (head_dim != TT_ATTN_HEAD_DIM)
+    return fail(TT_ATTN_BAD_ARG, "cache4_attention currently supports only head_dim=64");
+  tt_attn_status st = cache4_sizes("cache4_attention", batch, kv_heads, blocks);
+  if (st != TT_ATTN_OK) return st;
+  if (q_heads <= 0 || q_len <= 0) return fail(TT_ATTN_BAD_ARG, "cache4_attention: sizes must be positive");
+  if (q_heads % kv_heads != 0)
+    return fail(TT_ATTN_BAD_ARG, "cache4_attention: q heads must be a multiple of the K/V heads");
+  if (q_len > TT_ATTN_CACHE4_MAX_QUERIES)
+    return fail(TT_ATTN_BAD_ARG, "cache4_attention: at most 16 query tokens");
+  if (!cache4_shape_ok(batch, q_heads, kv_heads, q_len, blocks))
+    return fail(TT_ATTN_BAD_ARG, "cache4_attention: shape exceeds the supported CUDA grid limits");
+  const Shape4 qs = canonical(batch, q_heads, q_len, q_strides);
+  at::Params p{};
+  if (!operand_ok(q, qs))
+    return fail(TT_ATTN_UNSUPPORTED, "cache4_attention: q needs a unit last stride, other strides in multiples of "
+                                     "8 elements and a 16-byte aligned base; copy to aligned contiguous storage first");
+  if (!cache4_view(const_cast<void*>(cache_k), ck_strides, batch, kv_heads, blocks, &p.cache[0]) ||
+      !cache4_view(const_cast<void*>(cache_v), cv_strides, batch, kv_heads, blocks, &p.cache[1]))
+    return fail(TT_ATTN_UNSUPPORTED, std::string("cache4_attention") + kCache4Layout);
+  if (!aligned16(out)) return fail(TT_ATTN_BAD_ARG, "cache4_attention: out must be 16-byte aligned");
+  for (const void* ptr : {static_cast<const void*>(kv_lens), static_cast<const void*>(lse)})
+    if (reinterpret_cast<uintptr_t>(ptr) % 4 != 0)
+      return fail(TT_ATTN_BAD_ARG, "cache4_attention: kv_lens and lse must be 4-byte aligned");
+  const size_t need = tt_attn_cache4_workspace_size(batch, q_heads, kv_heads, q_len, blocks);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
+    return fail(TT_ATTN_BAD_ARG, "cache4_attention: workspace is smaller than tt_attn_cache4_workspace_size() or "
+                                 "not 16-byte aligned");
+  int dev = 0;
+  if ((st = prepare_device(&dev)) != TT_ATTN_OK) return st;
+  if ((st = set_cache4_attributes(dev)) != TT_ATTN_OK) return st;
+  const Cache4Plan pl = cache4_plan(batch, q_heads, kv_heads, q_len, blocks);
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_sb = qs.stride[0];
+  p.q_sh = qs.stride[1];
+  p.q_st = qs.stride[2];
+  p.lens = kv_lens;
+  p.B = static_cast<int>(batch);
+  p.Hkv = static_cast<int>(kv_heads);
+  p.G = static_cast<int>(q_heads / kv_heads);
+  p.T = static_cast<int>(q_len);
+  p.row_tiles = static_cast<int>(pl.row_tiles);
+  p.blocks = static_cast<int>(blocks);
+  p.cluster = pl.cluster;
+  p.parts = static_cast<int>(pl.parts);
+  p.o = static_cast<__nv_bfloat16*>(out);
+  p.lse = lse;
+  p.records = static_cast<float*>(workspace);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return check_launch("cache4_attention launch",
+                      pl.nt == 1 ? launch_cache4<1>(pl, p, s) : launch_cache4<2>(pl, p, s));
+}
+
+}  // extern "C"

@@ -589,6 +589,304 @@ torch::Tensor tree_commit(const pybind11::list& cache_k, const pybind11::list& c
   return new_lens;
 }
 
+// ------------------------------------------------------------------ query/key norm, 4-bit cache
+// A fused projection as [B, T, heads, 64] strides: given 5-D ([B, T, 3, H, 64], q, k and v heads) or 4-D.
+struct Projection {
+  torch::Tensor x;
+  int64_t B, T, Hq, Hkv;
+  int64_t strides[3];
+};
+
+Projection projection(const torch::Tensor& qkv, std::optional<int64_t> kv_heads, const char* what) {
+  TORCH_CHECK(qkv.defined() && qkv.is_cuda(), what, ": all tensors must be CUDA tensors");
+  TORCH_CHECK(qkv.scalar_type() == at::kBFloat16 && qkv.layout() == at::kStrided, what,
+              ": qkv must be a strided bf16 tensor");
+  Projection p;
+  p.x = qkv;
+  if (qkv.dim() == 5) {
+    TORCH_CHECK(qkv.size(2) == 3, what,
+                ": qkv must be [B, T, 3, H, 64] or [B, T, q_heads + 2 * kv_heads, 64]");
+    TORCH_CHECK(!kv_heads.has_value() || *kv_heads == qkv.size(3), what,
+                ": a [B, T, 3, H, 64] projection has H K/V heads");
+    p.Hq = p.Hkv = qkv.size(3);
+    p.x = qkv.flatten(2, 3);
+  } else {
+    TORCH_CHECK(qkv.dim() == 4 && kv_heads.has_value(), what,
+                ": qkv must be [B, T, 3, H, 64], or [B, T, q_heads + 2 * kv_heads, 64] with kv_heads given");
+    p.Hkv = *kv_heads;
+    TORCH_CHECK(p.Hkv > 0 && qkv.size(2) > 2 * p.Hkv && (qkv.size(2) - 2 * p.Hkv) % p.Hkv == 0, what,
+                ": q heads must be a positive multiple of the K/V heads");
+    p.Hq = qkv.size(2) - 2 * p.Hkv;
+  }
+  TORCH_CHECK(p.x.size(3) == TT_ATTN_HEAD_DIM, what, " currently supports only head_dim=64");
+  p.B = p.x.size(0);
+  p.T = p.x.size(1);
+  TORCH_CHECK(p.B > 0 && p.T > 0 && p.Hq > 0, what, ": batch, tokens and heads must be positive");
+  bool in_place = p.x.stride(3) == 1 && reinterpret_cast<uintptr_t>(p.x.data_ptr()) % 16 == 0;
+  for (int d = 0; d < 3; ++d)
+    in_place = in_place && (p.x.size(d) == 1 || (p.x.stride(d) > 0 && p.x.stride(d) % 8 == 0));
+  if (!in_place) p.x = p.x.clone(at::MemoryFormat::Contiguous);
+  for (int d = 0; d < 3; ++d) p.strides[d] = p.x.stride(d);
+  return p;
+}
+
+// Weights of the query and key norm: both or neither, [64], bf16 or FP32 alike.
+struct NormWeights {
+  torch::Tensor q, k;
+  bool f32 = false;
+  const void* qp() const { return q.defined() ? q.data_ptr() : nullptr; }
+  const void* kp() const { return k.defined() ? k.data_ptr() : nullptr; }
+};
+
+NormWeights norm_weights(const std::optional<torch::Tensor>& q, const std::optional<torch::Tensor>& k,
+                         const torch::Tensor& like, const char* what) {
+  NormWeights w;
+  TORCH_CHECK(q.has_value() == k.has_value(), what, ": give both norm weights or neither");
+  if (!q.has_value()) return w;
+  for (const torch::Tensor* t : {&*q, &*k}) {
+    TORCH_CHECK(t->defined() && t->is_cuda() && t->device() == like.device(), what,
+                ": all tensors must be on the same device");
+    TORCH_CHECK(t->dim() == 1 && t->size(0) == TT_ATTN_HEAD_DIM, what, ": norm weights must have shape [64]");
+    TORCH_CHECK((t->scalar_type() == at::kBFloat16 || t->scalar_type() == at::kFloat) &&
+                    t->scalar_type() == q->scalar_type(),
+                what, ": norm weights must both be bf16 or both be float32");
+  }
+  w.q = q->contiguous();
+  w.k = k->contiguous();
+  w.f32 = q->scalar_type() == at::kFloat;
+  return w;
+}
+
+void check_rope_tables(const torch::Tensor& cos, const torch::Tensor& sin, const torch::Tensor& like,
+                       const char* what) {
+  for (const torch::Tensor* t : {&cos, &sin}) {
+    TORCH_CHECK(t->defined() && t->is_cuda() && t->device() == like.device(), what,
+                ": all tensors must be on the same device");
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) > 0 &&
+                    t->size(1) == TT_ATTN_HEAD_DIM / 2 && t->is_contiguous(),
+                what, ": cos/sin must be contiguous float32 [L, 32] tables");
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, what,
+                ": cos/sin tables must be 16-byte aligned");
+  }
+  TORCH_CHECK(cos.sizes() == sin.sizes(), what, ": cos and sin must have the same shape");
+}
+
+// A position argument: a Python int, or an int64 CUDA tensor: one element, [B], or (with `every`) [B, T].
+struct Position {
+  int64_t host = 0;
+  torch::Tensor t;
+  const int64_t* dev = nullptr;
+  int64_t sb = 0, st = 0;
+};
+
+Position position_argument(const pybind11::object& position, const torch::Tensor& like, int64_t B, int64_t T,
+                           bool every, const char* what) {
+  Position p;
+  if (pybind11::isinstance<pybind11::int_>(position)) {
+    p.host = position.cast<int64_t>();
+    return p;
+  }
+  TORCH_CHECK(THPVariable_Check(position.ptr()), what, ": the position must be an int or an int64 CUDA tensor");
+  p.t = THPVariable_Unpack(position.ptr());
+  TORCH_CHECK(p.t.is_cuda() && p.t.device() == like.device() && p.t.scalar_type() == at::kLong, what,
+              ": a tensor position must be an int64 CUDA tensor on the same device");
+  const bool each = p.t.dim() == 1 && p.t.size(0) == B;
+  const bool per_token = every && p.t.dim() == 2 && p.t.size(0) == B && p.t.size(1) == T;
+  TORCH_CHECK(p.t.numel() == 1 || each || per_token, what, ": a tensor position must have one element",
+              every ? ", shape [B] or shape [B, T]" : " or shape [B]");
+  if (!p.t.is_contiguous()) p.t = p.t.contiguous();
+  p.dev = p.t.data_ptr<int64_t>();
+  if (per_token) {
+    p.sb = T;
+    p.st = T > 1 ? 1 : 0;
+  } else if (each) {
+    p.sb = 1;
+  }
+  return p;
+}
+
+// RMS norm and rotation of the query and key heads of a projection (tt_attn_qkv_norm_rope_bf16).
+std::tuple<torch::Tensor, torch::Tensor> qkv_norm_rope(
+    const torch::Tensor& qkv, std::optional<torch::Tensor> q_weight, std::optional<torch::Tensor> k_weight,
+    const torch::Tensor& cos, const torch::Tensor& sin, const pybind11::object& position, double eps,
+    std::optional<int64_t> kv_heads) {
+  const char* what = "qkv_norm_rope";
+  TORCH_CHECK(qkv.defined() && qkv.is_cuda(), what, ": all tensors must be CUDA tensors");
+  const c10::cuda::CUDAGuard device_guard(qkv.device());
+  const Projection x = projection(qkv, kv_heads, what);
+  check_rope_tables(cos, sin, x.x, what);
+  const NormWeights w = norm_weights(q_weight, k_weight, x.x, what);
+  const Position pos = position_argument(position, x.x, x.B, x.T, true, what);
+  check_sm100(x.x);
+  auto q = new_cuda({x.B, x.Hq, x.T, TT_ATTN_HEAD_DIM}, at::kBFloat16, x.x.device());
+  auto k = new_cuda({x.B, x.Hkv, x.T, TT_ATTN_HEAD_DIM}, at::kBFloat16, x.x.device());
+  auto stream = c10::cuda::getCurrentCUDAStream(x.x.get_device());
+  const tt_attn_status st = tt_attn_qkv_norm_rope_bf16(
+      x.x.data_ptr(), x.strides, x.B, x.T, x.Hq, x.Hkv, w.qp(), w.kp(), w.f32, cos.data_ptr<float>(),
+      sin.data_ptr<float>(), cos.size(0), pos.host, pos.dev, pos.sb, pos.st, eps, q.data_ptr(), k.data_ptr(),
+      static_cast<void*>(stream.stream()));
+  TORCH_CHECK(st == TT_ATTN_OK, "tt_attn_qkv_norm_rope_bf16 failed: ", tt_attn_status_string(st), ": ",
+              tt_attn_last_error());
+  return {q, k};
+}
+
+// Its gradients (tt_attn_qkv_norm_rope_backward_bf16): dqkv in qkv's shape, and the weights' (undefined without).
+std::tuple<torch::Tensor, std::optional<torch::Tensor>, std::optional<torch::Tensor>> qkv_norm_rope_backward(
+    const torch::Tensor& qkv, std::optional<torch::Tensor> q_weight, std::optional<torch::Tensor> k_weight,
+    const torch::Tensor& cos, const torch::Tensor& sin, const pybind11::object& position, double eps,
+    std::optional<int64_t> kv_heads, std::optional<torch::Tensor> dq, std::optional<torch::Tensor> dk,
+    std::optional<torch::Tensor> dv) {
+  const char* what = "qkv_norm_rope backward";
+  TORCH_CHECK(qkv.defined() && qkv.is_cuda(), what, ": all tensors must be CUDA tensors");
+  const c10::cuda::CUDAGuard device_guard(qkv.device());
+  const Projection x = projection(qkv, kv_heads, what);
+  check_rope_tables(cos, sin, x.x, what);
+  const NormWeights w = norm_weights(q_weight, k_weight, x.x, what);
+  const Position pos = position_argument(position, x.x, x.B, x.T, true, what);
+  check_sm100(x.x);
+  torch::Tensor g[3];
+  const void* gp[3] = {nullptr, nullptr, nullptr};
+  int64_t gs[3][4] = {};
+  std::optional<torch::Tensor>* given[3] = {&dq, &dk, &dv};
+  for (int i = 0; i < 3; ++i) {
+    if (!given[i]->has_value()) continue;
+    g[i] = **given[i];
+    TORCH_CHECK(g[i].defined() && g[i].is_cuda() && g[i].device() == x.x.device() &&
+                    g[i].scalar_type() == at::kBFloat16 && g[i].layout() == at::kStrided && g[i].dim() == 4 &&
+                    g[i].size(0) == x.B && g[i].size(1) == (i == 0 ? x.Hq : x.Hkv) && g[i].size(2) == x.T &&
+                    g[i].size(3) == TT_ATTN_HEAD_DIM,
+                what, ": gradients must be bf16 [B, heads, T, 64] tensors on the same device");
+    g[i] = aligned_contiguous(g[i]);
+    gp[i] = g[i].data_ptr();
+    for (int d = 0; d < 4; ++d) gs[i][d] = g[i].stride(d);
+  }
+  auto dx = new_cuda(qkv.sizes(), at::kBFloat16, x.x.device());
+  std::optional<torch::Tensor> dqw, dkw;
+  torch::Tensor ws;
+  const size_t ws_bytes = tt_attn_qkv_norm_rope_backward_workspace_size();
+  if (w.q.defined()) {
+    dqw = new_cuda({TT_ATTN_HEAD_DIM}, w.q.scalar_type(), x.x.device());
+    dkw = new_cuda({TT_ATTN_HEAD_DIM}, w.q.scalar_type(), x.x.device());
+    ws = new_cuda({static_cast<int64_t>(ws_bytes)}, at::kByte, x.x.device());
+  }
+  auto stream = c10::cuda::getCurrentCUDAStream(x.x.get_device());
+  const tt_attn_status st = tt_attn_qkv_norm_rope_backward_bf16(
+      x.x.data_ptr(), x.strides, x.B, x.T, x.Hq, x.Hkv, w.qp(), w.kp(), w.f32, cos.data_ptr<float>(),
+      sin.data_ptr<float>(), cos.size(0), pos.host, pos.dev, pos.sb, pos.st, eps, gp[0], gs[0], gp[1], gs[1],
+      gp[2], gs[2], dx.data_ptr(), dqw ? dqw->data_ptr() : nullptr, dkw ? dkw->data_ptr() : nullptr,
+      ws.defined() ? ws.data_ptr() : nullptr, ws_bytes, static_cast<void*>(stream.stream()));
+  TORCH_CHECK(st == TT_ATTN_OK, "tt_attn_qkv_norm_rope_backward_bf16 failed: ", tt_attn_status_string(st), ": ",
+              tt_attn_last_error());
+  return {dx, dqw, dkw};
+}
+
+struct Cache4 {
+  int64_t B, H, blocks;
+  int64_t s[4];
+};
+
+Cache4 cache4_tensor(const torch::Tensor& c, const torch::Tensor& like, const char* what) {
+  TORCH_CHECK(c.defined() && c.is_cuda() && c.device() == like.device(), what,
+              ": all tensors must be CUDA tensors on the same device");
+  TORCH_CHECK(c.scalar_type() == at::kByte && c.layout() == at::kStrided && c.dim() == 4 &&
+                  c.size(3) == TT_ATTN_CACHE4_BLOCK_BYTES,
+              what, ": a 4-bit cache must be a uint8 [B, kv_heads, blocks, 576] tensor");
+  return {c.size(0), c.size(1), c.size(2), {c.stride(0), c.stride(1), c.stride(2), c.stride(3)}};
+}
+
+// Norm, rotation and quantised append of a projection (tt_attn_cache4_append_bf16); returns q.
+torch::Tensor cache4_append(const torch::Tensor& qkv, const torch::Tensor& cos, const torch::Tensor& sin,
+                            const pybind11::object& position, const torch::Tensor& cache_k,
+                            const torch::Tensor& cache_v, std::optional<torch::Tensor> q_weight,
+                            std::optional<torch::Tensor> k_weight, double eps) {
+  const char* what = "cache4.append";
+  TORCH_CHECK(qkv.defined() && qkv.is_cuda(), what, ": all tensors must be CUDA tensors");
+  const Cache4 ck = cache4_tensor(cache_k, qkv, what), cv = cache4_tensor(cache_v, qkv, what);
+  const c10::cuda::CUDAGuard device_guard(qkv.device());
+  const Projection x = projection(qkv, ck.H, what);
+  TORCH_CHECK(cache_v.sizes() == cache_k.sizes() && ck.B == x.B, what,
+              ": the caches must have the same shape and the projection's batch size");
+  check_rope_tables(cos, sin, x.x, what);
+  const NormWeights w = norm_weights(q_weight, k_weight, x.x, what);
+  const Position pos = position_argument(position, x.x, x.B, x.T, false, what);
+  check_sm100(x.x);
+  auto q = new_cuda({x.B, x.Hq, x.T, TT_ATTN_HEAD_DIM}, at::kBFloat16, x.x.device());
+  auto stream = c10::cuda::getCurrentCUDAStream(x.x.get_device());
+  const tt_attn_status st = tt_attn_cache4_append_bf16(
+      x.x.data_ptr(), x.strides, x.B, x.T, x.Hq, x.Hkv, w.qp(), w.kp(), w.f32, cos.data_ptr<float>(),
+      sin.data_ptr<float>(), cos.size(0), pos.host, pos.dev, pos.sb, eps, q.data_ptr(), cache_k.data_ptr(), ck.s,
+      cache_v.data_ptr(), cv.s, ck.blocks, static_cast<void*>(stream.stream()));
+  TORCH_CHECK(st == TT_ATTN_OK, "tt_attn_cache4_append_bf16 failed: ", tt_attn_status_string(st), ": ",
+              tt_attn_last_error());
+  return q;
+}
+
+// Rows of a 4-bit cache as bf16 (tt_attn_cache4_read_bf16).
+std::tuple<torch::Tensor, torch::Tensor> cache4_read(const torch::Tensor& cache_k, const torch::Tensor& cache_v,
+                                                     const pybind11::object& start, int64_t rows) {
+  const char* what = "cache4.read";
+  TORCH_CHECK(cache_k.defined() && cache_k.is_cuda(), what, ": all tensors must be CUDA tensors");
+  const Cache4 ck = cache4_tensor(cache_k, cache_k, what), cv = cache4_tensor(cache_v, cache_k, what);
+  TORCH_CHECK(cache_v.sizes() == cache_k.sizes(), what, ": the caches must have the same shape");
+  TORCH_CHECK(rows > 0, what, ": the number of rows must be positive");
+  const c10::cuda::CUDAGuard device_guard(cache_k.device());
+  const Position pos = position_argument(start, cache_k, ck.B, 1, false, what);
+  check_sm100(cache_k);
+  TORCH_CHECK(pos.dev != nullptr || (pos.host >= 0 && pos.host <= ck.blocks * TT_ATTN_CACHE4_BLOCK_ROWS - rows),
+              what, ": start + rows exceeds the cache capacity");
+  auto k = new_cuda({ck.B, ck.H, rows, TT_ATTN_HEAD_DIM}, at::kBFloat16, cache_k.device());
+  auto v = new_cuda({ck.B, ck.H, rows, TT_ATTN_HEAD_DIM}, at::kBFloat16, cache_k.device());
+  auto stream = c10::cuda::getCurrentCUDAStream(cache_k.get_device());
+  const tt_attn_status st = tt_attn_cache4_read_bf16(
+      cache_k.data_ptr(), ck.s, cache_v.data_ptr(), cv.s, ck.B, ck.H, ck.blocks, pos.host, pos.dev, pos.sb, rows,
+      k.data_ptr(), v.data_ptr(), static_cast<void*>(stream.stream()));
+  TORCH_CHECK(st == TT_ATTN_OK, "tt_attn_cache4_read_bf16 failed: ", tt_attn_status_string(st), ": ",
+              tt_attn_last_error());
+  return {k, v};
+}
+
+// Attention over a 4-bit cache (tt_attn_cache4_forward_bf16).
+std::tuple<torch::Tensor, torch::Tensor> cache4_attention(torch::Tensor q, const torch::Tensor& cache_k,
+                                                          const torch::Tensor& cache_v,
+                                                          std::optional<torch::Tensor> kv_lens, bool with_lse) {
+  const char* what = "cache4.attention";
+  TORCH_CHECK(q.defined() && q.is_cuda(), what, ": all tensors must be CUDA tensors");
+  TORCH_CHECK(q.scalar_type() == at::kBFloat16 && q.layout() == at::kStrided && q.dim() == 4, what,
+              ": q must be a strided 4D bf16 tensor");
+  TORCH_CHECK(q.size(3) == TT_ATTN_HEAD_DIM, what, " currently supports only head_dim=64");
+  const Cache4 ck = cache4_tensor(cache_k, q, what), cv = cache4_tensor(cache_v, q, what);
+  const int64_t B = q.size(0), Hq = q.size(1), T = q.size(2);
+  TORCH_CHECK(cache_v.sizes() == cache_k.sizes() && ck.B == B, what,
+              ": the caches must have the same shape and q's batch size");
+  TORCH_CHECK(B > 0 && Hq > 0 && T > 0 && ck.H > 0 && ck.blocks > 0, what, ": sizes must be positive");
+  TORCH_CHECK(Hq % ck.H == 0, what, ": q heads must be a multiple of the K/V heads");
+  TORCH_CHECK(T <= TT_ATTN_CACHE4_MAX_QUERIES, what, ": at most 16 query tokens");
+  if (kv_lens.has_value())
+    TORCH_CHECK(kv_lens->defined() && kv_lens->dim() == 1 && kv_lens->size(0) == B, what,
+                ": kv_lens must have shape [B]");
+  const c10::cuda::CUDAGuard device_guard(q.device());
+  check_sm100(q);
+  torch::Tensor lens;
+  if (kv_lens.has_value()) lens = index32(*kv_lens, q, "kv_lens");
+  q = aligned_contiguous(q);
+  auto o = new_cuda({B, Hq, T, TT_ATTN_HEAD_DIM}, at::kBFloat16, q.device());
+  torch::Tensor lse;
+  if (with_lse) lse = new_cuda({B, Hq, T}, at::kFloat, q.device());
+  const size_t ws_bytes = tt_attn_cache4_workspace_size(B, Hq, ck.H, T, ck.blocks);
+  torch::Tensor ws;
+  if (ws_bytes > 0) ws = new_cuda({static_cast<int64_t>(ws_bytes)}, at::kByte, q.device());
+  const Strides qs(q);
+  auto stream = c10::cuda::getCurrentCUDAStream(q.get_device());
+  const tt_attn_status st = tt_attn_cache4_forward_bf16(
+      q.data_ptr(), qs.s, cache_k.data_ptr(), ck.s, cache_v.data_ptr(), cv.s, B, Hq, ck.H, T, ck.blocks,
+      TT_ATTN_HEAD_DIM, lens.defined() ? lens.data_ptr<int32_t>() : nullptr, o.data_ptr(),
+      with_lse ? lse.data_ptr<float>() : nullptr, ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes,
+      static_cast<void*>(stream.stream()));
+  TORCH_CHECK(st == TT_ATTN_OK, "tt_attn_cache4_forward_bf16 failed: ", tt_attn_status_string(st), ": ",
+              tt_attn_last_error());
+  return {o, lse};
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attention_forward", &attention_forward,
         "BF16 causal attention forward on sm_100a (returns O and natural-log FP32 LSE)",
@@ -623,6 +921,26 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("cache_k"), pybind11::arg("cache_v"), pybind11::arg("tree_k"),
         pybind11::arg("tree_v"), pybind11::arg("path"), pybind11::arg("counts"),
         pybind11::arg("cache_lens"));
+  m.def("qkv_norm_rope", &qkv_norm_rope,
+        "RMS norm and rotation of the query and key heads of a fused projection; returns q and k",
+        pybind11::arg("qkv"), pybind11::arg("q_weight"), pybind11::arg("k_weight"), pybind11::arg("cos"),
+        pybind11::arg("sin"), pybind11::arg("position"), pybind11::arg("eps"), pybind11::arg("kv_heads"));
+  m.def("qkv_norm_rope_backward", &qkv_norm_rope_backward,
+        "Gradients of qkv_norm_rope; returns dqkv and the norm weights' gradients",
+        pybind11::arg("qkv"), pybind11::arg("q_weight"), pybind11::arg("k_weight"), pybind11::arg("cos"),
+        pybind11::arg("sin"), pybind11::arg("position"), pybind11::arg("eps"), pybind11::arg("kv_heads"),
+        pybind11::arg("dq"), pybind11::arg("dk"), pybind11::arg("dv"));
+  m.def("cache4_append", &cache4_append,
+        "Norm, rotation and quantised append of a fused projection to a 4-bit cache; returns q",
+        pybind11::arg("qkv"), pybind11::arg("cos"), pybind11::arg("sin"), pybind11::arg("position"),
+        pybind11::arg("cache_k"), pybind11::arg("cache_v"), pybind11::arg("q_weight"),
+        pybind11::arg("k_weight"), pybind11::arg("eps"));
+  m.def("cache4_read", &cache4_read, "Rows of a 4-bit cache as bf16; returns K and V",
+        pybind11::arg("cache_k"), pybind11::arg("cache_v"), pybind11::arg("start"), pybind11::arg("rows"));
+  m.def("cache4_attention", &cache4_attention,
+        "Attention over a 4-bit KV cache; returns O and (with_lse) LSE", pybind11::arg("q"),
+        pybind11::arg("cache_k"), pybind11::arg("cache_v"), pybind11::arg("kv_lens") = pybind11::none(),
+        pybind11::arg("with_lse") = true);
   m.attr("HEAD_DIM") = TT_ATTN_HEAD_DIM;
   m.attr("ABI_VERSION") = TT_ATTN_ABI_VERSION;
 }

@@ -31,6 +31,9 @@
 #include "tree_persistent_sm100.cuh"
 #include "tree_verify_sm100.cuh"
 #include "tree_commit_sm100.cuh"
+#include "norm_rope_sm100.cuh"
+#include "cache4_sm100.cuh"
+#include "cache4_attention_sm100.cuh"
 
 namespace {
 
@@ -1300,3 +1303,6 @@ TT_ATTN_API tt_attn_status tt_attn_decode_bf16_noalloc(
 
 // ------------------------------------------------------------------ speculative decoding
 #include "speculative_abi.cuh"
+
+// ------------------------------------------------------------------ query/key norm, 4-bit cache
+#include "cache4_abi.cuh"

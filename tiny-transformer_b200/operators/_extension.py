@@ -94,6 +94,35 @@ def load_c_abi() -> ctypes.CDLL:
         voidpp, i64p, voidpp, i64p, voidpp, i64p, voidpp, i64p, ctypes.c_int64, ctypes.c_int64,
         ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
         ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+    projection = [ctypes.c_void_p, i64p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+                  ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p,
+                  ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64]
+    gradient = [ctypes.c_void_p, i64p]
+    lib.tt_attn_qkv_norm_rope_bf16.restype = ctypes.c_int
+    lib.tt_attn_qkv_norm_rope_bf16.argtypes = projection + [
+        ctypes.c_int64, ctypes.c_double, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+    lib.tt_attn_qkv_norm_rope_backward_bf16.restype = ctypes.c_int
+    lib.tt_attn_qkv_norm_rope_backward_bf16.argtypes = projection + [
+        ctypes.c_int64, ctypes.c_double] + 3 * gradient + [
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
+        ctypes.c_void_p]
+    lib.tt_attn_qkv_norm_rope_backward_workspace_size.restype = ctypes.c_size_t
+    lib.tt_attn_qkv_norm_rope_backward_workspace_size.argtypes = []
+    cache = 2 * [ctypes.c_void_p, i64p]
+    lib.tt_attn_cache4_append_bf16.restype = ctypes.c_int
+    lib.tt_attn_cache4_append_bf16.argtypes = projection + [
+        ctypes.c_double, ctypes.c_void_p] + cache + [ctypes.c_int64, ctypes.c_void_p]
+    lib.tt_attn_cache4_read_bf16.restype = ctypes.c_int
+    lib.tt_attn_cache4_read_bf16.argtypes = cache + [
+        ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
+        ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+    lib.tt_attn_cache4_forward_bf16.restype = ctypes.c_int
+    lib.tt_attn_cache4_forward_bf16.argtypes = [ctypes.c_void_p, i64p] + cache + [
+        ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
+        ctypes.c_void_p]
+    lib.tt_attn_cache4_workspace_size.restype = ctypes.c_size_t
+    lib.tt_attn_cache4_workspace_size.argtypes = [ctypes.c_int64] * 5
     lib.tt_attn_selftest_wait_timeout.restype = ctypes.c_int
     lib.tt_attn_selftest_wait_timeout.argtypes = [ctypes.c_int64, ctypes.c_void_p]
     lib.tt_attn_status_string.restype = ctypes.c_char_p
