@@ -25,6 +25,12 @@ is a multiple of 64, else after the cuBLAS projection
   full-capacity cache with per-sequence lengths ``kv_lens`` held on the device, so the same
   graph serves every step and the host only replays it.
 
+``DecoderConfig.qk_norm`` adds an RMS norm of every query and key head (the reference has none): with the
+student attention it runs with the rotation in one kernel, forward and backward
+(``operators.fused.qkv_norm_rope``). ``new_cache(..., bits=4)`` keeps the K/V rows in 4 bits (``KVCache4``):
+they are normed, turned and quantised in one kernel as they are written; steps attend to them as they are, and
+a prompt reads them back as BF16, so that what a token sees does not depend on how the prompt was cut.
+
 ``request`` measures TTFT / TPOT / tokens per second the way the reference's model benchmark
 does (tiny_transformer/benchmarks/model.py:19-37).
 """
@@ -52,6 +58,7 @@ class DecoderConfig:
     max_seq_len: int = 4096
     norm_eps: float = 1e-6
     rope_theta: float = 10000.0
+    qk_norm: bool = False   # RMS norm of every query and key head before the rotation
 
     @property
     def head_dim(self) -> int:
@@ -175,6 +182,37 @@ class KVCache:
         return sum(x.numel() * x.element_size() for x in self.keys + self.values if x is not None)
 
 
+class KVCache4:
+    """Inference cache held in 4 bits (``operators.cache4``): per layer two byte tensors ``[B, H, blocks, 576]``,
+    36 bytes a row, allocated on first use. ``length`` advances once per model call, as in :class:`KVCache`."""
+
+    def __init__(self, config: DecoderConfig, batch_size: int, capacity: int):
+        if not 0 < capacity <= config.max_seq_len or batch_size <= 0:
+            raise ValueError("invalid KV cache batch size or capacity")
+        if config.head_dim != 64:
+            raise ValueError("a 4-bit KV cache needs head_dim 64")
+        self.batch_size = batch_size
+        self.capacity = capacity
+        self.length = 0
+        self.keys = [None] * config.n_layers
+        self.values = [None] * config.n_layers
+
+    def reset(self):
+        self.length = 0
+
+    def storage_for(self, layer, heads, device):
+        if self.keys[layer] is None:
+            from .operators import cache4
+            self.keys[layer], self.values[layer] = (
+                cache4.new_cache(self.batch_size, heads, self.capacity, device) for _ in range(2))
+        elif self.keys[layer].device != device:
+            raise ValueError("KV cache device changed; create a new cache")
+        return self.keys[layer], self.values[layer]
+
+    def allocated_bytes(self):
+        return sum(x.numel() for x in self.keys + self.values if x is not None)
+
+
 # ------------------------------------------------------------------------ model
 
 class Block(nn.Module):
@@ -186,6 +224,11 @@ class Block(nn.Module):
         self.attn_norm = nn.Parameter(torch.ones(config.dim))
         self.ffn_norm = nn.Parameter(torch.ones(config.dim))
         self.qkv = nn.Parameter(torch.empty(3 * config.dim, config.dim))
+        if config.qk_norm:
+            self.q_norm = nn.Parameter(torch.ones(config.head_dim))
+            self.k_norm = nn.Parameter(torch.ones(config.head_dim))
+        else:
+            self.q_norm = self.k_norm = None
         self.proj = nn.Parameter(torch.empty(config.dim, config.dim))
         self.gate_up = nn.Parameter(torch.empty(2 * config.hidden_dim, config.dim))
         self.down = nn.Parameter(torch.empty(config.dim, config.hidden_dim))
@@ -196,7 +239,21 @@ class Block(nn.Module):
         h = rms_norm(x, self.attn_norm, cfg.norm_eps)
         qkv = F.linear(h, self.qkv).reshape(batch, time, 3, cfg.n_heads, cfg.head_dim)
         q, k, v = (t.transpose(1, 2) for t in qkv.unbind(dim=2))
+        q, k = self.norm_heads(q, k)
         return rope(q, cos, sin), rope(k, cos, sin), v
+
+    def norm_heads(self, q, k):
+        """The query/key norm, where the model has one."""
+        if self.q_norm is None:
+            return q, k
+        eps = self.config.norm_eps
+        return rms_norm(q, self.q_norm, eps), rms_norm(k, self.k_norm, eps)
+
+    def project_normed(self, x, tables, position):
+        """project_qkv of a model with a query/key norm, norm and rotation in one kernel (FP32, rounded once)."""
+        from .operators import fused
+        return fused.qkv_norm_rope(self.qkv_rows(x), self.q_norm, self.k_norm, *tables, position,
+                                   self.config.norm_eps)
 
     def finish(self, x, attended):
         cfg = self.config
@@ -206,8 +263,12 @@ class Block(nn.Module):
         gate, up = F.linear(h, self.gate_up).chunk(2, dim=-1)
         return x + F.linear(F.silu(gate) * up, self.down)
 
-    def forward(self, x, attention, cos, sin, layer, cache=None):
-        q, k, v = self.project_qkv(x, cos, sin)
+    def forward(self, x, attention, cos, sin, layer, cache=None, tables=None):
+        """With ``tables`` (every position's cos/sin) the norm and the rotation of q and k are one kernel."""
+        if tables is None:
+            q, k, v = self.project_qkv(x, cos, sin)
+        else:
+            q, k, v = self.project_normed(x, tables, 0 if cache is None else cache.length)
         past_len = 0 if cache is None else cache.length
         if cache is not None:
             k, v = cache.update(layer, k, v)
@@ -246,6 +307,22 @@ class Block(nn.Module):
         else:
             end = position + x.shape[1]
             attended = student.attention(q, keys[:, :, :end], values[:, :, :end], position)
+        return self.finish(x, attended)
+
+    def forward_cache4(self, x, tables, layer, cache, position, kv_lens):
+        """Student path over a 4-bit cache: norm, rotation and quantised append in one kernel, then attention over
+        the codes, or (more tokens than that takes) over the prefix read back as BF16. ``kv_lens`` counts the
+        new tokens too; ``position`` is an int, or for one token an int64 tensor on the device."""
+        from .operators import cache4, student
+        cfg = self.config
+        keys, values = cache.storage_for(layer, cfg.n_heads, x.device)
+        q = cache4.append(self.qkv_rows(x), *tables, position, keys, values, self.q_norm, self.k_norm,
+                          cfg.norm_eps)
+        if x.shape[1] <= cache4.MAX_QUERIES:
+            attended = cache4.attention(q, keys, values, kv_lens)
+        else:
+            k, v = cache4.read(keys, values, 0, position + x.shape[1])
+            attended = student.attention(q, k, v, position)
         return self.finish(x, attended)
 
 
@@ -294,11 +371,19 @@ class Decoder(nn.Module):
         self.attention = attention_operator(name)
 
     def uses_fused(self, cache) -> bool:
-        return cache is not None and self.fused_rope and self.attention_name == "student"
+        return (cache is not None and not isinstance(cache, KVCache4) and self.fused_rope
+                and self.attention_name == "student" and not self.config.qk_norm)
 
-    def new_cache(self, batch_size, capacity=None):
-        return KVCache(self.config, batch_size,
-                       self.config.max_seq_len if capacity is None else capacity)
+    def uses_fused_norm(self) -> bool:
+        return (self.config.qk_norm and self.attention_name == "student"
+                and self.embedding.is_cuda and self.embedding.dtype == torch.bfloat16)
+
+    def new_cache(self, batch_size, capacity=None, bits=16):
+        """A cache in the model's type, or with ``bits=4`` one whose rows are quantised (student attention)."""
+        if bits not in (4, 16):
+            raise ValueError("a KV cache has 16 or 4 bits")
+        kind = KVCache4 if bits == 4 else KVCache
+        return kind(self.config, batch_size, self.config.max_seq_len if capacity is None else capacity)
 
     def rope_tables(self, positions: torch.Tensor):
         """cos/sin [1, 1, T, D/2] for int positions [T], built in FP32 (model.py:114-118)."""
@@ -325,15 +410,22 @@ class Decoder(nn.Module):
             if time_ + past_len > cache.capacity or ids.shape[0] != cache.batch_size:
                 raise ValueError("KV cache capacity exceeded or batch size changed")
         x = F.embedding(ids, self.embedding)
-        if self.uses_fused(cache):
-            tables = (self.rope_cos, self.rope_sin)
+        tables = (self.rope_cos, self.rope_sin)
+        if isinstance(cache, KVCache4):
+            if self.attention_name != "student":
+                raise ValueError("a 4-bit KV cache needs the student attention")
+            lens = torch.full((ids.shape[0],), past_len + time_, dtype=torch.int32, device=ids.device)
+            for layer, block in enumerate(self.blocks):
+                x = block.forward_cache4(x, tables, layer, cache, past_len, lens)
+        elif self.uses_fused(cache):
             for layer, block in enumerate(self.blocks):
                 x = block.forward_fused(x, tables, layer, cache, past_len,
                                         fused_qkv=self.fused_qkv)
         else:
             cos, sin = self.rope_tables(torch.arange(past_len, past_len + time_, device=ids.device))
             for layer, block in enumerate(self.blocks):
-                x = block(x, self.attention, cos, sin, layer, cache)
+                x = block(x, self.attention, cos, sin, layer, cache,
+                          tables if self.uses_fused_norm() else None)
         if cache is not None:
             cache.length += time_
         if last_only:
@@ -353,7 +445,7 @@ class GraphedDecode:
     and advances the position and lengths, all on the device.
     """
 
-    def __init__(self, model: Decoder, cache: KVCache, max_new_tokens: int):
+    def __init__(self, model: Decoder, cache: KVCache | KVCache4, max_new_tokens: int):
         if model.attention_name != "student":
             raise ValueError("the graphed decode step runs the student attention kernels")
         self.model, self.cache = model, cache
@@ -389,15 +481,19 @@ class GraphedDecode:
         cap = cache.capacity
         x = F.embedding(self.token, model.embedding)
         self.kv_lens.copy_((self.position + 1).to(torch.int32).expand_as(self.kv_lens))
-        if model.fused_rope:
-            tables = (model.rope_cos, model.rope_sin)
+        tables = (model.rope_cos, model.rope_sin)
+        if isinstance(cache, KVCache4):
+            for layer, block in enumerate(model.blocks):
+                x = block.forward_cache4(x, tables, layer, cache, self.position, self.kv_lens)
+        elif model.uses_fused(cache):
             for layer, block in enumerate(model.blocks):
                 x = block.forward_fused(x, tables, layer, cache, self.position, self.kv_lens,
                                         fused_qkv=model.fused_qkv)
         else:
             cos, sin = model.rope_tables(self.position)
             for layer, block in enumerate(model.blocks):
-                q, k, v = block.project_qkv(x, cos, sin)
+                q, k, v = (block.project_normed(x, tables, self.position) if model.uses_fused_norm()
+                           else block.project_qkv(x, cos, sin))
                 keys, values = cache.append_at(layer, k, v, self.position)
                 attended = student.attention(q, keys, values, cap - 1, None, self.kv_lens)
                 x = block.finish(x, attended)
@@ -460,11 +556,13 @@ def _sync(device):
 
 
 @torch.inference_mode()
-def generate(model: Decoder, prompt: torch.Tensor, new_tokens: int, graphed: bool = False):
-    """Greedy generation (generate.py:9-29 with temperature 0): returns [B, new_tokens] ids."""
+def generate(model: Decoder, prompt: torch.Tensor, new_tokens: int, graphed: bool = False,
+             cache_bits: int = 16):
+    """Greedy generation (generate.py:9-29 with temperature 0): returns [B, new_tokens] ids.
+    ``cache_bits=4`` keeps the K/V rows in a 4-bit cache (student attention)."""
     if new_tokens <= 0:
         raise ValueError("new_tokens must be positive")
-    cache = model.new_cache(prompt.shape[0], prompt.shape[1] + new_tokens)
+    cache = model.new_cache(prompt.shape[0], prompt.shape[1] + new_tokens, cache_bits)
     token = model(prompt, cache=cache, last_only=True)[:, -1, :].argmax(dim=-1, keepdim=True)
     if graphed and new_tokens > 1:
         g = GraphedDecode(model, cache, new_tokens)
@@ -480,7 +578,8 @@ def generate(model: Decoder, prompt: torch.Tensor, new_tokens: int, graphed: boo
 
 
 @torch.inference_mode()
-def request(model: Decoder, prompt: torch.Tensor, new_tokens: int, graphed: bool = False):
+def request(model: Decoder, prompt: torch.Tensor, new_tokens: int, graphed: bool = False,
+            cache_bits: int = 16):
     """One timed request (benchmarks/model.py:19-37): cache allocation, prefill through the first
     token (TTFT), then the remaining decode steps with no per-token host synchronisation
     (TPOT). Host wall time around device synchronisations. In graphed mode the capture of the
@@ -494,7 +593,7 @@ def request(model: Decoder, prompt: torch.Tensor, new_tokens: int, graphed: bool
     g = None
     if graphed:
         # Graphs are bound to cache storage: build the cache and capture before timing.
-        cache = model.new_cache(prompt.shape[0], prompt.shape[1] + new_tokens)
+        cache = model.new_cache(prompt.shape[0], prompt.shape[1] + new_tokens, cache_bits)
         token = model(prompt, cache=cache, last_only=True)[:, -1, :].argmax(dim=-1, keepdim=True)
         g = GraphedDecode(model, cache, new_tokens)
         g.prepare(token)
@@ -505,7 +604,7 @@ def request(model: Decoder, prompt: torch.Tensor, new_tokens: int, graphed: bool
     _sync(device)
     start = time.perf_counter()
     if g is None:
-        cache = model.new_cache(prompt.shape[0], prompt.shape[1] + new_tokens)
+        cache = model.new_cache(prompt.shape[0], prompt.shape[1] + new_tokens, cache_bits)
     token = model(prompt, cache=cache, last_only=True)[:, -1, :].argmax(dim=-1, keepdim=True)
     _sync(device)
     first = time.perf_counter()

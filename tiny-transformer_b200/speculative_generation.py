@@ -72,6 +72,7 @@ def forward_tree(model: Decoder, ids, tree_parents, depths, cache: KVCache, lens
         h = rms_norm(x, block.attn_norm, cfg.norm_eps)
         qkv = F.linear(h, block.qkv).view(batch, nodes, 3, cfg.n_heads, cfg.head_dim)
         q, k, v = (t.transpose(1, 2) for t in qkv.unbind(dim=2))
+        q, k = block.norm_heads(q, k)
         q, k = rope(q, cos, sin), rope(k, cos, sin)
         attended = ops.tree_attention(q, k, v, cache.keys[layer], cache.values[layer], tree_parents,
                                       lens)
