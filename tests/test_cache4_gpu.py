@@ -348,6 +348,43 @@ def test_attention_matches_oracle(c4, B, Hq, Hkv, T, C, lens):
     _check_attention(c4, _queries(B, Hq, T, C), kb, vb, kv, vv, lens)
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,T", [(160, 1, 1, 1), (80, 2, 2, 1), (160, 4, 1, 1), (150, 4, 1, 3), (40, 8, 4, 5),
+                                        (300, 1, 1, 2)])
+def test_attention_many_sequences(c4, B, Hq, Hkv, T):
+    """Many sequences with room for long ones: empty, short and a few long ones, their tiles in equal shares for all
+    warps. What is behind the lengths is NaN."""
+    blocks, rows = 450, 1600
+    rs = np.random.RandomState(B + T)
+    lens = rs.randint(0, 200, B)
+    lens[[0, 1, B - 1]] = 0
+    lens[[5, B // 2]] = rows, 1111
+    kb, kv = _random_cache(B, Hkv, rows, 71)
+    vb, vv = _random_cache(B, Hkv, rows, 72)
+    full = [torch.full((B, Hkv, blocks, 576), 0xFF, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    for dst, src in zip(full, (kb, vb)):
+        codes, scales = oracle.unpack(src)
+        for b, n in enumerate(lens):
+            scales[b, :, n:] = 0xFF
+        dst[:, :, :rows // 16] = torch.from_numpy(oracle.pack(codes, scales)).cuda()
+    q = _queries(B, Hq, T, 73)
+    for order in (np.arange(B), np.argsort(lens)):
+        dev = torch.from_numpy(lens[order]).cuda()
+        args = (q[order].cuda(), *(x[order] for x in full), dev)
+        o, lse = c4.attention_with_lse(*args)
+        ref, ref_lse, A = oracle.attention(_np(q)[order], kv[order], vv[order], lens[order])
+        S = np.abs(vv[order]).sum(2, keepdims=True).repeat(Hq // Hkv, axis=1)
+        got, got_lse = _np(o), _np(lse)
+        empty = np.isneginf(ref_lse)
+        assert (got[empty] == 0).all() and np.isneginf(got_lse[empty]).all()
+        assert (np.abs(got - ref) <= 2.0 ** -8 * np.abs(ref) + 2.0 ** -9 * A + 2.0 ** -32 * S).all()
+        lerr = np.abs(got_lse[~empty] - ref_lse[~empty])
+        assert (lerr <= 2.0 ** -12 + 2.0 ** -20 * np.abs(ref_lse[~empty])).all()
+        assert torch.equal(o, c4.attention(*args))
+    # Nothing to see at all.
+    o, lse = c4.attention_with_lse(*args[:3], torch.zeros(B, dtype=torch.int32, device="cuda"))
+    assert (o == 0).all() and torch.isneginf(lse).all()
+
+
 def test_attention_weights_reach_every_row(c4):
     """One row at a time has all the weight: a wrong row, feature or scale shows."""
     C, H = 400, 1

@@ -126,7 +126,11 @@ struct Cache4Plan {
   int64_t row_tiles = 1;
   int cluster = 1;
   int64_t parts = 1;
+  int64_t flat_ctas = 0;  // the flat kernel's CTAs; 0: the cluster kernel
 };
+
+// From here on equal shares of all tiles beat a cluster for each unit.
+constexpr int64_t kCache4FlatTiles = 16384;
 
 Cache4Plan cache4_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t blocks) {
   namespace at = tt::cache4::attn;
@@ -136,6 +140,11 @@ Cache4Plan cache4_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t
   pl.row_tiles = (rows + 8 * pl.nt - 1) / (8 * pl.nt);
   const int64_t units = batch * kv_heads * pl.row_tiles;
   const int64_t tiles = (blocks + at::TILE_BLOCKS - 1) / at::TILE_BLOCKS;
+  // (The flat kernel counts tiles in 32 bits.)
+  if (units >= kPlanSms && units * tiles > kCache4FlatTiles && tiles <= INT32_MAX / units) {
+    pl.flat_ctas = kPlanSms;
+    return pl;
+  }
   // CTAs of a unit: enough to fill three to an SM, each warp with a tile at least; for long caches CTAs of about 64
   // tiles whatever their number, so that uneven lengths leave short ends.
   const int64_t most = (tiles + at::WARPS - 1) / at::WARPS;
@@ -145,6 +154,10 @@ Cache4Plan cache4_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t
   return pl;
 }
 
+int64_t cache4_flat_warps(const Cache4Plan& pl) {
+  return pl.nt == 1 ? tt::cache4::attn::Flat<1>::WARPS : tt::cache4::attn::Flat<2>::WARPS;
+}
+
 bool cache4_shape_ok(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t blocks) {
   constexpr int64_t kMax = INT32_MAX / (tt::cache4::MAX_QUERIES * tt::cache4::attn::MAX_CLUSTER);
   return batch > 0 && q_heads > 0 && kv_heads > 0 && q_len > 0 && blocks > 0 && q_heads % kv_heads == 0 &&
@@ -152,12 +165,23 @@ bool cache4_shape_ok(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t q
          batch <= kMax && q_heads <= kMax / batch;
 }
 
-template <int NT>
+template <int NT, bool ONE>
 cudaError_t launch_cache4(const Cache4Plan& pl, const tt::cache4::attn::Params& p, cudaStream_t stream) {
   namespace at = tt::cache4::attn;
+  if (pl.flat_ctas > 0) {
+    const Launch launch(dim3(static_cast<unsigned>(pl.flat_ctas)), at::Flat<NT>::WARPS * 32,
+                        at::Flat<NT>::SMEM, 1, stream);
+    cudaError_t e = cudaLaunchKernelEx(&launch.cfg, at::flat_kernel<NT, ONE>, p);
+    if (e != cudaSuccess) return e;
+    const int64_t rows = static_cast<int64_t>(p.B) * p.Hkv * p.G * p.T;
+    const Launch merge(dim3(static_cast<unsigned>((rows + at::FLAT_COMBINE_WARPS - 1) / at::FLAT_COMBINE_WARPS)),
+                       at::FLAT_COMBINE_WARPS * 32, 0, 1, stream);
+    return cudaLaunchKernelEx(&merge.cfg, at::flat_combine_kernel, p, 8 * NT,
+                              static_cast<int>(pl.flat_ctas) * at::Flat<NT>::WARPS);
+  }
   const int64_t grid = static_cast<int64_t>(p.B) * p.Hkv * pl.row_tiles * pl.parts * pl.cluster;
   const Launch launch(dim3(static_cast<unsigned>(grid)), at::THREADS, sizeof(at::Smem<NT>), pl.cluster, stream);
-  cudaError_t e = cudaLaunchKernelEx(&launch.cfg, at::attention_kernel<NT>, p);
+  cudaError_t e = cudaLaunchKernelEx(&launch.cfg, at::attention_kernel<NT, ONE>, p);
   if (e == cudaSuccess && pl.parts > 1) {
     const Launch merge(dim3(static_cast<unsigned>(static_cast<int64_t>(p.B) * p.Hkv * p.G * p.T)),
                        at::COMBINE_WARPS * 32, 0, 1, stream);
@@ -170,11 +194,21 @@ tt_attn_status set_cache4_attributes(int dev) {
   namespace at = tt::cache4::attn;
   static std::atomic<bool> done[kMaxDevices] = {};
   if (done[dev].load(std::memory_order_acquire)) return TT_ATTN_OK;
-  cudaError_t e = cudaFuncSetAttribute(at::attention_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(sizeof(at::Smem<1>)));
+  cudaError_t e = cudaSuccess;
+  for (auto fn : {at::attention_kernel<1, true>, at::attention_kernel<1, false>})
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(sizeof(at::Smem<1>)));
   if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(at::attention_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(at::attention_kernel<2, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(sizeof(at::Smem<2>)));
+  for (auto fn : {at::flat_kernel<1, true>, at::flat_kernel<1, false>})
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(at::Flat<1>::SMEM));
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(at::flat_kernel<2, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(at::Flat<2>::SMEM));
   if (e != cudaSuccess) return cuda_fail("cudaFuncSetAttribute", e);
   done[dev].store(true, std::memory_order_release);
   return TT_ATTN_OK;
@@ -354,8 +388,10 @@ TT_ATTN_API size_t tt_attn_cache4_workspace_size(int64_t batch, int64_t q_heads,
                                                  int64_t q_len, int64_t blocks) {
   if (!cache4_shape_ok(batch, q_heads, kv_heads, q_len, blocks)) return 0;
   const Cache4Plan pl = cache4_plan(batch, q_heads, kv_heads, q_len, blocks);
-  if (pl.parts == 1) return 0;
-  return static_cast<size_t>(batch * kv_heads * pl.row_tiles * pl.parts) * 8 * pl.nt *
+  const int64_t units = batch * kv_heads * pl.row_tiles;
+  if (pl.flat_ctas == 0 && pl.parts == 1) return 0;
+  const int64_t slots = pl.flat_ctas > 0 ? units + pl.flat_ctas * cache4_flat_warps(pl) : units * pl.parts;
+  return static_cast<size_t>(slots) * 8 * pl.nt *
          tt::cache4::attn::REC * sizeof(float);
 }
 
@@ -416,7 +452,9 @@ TT_ATTN_API tt_attn_status tt_attn_cache4_forward_bf16(
   p.records = static_cast<float*>(workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return check_launch("cache4_attention launch",
-                      pl.nt == 1 ? launch_cache4<1>(pl, p, s) : launch_cache4<2>(pl, p, s));
+                      pl.nt == 2                  ? launch_cache4<2, false>(pl, p, s)
+                      : q_heads * q_len == kv_heads ? launch_cache4<1, true>(pl, p, s)
+                                                    : launch_cache4<1, false>(pl, p, s));
 }
 
 }  // extern "C"
