@@ -172,9 +172,11 @@ def test_attention_rejects_before_cuda(lib, kwargs, status, fragment):
 
 
 def test_workspace_sizes(lib):
-    assert lib.tt_attn_cache4_workspace_size(64, 12, 12, 1, 512) == 0      # enough sequences
+    assert lib.tt_attn_cache4_workspace_size(8, 12, 12, 1, 32) == 0        # a cluster for each sequence
     n = lib.tt_attn_cache4_workspace_size(1, 16, 2, 1, 8192)               # few sequences, a long cache
     assert n > 0 and n % (2 * 8 * 66 * 4) == 0
+    n = lib.tt_attn_cache4_workspace_size(64, 12, 12, 1, 512)              # many sequences
+    assert n % (8 * 66 * 4) == 0 and n // (8 * 66 * 4) == 64 * 12 + 148 * 16
     for bad in ((0, 1, 1, 1, 1), (1, 3, 2, 1, 1), (1, 1, 1, 17, 1), (1, 1, 1, 1, 0), (2**40, 1, 1, 1, 1)):
         assert lib.tt_attn_cache4_workspace_size(*bad) == 0
     assert lib.tt_attn_qkv_norm_rope_backward_workspace_size() % (2 * 64 * 4) == 0

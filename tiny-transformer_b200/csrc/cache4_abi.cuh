@@ -75,21 +75,25 @@ tt_attn_status norm_rope_common(const std::string& what, const NormRopeArgs& a, 
   return TT_ATTN_OK;
 }
 
-// Splits the heads of a group of four tokens into warp items: as many heads to an item as leave `warps` items, at
-// most `most`. Returns the items.
-int64_t norm_rope_items(tt::norm_rope::Common* c, int64_t heads, int64_t warps, int64_t most) {
+// Splits the heads of a group of four tokens into warp items: up to four to an item, fewer where that leaves less than
+// `warps` items. Returns the items.
+int norm_rope_items(tt::norm_rope::Common* c, bool values, int64_t warps) {
   const int64_t groups = static_cast<int64_t>(c->B) * ((c->T + tt::norm_rope::ROWS - 1) / tt::norm_rope::ROWS);
-  const int64_t per = std::max<int64_t>(1, std::min<int64_t>({most, heads, groups * heads / warps}));
-  c->items_per_group = static_cast<int>((heads + per - 1) / per);
-  c->heads_per_item = static_cast<int>((heads + c->items_per_group - 1) / c->items_per_group);
-  return groups * c->items_per_group;
+  const int64_t heads = c->Hq + (values ? 2 : 1) * c->Hkv;
+  const int per = static_cast<int>(
+      std::max<int64_t>(1, std::min<int64_t>(tt::norm_rope::MAX_HEADS, groups * heads / warps)));
+  c->per_item = per;
+  c->items[0] = (c->Hq + per - 1) / per;
+  c->items[1] = (c->Hkv + per - 1) / per;
+  c->items[2] = values ? c->items[1] : 0;
+  return static_cast<int>(groups * (c->items[0] + c->items[1] + c->items[2]));
 }
 
 unsigned norm_rope_grid(int64_t items) {
   return static_cast<unsigned>((items + tt::norm_rope::WARPS - 1) / tt::norm_rope::WARPS);
 }
 
-constexpr int64_t kNormBackwardCtas = 6 * kPlanSms;   // also the rows of its workspace
+constexpr int64_t kNormBackwardCtas = 5 * kPlanSms;   // also the rows of its workspace
 
 // ------------------------------------------------------------------ 4-bit cache
 
@@ -235,10 +239,10 @@ TT_ATTN_API tt_attn_status tt_attn_qkv_norm_rope_bf16(
     return fail(TT_ATTN_BAD_ARG, "qkv_norm_rope: the outputs must not be NULL and be 16-byte aligned");
   int dev = 0;
   if ((st = prepare_device(&dev)) != TT_ATTN_OK) return st;
-  p.q_out = static_cast<__nv_bfloat16*>(q_out);
-  p.k_out = static_cast<__nv_bfloat16*>(k_out);
-  const int64_t items = norm_rope_items(&p.c, q_heads + kv_heads, 16 * kPlanSms, 8);
-  const Launch launch(dim3(norm_rope_grid(items)), nr::THREADS, 0, 1, static_cast<cudaStream_t>(stream));
+  p.out[0] = static_cast<__nv_bfloat16*>(q_out);
+  p.out[1] = static_cast<__nv_bfloat16*>(k_out);
+  p.total = norm_rope_items(&p.c, false, 16 * kPlanSms);
+  const Launch launch(dim3(norm_rope_grid(p.total)), nr::THREADS, 0, 1, static_cast<cudaStream_t>(stream));
   const cudaError_t le = q_weight != nullptr ? cudaLaunchKernelEx(&launch.cfg, nr::forward_kernel<true>, p)
                                              : cudaLaunchKernelEx(&launch.cfg, nr::forward_kernel<false>, p);
   return check_launch("qkv_norm_rope launch", le);
@@ -295,8 +299,8 @@ TT_ATTN_API tt_attn_status tt_attn_qkv_norm_rope_backward_bf16(
   p.partial = static_cast<float*>(workspace);
   p.dw[0] = dq_weight;
   p.dw[1] = dk_weight;
-  const int64_t items = norm_rope_items(&p.c, q_heads + 2 * kv_heads, 16 * kPlanSms, 8);
-  p.blocks = static_cast<int>(std::min<int64_t>(norm_rope_grid(items), kNormBackwardCtas));
+  p.total = norm_rope_items(&p.c, true, 16 * kPlanSms);
+  p.blocks = static_cast<int>(std::min<int64_t>(norm_rope_grid(p.total), kNormBackwardCtas));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const Launch launch(dim3(static_cast<unsigned>(p.blocks)), nr::THREADS, 0, 1, s);
   cudaError_t le = norm ? cudaLaunchKernelEx(&launch.cfg, nr::backward_kernel<true>, p)
@@ -336,8 +340,8 @@ TT_ATTN_API tt_attn_status tt_attn_cache4_append_bf16(
   int dev = 0;
   if ((st = prepare_device(&dev)) != TT_ATTN_OK) return st;
   p.q_out = static_cast<__nv_bfloat16*>(q_out);
-  const int64_t items = norm_rope_items(&p.c, q_heads + 2 * kv_heads, 16 * kPlanSms, 8);
-  const Launch launch(dim3(norm_rope_grid(items)), nr::THREADS, 0, 1, static_cast<cudaStream_t>(stream));
+  p.total = norm_rope_items(&p.c, true, 16 * kPlanSms);
+  const Launch launch(dim3(norm_rope_grid(p.total)), nr::THREADS, 0, 1, static_cast<cudaStream_t>(stream));
   const cudaError_t le = q_weight != nullptr ? cudaLaunchKernelEx(&launch.cfg, c4::append_kernel<true>, p)
                                              : cudaLaunchKernelEx(&launch.cfg, c4::append_kernel<false>, p);
   return check_launch("cache4_append launch", le);
@@ -357,8 +361,8 @@ TT_ATTN_API tt_attn_status tt_attn_cache4_read_bf16(
                                  "outputs 16-byte aligned");
   if (rows <= 0) return fail(TT_ATTN_BAD_ARG, "cache4_read: sizes must be positive");
   constexpr int64_t kMax = INT32_MAX / 8;
-  if (batch > kMax || kv_heads > kMax / batch || rows > INT64_MAX / 2 / (batch * kv_heads) ||
-      batch * kv_heads * rows > kMax * (c4::READ_THREADS / 8) || rows > INT32_MAX)
+  const int64_t chunks = rows / c4::READ_ROWS + 1;
+  if (batch > kMax || kv_heads > kMax / batch || rows > INT32_MAX / 2 || chunks > kMax / (batch * kv_heads))
     return fail(TT_ATTN_BAD_ARG, "cache4_read: shape exceeds the supported CUDA grid limits");
   if (start_sb < 0 || reinterpret_cast<uintptr_t>(start_dev) % 8 != 0)
     return fail(TT_ATTN_BAD_ARG, "cache4_read: the start needs a stride that is not negative and 8-byte alignment");
@@ -378,9 +382,9 @@ TT_ATTN_API tt_attn_status tt_attn_cache4_read_bf16(
   p.start = start;
   p.start_dev = start_dev;
   p.start_sb = start_sb;
-  constexpr int64_t per_block = c4::READ_THREADS / 8 * c4::READ_STEPS;
-  const Launch launch(dim3(static_cast<unsigned>((2 * batch * kv_heads * rows + per_block - 1) / per_block)),
-                      c4::READ_THREADS, 0, 1, static_cast<cudaStream_t>(stream));
+  const int64_t items = 2 * batch * kv_heads * ((rows + c4::READ_ROWS - 1) / c4::READ_ROWS);
+  const Launch launch(dim3(static_cast<unsigned>((items + c4::READ_WARPS - 1) / c4::READ_WARPS)),
+                      c4::READ_WARPS * 32, 0, 1, static_cast<cudaStream_t>(stream));
   return check_launch("cache4_read launch", cudaLaunchKernelEx(&launch.cfg, c4::read_kernel, p));
 }
 

@@ -9,10 +9,11 @@
 // (with 4, a group whose largest value is below 0.09 would lose bits), and a scale becomes a half by a shift.
 //
 // Quantising 16 values x: scale = max|x| / 6 rounded to nearest even (to 10240 at most), code = x / scale rounded to
-// nearest, ties to the even code, saturating at 6. Values are bf16, so borders are exact: a tie x = border x scale
-// (3 x 4 bits) is a bf16 number, every other bf16 number is at least 2^-8 of itself away, and the product
-// x * (1 / scale) is off by 2^-22 of itself at most. Rounding it to multiples of 2^-13 restores ties and
-// crosses none. A group with a NaN gets the scale NaN; infinities saturate.
+// nearest, ties to the even code, saturating at 6. Values are bf16, so borders are exact numbers: a tie x =
+// border x scale (3 x 4 bits) is a bf16 number, every other bf16 number is at least 2^-8 of itself away, and
+// x * (1 / scale) is off by 2^-21 of itself at most; rounding it to multiples of 2^-13 restores ties and crosses none.
+// In the same way max|x| times 1/6 is off by 2^-23, a tie of the scale has 5 significant bits, and rounding to 20 bits
+// first restores it. A group with a NaN gets the scale NaN; infinities saturate.
 //
 // Append: key rows are the bf16 values of the rotation, correctly rounded: an error of the last bit next to a
 // border would be a whole step of a code. FP32 decides wherever the value is farther from a bf16 border than
@@ -67,103 +68,133 @@ __device__ __forceinline__ uint32_t scale_pair(uint32_t byte) { return byte * 0x
 
 // ------------------------------------------------------------------------------- quantising
 
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
 // Eight bf16 values (this lane's half of a group of 16; the other half is in lane ^ 1) to a word of codes.
 // Returns the group's scale byte.
 __device__ __forceinline__ uint32_t quantise8(const uint4& v, uint32_t& codes) {
   const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-  uint32_t top = 0;   // largest |x| as bits: a NaN is above infinity
-#pragma unroll
-  for (int i = 0; i < 4; ++i) top = max(top, max(u[i] & 0x7fffu, (u[i] >> 16) & 0x7fffu));
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  // To four significant bits (the quotient of an 8-bit number and 6 is never close to a tie it is not).
-  const float want = __fdiv_rn(__uint_as_float(top << 16), 6.0f);
-  const uint32_t bits = __float_as_uint(want);
-  uint32_t byte;
-  if (want >= 6.103515625e-05f)   // 2^-14
-    byte = ((bits + 0x7ffffu + ((bits >> 20) & 1u)) >> 20) - (112u << 3);
-  else
-    byte = static_cast<uint32_t>(__float2int_rn(want * 131072.0f));
-  byte = min(byte, MAX_SCALE_BYTE);
+  // Largest |x| as bits: a NaN is above infinity.
+  uint32_t two = max_u16x2(max_u16x2(u[0] & 0x7fff7fffu, u[1] & 0x7fff7fffu),
+                           max_u16x2(u[2] & 0x7fff7fffu, u[3] & 0x7fff7fffu));
+  two = max_u16x2(two, __shfl_xor_sync(0xffffffffu, two, 1));
+  const uint32_t top = max(two & 0xffffu, two >> 16);
+  const uint32_t sixth = __float_as_uint(__uint_as_float(top << 16) * (1.0f / 6.0f));
+  // Times 2^-112 a float's exponent and mantissa are those of the scale byte, subnormals included.
+  const uint32_t bits = __float_as_uint(__uint_as_float((sixth + 8u) & ~15u) * 1.92592994438723586e-34f);
+  uint32_t byte = min((bits + 0x7ffffu + ((bits >> 20) & 1u)) >> 20, MAX_SCALE_BYTE);
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(__uint_as_float(byte << 20) * 5.192296858534828e33f));
+  if (byte == 0) inv = 0.0f;
   if (top > 0x7f80u) byte = 0xffu;
-  const float scale = __half2float(__ushort_as_half(static_cast<unsigned short>(byte << 7)));
-  const float inv = byte == 0 ? 0.0f : __frcp_rn(scale);
-  codes = 0;
+  float y[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float lo = __fadd_rn(__fadd_rn(bf16_lo(u[i]) * inv, 1536.0f), -1536.0f);
-    const float hi = __fadd_rn(__fadd_rn(bf16_hi(u[i]) * inv, 1536.0f), -1536.0f);
-    uint32_t two;
-    asm("{\n\t.reg .b8 t, z;\n\t.reg .b16 q;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\t"
-        "mov.b16 q, {t, 0};\n\t"
-        "cvt.u32.u16 %0, q;\n\t}"
-        : "=r"(two)
-        : "f"(hi), "f"(lo));
-    codes |= two << (8 * i);
+    y[2 * i] = __fadd_rn(__fmaf_rn(bf16_lo(u[i]), inv, 1536.0f), -1536.0f);
+    y[2 * i + 1] = __fadd_rn(__fmaf_rn(bf16_hi(u[i]), inv, 1536.0f), -1536.0f);
   }
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(codes)
+      : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
   return byte;
 }
 
-// Stores a row's codes and scales; lane8 holds features 8 lane8 to 8 lane8 + 7 and its group's scale byte.
-__device__ __forceinline__ void store_row(const View& c, int b, int h, int64_t pos, int lane8, bool ok,
-                                          uint32_t codes, uint32_t byte) {
+// Where a lane's part of a row stands in each head of a cache: 4 bytes of codes, and the row's scales.
+struct RowPlace {
+  uint8_t* codes;
+  uint8_t* scales;
+
+  __device__ __forceinline__ void set(const View& c, int b, int64_t pos, int lane8) {
+    uint8_t* block = c.p + b * c.sb + (pos / BLOCK_ROWS) * c.sn;
+    const int r = static_cast<int>(pos % BLOCK_ROWS);
+    codes = block + r * (HD / 2) + lane8 * 4;
+    scales = block + CODE_BYTES + r * GROUPS;
+  }
+};
+
+// Quantises a row (8 features a lane) and stores its codes and scales.
+__device__ __forceinline__ void store_row(const RowPlace& at, int64_t head, int lane8, bool ok, const uint4& v) {
+  uint32_t codes;
+  const uint32_t byte = quantise8(v, codes);
   uint32_t scales = (lane8 & 1) ? 0u : byte << (4 * lane8);
   scales |= __shfl_xor_sync(0xffffffffu, scales, 2);
   scales |= __shfl_xor_sync(0xffffffffu, scales, 4);
   if (!ok) return;
-  uint8_t* block = c.p + b * c.sb + h * c.sh + (pos / BLOCK_ROWS) * c.sn;
-  const int r = static_cast<int>(pos % BLOCK_ROWS);
-  *reinterpret_cast<uint32_t*>(block + r * (HD / 2) + lane8 * 4) = codes;
-  if (lane8 == 0) *reinterpret_cast<uint32_t*>(block + CODE_BYTES + r * GROUPS) = scales;
+  *reinterpret_cast<uint32_t*>(at.codes + head) = codes;
+  if (lane8 == 0) *reinterpret_cast<uint32_t*>(at.scales + head) = scales;
 }
 
 // ------------------------------------------------------------------------------- append
 
 struct AppendParams {
   norm_rope::Common c;
+  int total;              // items
   __nv_bfloat16* q_out;   // [B, Hq, T, 64]
   View cache[2];          // keys, values
   int64_t capacity;       // rows
 };
 
-// The correctly rounded bf16 values of a key row (up to FP64's own rounding).
+// The bf16 values of a key row from FP32; false in a lane that cannot tell how one of them is rounded.
 template <bool NORM>
-__device__ __forceinline__ uint4 key_row(const float (&x)[norm_rope::E], const float (&w)[norm_rope::E],
-                                         const norm_rope::Turn& u, double eps) {
-  using norm_rope::E;
-  float r = 1.0f;
-  if (NORM) r = norm_rope::inverse_rms(x, static_cast<float>(eps));
-  uint32_t out[4];
-  bool unsure = false;
+__device__ __forceinline__ bool key_row(const uint4& v, const norm_rope::Coefficients& k, float eps, uint4& out) {
+  constexpr int E = norm_rope::E;
+  constexpr float UNIT = 9.5367431640625e-07f;   // 2^-20
+  float x[E];
+  norm_rope::unpack8(v, x);
+  const float r = NORM ? norm_rope::inverse_rms(x, eps) : 1.0f;
+  uint32_t y[4];
+  bool sure = true;
 #pragma unroll
   for (int i = 0; i < E / 2; ++i) {
-    const float a = x[2 * i] * w[2 * i] * r, b = x[2 * i + 1] * w[2 * i + 1] * r;
-    const float ac = a * u.c[i], bs = b * u.s[i], as = a * u.s[i], bc = b * u.c[i];
-    const float y0 = ac - bs, y1 = as + bc;
+    const float a = x[2 * i] * r, b = x[2 * i + 1] * r;
+    const float a0 = a * k.ec[i], b0 = b * k.os[i], a1 = a * k.es[i], b1 = b * k.oc[i];
+    const float y0 = a0 - b0, y1 = a1 + b1;
     // In units of 2^-20 of the terms: rsqrtf .25, the sum of squares .35, six roundings .0625 each.
-    const float e0 = (fabsf(ac) + fabsf(bs)) * 9.5367431640625e-07f;   // 2^-20
-    const float e1 = (fabsf(as) + fabsf(bc)) * 9.5367431640625e-07f;
-    out[i] = pack_bf16x2(y0 - e0, y1 - e1);
-    unsure = unsure || out[i] != pack_bf16x2(y0 + e0, y1 + e1);
+    const float m0 = fabsf(a0) + fabsf(b0), m1 = fabsf(a1) + fabsf(b1);
+    y[i] = pack_bf16x2(fmaf(m0, -UNIT, y0), fmaf(m1, -UNIT, y1));
+    sure = sure && y[i] == pack_bf16x2(fmaf(m0, UNIT, y0), fmaf(m1, UNIT, y1));
   }
-  if (__any_sync(0xffffffffu, unsure)) {
-    double rd = 1.0;
-    if (NORM) {
-      double ss = 0.0;
+  out = make_uint4(y[0], y[1], y[2], y[3]);
+  return sure;
+}
+
+// The same from FP64: correctly rounded but for FP64's own errors.
+template <bool NORM>
+__device__ __forceinline__ uint4 key_row_exact(const norm_rope::Common& p, const uint4& v, int64_t pos, int lane8) {
+  constexpr int E = norm_rope::E;
+  float x[E], w[E];
+  norm_rope::unpack8(v, x);
+  norm_rope::Turn u;
+  norm_rope::load_turn(p, pos, lane8, u);
 #pragma unroll
-      for (int i = 0; i < E; ++i) ss += static_cast<double>(x[i]) * x[i];
+  for (int i = 0; i < E; ++i) w[i] = 1.0f;
+  double r = 1.0;
+  if (NORM) {
+    norm_rope::load_weight(p, 1, lane8, w);
+    double ss = 0.0;
 #pragma unroll
-      for (int m = 1; m < 8; m *= 2) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-      rd = 1.0 / sqrt(ss / HD + eps);
-    }
+    for (int i = 0; i < E; ++i) ss += static_cast<double>(x[i]) * x[i];
 #pragma unroll
-    for (int i = 0; i < E / 2; ++i) {
-      const double a = x[2 * i] * rd * w[2 * i], b = x[2 * i + 1] * rd * w[2 * i + 1];
-      const double c = u.c[i], s = u.s[i];
-      out[i] = pack_bf16x2(static_cast<float>(a * c - b * s), static_cast<float>(a * s + b * c));
-    }
+    for (int m = 1; m < 8; m *= 2) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+    r = 1.0 / sqrt(ss / HD + p.eps);
   }
-  return make_uint4(out[0], out[1], out[2], out[3]);
+  uint32_t y[4];
+#pragma unroll
+  for (int i = 0; i < E / 2; ++i) {
+    const double a = x[2 * i] * r * w[2 * i], b = x[2 * i + 1] * r * w[2 * i + 1];
+    const double c = u.c[i], s = u.s[i];
+    y[i] = pack_bf16x2(static_cast<float>(a * c - b * s), static_cast<float>(a * s + b * c));
+  }
+  return make_uint4(y[0], y[1], y[2], y[3]);
 }
 
 template <bool NORM>
@@ -172,52 +203,62 @@ __global__ void __launch_bounds__(norm_rope::THREADS)
   namespace nr = norm_rope;
   const nr::Common& p = ap.c;
   const int lane = threadIdx.x & 31, lane8 = lane & 7;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * nr::WARPS + (threadIdx.x >> 5);
-  const int groups = (p.T + nr::ROWS - 1) / nr::ROWS;
+  const int index = static_cast<int>(blockIdx.x) * nr::WARPS + (threadIdx.x >> 5);
   wait_for_previous_kernel();
-  if (item >= static_cast<int64_t>(p.B) * groups * p.items_per_group) return;  // whole warps
-  const int64_t bg = item / p.items_per_group;
-  const int first = static_cast<int>(item % p.items_per_group) * p.heads_per_item;
-  const int last = min(first + p.heads_per_item, p.Hq + 2 * p.Hkv);
-  const int b = static_cast<int>(bg / groups);
-  const int t = static_cast<int>(bg % groups) * nr::ROWS + (lane >> 3);
-  const bool row = t < p.T;
-  const int64_t pos = row ? nr::position_of(p, b, t) : 0;
-  const bool ok = row && pos >= 0 && pos < p.table_len && pos < ap.capacity;
-  if (row && !ok && lane8 == 0) atomicOr(&g_tt_status, TT_ERR_RANGE);
-  nr::Turn u;
-  nr::load_turn(p, ok ? pos : 0, lane8, u);
-  const __nv_bfloat16* src = p.qkv + b * p.x_sb + static_cast<int64_t>(row ? t : 0) * p.x_st + lane8 * nr::E;
-  float w[nr::E];
+  if (index >= ap.total) return;  // whole warps
+  nr::Item it;
+  it.set(p, index, lane);
+  const __nv_bfloat16* src = p.qkv + it.b * p.x_sb + static_cast<int64_t>(it.row ? it.t : 0) * p.x_st +
+                             it.head0(p) * p.x_sh + lane8 * nr::E;
+  uint4 v[nr::MAX_HEADS];
 #pragma unroll
-  for (int i = 0; i < nr::E; ++i) w[i] = 1.0f;
-  int kind = -1;
-#pragma unroll 2
-  for (int h = first; h < last; ++h) {
-    const int now = h < p.Hq ? 0 : h < p.Hq + p.Hkv ? 1 : 2;
-    if (NORM && now != kind && now < 2) nr::load_weight(p, now, lane8, w);
-    kind = now;
-    uint4 v = *reinterpret_cast<const uint4*>(src + h * p.x_sh);
-    float x[nr::E];
-    if (now == 0) {
-      float y[nr::E], r = 1.0f;
-      nr::unpack8(v, x);
-      if (NORM) r = nr::inverse_rms(x, static_cast<float>(p.eps));
-      nr::turn_row(x, w, r, u, y);
+  for (int h = 0; h < nr::MAX_HEADS; ++h)
+    if (h < it.heads) v[h] = *reinterpret_cast<const uint4*>(src + h * p.x_sh);
+  const int64_t pos = it.row ? nr::position_of(p, it.b, it.t) : 0;
+  const bool ok = it.row && pos >= 0 && pos < p.table_len && pos < ap.capacity;
+  if (it.row && !ok && lane8 == 0) atomicOr(&g_tt_status, TT_ERR_RANGE);
+  const int64_t at = ok ? pos : 0;
+  if (it.kind == 2) {
+    RowPlace place;
+    place.set(ap.cache[1], it.b, at, lane8);
+#pragma unroll
+    for (int h = 0; h < nr::MAX_HEADS; ++h)
+      if (h < it.heads) store_row(place, (it.first + h) * ap.cache[1].sh, lane8, ok, v[h]);
+    return;
+  }
+  nr::Turn u;
+  nr::load_turn(p, at, lane8, u);
+  nr::Coefficients k;
+  k.set<NORM>(p, it.kind, u, lane8);
+  const float eps = static_cast<float>(p.eps);
+  if (it.kind == 0) {
+    __nv_bfloat16* dst = ap.q_out + ((static_cast<int64_t>(it.b) * p.Hq + it.first) * p.T + it.t) * HD + lane8 * nr::E;
+#pragma unroll
+    for (int h = 0; h < nr::MAX_HEADS; ++h) {
+      if (h >= it.heads) break;
+      const uint4 y = nr::turn_row<NORM>(v[h], k, eps);
       // A row whose position is outside the cache or the table is zero.
-      const uint4 out = ok ? nr::pack8(y) : make_uint4(0, 0, 0, 0);
-      if (row)
-        *reinterpret_cast<uint4*>(ap.q_out + ((static_cast<int64_t>(b) * p.Hq + h) * p.T + t) * HD +
-                                  lane8 * nr::E) = out;
-      continue;
+      if (it.row)
+        *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(h) * p.T * HD) = ok ? y : make_uint4(0, 0, 0, 0);
     }
-    if (now == 1) {
-      nr::unpack8(v, x);
-      v = key_row<NORM>(x, w, u, p.eps);
-    }
-    uint32_t codes;
-    const uint32_t byte = quantise8(v, codes);
-    store_row(ap.cache[now - 1], b, h - p.Hq - (now - 1) * p.Hkv, pos, lane8, ok, codes, byte);
+    return;
+  }
+  RowPlace place;
+  place.set(ap.cache[0], it.b, at, lane8);
+  unsigned unsure = 0;   // heads
+#pragma unroll
+  for (int h = 0; h < nr::MAX_HEADS; ++h) {
+    if (h >= it.heads) break;
+    uint4 y;
+    const bool sure = key_row<NORM>(v[h], k, eps, y);
+    if (__any_sync(0xffffffffu, !sure)) unsure |= 1u << h;
+    store_row(place, (it.first + h) * ap.cache[0].sh, lane8, ok, y);
+  }
+  while (unsure != 0) {
+    const int h = __ffs(static_cast<int>(unsure)) - 1;
+    unsure &= unsure - 1;
+    const uint4 x = *reinterpret_cast<const uint4*>(src + h * p.x_sh);
+    store_row(place, (it.first + h) * ap.cache[0].sh, lane8, ok, key_row_exact<NORM>(p, x, at, lane8));
   }
 }
 
@@ -233,54 +274,57 @@ struct ReadParams {
   int64_t start_sb;
 };
 
-constexpr int READ_THREADS = 256;
-constexpr int READ_STEPS = 4;     // rows of a thread, so that as many loads are in flight
+constexpr int READ_WARPS = 4;
+constexpr int READ_ROWS = 16;     // rows of a warp: four steps of four, all loads in flight together
 
 // Eight lanes a row: 4 bytes of codes and the group's scale each, 16 bytes out.
-__global__ void __launch_bounds__(READ_THREADS) read_kernel(const __grid_constant__ ReadParams p) {
-  const int lane8 = threadIdx.x & 7;
+__global__ void __launch_bounds__(READ_WARPS * 32) read_kernel(const __grid_constant__ ReadParams p) {
+  constexpr int STEPS = READ_ROWS / 4;
+  const int lane = threadIdx.x & 31, lane8 = lane & 7;
   wait_for_previous_kernel();
-  const int64_t per_cache = static_cast<int64_t>(p.B) * p.Hkv * p.rows;
-  constexpr int ROWS_PER_STEP = READ_THREADS / 8;
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * (ROWS_PER_STEP * READ_STEPS) + (threadIdx.x >> 3);
-  uint32_t codes[READ_STEPS], byte[READ_STEPS];
+  // Item: (K or V, sequence, head, 16 rows).
+  const unsigned chunks = (static_cast<unsigned>(p.rows) + READ_ROWS - 1) / READ_ROWS;
+  const unsigned index = blockIdx.x * READ_WARPS + (threadIdx.x >> 5);
+  const unsigned row_of = index / chunks, heads = static_cast<unsigned>(p.B) * p.Hkv;
+  if (row_of >= 2 * heads) return;   // whole warps
+  const int kv = row_of >= heads ? 1 : 0;
+  const int bh = static_cast<int>(row_of - kv * heads);
+  const int b = bh / p.Hkv, h = bh - b * p.Hkv;
+  const int first = static_cast<int>(index - row_of * chunks) * READ_ROWS + (lane >> 3);
+  const View& c = p.cache[kv];
+  const uint8_t* base = c.p + b * c.sb + h * c.sh;
+  const int64_t start = (p.start_dev != nullptr ? p.start_dev[b * p.start_sb] : p.start) + first;
+  uint32_t codes[STEPS], byte[STEPS];
+  bool outside = false;
 #pragma unroll
-  for (int s = 0; s < READ_STEPS; ++s) {
-    const int64_t at = base + s * ROWS_PER_STEP;
+  for (int s = 0; s < STEPS; ++s) {
+    const int64_t pos = start + 4 * s;
     codes[s] = byte[s] = 0;
-    if (at >= 2 * per_cache) continue;
-    const int kv = at >= per_cache ? 1 : 0;
-    const int64_t rest = at - kv * per_cache;
-    const int i = static_cast<int>(rest % p.rows);
-    const int bh = static_cast<int>(rest / p.rows);
-    const int b = bh / p.Hkv, h = bh - b * p.Hkv;
-    const int64_t pos = (p.start_dev != nullptr ? p.start_dev[b * p.start_sb] : p.start) + i;
+    if (first + 4 * s >= p.rows) continue;
     if (pos < 0 || pos >= p.capacity) {   // reads as zero
-      if (lane8 == 0) atomicOr(&g_tt_status, TT_ERR_RANGE);
+      outside = true;
       continue;
     }
-    const View& c = p.cache[kv];
-    const uint8_t* block = c.p + b * c.sb + h * c.sh + (pos / BLOCK_ROWS) * c.sn;
+    const uint8_t* block = base + (pos / BLOCK_ROWS) * c.sn;
     const int r = static_cast<int>(pos % BLOCK_ROWS);
     codes[s] = *reinterpret_cast<const uint32_t*>(block + r * (HD / 2) + lane8 * 4);
     byte[s] = block[CODE_BYTES + r * GROUPS + (lane8 >> 1)];
   }
+  if (outside && lane8 == 0) atomicOr(&g_tt_status, TT_ERR_RANGE);
+  __nv_bfloat16* out = p.out[kv] + (static_cast<int64_t>(bh) * p.rows + first) * HD + lane8 * 8;
 #pragma unroll
-  for (int s = 0; s < READ_STEPS; ++s) {
-    const int64_t at = base + s * ROWS_PER_STEP;
-    if (at >= 2 * per_cache) continue;
-    const int kv = at >= per_cache ? 1 : 0;
-    uint32_t pairs[4], out[4];
+  for (int s = 0; s < STEPS; ++s) {
+    if (first + 4 * s >= p.rows) break;
+    uint32_t pairs[4], y[4];
     decode8(codes[s], pairs);
     const uint32_t scale = scale_pair(byte[s]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t y = mul_half2(pairs[i], scale);
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&y));
-      out[i] = pack_bf16x2(f.x, f.y);
+      const uint32_t two = mul_half2(pairs[i], scale);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two));
+      y[i] = pack_bf16x2(f.x, f.y);
     }
-    *reinterpret_cast<uint4*>(p.out[kv] + (at - kv * per_cache) * HD + lane8 * 8) =
-        make_uint4(out[0], out[1], out[2], out[3]);
+    *reinterpret_cast<uint4*>(out + s * 4 * HD) = make_uint4(y[0], y[1], y[2], y[3]);
   }
 }
 

@@ -11,9 +11,9 @@
 //
 // Bound by memory: 128 bytes in and 128 out per head forward; backward reads x and dy and writes dx. Eight
 // lanes hold a row, 16 bytes each, so a warp's loads and stores are 4 whole rows; the pairs of the rotation stay
-// inside a lane and the norm's sums take three shuffles. A warp's four rows are four tokens of one head: their
-// rows of q and k are adjacent in the [B, H, T, 64] outputs, and the table rows stay in registers while
-// the warp goes through heads.
+// inside a lane and the norm's sums take three shuffles. A warp's item is four tokens of up to four heads of one kind
+// (query, key or value): the tokens' rows of q and k are adjacent in the [B, H, T, 64] outputs, all of an item's loads
+// are in flight together, and the weights are multiplied into the table rows once for its heads.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -31,14 +31,15 @@ constexpr int THREADS = WARPS * 32;
 constexpr int ROWS = 4;   // tokens of a warp's step
 constexpr int LANES = 8;  // lanes of a row
 constexpr int E = HD / LANES;
+constexpr int MAX_HEADS = 4;
 
 // What a call of any of the kernels here and of the cache's append has in common.
 struct Common {
   const __nv_bfloat16* qkv;
   int64_t x_sb, x_st, x_sh;   // element strides of qkv (batch, token, head)
   int B, T, Hq, Hkv;
-  int heads_per_item;         // a warp's item: 4 tokens, this many heads
-  int items_per_group;        // items of one group of 4 tokens
+  int per_item;               // heads of an item, at most MAX_HEADS
+  int items[3];               // items of the query, key and value heads of a group of four tokens
   const void* w[2];           // q and k weight [64], both NULL: no norm
   bool w_f32;                 // else bf16
   const float* cos;           // [table_len, 32]
@@ -71,11 +72,34 @@ __device__ __forceinline__ void load_weight(const Common& p, int kind, int lane8
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     const int at = lane8 * E + i;
-    w[i] = p.w[kind] == nullptr ? 1.0f
-           : p.w_f32 ? static_cast<const float*>(p.w[kind])[at]
-                     : __bfloat162float(static_cast<const __nv_bfloat16*>(p.w[kind])[at]);
+    w[i] = p.w_f32 ? static_cast<const float*>(p.w[kind])[at]
+                   : __bfloat162float(static_cast<const __nv_bfloat16*>(p.w[kind])[at]);
   }
 }
+
+// A warp's item.
+struct Item {
+  int b, t;          // sequence, this lane's token
+  int kind;          // 0 query, 1 key, 2 value heads
+  int first, heads;  // of its kind
+  bool row;          // this lane's token is there
+
+  __device__ __forceinline__ void set(const Common& p, int index, int lane) {
+    const int per_group = p.items[0] + p.items[1] + p.items[2], groups = (p.T + ROWS - 1) / ROWS;
+    const int bg = index / per_group;
+    int at = index - bg * per_group;
+    kind = at < p.items[0] ? 0 : at < p.items[0] + p.items[1] ? 1 : 2;
+    at -= kind == 0 ? 0 : kind == 1 ? p.items[0] : p.items[0] + p.items[1];
+    first = at * p.per_item;
+    heads = min(p.per_item, (kind == 0 ? p.Hq : p.Hkv) - first);
+    b = bg / groups;
+    t = (bg - b * groups) * ROWS + (lane >> 3);
+    row = t < p.T;
+  }
+  __device__ __forceinline__ int head0(const Common& p) const {   // of the projection
+    return first + (kind == 0 ? 0 : kind == 1 ? p.Hq : p.Hq + p.Hkv);
+  }
+};
 
 __device__ __forceinline__ void unpack8(const uint4& v, float (&x)[E]) {
   const uint32_t u[4] = {v.x, v.y, v.z, v.w};
@@ -105,67 +129,79 @@ __device__ __forceinline__ float inverse_rms(const float (&x)[E], float eps) {
   return rsqrtf(row_sum(ss) * (1.0f / HD) + eps);
 }
 
-// y = rotation of x r w (r = 1 and w = 1 without a norm).
-__device__ __forceinline__ void turn_row(const float (&x)[E], const float (&w)[E], float r, const Turn& u,
-                                         float (&y)[E]) {
+// The rotation with the weights in it: y_2i = x_2i ec - x_2i+1 os, y_2i+1 = x_2i es + x_2i+1 oc (x normed).
+struct Coefficients {
+  float ec[E / 2], es[E / 2], oc[E / 2], os[E / 2];
+
+  template <bool NORM>
+  __device__ __forceinline__ void set(const Common& p, int kind, const Turn& u, int lane8) {
+    float w[E];
+    if (NORM) load_weight(p, kind, lane8, w);
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      const float we = NORM ? w[2 * i] : 1.0f, wo = NORM ? w[2 * i + 1] : 1.0f;
+      ec[i] = we * u.c[i];
+      es[i] = we * u.s[i];
+      oc[i] = wo * u.c[i];
+      os[i] = wo * u.s[i];
+    }
+  }
+};
+
+template <bool NORM>
+__device__ __forceinline__ uint4 turn_row(const uint4& v, const Coefficients& k, float eps) {
+  float x[E], y[E];
+  unpack8(v, x);
+  const float r = NORM ? inverse_rms(x, eps) : 1.0f;
 #pragma unroll
   for (int i = 0; i < E / 2; ++i) {
-    const float a = x[2 * i] * w[2 * i] * r, b = x[2 * i + 1] * w[2 * i + 1] * r;
-    y[2 * i] = a * u.c[i] - b * u.s[i];
-    y[2 * i + 1] = a * u.s[i] + b * u.c[i];
+    const float a = x[2 * i] * r, b = x[2 * i + 1] * r;
+    y[2 * i] = a * k.ec[i] - b * k.os[i];
+    y[2 * i + 1] = a * k.es[i] + b * k.oc[i];
   }
+  return pack8(y);
 }
 
 // ------------------------------------------------------------------------------- forward
 
 struct ForwardParams {
   Common c;
-  __nv_bfloat16* q_out;   // [B, Hq, T, 64]
-  __nv_bfloat16* k_out;   // [B, Hkv, T, 64]
+  int total;              // items
+  __nv_bfloat16* out[2];  // q [B, Hq, T, 64], k [B, Hkv, T, 64]
 };
 
 template <bool NORM>
 __global__ void __launch_bounds__(THREADS) forward_kernel(const __grid_constant__ ForwardParams fp) {
   const Common& p = fp.c;
   const int lane = threadIdx.x & 31, lane8 = lane & 7;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * WARPS + (threadIdx.x >> 5);
-  const int groups = (p.T + ROWS - 1) / ROWS;
+  const int index = static_cast<int>(blockIdx.x) * WARPS + (threadIdx.x >> 5);
   wait_for_previous_kernel();
-  if (item >= static_cast<int64_t>(p.B) * groups * p.items_per_group) return;  // whole warps
-  const int64_t bg = item / p.items_per_group;
-  const int first = static_cast<int>(item % p.items_per_group) * p.heads_per_item;
-  const int last = min(first + p.heads_per_item, p.Hq + p.Hkv);
-  const int b = static_cast<int>(bg / groups);
-  const int t = static_cast<int>(bg % groups) * ROWS + (lane >> 3);
-  const bool row = t < p.T;
-  const int64_t pos = row ? position_of(p, b, t) : 0;
-  const bool ok = row && pos >= 0 && pos < p.table_len;
-  if (row && !ok && lane8 == 0) atomicOr(&g_tt_status, TT_ERR_RANGE);
+  if (index >= fp.total) return;  // whole warps
+  Item it;
+  it.set(p, index, lane);
+  const __nv_bfloat16* src = p.qkv + it.b * p.x_sb + static_cast<int64_t>(it.row ? it.t : 0) * p.x_st +
+                             it.head0(p) * p.x_sh + lane8 * E;
+  uint4 v[MAX_HEADS];
+#pragma unroll
+  for (int h = 0; h < MAX_HEADS; ++h)
+    if (h < it.heads) v[h] = *reinterpret_cast<const uint4*>(src + h * p.x_sh);
+  const int64_t pos = it.row ? position_of(p, it.b, it.t) : 0;
+  const bool ok = it.row && pos >= 0 && pos < p.table_len;
+  if (it.row && !ok && lane8 == 0) atomicOr(&g_tt_status, TT_ERR_RANGE);
   Turn u;
   load_turn(p, ok ? pos : 0, lane8, u);
-  const __nv_bfloat16* src = p.qkv + b * p.x_sb + static_cast<int64_t>(row ? t : 0) * p.x_st + lane8 * E;
-  float w[E];
-  int kind = -1;
-#pragma unroll 2
-  for (int h = first; h < last; ++h) {
-    const int now = h < p.Hq ? 0 : 1;
-    if (NORM && now != kind) load_weight(p, now, lane8, w);
-    kind = now;
-    float x[E], y[E];
-    unpack8(*reinterpret_cast<const uint4*>(src + h * p.x_sh), x);
-    float r = 1.0f;
-    if (NORM) {
-      r = inverse_rms(x, static_cast<float>(p.eps));
-    } else {
+  Coefficients k;
+  k.set<NORM>(p, it.kind, u, lane8);
+  const int heads = it.kind == 0 ? p.Hq : p.Hkv;
+  __nv_bfloat16* dst = fp.out[it.kind] +
+                       ((static_cast<int64_t>(it.b) * heads + it.first) * p.T + it.t) * HD + lane8 * E;
 #pragma unroll
-      for (int i = 0; i < E; ++i) w[i] = 1.0f;
-    }
-    turn_row(x, w, r, u, y);
+  for (int h = 0; h < MAX_HEADS; ++h) {
+    if (h >= it.heads) break;
+    const uint4 y = turn_row<NORM>(v[h], k, static_cast<float>(p.eps));
     // A row whose position is outside the table is zero.
-    const uint4 out = ok ? pack8(y) : make_uint4(0, 0, 0, 0);
-    __nv_bfloat16* dst = now == 0 ? fp.q_out + ((static_cast<int64_t>(b) * p.Hq + h) * p.T + t) * HD
-                                  : fp.k_out + ((static_cast<int64_t>(b) * p.Hkv + h - p.Hq) * p.T + t) * HD;
-    if (row) *reinterpret_cast<uint4*>(dst + lane8 * E) = out;
+    if (it.row)
+      *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(h) * p.T * HD) = ok ? y : make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -173,6 +209,7 @@ __global__ void __launch_bounds__(THREADS) forward_kernel(const __grid_constant_
 
 struct BackwardParams {
   Common c;
+  int total;                           // items
   const __nv_bfloat16* g[3];           // dq, dk [B, H, T, 64] after the rotation, dv; NULL: zero
   int64_t g_sb[3], g_sh[3], g_st[3];
   __nv_bfloat16* dx;                   // [B, T, Hq + 2 Hkv, 64]
@@ -181,77 +218,48 @@ struct BackwardParams {
   int blocks;
 };
 
-// dx of every head (a value head's gradient is copied), and per CTA the sum of dw over its rows, added in a
-// fixed order so that it does not depend on timing: registers, then the CTA's rows through shared memory.
+constexpr int BATCH = 2;   // heads whose x and g are in flight together (backward)
+
+// One item of query or key heads: dx, and dw added to `dw`.
 template <bool NORM>
-__global__ void __launch_bounds__(THREADS) backward_kernel(const __grid_constant__ BackwardParams bp) {
+__device__ __forceinline__ void backward_item(const BackwardParams& bp, const Item& it, int lane8,
+                                              const __nv_bfloat16* src, const __nv_bfloat16* grad, int64_t g_sh,
+                                              __nv_bfloat16* dst, bool ok, const Turn& u, const float (&w)[E],
+                                              float (&dw)[E]) {
   const Common& p = bp.c;
-  const int lane = threadIdx.x & 31, lane8 = lane & 7, warp = threadIdx.x >> 5;
-  const int groups = (p.T + ROWS - 1) / ROWS;
-  const int heads = p.Hq + 2 * p.Hkv;
-  const int64_t items = static_cast<int64_t>(p.B) * groups * p.items_per_group;
-  wait_for_previous_kernel();
-  float w[2][E], dw[2][E];
+#pragma unroll 1
+  for (int h0 = 0; h0 < it.heads; h0 += BATCH) {
+    uint4 xv[BATCH], gv[BATCH];
 #pragma unroll
-  for (int kind = 0; kind < 2; ++kind) {
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      w[kind][i] = 1.0f;
-      dw[kind][i] = 0.0f;
-    }
-    if (NORM) load_weight(p, kind, lane8, w[kind]);
-  }
-  for (int64_t item = static_cast<int64_t>(blockIdx.x) * WARPS + warp; item < items;
-       item += static_cast<int64_t>(gridDim.x) * WARPS) {
-    const int64_t bg = item / p.items_per_group;
-    const int first = static_cast<int>(item % p.items_per_group) * p.heads_per_item;
-    const int last = min(first + p.heads_per_item, heads);
-    const int b = static_cast<int>(bg / groups);
-    const int t = static_cast<int>(bg % groups) * ROWS + (lane >> 3);
-    const bool row = t < p.T;
-    const int64_t pos = row ? position_of(p, b, t) : 0;
-    const bool ok = row && pos >= 0 && pos < p.table_len;
-    if (row && !ok && lane8 == 0) atomicOr(&g_tt_status, TT_ERR_RANGE);
-    Turn u;
-    load_turn(p, ok ? pos : 0, lane8, u);
-    const int tt = row ? t : 0;
-    const __nv_bfloat16* src = p.qkv + b * p.x_sb + static_cast<int64_t>(tt) * p.x_st + lane8 * E;
-    __nv_bfloat16* dst = bp.dx + ((static_cast<int64_t>(b) * p.T + tt) * heads) * HD + lane8 * E;
-#pragma unroll 2
-    for (int h = first; h < last; ++h) {
-      const int part = h < p.Hq ? 0 : h < p.Hq + p.Hkv ? 1 : 2;
-      const int hp = h - (part == 0 ? 0 : part == 1 ? p.Hq : p.Hq + p.Hkv);
-      uint4 gv = make_uint4(0, 0, 0, 0);
-      if (bp.g[part] != nullptr)
-        gv = *reinterpret_cast<const uint4*>(bp.g[part] + b * bp.g_sb[part] + hp * bp.g_sh[part] +
-                                             static_cast<int64_t>(tt) * bp.g_st[part] + lane8 * E);
-      if (part == 2) {
-        if (row) *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(h) * HD) = gv;
-        continue;
+    for (int j = 0; j < BATCH; ++j) {
+      gv[j] = make_uint4(0, 0, 0, 0);
+      if (h0 + j < it.heads) {
+        xv[j] = *reinterpret_cast<const uint4*>(src + (h0 + j) * p.x_sh);
+        if (grad != nullptr) gv[j] = *reinterpret_cast<const uint4*>(grad + (h0 + j) * g_sh);
       }
-      float x[E], gy[E], g[E];
-      unpack8(*reinterpret_cast<const uint4*>(src + h * p.x_sh), x);
-      unpack8(gv, gy);
+    }
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      if (h0 + j >= it.heads) break;
+      float x[E], gy[E], g[E], dx[E];
+      unpack8(xv[j], x);
+      unpack8(gv[j], gy);
+      // Turned back; a row outside the table was not turned but zeroed, and has no gradient.
 #pragma unroll
       for (int i = 0; i < E / 2; ++i) {
-        // A row outside the table was not turned but zeroed: no gradient.
         const float a = ok ? gy[2 * i] : 0.0f, c = ok ? gy[2 * i + 1] : 0.0f;
         g[2 * i] = a * u.c[i] + c * u.s[i];
         g[2 * i + 1] = c * u.c[i] - a * u.s[i];
       }
-      float dx[E];
       if (NORM) {
         const float r = inverse_rms(x, static_cast<float>(p.eps));
         float dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-          const float n = x[i] * r;
-          const float gw = g[i] * (part == 0 ? w[0][i] : w[1][i]);
-          const float add = ok ? g[i] * n : 0.0f;
-          if (part == 0) dw[0][i] += add; else dw[1][i] += add;
-          x[i] = n;
-          g[i] = gw;
-          dot = fmaf(gw, n, dot);
+          x[i] *= r;
+          dw[i] += ok ? g[i] * x[i] : 0.0f;
+          g[i] *= w[i];
+          dot = fmaf(g[i], x[i], dot);
         }
         dot = row_sum(dot) * (1.0f / HD);
 #pragma unroll
@@ -260,8 +268,57 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const __grid_constant
 #pragma unroll
         for (int i = 0; i < E; ++i) dx[i] = ok ? g[i] : 0.0f;
       }
-      if (row) *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(h) * HD) = pack8(dx);
+      if (it.row) *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(h0 + j) * HD) = pack8(dx);
     }
+  }
+}
+
+// dx of every head (a value head's gradient is copied), and per CTA the sum of dw over its rows, added in a
+// fixed order so that it does not depend on timing: registers, then the CTA's rows through shared memory.
+template <bool NORM>
+__global__ void __launch_bounds__(THREADS, 5) backward_kernel(const __grid_constant__ BackwardParams bp) {
+  const Common& p = bp.c;
+  const int lane = threadIdx.x & 31, lane8 = lane & 7, warp = threadIdx.x >> 5;
+  const int heads = p.Hq + 2 * p.Hkv;
+  wait_for_previous_kernel();
+  float dw[2][E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) dw[0][i] = dw[1][i] = 0.0f;
+  for (int index = static_cast<int>(blockIdx.x) * WARPS + warp; index < bp.total;
+       index += static_cast<int>(gridDim.x) * WARPS) {
+    Item it;
+    it.set(p, index, lane);
+    const int64_t t = it.row ? it.t : 0;
+    const __nv_bfloat16* grad = bp.g[it.kind];
+    if (grad != nullptr)
+      grad += it.b * bp.g_sb[it.kind] + it.first * bp.g_sh[it.kind] + t * bp.g_st[it.kind] + lane8 * E;
+    const int64_t g_sh = bp.g_sh[it.kind];
+    __nv_bfloat16* dst =
+        bp.dx + ((static_cast<int64_t>(it.b) * p.T + t) * heads + it.head0(p)) * HD + lane8 * E;
+    if (it.kind == 2) {
+      uint4 v[MAX_HEADS];
+#pragma unroll
+      for (int h = 0; h < MAX_HEADS; ++h) {
+        v[h] = make_uint4(0, 0, 0, 0);
+        if (h < it.heads && grad != nullptr) v[h] = *reinterpret_cast<const uint4*>(grad + h * g_sh);
+      }
+#pragma unroll
+      for (int h = 0; h < MAX_HEADS; ++h)
+        if (h < it.heads && it.row) *reinterpret_cast<uint4*>(dst + h * HD) = v[h];
+      continue;
+    }
+    const int64_t pos = it.row ? position_of(p, it.b, it.t) : 0;
+    const bool ok = it.row && pos >= 0 && pos < p.table_len;
+    if (it.row && !ok && lane8 == 0) atomicOr(&g_tt_status, TT_ERR_RANGE);
+    Turn u;
+    load_turn(p, ok ? pos : 0, lane8, u);
+    float w[E];
+    if (NORM) load_weight(p, it.kind, lane8, w);
+    const __nv_bfloat16* src = p.qkv + it.b * p.x_sb + t * p.x_st + it.head0(p) * p.x_sh + lane8 * E;
+    if (it.kind == 0)
+      backward_item<NORM>(bp, it, lane8, src, grad, g_sh, dst, ok, u, w, dw[0]);
+    else
+      backward_item<NORM>(bp, it, lane8, src, grad, g_sh, dst, ok, u, w, dw[1]);
   }
   if constexpr (NORM) {
     __shared__ float sums[2][WARPS * ROWS][HD];
