@@ -350,7 +350,8 @@ TT_ATTN_API tt_attn_status tt_attn_tree_commit_bf16(
  *   qkv        [batch, q_len, q_heads + 2 kv_heads, 64] bf16 (query, key, value heads), features adjacent, element
  *              strides qkv_strides[3] (batch, token, head) in multiples of 8, 16-byte aligned
  *              (TT_ATTN_UNSUPPORTED otherwise)
- *   q_weight, k_weight  [64] bf16, or FP32 with weights_f32 != 0; both NULL: no norm, the rotation alone
+ *   q_weight, k_weight  [64] bf16, or FP32 with weights_f32 != 0, 16-byte aligned; both NULL: no norm, the
+ *              rotation alone
  *   cos, sin   [table_len, 32] FP32, row = position, 16-byte aligned; used in FP32
  *   position   of token 0 (validated here), or position_dev: token (b, t) is at
  *              position_dev[b * position_sb + t * position_st], + t where position_st is 0

@@ -50,8 +50,8 @@ COMMON = [
     (dict(pos=2**63 - 1), BAD_ARG, "exceeds the cos/sin table"),
     (dict(sb=-1), BAD_ARG, "negative"),
     (dict(dev=20), BAD_ARG, "8-byte"),
-    (dict(kw=17), BAD_ARG, "weights must be aligned"),
-    (dict(qw=18, f32=1), BAD_ARG, "weights must be aligned"),
+    (dict(kw=24), BAD_ARG, "16-byte"),
+    (dict(qw=20, f32=1), BAD_ARG, "16-byte"),
     (dict(sin=8), BAD_ARG, "16-byte"),
     (dict(qkv=24), UNSUPPORTED, "aligned"),
     (dict(strides=_s(5 * 8 * 64 + 4, 8 * 64, 64)), UNSUPPORTED, "multiples of 8"),
@@ -179,7 +179,7 @@ def test_workspace_sizes(lib):
     assert n % (8 * 66 * 4) == 0 and n // (8 * 66 * 4) == 64 * 12 + 148 * 16
     for bad in ((0, 1, 1, 1, 1), (1, 3, 2, 1, 1), (1, 1, 1, 17, 1), (1, 1, 1, 1, 0), (2**40, 1, 1, 1, 1)):
         assert lib.tt_attn_cache4_workspace_size(*bad) == 0
-    assert lib.tt_attn_qkv_norm_rope_backward_workspace_size() % (2 * 64 * 4) == 0
+    assert lib.tt_attn_qkv_norm_rope_backward_workspace_size() % (64 * 4) == 0
 
 
 def test_format_constants_agree():

@@ -41,11 +41,8 @@ tt_attn_status norm_rope_common(const std::string& what, const NormRopeArgs& a, 
     return fail(TT_ATTN_BAD_ARG, what + ": position strides must not be negative");
   if (reinterpret_cast<uintptr_t>(a.position_dev) % 8 != 0)
     return fail(TT_ATTN_BAD_ARG, what + ": the position must be 8-byte aligned");
-  for (const void* w : {a.q_weight, a.k_weight})
-    if (reinterpret_cast<uintptr_t>(w) % (a.weights_f32 ? 4 : 2) != 0)
-      return fail(TT_ATTN_BAD_ARG, what + ": the weights must be aligned to their type");
-  if (!aligned16(a.cos) || !aligned16(a.sin))
-    return fail(TT_ATTN_BAD_ARG, what + ": the cos/sin tables must be 16-byte aligned");
+  if (!aligned16(a.q_weight) || !aligned16(a.k_weight) || !aligned16(a.cos) || !aligned16(a.sin))
+    return fail(TT_ATTN_BAD_ARG, what + ": the weights and the cos/sin tables must be 16-byte aligned");
   const int64_t size[3] = {a.batch, a.q_len, a.q_heads + 2 * a.kv_heads};
   for (int d = 0; d < 3; ++d)
     if (size[d] > 1 && (a.strides[d] <= 0 || a.strides[d] % 8 != 0))
@@ -76,9 +73,9 @@ tt_attn_status norm_rope_common(const std::string& what, const NormRopeArgs& a, 
 }
 
 // Splits the heads of a group of four tokens into warp items: up to four to an item, fewer where that leaves less than
-// `warps` items. Returns the items.
-int norm_rope_items(tt::norm_rope::Common* c, bool values, int64_t warps) {
-  const int64_t groups = static_cast<int64_t>(c->B) * ((c->T + tt::norm_rope::ROWS - 1) / tt::norm_rope::ROWS);
+// `warps` items. Returns the groups.
+int64_t norm_rope_items(tt::norm_rope::Common* c, bool values, int64_t warps) {
+  const int64_t per_seq = (c->T + tt::norm_rope::ROWS - 1) / tt::norm_rope::ROWS, groups = c->B * per_seq;
   const int64_t heads = c->Hq + (values ? 2 : 1) * c->Hkv;
   const int per = static_cast<int>(
       std::max<int64_t>(1, std::min<int64_t>(tt::norm_rope::MAX_HEADS, groups * heads / warps)));
@@ -86,14 +83,17 @@ int norm_rope_items(tt::norm_rope::Common* c, bool values, int64_t warps) {
   c->items[0] = (c->Hq + per - 1) / per;
   c->items[1] = (c->Hkv + per - 1) / per;
   c->items[2] = values ? c->items[1] : 0;
-  return static_cast<int>(groups * (c->items[0] + c->items[1] + c->items[2]));
+  c->groups.set(static_cast<uint32_t>(per_seq));
+  c->per_group.set(static_cast<uint32_t>(c->items[0] + c->items[1] + c->items[2]));
+  for (int i = 0; i < 3; ++i) c->each[i].set(static_cast<uint32_t>(std::max(1, c->items[i])));
+  return groups;
 }
 
 unsigned norm_rope_grid(int64_t items) {
   return static_cast<unsigned>((items + tt::norm_rope::WARPS - 1) / tt::norm_rope::WARPS);
 }
 
-constexpr int64_t kNormBackwardCtas = 5 * kPlanSms;   // also the rows of its workspace
+constexpr int64_t kNormBackwardCtas = 5 * kPlanSms;   // but for rounding; its workspace has a row for each
 
 // ------------------------------------------------------------------ 4-bit cache
 
@@ -241,7 +241,7 @@ TT_ATTN_API tt_attn_status tt_attn_qkv_norm_rope_bf16(
   if ((st = prepare_device(&dev)) != TT_ATTN_OK) return st;
   p.out[0] = static_cast<__nv_bfloat16*>(q_out);
   p.out[1] = static_cast<__nv_bfloat16*>(k_out);
-  p.total = norm_rope_items(&p.c, false, 16 * kPlanSms);
+  p.total = static_cast<int>(norm_rope_items(&p.c, false, 16 * kPlanSms) * p.c.per_group.d);
   const Launch launch(dim3(norm_rope_grid(p.total)), nr::THREADS, 0, 1, static_cast<cudaStream_t>(stream));
   const cudaError_t le = q_weight != nullptr ? cudaLaunchKernelEx(&launch.cfg, nr::forward_kernel<true>, p)
                                              : cudaLaunchKernelEx(&launch.cfg, nr::forward_kernel<false>, p);
@@ -249,7 +249,7 @@ TT_ATTN_API tt_attn_status tt_attn_qkv_norm_rope_bf16(
 }
 
 TT_ATTN_API size_t tt_attn_qkv_norm_rope_backward_workspace_size(void) {
-  return static_cast<size_t>(kNormBackwardCtas) * 2 * TT_ATTN_HEAD_DIM * sizeof(float);
+  return static_cast<size_t>(kNormBackwardCtas + 2) * TT_ATTN_HEAD_DIM * sizeof(float);
 }
 
 TT_ATTN_API tt_attn_status tt_attn_qkv_norm_rope_backward_bf16(
@@ -299,14 +299,22 @@ TT_ATTN_API tt_attn_status tt_attn_qkv_norm_rope_backward_bf16(
   p.partial = static_cast<float*>(workspace);
   p.dw[0] = dq_weight;
   p.dw[1] = dk_weight;
-  p.total = norm_rope_items(&p.c, true, 16 * kPlanSms);
-  p.blocks = static_cast<int>(std::min<int64_t>(norm_rope_grid(p.total), kNormBackwardCtas));
+  // CTAs for each kind of heads in proportion to what they read and write: x, dy and dx, or dv twice.
+  const int64_t groups = norm_rope_items(&p.c, true, 16 * kPlanSms);
+  const int64_t weight[3] = {3 * q_heads, 3 * kv_heads, 2 * kv_heads}, sum = weight[0] + weight[1] + weight[2];
+  int64_t blocks = 0;
+  for (int i = 0; i < 3; ++i) {
+    p.total[i] = static_cast<int>(groups * p.c.items[i]);
+    p.ctas[i] = static_cast<int>(std::max<int64_t>(
+        1, std::min<int64_t>(norm_rope_grid(p.total[i]), kNormBackwardCtas * weight[i] / sum)));
+    blocks += p.ctas[i];
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const Launch launch(dim3(static_cast<unsigned>(p.blocks)), nr::THREADS, 0, 1, s);
+  const Launch launch(dim3(static_cast<unsigned>(blocks)), nr::THREADS, 0, 1, s);
   cudaError_t le = norm ? cudaLaunchKernelEx(&launch.cfg, nr::backward_kernel<true>, p)
                         : cudaLaunchKernelEx(&launch.cfg, nr::backward_kernel<false>, p);
   if (le == cudaSuccess && norm) {
-    const Launch reduce(dim3(2 * nr::HD / nr::REDUCE_FEATURES), 32 * nr::REDUCE_FEATURES, 0, 1, s);
+    const Launch reduce(dim3(2 * nr::HD / nr::REDUCE_FEATURES), nr::REDUCE_THREADS * nr::REDUCE_FEATURES, 0, 1, s);
     le = cudaLaunchKernelEx(&reduce.cfg, nr::reduce_kernel, p);
   }
   return check_launch("qkv_norm_rope backward launch", le);
@@ -340,7 +348,7 @@ TT_ATTN_API tt_attn_status tt_attn_cache4_append_bf16(
   int dev = 0;
   if ((st = prepare_device(&dev)) != TT_ATTN_OK) return st;
   p.q_out = static_cast<__nv_bfloat16*>(q_out);
-  p.total = norm_rope_items(&p.c, true, 16 * kPlanSms);
+  p.total = static_cast<int>(norm_rope_items(&p.c, true, 16 * kPlanSms) * p.c.per_group.d);
   const Launch launch(dim3(norm_rope_grid(p.total)), nr::THREADS, 0, 1, static_cast<cudaStream_t>(stream));
   const cudaError_t le = q_weight != nullptr ? cudaLaunchKernelEx(&launch.cfg, c4::append_kernel<true>, p)
                                              : cudaLaunchKernelEx(&launch.cfg, c4::append_kernel<false>, p);

@@ -33,6 +33,21 @@ constexpr int LANES = 8;  // lanes of a row
 constexpr int E = HD / LANES;
 constexpr int MAX_HEADS = 4;
 
+// Division of n < 2^31 by a number known on the host (Granlund and Montgomery, 1994): a product and a shift.
+struct Divisor {
+  uint32_t d, multiply, shift;
+
+  void set(uint32_t by) {
+    d = by;
+    shift = 0;
+    while ((1ull << shift) < by) ++shift;
+    multiply = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - by)) / by + 1);
+  }
+  __device__ __forceinline__ int of(int n) const {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), multiply) + static_cast<uint32_t>(n)) >> shift);
+  }
+};
+
 // What a call of any of the kernels here and of the cache's append has in common.
 struct Common {
   const __nv_bfloat16* qkv;
@@ -40,6 +55,7 @@ struct Common {
   int B, T, Hq, Hkv;
   int per_item;               // heads of an item, at most MAX_HEADS
   int items[3];               // items of the query, key and value heads of a group of four tokens
+  Divisor groups, per_group, each[3];   // divisions by groups, by all items of one, by those of a kind
   const void* w[2];           // q and k weight [64], both NULL: no norm
   bool w_f32;                 // else bf16
   const float* cos;           // [table_len, 32]
@@ -68,12 +84,23 @@ __device__ __forceinline__ void load_turn(const Common& p, int64_t pos, int lane
   u.s[0] = s.x; u.s[1] = s.y; u.s[2] = s.z; u.s[3] = s.w;
 }
 
-__device__ __forceinline__ void load_weight(const Common& p, int kind, int lane8, float (&w)[E]) {
+__device__ __forceinline__ void unpack8(const uint4& v, float (&x)[E]) {
+  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const int at = lane8 * E + i;
-    w[i] = p.w_f32 ? static_cast<const float*>(p.w[kind])[at]
-                   : __bfloat162float(static_cast<const __nv_bfloat16*>(p.w[kind])[at]);
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = bf16_lo(u[i]);
+    x[2 * i + 1] = bf16_hi(u[i]);
+  }
+}
+
+__device__ __forceinline__ void load_weight(const Common& p, int kind, int lane8, float (&w)[E]) {
+  if (p.w_f32) {
+    const float* src = static_cast<const float*>(p.w[kind]) + lane8 * E;
+    const float4 lo = *reinterpret_cast<const float4*>(src), hi = *reinterpret_cast<const float4*>(src + 4);
+    w[0] = lo.x; w[1] = lo.y; w[2] = lo.z; w[3] = lo.w;
+    w[4] = hi.x; w[5] = hi.y; w[6] = hi.z; w[7] = hi.w;
+  } else {
+    unpack8(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.w[kind]) + lane8 * E), w);
   }
 }
 
@@ -85,30 +112,24 @@ struct Item {
   bool row;          // this lane's token is there
 
   __device__ __forceinline__ void set(const Common& p, int index, int lane) {
-    const int per_group = p.items[0] + p.items[1] + p.items[2], groups = (p.T + ROWS - 1) / ROWS;
-    const int bg = index / per_group;
-    int at = index - bg * per_group;
-    kind = at < p.items[0] ? 0 : at < p.items[0] + p.items[1] ? 1 : 2;
-    at -= kind == 0 ? 0 : kind == 1 ? p.items[0] : p.items[0] + p.items[1];
+    const int bg = p.per_group.of(index);
+    const int at = index - bg * static_cast<int>(p.per_group.d);
+    const int k = at < p.items[0] ? 0 : at < p.items[0] + p.items[1] ? 1 : 2;
+    set_kind(p, k, bg, at - (k == 0 ? 0 : k == 1 ? p.items[0] : p.items[0] + p.items[1]), lane);
+  }
+  // Item `at` of kind k in group bg.
+  __device__ __forceinline__ void set_kind(const Common& p, int k, int bg, int at, int lane) {
+    kind = k;
     first = at * p.per_item;
     heads = min(p.per_item, (kind == 0 ? p.Hq : p.Hkv) - first);
-    b = bg / groups;
-    t = (bg - b * groups) * ROWS + (lane >> 3);
+    b = p.groups.of(bg);
+    t = (bg - b * static_cast<int>(p.groups.d)) * ROWS + (lane >> 3);
     row = t < p.T;
   }
   __device__ __forceinline__ int head0(const Common& p) const {   // of the projection
     return first + (kind == 0 ? 0 : kind == 1 ? p.Hq : p.Hq + p.Hkv);
   }
 };
-
-__device__ __forceinline__ void unpack8(const uint4& v, float (&x)[E]) {
-  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = bf16_lo(u[i]);
-    x[2 * i + 1] = bf16_hi(u[i]);
-  }
-}
 
 __device__ __forceinline__ uint4 pack8(const float (&y)[E]) {
   return make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
@@ -209,150 +230,147 @@ __global__ void __launch_bounds__(THREADS) forward_kernel(const __grid_constant_
 
 struct BackwardParams {
   Common c;
-  int total;                           // items
+  int total[3], ctas[3];               // items of each kind of heads, and CTAs for them (0 where none)
   const __nv_bfloat16* g[3];           // dq, dk [B, H, T, 64] after the rotation, dv; NULL: zero
   int64_t g_sb[3], g_sh[3], g_st[3];
   __nv_bfloat16* dx;                   // [B, T, Hq + 2 Hkv, 64]
-  float* partial;                      // [grid, 2, 64]: this CTA's sums of dw
+  float* partial;                      // [query and key CTAs, 64]: their sums of dw
   void* dw[2];                         // in the weights' type
-  int blocks;
 };
 
-constexpr int BATCH = 2;   // heads whose x and g are in flight together (backward)
-
-// One item of query or key heads: dx, and dw added to `dw`.
-template <bool NORM>
-__device__ __forceinline__ void backward_item(const BackwardParams& bp, const Item& it, int lane8,
-                                              const __nv_bfloat16* src, const __nv_bfloat16* grad, int64_t g_sh,
-                                              __nv_bfloat16* dst, bool ok, const Turn& u, const float (&w)[E],
-                                              float (&dw)[E]) {
-  const Common& p = bp.c;
-#pragma unroll 1
-  for (int h0 = 0; h0 < it.heads; h0 += BATCH) {
-    uint4 xv[BATCH], gv[BATCH];
-#pragma unroll
-    for (int j = 0; j < BATCH; ++j) {
-      gv[j] = make_uint4(0, 0, 0, 0);
-      if (h0 + j < it.heads) {
-        xv[j] = *reinterpret_cast<const uint4*>(src + (h0 + j) * p.x_sh);
-        if (grad != nullptr) gv[j] = *reinterpret_cast<const uint4*>(grad + (h0 + j) * g_sh);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < BATCH; ++j) {
-      if (h0 + j >= it.heads) break;
-      float x[E], gy[E], g[E], dx[E];
-      unpack8(xv[j], x);
-      unpack8(gv[j], gy);
-      // Turned back; a row outside the table was not turned but zeroed, and has no gradient.
-#pragma unroll
-      for (int i = 0; i < E / 2; ++i) {
-        const float a = ok ? gy[2 * i] : 0.0f, c = ok ? gy[2 * i + 1] : 0.0f;
-        g[2 * i] = a * u.c[i] + c * u.s[i];
-        g[2 * i + 1] = c * u.c[i] - a * u.s[i];
-      }
-      if (NORM) {
-        const float r = inverse_rms(x, static_cast<float>(p.eps));
-        float dot = 0.0f;
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          x[i] *= r;
-          dw[i] += ok ? g[i] * x[i] : 0.0f;
-          g[i] *= w[i];
-          dot = fmaf(g[i], x[i], dot);
-        }
-        dot = row_sum(dot) * (1.0f / HD);
-#pragma unroll
-        for (int i = 0; i < E; ++i) dx[i] = ok ? (g[i] - x[i] * dot) * r : 0.0f;
-      } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i) dx[i] = ok ? g[i] : 0.0f;
-      }
-      if (it.row) *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(h0 + j) * HD) = pack8(dx);
-    }
-  }
-}
-
-// dx of every head (a value head's gradient is copied), and per CTA the sum of dw over its rows, added in a
-// fixed order so that it does not depend on timing: registers, then the CTA's rows through shared memory.
+// A CTA's items are of one kind. Query and key heads: dx, and dw summed over the CTA's rows in a fixed order, so
+// that it does not depend on timing (registers, then shared memory). Value heads: dv copied.
 template <bool NORM>
 __global__ void __launch_bounds__(THREADS, 5) backward_kernel(const __grid_constant__ BackwardParams bp) {
   const Common& p = bp.c;
   const int lane = threadIdx.x & 31, lane8 = lane & 7, warp = threadIdx.x >> 5;
   const int heads = p.Hq + 2 * p.Hkv;
+  int cta = static_cast<int>(blockIdx.x), kind = 0;
+  while (cta >= bp.ctas[kind]) cta -= bp.ctas[kind++];
+  const int total = bp.total[kind], stride = bp.ctas[kind] * WARPS;
+  const __nv_bfloat16* const grad0 = bp.g[kind];
+  const int64_t g_sb = bp.g_sb[kind], g_sh = bp.g_sh[kind], g_st = bp.g_st[kind];
   wait_for_previous_kernel();
-  float dw[2][E];
-#pragma unroll
-  for (int i = 0; i < E; ++i) dw[0][i] = dw[1][i] = 0.0f;
-  for (int index = static_cast<int>(blockIdx.x) * WARPS + warp; index < bp.total;
-       index += static_cast<int>(gridDim.x) * WARPS) {
-    Item it;
-    it.set(p, index, lane);
-    const int64_t t = it.row ? it.t : 0;
-    const __nv_bfloat16* grad = bp.g[it.kind];
-    if (grad != nullptr)
-      grad += it.b * bp.g_sb[it.kind] + it.first * bp.g_sh[it.kind] + t * bp.g_st[it.kind] + lane8 * E;
-    const int64_t g_sh = bp.g_sh[it.kind];
-    __nv_bfloat16* dst =
-        bp.dx + ((static_cast<int64_t>(it.b) * p.T + t) * heads + it.head0(p)) * HD + lane8 * E;
-    if (it.kind == 2) {
+  if (kind == 2) {
+    for (int index = cta * WARPS + warp; index < total; index += stride) {
+      Item it;
+      const int bg = p.each[2].of(index);
+      it.set_kind(p, 2, bg, index - bg * static_cast<int>(p.each[2].d), lane);
+      if (!it.row) continue;
+      const __nv_bfloat16* grad = grad0 + it.b * g_sb + it.first * g_sh + it.t * g_st + lane8 * E;
+      __nv_bfloat16* dst =
+          bp.dx + ((static_cast<int64_t>(it.b) * p.T + it.t) * heads + it.head0(p)) * HD + lane8 * E;
       uint4 v[MAX_HEADS];
 #pragma unroll
       for (int h = 0; h < MAX_HEADS; ++h) {
         v[h] = make_uint4(0, 0, 0, 0);
-        if (h < it.heads && grad != nullptr) v[h] = *reinterpret_cast<const uint4*>(grad + h * g_sh);
+        if (h < it.heads && grad0 != nullptr) v[h] = *reinterpret_cast<const uint4*>(grad + h * g_sh);
       }
 #pragma unroll
       for (int h = 0; h < MAX_HEADS; ++h)
-        if (h < it.heads && it.row) *reinterpret_cast<uint4*>(dst + h * HD) = v[h];
-      continue;
+        if (h < it.heads) *reinterpret_cast<uint4*>(dst + h * HD) = v[h];
     }
+    return;
+  }
+  float w[E], dw[E];
+  if (NORM) load_weight(p, kind, lane8, w);
+#pragma unroll
+  for (int i = 0; i < E; ++i) dw[i] = 0.0f;
+  for (int index = cta * WARPS + warp; index < total; index += stride) {
+    Item it;
+    const int bg = p.each[kind].of(index);
+    it.set_kind(p, kind, bg, index - bg * static_cast<int>(p.each[kind].d), lane);
     const int64_t pos = it.row ? position_of(p, it.b, it.t) : 0;
     const bool ok = it.row && pos >= 0 && pos < p.table_len;
     if (it.row && !ok && lane8 == 0) atomicOr(&g_tt_status, TT_ERR_RANGE);
+    const int64_t t = it.row ? it.t : 0;
+    const __nv_bfloat16* src = p.qkv + it.b * p.x_sb + t * p.x_st + it.head0(p) * p.x_sh + lane8 * E;
+    const __nv_bfloat16* grad = grad0 + it.b * g_sb + it.first * g_sh + t * g_st + lane8 * E;
+    __nv_bfloat16* dst = bp.dx + ((static_cast<int64_t>(it.b) * p.T + t) * heads + it.head0(p)) * HD + lane8 * E;
+    // A row outside the table was not turned but zeroed: its x and g count as zeros.
+    uint4 xv[MAX_HEADS], gv[MAX_HEADS];
+#pragma unroll
+    for (int h = 0; h < MAX_HEADS; ++h) {
+      xv[h] = gv[h] = make_uint4(0, 0, 0, 0);
+      if (h < it.heads && ok) {
+        xv[h] = *reinterpret_cast<const uint4*>(src + h * p.x_sh);
+        if (grad0 != nullptr) gv[h] = *reinterpret_cast<const uint4*>(grad + h * g_sh);
+      }
+    }
     Turn u;
     load_turn(p, ok ? pos : 0, lane8, u);
-    float w[E];
-    if (NORM) load_weight(p, it.kind, lane8, w);
-    const __nv_bfloat16* src = p.qkv + it.b * p.x_sb + t * p.x_st + it.head0(p) * p.x_sh + lane8 * E;
-    if (it.kind == 0)
-      backward_item<NORM>(bp, it, lane8, src, grad, g_sh, dst, ok, u, w, dw[0]);
-    else
-      backward_item<NORM>(bp, it, lane8, src, grad, g_sh, dst, ok, u, w, dw[1]);
+#pragma unroll
+    for (int h = 0; h < MAX_HEADS; ++h) {
+      if (h >= it.heads) break;
+      float x[E], gy[E], g[E], dx[E];
+      unpack8(xv[h], x);
+      unpack8(gv[h], gy);
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) {
+        g[2 * i] = gy[2 * i] * u.c[i] + gy[2 * i + 1] * u.s[i];
+        g[2 * i + 1] = gy[2 * i + 1] * u.c[i] - gy[2 * i] * u.s[i];
+      }
+      if (NORM) {
+        const float rms = inverse_rms(x, static_cast<float>(p.eps));   // all lanes: it shuffles
+        const float r = ok ? rms : 0.0f;
+        float dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          x[i] *= r;
+          dw[i] = fmaf(g[i], x[i], dw[i]);
+          g[i] *= w[i];
+          dot = fmaf(g[i], x[i], dot);
+        }
+        dot = row_sum(dot) * (1.0f / HD);
+#pragma unroll
+        for (int i = 0; i < E; ++i) dx[i] = (g[i] - x[i] * dot) * r;
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) dx[i] = g[i];
+      }
+      if (it.row) *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(h) * HD) = pack8(dx);
+    }
   }
   if constexpr (NORM) {
-    __shared__ float sums[2][WARPS * ROWS][HD];
+    __shared__ float sums[WARPS * ROWS][HD];
 #pragma unroll
-    for (int kind = 0; kind < 2; ++kind)
-#pragma unroll
-      for (int i = 0; i < E; ++i) sums[kind][warp * ROWS + (lane >> 3)][lane8 * E + i] = dw[kind][i];
+    for (int i = 0; i < E; ++i) sums[warp * ROWS + (lane >> 3)][lane8 * E + i] = dw[i];
     __syncthreads();
-    for (int i = threadIdx.x; i < 2 * HD; i += THREADS) {
+    if (threadIdx.x < HD) {
       float s = 0.0f;
 #pragma unroll
-      for (int j = 0; j < WARPS * ROWS; ++j) s += sums[i / HD][j][i % HD];
-      bp.partial[static_cast<int64_t>(blockIdx.x) * 2 * HD + i] = s;
+      for (int j = 0; j < WARPS * ROWS; ++j) s += sums[j][threadIdx.x];
+      bp.partial[static_cast<int64_t>(blockIdx.x) * HD + threadIdx.x] = s;
     }
   }
 }
 
-// dw: the CTAs' sums, added in a fixed order. One block for eight of the 128 features; 32 threads a feature.
+// dw: the CTAs' sums, added in a fixed order. One block for eight of the 128 features; 64 threads a feature.
 constexpr int REDUCE_FEATURES = 8;
+constexpr int REDUCE_THREADS = 64;
 
-__global__ void __launch_bounds__(32 * REDUCE_FEATURES)
+__global__ void __launch_bounds__(REDUCE_THREADS * REDUCE_FEATURES)
     reduce_kernel(const __grid_constant__ BackwardParams bp) {
-  __shared__ double part[32][REDUCE_FEATURES + 1];
+  __shared__ double part[REDUCE_THREADS][REDUCE_FEATURES + 1];
   const int f = threadIdx.x % REDUCE_FEATURES, j = threadIdx.x / REDUCE_FEATURES;
-  const int at = blockIdx.x * REDUCE_FEATURES + f;
+  const int at = blockIdx.x * REDUCE_FEATURES + f, kind = at / HD;
+  const float* src = bp.partial + static_cast<int64_t>(kind == 0 ? 0 : bp.ctas[0]) * HD + at % HD;
   wait_for_previous_kernel();
   double s = 0.0;
-#pragma unroll 4
-  for (int i = j; i < bp.blocks; i += 32) s += bp.partial[static_cast<int64_t>(i) * 2 * HD + at];
+#pragma unroll 8
+  for (int i = j; i < bp.ctas[kind]; i += REDUCE_THREADS) s += src[static_cast<int64_t>(i) * HD];
   part[j][f] = s;
   __syncthreads();
+  if (j >= 8) return;
+#pragma unroll
+  for (int i = 8; i < REDUCE_THREADS; i += 8) s += part[j + i][f];
+  // The eight sums of a feature are in lanes f, f + 8, .. of two warps.
+  part[j][f] = s;
+  __syncwarp();
+  asm volatile("bar.sync 1, 64;" ::: "memory");
   if (j != 0) return;
-  for (int i = 1; i < 32; ++i) s += part[i][f];
-  void* out = bp.dw[at / HD];
+  for (int i = 1; i < 8; ++i) s += part[i][f];
+  void* out = bp.dw[kind];
   if (bp.c.w_f32)
     static_cast<float*>(out)[at % HD] = static_cast<float>(s);
   else

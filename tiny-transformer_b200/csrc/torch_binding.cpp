@@ -651,8 +651,8 @@ NormWeights norm_weights(const std::optional<torch::Tensor>& q, const std::optio
                     t->scalar_type() == q->scalar_type(),
                 what, ": norm weights must both be bf16 or both be float32");
   }
-  w.q = q->contiguous();
-  w.k = k->contiguous();
+  w.q = contiguous_aligned(*q);
+  w.k = contiguous_aligned(*k);
   w.f32 = q->scalar_type() == at::kFloat;
   return w;
 }
