@@ -72,8 +72,8 @@ tt_attn_status norm_rope_common(const std::string& what, const NormRopeArgs& a, 
   return TT_ATTN_OK;
 }
 
-// Splits the heads of a group of four tokens into warp items: up to four to an item, fewer where that leaves less than
-// `warps` items. Returns the groups.
+// Splits the heads of a group of four tokens into warp items: up to sixteen to an item, fewer where that leaves less than
+// `warps` items. Returns the items.
 int64_t norm_rope_items(tt::norm_rope::Common* c, bool values, int64_t warps) {
   const int64_t per_seq = (c->T + tt::norm_rope::ROWS - 1) / tt::norm_rope::ROWS, groups = c->B * per_seq;
   const int64_t heads = c->Hq + (values ? 2 : 1) * c->Hkv;
@@ -84,9 +84,13 @@ int64_t norm_rope_items(tt::norm_rope::Common* c, bool values, int64_t warps) {
   c->items[1] = (c->Hkv + per - 1) / per;
   c->items[2] = values ? c->items[1] : 0;
   c->groups.set(static_cast<uint32_t>(per_seq));
-  c->per_group.set(static_cast<uint32_t>(c->items[0] + c->items[1] + c->items[2]));
-  for (int i = 0; i < 3; ++i) c->each[i].set(static_cast<uint32_t>(std::max(1, c->items[i])));
-  return groups;
+  int64_t all = 0;
+  for (int i = 0; i < 3; ++i) {
+    c->each[i].set(static_cast<uint32_t>(std::max(1, c->items[i])));
+    c->total[i] = static_cast<int>(groups * c->items[i]);
+    all += c->total[i];
+  }
+  return all;
 }
 
 unsigned norm_rope_grid(int64_t items) {
@@ -241,8 +245,8 @@ TT_ATTN_API tt_attn_status tt_attn_qkv_norm_rope_bf16(
   if ((st = prepare_device(&dev)) != TT_ATTN_OK) return st;
   p.out[0] = static_cast<__nv_bfloat16*>(q_out);
   p.out[1] = static_cast<__nv_bfloat16*>(k_out);
-  p.total = static_cast<int>(norm_rope_items(&p.c, false, 16 * kPlanSms) * p.c.per_group.d);
-  const Launch launch(dim3(norm_rope_grid(p.total)), nr::THREADS, 0, 1, static_cast<cudaStream_t>(stream));
+  const int64_t items = norm_rope_items(&p.c, false, 16 * kPlanSms);
+  const Launch launch(dim3(norm_rope_grid(items)), nr::THREADS, 0, 1, static_cast<cudaStream_t>(stream));
   const cudaError_t le = q_weight != nullptr ? cudaLaunchKernelEx(&launch.cfg, nr::forward_kernel<true>, p)
                                              : cudaLaunchKernelEx(&launch.cfg, nr::forward_kernel<false>, p);
   return check_launch("qkv_norm_rope launch", le);
@@ -300,13 +304,12 @@ TT_ATTN_API tt_attn_status tt_attn_qkv_norm_rope_backward_bf16(
   p.dw[0] = dq_weight;
   p.dw[1] = dk_weight;
   // CTAs for each kind of heads in proportion to what they read and write: x, dy and dx, or dv twice.
-  const int64_t groups = norm_rope_items(&p.c, true, 16 * kPlanSms);
+  norm_rope_items(&p.c, true, 16 * kPlanSms);
   const int64_t weight[3] = {3 * q_heads, 3 * kv_heads, 2 * kv_heads}, sum = weight[0] + weight[1] + weight[2];
   int64_t blocks = 0;
   for (int i = 0; i < 3; ++i) {
-    p.total[i] = static_cast<int>(groups * p.c.items[i]);
     p.ctas[i] = static_cast<int>(std::max<int64_t>(
-        1, std::min<int64_t>(norm_rope_grid(p.total[i]), kNormBackwardCtas * weight[i] / sum)));
+        1, std::min<int64_t>(norm_rope_grid(p.c.total[i]), kNormBackwardCtas * weight[i] / sum)));
     blocks += p.ctas[i];
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -348,8 +351,8 @@ TT_ATTN_API tt_attn_status tt_attn_cache4_append_bf16(
   int dev = 0;
   if ((st = prepare_device(&dev)) != TT_ATTN_OK) return st;
   p.q_out = static_cast<__nv_bfloat16*>(q_out);
-  p.total = static_cast<int>(norm_rope_items(&p.c, true, 16 * kPlanSms) * p.c.per_group.d);
-  const Launch launch(dim3(norm_rope_grid(p.total)), nr::THREADS, 0, 1, static_cast<cudaStream_t>(stream));
+  const int64_t items = norm_rope_items(&p.c, true, 16 * kPlanSms);
+  const Launch launch(dim3(norm_rope_grid(items)), nr::THREADS, 0, 1, static_cast<cudaStream_t>(stream));
   const cudaError_t le = q_weight != nullptr ? cudaLaunchKernelEx(&launch.cfg, c4::append_kernel<true>, p)
                                              : cudaLaunchKernelEx(&launch.cfg, c4::append_kernel<false>, p);
   return check_launch("cache4_append launch", le);

@@ -15,9 +15,10 @@
 // In the same way max|x| times 1/6 is off by 2^-23, a tie of the scale has 5 significant bits, and rounding to 20 bits
 // first restores it. A group with a NaN gets the scale NaN; infinities saturate.
 //
-// Append: key rows are the bf16 values of the rotation, correctly rounded: an error of the last bit next to a
-// border would be a whole step of a code. FP32 decides wherever the value is farther from a bf16 border than
-// its error bound; the others (about one in 2^11) are computed again in FP64.
+// Append: key rows are quantised from the bf16 values of the rotation, correctly rounded: an error of the last bit
+// next to a border would be a whole step of a code. FP32 decides wherever a value is farther from a bf16 border
+// than its error bound. Of the others (one in 2^10) both neighbours are quantised, and where that gives different
+// codes the row is computed again in FP64.
 //
 // Both kernels are bound by memory (append: 128 bytes a head in, 128 or 36 out; read: 36 in, 128 out).
 #pragma once
@@ -92,10 +93,12 @@ __device__ __forceinline__ uint32_t quantise8(const uint4& v, uint32_t& codes) {
   if (byte == 0) inv = 0.0f;
   if (top > 0x7f80u) byte = 0xffu;
   float y[8];
+  const uint64_t inv2 = f2_pack(inv, inv);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    y[2 * i] = __fadd_rn(__fmaf_rn(bf16_lo(u[i]), inv, 1536.0f), -1536.0f);
-    y[2 * i + 1] = __fadd_rn(__fmaf_rn(bf16_hi(u[i]), inv, 1536.0f), -1536.0f);
+    const uint64_t x = f2_pack(bf16_lo(u[i]), bf16_hi(u[i]));
+    f2_unpack(f2_add(f2_fma(x, inv2, f2_pack(1536.0f, 1536.0f)), f2_pack(-1536.0f, -1536.0f)), y[2 * i],
+              y[2 * i + 1]);
   }
   asm("{\n\t.reg .b8 a, b, c, d;\n\t"
       "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
@@ -121,10 +124,9 @@ struct RowPlace {
   }
 };
 
-// Quantises a row (8 features a lane) and stores its codes and scales.
-__device__ __forceinline__ void store_row(const RowPlace& at, int64_t head, int lane8, bool ok, const uint4& v) {
-  uint32_t codes;
-  const uint32_t byte = quantise8(v, codes);
+// Stores a row's codes and scales (each lane its word and its group's byte).
+__device__ __forceinline__ void store_row(const RowPlace& at, int64_t head, int lane8, bool ok, uint32_t codes,
+                                          uint32_t byte) {
   uint32_t scales = (lane8 & 1) ? 0u : byte << (4 * lane8);
   scales |= __shfl_xor_sync(0xffffffffu, scales, 2);
   scales |= __shfl_xor_sync(0xffffffffu, scales, 4);
@@ -137,34 +139,57 @@ __device__ __forceinline__ void store_row(const RowPlace& at, int64_t head, int 
 
 struct AppendParams {
   norm_rope::Common c;
-  int total;              // items
   __nv_bfloat16* q_out;   // [B, Hq, T, 64]
   View cache[2];          // keys, values
   int64_t capacity;       // rows
 };
 
-// The bf16 values of a key row from FP32; false in a lane that cannot tell how one of them is rounded.
+// The bf16 values of a key row from FP32, `up` those from above; they differ where FP32 cannot tell how a value is
+// rounded. `most` is the largest coefficient of each pair, times 2^-20.
 template <bool NORM>
-__device__ __forceinline__ bool key_row(const uint4& v, const norm_rope::Coefficients& k, float eps, uint4& out) {
-  constexpr int E = norm_rope::E;
-  constexpr float UNIT = 9.5367431640625e-07f;   // 2^-20
-  float x[E];
-  norm_rope::unpack8(v, x);
-  const float r = NORM ? norm_rope::inverse_rms(x, eps) : 1.0f;
-  uint32_t y[4];
-  bool sure = true;
+__device__ __forceinline__ void key_row(const uint4& v, const norm_rope::Coefficients& k, const uint64_t (&most)[2],
+                                        float eps, uint4& out, uint4& up) {
+  norm_rope::Pairs x;
+  x.unpack(v);
+  if (NORM) x.scale(norm_rope::inverse_rms(x, eps));
+  const norm_rope::Pairs y = k.turn(x);
+  norm_rope::Pairs lo, hi;
 #pragma unroll
-  for (int i = 0; i < E / 2; ++i) {
-    const float a = x[2 * i] * r, b = x[2 * i + 1] * r;
-    const float a0 = a * k.ec[i], b0 = b * k.os[i], a1 = a * k.es[i], b1 = b * k.oc[i];
-    const float y0 = a0 - b0, y1 = a1 + b1;
-    // In units of 2^-20 of the terms: rsqrtf .25, the sum of squares .35, six roundings .0625 each.
-    const float m0 = fabsf(a0) + fabsf(b0), m1 = fabsf(a1) + fabsf(b1);
-    y[i] = pack_bf16x2(fmaf(m0, -UNIT, y0), fmaf(m1, -UNIT, y1));
-    sure = sure && y[i] == pack_bf16x2(fmaf(m0, UNIT, y0), fmaf(m1, UNIT, y1));
+  for (int i = 0; i < 2; ++i) {
+    // An element's terms are below (|x_2i| + |x_2i+1|) most; in units of 2^-20 of that it is off by: rsqrtf .25,
+    // the sum of squares .25 (8 roundings), eps .03, five more roundings .0625 each, and the one here.
+    float e0, e1, o0, o1;
+    f2_unpack(x.e[i], e0, e1);
+    f2_unpack(x.o[i], o0, o1);
+    const uint64_t size = f2_pack(fabsf(e0) + fabsf(o0), fabsf(e1) + fabsf(o1));
+    const uint64_t off = f2_mul(size, most[i]), minus = f2_pack(-1.0f, -1.0f);
+    lo.e[i] = f2_fma(off, minus, y.e[i]);
+    lo.o[i] = f2_fma(off, minus, y.o[i]);
+    hi.e[i] = f2_add(off, y.e[i]);
+    hi.o[i] = f2_add(off, y.o[i]);
   }
-  out = make_uint4(y[0], y[1], y[2], y[3]);
-  return sure;
+  out = lo.pack();
+  up = hi.pack();
+}
+
+__device__ __forceinline__ uint32_t min_u16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("min.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+// Two candidates for each value to the smaller and the larger magnitudes. The true row lies between these in every
+// place, and scales and codes grow with magnitudes: where both have the same, it has them too. (Candidates of different
+// signs keep the first one's; next to zero both codes are zero.)
+__device__ __forceinline__ void order(uint4& a, uint4& b) {
+  uint32_t* x[4] = {&a.x, &a.y, &a.z, &a.w};
+  uint32_t* y[4] = {&b.x, &b.y, &b.z, &b.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t sign = *x[i] & 0x80008000u, p = *x[i] & 0x7fff7fffu, q = *y[i] & 0x7fff7fffu;
+    *x[i] = min_u16x2(p, q) | sign;
+    *y[i] = max_u16x2(p, q) | sign;
+  }
 }
 
 // The same from FP64: correctly rounded but for FP64's own errors.
@@ -198,22 +223,29 @@ __device__ __forceinline__ uint4 key_row_exact(const norm_rope::Common& p, const
 }
 
 template <bool NORM>
-__global__ void __launch_bounds__(norm_rope::THREADS)
+__global__ void __launch_bounds__(norm_rope::THREADS, 7)
     append_kernel(const __grid_constant__ AppendParams ap) {
   namespace nr = norm_rope;
   const nr::Common& p = ap.c;
   const int lane = threadIdx.x & 31, lane8 = lane & 7;
-  const int index = static_cast<int>(blockIdx.x) * nr::WARPS + (threadIdx.x >> 5);
+  // Keys first: they take longest.
+  int index = static_cast<int>(blockIdx.x) * nr::WARPS + (threadIdx.x >> 5), kind = 1;
   wait_for_previous_kernel();
-  if (index >= ap.total) return;  // whole warps
+  if (index >= p.total[1]) {
+    index -= p.total[1];
+    kind = 2;
+    if (index >= p.total[2]) {
+      index -= p.total[2];
+      kind = 0;
+    }
+  }
+  if (index >= p.total[kind]) return;  // whole warps
   nr::Item it;
-  it.set(p, index, lane);
+  it.set(p, kind, index, lane);
   const __nv_bfloat16* src = p.qkv + it.b * p.x_sb + static_cast<int64_t>(it.row ? it.t : 0) * p.x_st +
                              it.head0(p) * p.x_sh + lane8 * nr::E;
-  uint4 v[nr::MAX_HEADS];
-#pragma unroll
-  for (int h = 0; h < nr::MAX_HEADS; ++h)
-    if (h < it.heads) v[h] = *reinterpret_cast<const uint4*>(src + h * p.x_sh);
+  nr::HeadRows<nr::SMALL_BATCH> in;
+  in.start(src, p.x_sh, it.heads);
   const int64_t pos = it.row ? nr::position_of(p, it.b, it.t) : 0;
   const bool ok = it.row && pos >= 0 && pos < p.table_len && pos < ap.capacity;
   if (it.row && !ok && lane8 == 0) atomicOr(&g_tt_status, TT_ERR_RANGE);
@@ -221,9 +253,17 @@ __global__ void __launch_bounds__(norm_rope::THREADS)
   if (it.kind == 2) {
     RowPlace place;
     place.set(ap.cache[1], it.b, at, lane8);
+    int64_t head = it.first * ap.cache[1].sh;
+    do {
+      in.prefetch();
 #pragma unroll
-    for (int h = 0; h < nr::MAX_HEADS; ++h)
-      if (h < it.heads) store_row(place, (it.first + h) * ap.cache[1].sh, lane8, ok, v[h]);
+      for (int j = 0; j < nr::SMALL_BATCH; ++j, head += ap.cache[1].sh)
+        if (j < in.left) {
+          uint32_t codes;
+          const uint32_t byte = quantise8(in.now[j], codes);
+          store_row(place, head, lane8, ok, codes, byte);
+        }
+    } while (in.advance());
     return;
   }
   nr::Turn u;
@@ -232,33 +272,57 @@ __global__ void __launch_bounds__(norm_rope::THREADS)
   k.set<NORM>(p, it.kind, u, lane8);
   const float eps = static_cast<float>(p.eps);
   if (it.kind == 0) {
-    __nv_bfloat16* dst = ap.q_out + ((static_cast<int64_t>(it.b) * p.Hq + it.first) * p.T + it.t) * HD + lane8 * nr::E;
-#pragma unroll
-    for (int h = 0; h < nr::MAX_HEADS; ++h) {
-      if (h >= it.heads) break;
-      const uint4 y = nr::turn_row<NORM>(v[h], k, eps);
-      // A row whose position is outside the cache or the table is zero.
-      if (it.row)
-        *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(h) * p.T * HD) = ok ? y : make_uint4(0, 0, 0, 0);
-    }
+    nr::turn_heads<NORM>(
+        in, k, eps,
+        ap.q_out + ((static_cast<int64_t>(it.b) * p.Hq + it.first) * p.T + it.t) * HD + lane8 * nr::E,
+        static_cast<int64_t>(p.T) * HD, it.row, ok);
     return;
   }
   RowPlace place;
   place.set(ap.cache[0], it.b, at, lane8);
-  unsigned unsure = 0;   // heads
+  uint64_t most[2];
 #pragma unroll
-  for (int h = 0; h < nr::MAX_HEADS; ++h) {
-    if (h >= it.heads) break;
-    uint4 y;
-    const bool sure = key_row<NORM>(v[h], k, eps, y);
-    if (__any_sync(0xffffffffu, !sure)) unsure |= 1u << h;
-    store_row(place, (it.first + h) * ap.cache[0].sh, lane8, ok, y);
+  for (int i = 0; i < 2; ++i) {
+    float a[4], b[4];
+    f2_unpack(k.ec[i], a[0], b[0]);
+    f2_unpack(k.es[i], a[1], b[1]);
+    f2_unpack(k.oc[i], a[2], b[2]);
+    f2_unpack(k.os[i], a[3], b[3]);
+    constexpr float UNIT = 9.5367431640625e-07f;   // 2^-20
+    most[i] = f2_pack(UNIT * fmaxf(fmaxf(fabsf(a[0]), fabsf(a[1])), fmaxf(fabsf(a[2]), fabsf(a[3]))),
+                      UNIT * fmaxf(fmaxf(fabsf(b[0]), fabsf(b[1])), fmaxf(fabsf(b[2]), fabsf(b[3]))));
   }
+  unsigned unsure = 0;   // heads
+  int64_t head = it.first * ap.cache[0].sh;
+  int h = 0;
+  do {
+    in.prefetch();
+#pragma unroll
+    for (int j = 0; j < nr::SMALL_BATCH; ++j, ++h, head += ap.cache[0].sh) {
+      if (j >= in.left) break;
+      uint4 y, up;
+      key_row<NORM>(in.now[j], k, most, eps, y, up);
+      uint32_t codes, byte;
+      const bool sure = ((y.x ^ up.x) | (y.y ^ up.y) | (y.z ^ up.z) | (y.w ^ up.w)) == 0;
+      if (__any_sync(0xffffffffu, !sure)) {
+        order(y, up);
+        uint32_t above;
+        const uint32_t byte_above = quantise8(up, above);
+        byte = quantise8(y, codes);
+        if (__any_sync(0xffffffffu, codes != above || byte != byte_above)) unsure |= 1u << h;
+      } else {
+        byte = quantise8(y, codes);
+      }
+      store_row(place, head, lane8, ok, codes, byte);
+    }
+  } while (in.advance());
   while (unsure != 0) {
-    const int h = __ffs(static_cast<int>(unsure)) - 1;
+    h = __ffs(static_cast<int>(unsure)) - 1;
     unsure &= unsure - 1;
     const uint4 x = *reinterpret_cast<const uint4*>(src + h * p.x_sh);
-    store_row(place, (it.first + h) * ap.cache[0].sh, lane8, ok, key_row_exact<NORM>(p, x, at, lane8));
+    uint32_t codes;
+    const uint32_t byte = quantise8(key_row_exact<NORM>(p, x, at, lane8), codes);
+    store_row(place, (it.first + h) * ap.cache[0].sh, lane8, ok, codes, byte);
   }
 }
 

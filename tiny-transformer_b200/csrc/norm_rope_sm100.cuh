@@ -11,9 +11,9 @@
 //
 // Bound by memory: 128 bytes in and 128 out per head forward; backward reads x and dy and writes dx. Eight
 // lanes hold a row, 16 bytes each, so a warp's loads and stores are 4 whole rows; the pairs of the rotation stay
-// inside a lane and the norm's sums take three shuffles. A warp's item is four tokens of up to four heads of one kind
-// (query, key or value): the tokens' rows of q and k are adjacent in the [B, H, T, 64] outputs, all of an item's loads
-// are in flight together, and the weights are multiplied into the table rows once for its heads.
+// inside a lane and the norm's sums take three shuffles. A warp's item is four tokens of up to sixteen heads of one
+// kind (query, key or value): the tokens' rows of q and k are adjacent in the [B, H, T, 64] outputs, the weights are
+// multiplied into the table rows once, and the next heads are loaded while these are computed.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -31,7 +31,9 @@ constexpr int THREADS = WARPS * 32;
 constexpr int ROWS = 4;   // tokens of a warp's step
 constexpr int LANES = 8;  // lanes of a row
 constexpr int E = HD / LANES;
-constexpr int MAX_HEADS = 4;
+constexpr int MAX_HEADS = 16;      // of an item
+constexpr int BATCH = 4;           // heads in flight together
+constexpr int SMALL_BATCH = 2;     // (backward: each with two rows to load; append)
 
 // Division of n < 2^31 by a number known on the host (Granlund and Montgomery, 1994): a product and a shift.
 struct Divisor {
@@ -55,7 +57,8 @@ struct Common {
   int B, T, Hq, Hkv;
   int per_item;               // heads of an item, at most MAX_HEADS
   int items[3];               // items of the query, key and value heads of a group of four tokens
-  Divisor groups, per_group, each[3];   // divisions by groups, by all items of one, by those of a kind
+  int total[3];               // items of each kind in all groups
+  Divisor groups, each[3];    // divisions by the groups of a sequence, by items[]
   const void* w[2];           // q and k weight [64], both NULL: no norm
   bool w_f32;                 // else bf16
   const float* cos;           // [table_len, 32]
@@ -111,16 +114,11 @@ struct Item {
   int first, heads;  // of its kind
   bool row;          // this lane's token is there
 
-  __device__ __forceinline__ void set(const Common& p, int index, int lane) {
-    const int bg = p.per_group.of(index);
-    const int at = index - bg * static_cast<int>(p.per_group.d);
-    const int k = at < p.items[0] ? 0 : at < p.items[0] + p.items[1] ? 1 : 2;
-    set_kind(p, k, bg, at - (k == 0 ? 0 : k == 1 ? p.items[0] : p.items[0] + p.items[1]), lane);
-  }
-  // Item `at` of kind k in group bg.
-  __device__ __forceinline__ void set_kind(const Common& p, int k, int bg, int at, int lane) {
+  // Item `index` of kind k.
+  __device__ __forceinline__ void set(const Common& p, int k, int index, int lane) {
     kind = k;
-    first = at * p.per_item;
+    const int bg = p.each[k].of(index);
+    first = (index - bg * static_cast<int>(p.each[k].d)) * p.per_item;
     heads = min(p.per_item, (kind == 0 ? p.Hq : p.Hkv) - first);
     b = p.groups.of(bg);
     t = (bg - b * static_cast<int>(p.groups.d)) * ROWS + (lane >> 3);
@@ -131,10 +129,51 @@ struct Item {
   }
 };
 
-__device__ __forceinline__ uint4 pack8(const float (&y)[E]) {
-  return make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
-                    pack_bf16x2(y[6], y[7]));
-}
+// A lane's eight features as packed FP32 pairs: even features (0, 2), (4, 6), odd ones (1, 3), (5, 7), so that the
+// two of a rotation stand in the same place of two registers.
+struct Pairs {
+  uint64_t e[2], o[2];
+
+  __device__ __forceinline__ void unpack(const uint4& v) {
+    e[0] = f2_pack(bf16_lo(v.x), bf16_lo(v.y));
+    e[1] = f2_pack(bf16_lo(v.z), bf16_lo(v.w));
+    o[0] = f2_pack(bf16_hi(v.x), bf16_hi(v.y));
+    o[1] = f2_pack(bf16_hi(v.z), bf16_hi(v.w));
+  }
+  __device__ __forceinline__ void set(const float (&x)[E]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      e[i] = f2_pack(x[4 * i], x[4 * i + 2]);
+      o[i] = f2_pack(x[4 * i + 1], x[4 * i + 3]);
+    }
+  }
+  __device__ __forceinline__ uint4 pack() const {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float e0, e1, o0, o1;
+      f2_unpack(e[i], e0, e1);
+      f2_unpack(o[i], o0, o1);
+      u[2 * i] = pack_bf16x2(e0, o0);
+      u[2 * i + 1] = pack_bf16x2(e1, o1);
+    }
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+  __device__ __forceinline__ void scale(float r) {
+    const uint64_t r2 = f2_pack(r, r);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      e[i] = f2_mul(e[i], r2);
+      o[i] = f2_mul(o[i], r2);
+    }
+  }
+  __device__ __forceinline__ float dot(const Pairs& b) const {
+    const uint64_t s = f2_add(f2_fma(e[1], b.e[1], f2_mul(e[0], b.e[0])), f2_fma(o[1], b.o[1], f2_mul(o[0], b.o[0])));
+    float lo, hi;
+    f2_unpack(s, lo, hi);
+    return lo + hi;
+  }
+};
 
 // Sum over the eight lanes of a row, in every one of them.
 __device__ __forceinline__ float row_sum(float v) {
@@ -143,51 +182,99 @@ __device__ __forceinline__ float row_sum(float v) {
   return v + __shfl_xor_sync(0xffffffffu, v, 4);
 }
 
-__device__ __forceinline__ float inverse_rms(const float (&x)[E], float eps) {
-  float ss = 0.0f;
-#pragma unroll
-  for (int i = 0; i < E; ++i) ss = fmaf(x[i], x[i], ss);
-  return rsqrtf(row_sum(ss) * (1.0f / HD) + eps);
+__device__ __forceinline__ float inverse_rms(const Pairs& x, float eps) {
+  return rsqrtf(row_sum(x.dot(x)) * (1.0f / HD) + eps);
 }
 
-// The rotation with the weights in it: y_2i = x_2i ec - x_2i+1 os, y_2i+1 = x_2i es + x_2i+1 oc (x normed).
+// The rotation with the weights in it: y_2i = x_2i ec + x_2i+1 os, y_2i+1 = x_2i es + x_2i+1 oc (x normed; os has
+// the rotation's minus).
 struct Coefficients {
-  float ec[E / 2], es[E / 2], oc[E / 2], os[E / 2];
+  uint64_t ec[2], es[2], oc[2], os[2];
 
   template <bool NORM>
   __device__ __forceinline__ void set(const Common& p, int kind, const Turn& u, int lane8) {
     float w[E];
     if (NORM) load_weight(p, kind, lane8, w);
 #pragma unroll
-    for (int i = 0; i < E / 2; ++i) {
-      const float we = NORM ? w[2 * i] : 1.0f, wo = NORM ? w[2 * i + 1] : 1.0f;
-      ec[i] = we * u.c[i];
-      es[i] = we * u.s[i];
-      oc[i] = wo * u.c[i];
-      os[i] = wo * u.s[i];
+    for (int i = 0; i < 2; ++i) {
+      const uint64_t c = f2_pack(u.c[2 * i], u.c[2 * i + 1]), s = f2_pack(u.s[2 * i], u.s[2 * i + 1]);
+      const uint64_t minus = f2_pack(-u.s[2 * i], -u.s[2 * i + 1]);
+      const uint64_t we = NORM ? f2_pack(w[4 * i], w[4 * i + 2]) : f2_pack(1.0f, 1.0f);
+      const uint64_t wo = NORM ? f2_pack(w[4 * i + 1], w[4 * i + 3]) : f2_pack(1.0f, 1.0f);
+      ec[i] = f2_mul(we, c);
+      es[i] = f2_mul(we, s);
+      oc[i] = f2_mul(wo, c);
+      os[i] = f2_mul(wo, minus);
     }
+  }
+  __device__ __forceinline__ Pairs turn(const Pairs& x) const {
+    Pairs y;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      y.e[i] = f2_fma(x.e[i], ec[i], f2_mul(x.o[i], os[i]));
+      y.o[i] = f2_fma(x.e[i], es[i], f2_mul(x.o[i], oc[i]));
+    }
+    return y;
   }
 };
 
 template <bool NORM>
 __device__ __forceinline__ uint4 turn_row(const uint4& v, const Coefficients& k, float eps) {
-  float x[E], y[E];
-  unpack8(v, x);
-  const float r = NORM ? inverse_rms(x, eps) : 1.0f;
+  Pairs x;
+  x.unpack(v);
+  if (NORM) x.scale(inverse_rms(x, eps));
+  return k.turn(x).pack();
+}
+
+// An item's rows, head by head: N of them are in registers while the next are on their way.
+template <int N>
+struct HeadRows {
+  const __nv_bfloat16* src;   // of the batch in `now`
+  int64_t step;               // elements from head to head
+  int left;                   // heads from `now` on
+  uint4 now[N], next[N];
+
+  __device__ __forceinline__ static void load(uint4 (&v)[N], const __nv_bfloat16* from, int64_t step, int count) {
 #pragma unroll
-  for (int i = 0; i < E / 2; ++i) {
-    const float a = x[2 * i] * r, b = x[2 * i + 1] * r;
-    y[2 * i] = a * k.ec[i] - b * k.os[i];
-    y[2 * i + 1] = a * k.es[i] + b * k.oc[i];
+    for (int j = 0; j < N; ++j)
+      if (j < count) v[j] = *reinterpret_cast<const uint4*>(from + j * step);
   }
-  return pack8(y);
+  __device__ __forceinline__ void start(const __nv_bfloat16* from, int64_t by, int heads) {
+    src = from;
+    step = by;
+    left = heads;
+    load(now, src, step, left);
+  }
+  __device__ __forceinline__ void prefetch() { load(next, src + N * step, step, left - N); }
+  __device__ __forceinline__ bool advance() {
+    left -= N;
+    src += N * step;
+#pragma unroll
+    for (int j = 0; j < N; ++j) now[j] = next[j];
+    return left > 0;
+  }
+};
+
+// Turns an item's heads. A row whose position is outside the table (or the cache) is zero.
+template <bool NORM, int N>
+__device__ __forceinline__ void turn_heads(HeadRows<N>& in, const Coefficients& k, float eps, __nv_bfloat16* dst,
+                                           int64_t step, bool row, bool ok) {
+  do {
+    in.prefetch();
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (j >= in.left) break;
+      const uint4 y = turn_row<NORM>(in.now[j], k, eps);
+      if (row) *reinterpret_cast<uint4*>(dst) = ok ? y : make_uint4(0, 0, 0, 0);
+      dst += step;
+    }
+  } while (in.advance());
 }
 
 // ------------------------------------------------------------------------------- forward
 
 struct ForwardParams {
   Common c;
-  int total;              // items
   __nv_bfloat16* out[2];  // q [B, Hq, T, 64], k [B, Hkv, T, 64]
 };
 
@@ -195,17 +282,19 @@ template <bool NORM>
 __global__ void __launch_bounds__(THREADS) forward_kernel(const __grid_constant__ ForwardParams fp) {
   const Common& p = fp.c;
   const int lane = threadIdx.x & 31, lane8 = lane & 7;
-  const int index = static_cast<int>(blockIdx.x) * WARPS + (threadIdx.x >> 5);
+  int index = static_cast<int>(blockIdx.x) * WARPS + (threadIdx.x >> 5), kind = 0;
   wait_for_previous_kernel();
-  if (index >= fp.total) return;  // whole warps
+  if (index >= p.total[0]) {
+    index -= p.total[0];
+    kind = 1;
+  }
+  if (index >= p.total[kind]) return;  // whole warps
   Item it;
-  it.set(p, index, lane);
+  it.set(p, kind, index, lane);
   const __nv_bfloat16* src = p.qkv + it.b * p.x_sb + static_cast<int64_t>(it.row ? it.t : 0) * p.x_st +
                              it.head0(p) * p.x_sh + lane8 * E;
-  uint4 v[MAX_HEADS];
-#pragma unroll
-  for (int h = 0; h < MAX_HEADS; ++h)
-    if (h < it.heads) v[h] = *reinterpret_cast<const uint4*>(src + h * p.x_sh);
+  HeadRows<BATCH> in;
+  in.start(src, p.x_sh, it.heads);
   const int64_t pos = it.row ? position_of(p, it.b, it.t) : 0;
   const bool ok = it.row && pos >= 0 && pos < p.table_len;
   if (it.row && !ok && lane8 == 0) atomicOr(&g_tt_status, TT_ERR_RANGE);
@@ -214,23 +303,16 @@ __global__ void __launch_bounds__(THREADS) forward_kernel(const __grid_constant_
   Coefficients k;
   k.set<NORM>(p, it.kind, u, lane8);
   const int heads = it.kind == 0 ? p.Hq : p.Hkv;
-  __nv_bfloat16* dst = fp.out[it.kind] +
-                       ((static_cast<int64_t>(it.b) * heads + it.first) * p.T + it.t) * HD + lane8 * E;
-#pragma unroll
-  for (int h = 0; h < MAX_HEADS; ++h) {
-    if (h >= it.heads) break;
-    const uint4 y = turn_row<NORM>(v[h], k, static_cast<float>(p.eps));
-    // A row whose position is outside the table is zero.
-    if (it.row)
-      *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(h) * p.T * HD) = ok ? y : make_uint4(0, 0, 0, 0);
-  }
+  turn_heads<NORM>(in, k, static_cast<float>(p.eps),
+                   fp.out[it.kind] + ((static_cast<int64_t>(it.b) * heads + it.first) * p.T + it.t) * HD + lane8 * E,
+                   static_cast<int64_t>(p.T) * HD, it.row, ok);
 }
 
 // ------------------------------------------------------------------------------- backward
 
 struct BackwardParams {
   Common c;
-  int total[3], ctas[3];               // items of each kind of heads, and CTAs for them (0 where none)
+  int ctas[3];                         // CTAs for each kind of heads
   const __nv_bfloat16* g[3];           // dq, dk [B, H, T, 64] after the rotation, dv; NULL: zero
   int64_t g_sb[3], g_sh[3], g_st[3];
   __nv_bfloat16* dx;                   // [B, T, Hq + 2 Hkv, 64]
@@ -247,39 +329,44 @@ __global__ void __launch_bounds__(THREADS, 5) backward_kernel(const __grid_const
   const int heads = p.Hq + 2 * p.Hkv;
   int cta = static_cast<int>(blockIdx.x), kind = 0;
   while (cta >= bp.ctas[kind]) cta -= bp.ctas[kind++];
-  const int total = bp.total[kind], stride = bp.ctas[kind] * WARPS;
+  const int total = p.total[kind], stride = bp.ctas[kind] * WARPS;
   const __nv_bfloat16* const grad0 = bp.g[kind];
   const int64_t g_sb = bp.g_sb[kind], g_sh = bp.g_sh[kind], g_st = bp.g_st[kind];
   wait_for_previous_kernel();
   if (kind == 2) {
     for (int index = cta * WARPS + warp; index < total; index += stride) {
       Item it;
-      const int bg = p.each[2].of(index);
-      it.set_kind(p, 2, bg, index - bg * static_cast<int>(p.each[2].d), lane);
+      it.set(p, 2, index, lane);
       if (!it.row) continue;
       const __nv_bfloat16* grad = grad0 + it.b * g_sb + it.first * g_sh + it.t * g_st + lane8 * E;
       __nv_bfloat16* dst =
           bp.dx + ((static_cast<int64_t>(it.b) * p.T + it.t) * heads + it.head0(p)) * HD + lane8 * E;
-      uint4 v[MAX_HEADS];
-#pragma unroll
-      for (int h = 0; h < MAX_HEADS; ++h) {
-        v[h] = make_uint4(0, 0, 0, 0);
-        if (h < it.heads && grad0 != nullptr) v[h] = *reinterpret_cast<const uint4*>(grad + h * g_sh);
+      if (grad0 == nullptr) {
+        for (int h = 0; h < it.heads; ++h) *reinterpret_cast<uint4*>(dst + h * HD) = make_uint4(0, 0, 0, 0);
+        continue;
       }
+      HeadRows<BATCH> in;
+      in.start(grad, g_sh, it.heads);
+      do {
+        in.prefetch();
 #pragma unroll
-      for (int h = 0; h < MAX_HEADS; ++h)
-        if (h < it.heads) *reinterpret_cast<uint4*>(dst + h * HD) = v[h];
+        for (int j = 0; j < BATCH; ++j, dst += HD)
+          if (j < in.left) *reinterpret_cast<uint4*>(dst) = in.now[j];
+      } while (in.advance());
     }
     return;
   }
-  float w[E], dw[E];
-  if (NORM) load_weight(p, kind, lane8, w);
+  Pairs w, dw;
+  if (NORM) {
+    float each[E];
+    load_weight(p, kind, lane8, each);
+    w.set(each);
+  }
 #pragma unroll
-  for (int i = 0; i < E; ++i) dw[i] = 0.0f;
+  for (int i = 0; i < 2; ++i) dw.e[i] = dw.o[i] = f2_pack(0.0f, 0.0f);
   for (int index = cta * WARPS + warp; index < total; index += stride) {
     Item it;
-    const int bg = p.each[kind].of(index);
-    it.set_kind(p, kind, bg, index - bg * static_cast<int>(p.each[kind].d), lane);
+    it.set(p, kind, index, lane);
     const int64_t pos = it.row ? position_of(p, it.b, it.t) : 0;
     const bool ok = it.row && pos >= 0 && pos < p.table_len;
     if (it.row && !ok && lane8 == 0) atomicOr(&g_tt_status, TT_ERR_RANGE);
@@ -288,53 +375,80 @@ __global__ void __launch_bounds__(THREADS, 5) backward_kernel(const __grid_const
     const __nv_bfloat16* grad = grad0 + it.b * g_sb + it.first * g_sh + t * g_st + lane8 * E;
     __nv_bfloat16* dst = bp.dx + ((static_cast<int64_t>(it.b) * p.T + t) * heads + it.head0(p)) * HD + lane8 * E;
     // A row outside the table was not turned but zeroed: its x and g count as zeros.
-    uint4 xv[MAX_HEADS], gv[MAX_HEADS];
+    constexpr int N = SMALL_BATCH;
+    uint4 xv[N], gv[N];
+    auto load = [&](uint4 (&x)[N], uint4 (&g)[N], int h0) {
 #pragma unroll
-    for (int h = 0; h < MAX_HEADS; ++h) {
-      xv[h] = gv[h] = make_uint4(0, 0, 0, 0);
-      if (h < it.heads && ok) {
-        xv[h] = *reinterpret_cast<const uint4*>(src + h * p.x_sh);
-        if (grad0 != nullptr) gv[h] = *reinterpret_cast<const uint4*>(grad + h * g_sh);
+      for (int j = 0; j < N; ++j) {
+        x[j] = g[j] = make_uint4(0, 0, 0, 0);
+        if (h0 + j < it.heads && ok) {
+          x[j] = *reinterpret_cast<const uint4*>(src + (h0 + j) * p.x_sh);
+          if (grad0 != nullptr) g[j] = *reinterpret_cast<const uint4*>(grad + (h0 + j) * g_sh);
+        }
       }
-    }
+    };
+    load(xv, gv, 0);
     Turn u;
     load_turn(p, ok ? pos : 0, lane8, u);
+    uint64_t c[2], s[2], minus[2];
 #pragma unroll
-    for (int h = 0; h < MAX_HEADS; ++h) {
-      if (h >= it.heads) break;
-      float x[E], gy[E], g[E], dx[E];
-      unpack8(xv[h], x);
-      unpack8(gv[h], gy);
+    for (int i = 0; i < 2; ++i) {
+      c[i] = f2_pack(u.c[2 * i], u.c[2 * i + 1]);
+      s[i] = f2_pack(u.s[2 * i], u.s[2 * i + 1]);
+      minus[i] = f2_pack(-u.s[2 * i], -u.s[2 * i + 1]);
+    }
+#pragma unroll 1
+    for (int h0 = 0; h0 < it.heads; h0 += N) {
+      uint4 xn[N], gn[N];
+      load(xn, gn, h0 + N);
 #pragma unroll
-      for (int i = 0; i < E / 2; ++i) {
-        g[2 * i] = gy[2 * i] * u.c[i] + gy[2 * i + 1] * u.s[i];
-        g[2 * i + 1] = gy[2 * i + 1] * u.c[i] - gy[2 * i] * u.s[i];
-      }
-      if (NORM) {
-        const float rms = inverse_rms(x, static_cast<float>(p.eps));   // all lanes: it shuffles
-        const float r = ok ? rms : 0.0f;
-        float dot = 0.0f;
+      for (int j = 0; j < N; ++j) {
+        if (h0 + j >= it.heads) break;
+        Pairs x, gy, g;
+        x.unpack(xv[j]);
+        gy.unpack(gv[j]);
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-          x[i] *= r;
-          dw[i] = fmaf(g[i], x[i], dw[i]);
-          g[i] *= w[i];
-          dot = fmaf(g[i], x[i], dot);
+        for (int i = 0; i < 2; ++i) {
+          g.e[i] = f2_fma(gy.e[i], c[i], f2_mul(gy.o[i], s[i]));
+          g.o[i] = f2_fma(gy.o[i], c[i], f2_mul(gy.e[i], minus[i]));
         }
-        dot = row_sum(dot) * (1.0f / HD);
+        if (NORM) {
+          const float rms = inverse_rms(x, static_cast<float>(p.eps));   // all lanes: it shuffles
+          const float r = ok ? rms : 0.0f;
+          x.scale(r);
 #pragma unroll
-        for (int i = 0; i < E; ++i) dx[i] = (g[i] - x[i] * dot) * r;
-      } else {
+          for (int i = 0; i < 2; ++i) {
+            dw.e[i] = f2_fma(g.e[i], x.e[i], dw.e[i]);
+            dw.o[i] = f2_fma(g.o[i], x.o[i], dw.o[i]);
+            g.e[i] = f2_mul(g.e[i], w.e[i]);
+            g.o[i] = f2_mul(g.o[i], w.o[i]);
+          }
+          const float dot = row_sum(g.dot(x)) * (-1.0f / HD);
+          const uint64_t dot2 = f2_pack(dot, dot);
 #pragma unroll
-        for (int i = 0; i < E; ++i) dx[i] = g[i];
+          for (int i = 0; i < 2; ++i) {
+            g.e[i] = f2_fma(x.e[i], dot2, g.e[i]);
+            g.o[i] = f2_fma(x.o[i], dot2, g.o[i]);
+          }
+          g.scale(r);
+        }
+        if (it.row) *reinterpret_cast<uint4*>(dst + (h0 + j) * HD) = g.pack();
       }
-      if (it.row) *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(h) * HD) = pack8(dx);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        xv[j] = xn[j];
+        gv[j] = gn[j];
+      }
     }
   }
   if constexpr (NORM) {
     __shared__ float sums[WARPS * ROWS][HD];
+    float* sum = &sums[warp * ROWS + (lane >> 3)][lane8 * E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) sums[warp * ROWS + (lane >> 3)][lane8 * E + i] = dw[i];
+    for (int i = 0; i < 2; ++i) {
+      f2_unpack(dw.e[i], sum[4 * i], sum[4 * i + 2]);
+      f2_unpack(dw.o[i], sum[4 * i + 1], sum[4 * i + 3]);
+    }
     __syncthreads();
     if (threadIdx.x < HD) {
       float s = 0.0f;
