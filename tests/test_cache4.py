@@ -225,7 +225,8 @@ def test_entry_points_forward_and_guard():
                 call()
             t[1].is_cuda = True
     with pytest.raises(RuntimeError, match="CUDA"):
-        fused.qkv_norm_rope(torch.zeros(1, 1, 3, 1, 64), None, None, None, None)
+        table = torch.zeros(4, 32)
+        fused.qkv_norm_rope(torch.zeros(1, 1, 3, 1, 64), None, None, table, table)
     for bad in ((0, 1, 1), (1, 0, 1), (1, 1, 0)):
         with pytest.raises(ValueError, match="positive"):
             cache4.new_cache(*bad, device="cpu")

@@ -321,6 +321,25 @@ def test_refusals(op, change, match):
         op(qkv.cuda(), *[x.cuda() for x in w], cos.requires_grad_(), sin, 0, EPS, 2)
 
 
+def test_gradients_have_no_backward(op):
+    qkv, w, g = _inputs(1, 4, 1, 1, torch.bfloat16, 1)
+    cos, sin = (t.cuda() for t in _tables())
+    leaves = [x.cuda().requires_grad_() for x in (qkv, *w)]
+    want = torch.autograd.grad(op(*leaves, cos, sin, 0, EPS, 1), leaves, [x.cuda() for x in g])
+    grads = torch.autograd.grad(op(*leaves, cos, sin, 0, EPS, 1), leaves, [x.cuda() for x in g], create_graph=True)
+    assert all(map(torch.equal, want, grads))
+    with pytest.raises(RuntimeError, match="no backward"):
+        grads[0].sum().backward()
+    # A projection changed between forward and backward is noticed.
+    x = leaves[0].detach().clone().requires_grad_()
+    y = x * 1
+    out = op(y, *leaves[1:], cos, sin, 0, EPS, 1)
+    with torch.no_grad():
+        y.add_(1)
+    with pytest.raises(RuntimeError, match="modified"):
+        torch.autograd.grad(out, x, [t.cuda() for t in g])
+
+
 def test_autocast_is_refused(op):
     qkv, w, _ = _inputs(1, 3, 1, 1, torch.bfloat16, 1)
     cos, sin = (t.cuda() for t in _tables())

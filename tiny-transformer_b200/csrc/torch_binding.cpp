@@ -13,6 +13,7 @@
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <cstdint>
 #include <limits>
@@ -679,15 +680,10 @@ struct Position {
   int64_t sb = 0, st = 0;
 };
 
-Position position_argument(const pybind11::object& position, const torch::Tensor& like, int64_t B, int64_t T,
-                           bool every, const char* what) {
+Position position_tensor(const torch::Tensor& position, const torch::Tensor& like, int64_t B, int64_t T, bool every,
+                         const char* what) {
   Position p;
-  if (pybind11::isinstance<pybind11::int_>(position)) {
-    p.host = position.cast<int64_t>();
-    return p;
-  }
-  TORCH_CHECK(THPVariable_Check(position.ptr()), what, ": the position must be an int or an int64 CUDA tensor");
-  p.t = THPVariable_Unpack(position.ptr());
+  p.t = position;
   TORCH_CHECK(p.t.is_cuda() && p.t.device() == like.device() && p.t.scalar_type() == at::kLong, what,
               ": a tensor position must be an int64 CUDA tensor on the same device");
   const bool each = p.t.dim() == 1 && p.t.size(0) == B;
@@ -705,79 +701,193 @@ Position position_argument(const pybind11::object& position, const torch::Tensor
   return p;
 }
 
+Position position_argument(const pybind11::object& position, const torch::Tensor& like, int64_t B, int64_t T,
+                           bool every, const char* what) {
+  Position p;
+  if (pybind11::isinstance<pybind11::int_>(position)) {
+    p.host = position.cast<int64_t>();
+    return p;
+  }
+  TORCH_CHECK(THPVariable_Check(position.ptr()), what, ": the position must be an int or an int64 CUDA tensor");
+  return position_tensor(THPVariable_Unpack(position.ptr()), like, B, T, every, what);
+}
+
+// Everything about a call but the tensors that its gradients need again.
+struct NormRopeCall {
+  Projection x;
+  NormWeights w;
+  Position pos;
+};
+
+NormRopeCall norm_rope_call(const torch::Tensor& qkv, const std::optional<torch::Tensor>& q_weight,
+                            const std::optional<torch::Tensor>& k_weight, const torch::Tensor& cos,
+                            const torch::Tensor& sin, const Position& pos, std::optional<int64_t> kv_heads,
+                            const char* what) {
+  NormRopeCall c{projection(qkv, kv_heads, what), {}, pos};
+  check_rope_tables(cos, sin, c.x.x, what);
+  c.w = norm_weights(q_weight, k_weight, c.x.x, what);
+  check_sm100(c.x.x);
+  return c;
+}
+
 // RMS norm and rotation of the query and key heads of a projection (tt_attn_qkv_norm_rope_bf16).
-std::tuple<torch::Tensor, torch::Tensor> qkv_norm_rope(
-    const torch::Tensor& qkv, std::optional<torch::Tensor> q_weight, std::optional<torch::Tensor> k_weight,
-    const torch::Tensor& cos, const torch::Tensor& sin, const pybind11::object& position, double eps,
-    std::optional<int64_t> kv_heads) {
-  const char* what = "qkv_norm_rope";
-  TORCH_CHECK(qkv.defined() && qkv.is_cuda(), what, ": all tensors must be CUDA tensors");
-  const c10::cuda::CUDAGuard device_guard(qkv.device());
-  const Projection x = projection(qkv, kv_heads, what);
-  check_rope_tables(cos, sin, x.x, what);
-  const NormWeights w = norm_weights(q_weight, k_weight, x.x, what);
-  const Position pos = position_argument(position, x.x, x.B, x.T, true, what);
-  check_sm100(x.x);
+std::tuple<torch::Tensor, torch::Tensor> norm_rope_forward(const NormRopeCall& c, const torch::Tensor& cos,
+                                                           const torch::Tensor& sin, double eps) {
+  const Projection& x = c.x;
   auto q = new_cuda({x.B, x.Hq, x.T, TT_ATTN_HEAD_DIM}, at::kBFloat16, x.x.device());
   auto k = new_cuda({x.B, x.Hkv, x.T, TT_ATTN_HEAD_DIM}, at::kBFloat16, x.x.device());
   auto stream = c10::cuda::getCurrentCUDAStream(x.x.get_device());
   const tt_attn_status st = tt_attn_qkv_norm_rope_bf16(
-      x.x.data_ptr(), x.strides, x.B, x.T, x.Hq, x.Hkv, w.qp(), w.kp(), w.f32, cos.data_ptr<float>(),
-      sin.data_ptr<float>(), cos.size(0), pos.host, pos.dev, pos.sb, pos.st, eps, q.data_ptr(), k.data_ptr(),
-      static_cast<void*>(stream.stream()));
+      x.x.data_ptr(), x.strides, x.B, x.T, x.Hq, x.Hkv, c.w.qp(), c.w.kp(), c.w.f32, cos.data_ptr<float>(),
+      sin.data_ptr<float>(), cos.size(0), c.pos.host, c.pos.dev, c.pos.sb, c.pos.st, eps, q.data_ptr(),
+      k.data_ptr(), static_cast<void*>(stream.stream()));
   TORCH_CHECK(st == TT_ATTN_OK, "tt_attn_qkv_norm_rope_bf16 failed: ", tt_attn_status_string(st), ": ",
               tt_attn_last_error());
   return {q, k};
 }
 
-// Its gradients (tt_attn_qkv_norm_rope_backward_bf16): dqkv in qkv's shape, and the weights' (undefined without).
-std::tuple<torch::Tensor, std::optional<torch::Tensor>, std::optional<torch::Tensor>> qkv_norm_rope_backward(
-    const torch::Tensor& qkv, std::optional<torch::Tensor> q_weight, std::optional<torch::Tensor> k_weight,
-    const torch::Tensor& cos, const torch::Tensor& sin, const pybind11::object& position, double eps,
-    std::optional<int64_t> kv_heads, std::optional<torch::Tensor> dq, std::optional<torch::Tensor> dk,
-    std::optional<torch::Tensor> dv) {
-  const char* what = "qkv_norm_rope backward";
-  TORCH_CHECK(qkv.defined() && qkv.is_cuda(), what, ": all tensors must be CUDA tensors");
-  const c10::cuda::CUDAGuard device_guard(qkv.device());
-  const Projection x = projection(qkv, kv_heads, what);
-  check_rope_tables(cos, sin, x.x, what);
-  const NormWeights w = norm_weights(q_weight, k_weight, x.x, what);
-  const Position pos = position_argument(position, x.x, x.B, x.T, true, what);
-  check_sm100(x.x);
+// The value heads of a projection as a [B, Hkv, T, 64] view.
+torch::Tensor value_heads(const torch::Tensor& qkv, int64_t kv_heads) {
+  return (qkv.dim() == 5 ? qkv.select(2, 2) : qkv.narrow(2, qkv.size(2) - kv_heads, kv_heads)).transpose(1, 2);
+}
+
+// Gradients of norm_rope_forward (tt_attn_qkv_norm_rope_backward_bf16): dqkv in qkv's shape, and the weights'
+// (undefined without).
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> norm_rope_backward(
+    const NormRopeCall& c, const torch::Tensor& qkv, const torch::Tensor& cos, const torch::Tensor& sin, double eps,
+    const torch::Tensor& dq, const torch::Tensor& dk, const torch::Tensor& dv) {
+  const Projection& x = c.x;
+  const torch::Tensor* given[3] = {&dq, &dk, &dv};
   torch::Tensor g[3];
   const void* gp[3] = {nullptr, nullptr, nullptr};
   int64_t gs[3][4] = {};
-  std::optional<torch::Tensor>* given[3] = {&dq, &dk, &dv};
   for (int i = 0; i < 3; ++i) {
-    if (!given[i]->has_value()) continue;
-    g[i] = **given[i];
-    TORCH_CHECK(g[i].defined() && g[i].is_cuda() && g[i].device() == x.x.device() &&
-                    g[i].scalar_type() == at::kBFloat16 && g[i].layout() == at::kStrided && g[i].dim() == 4 &&
-                    g[i].size(0) == x.B && g[i].size(1) == (i == 0 ? x.Hq : x.Hkv) && g[i].size(2) == x.T &&
+    if (!given[i]->defined()) continue;
+    g[i] = *given[i];
+    TORCH_CHECK(g[i].is_cuda() && g[i].device() == x.x.device() && g[i].scalar_type() == at::kBFloat16 &&
+                    g[i].layout() == at::kStrided && g[i].dim() == 4 && g[i].size(0) == x.B &&
+                    g[i].size(1) == (i == 0 ? x.Hq : x.Hkv) && g[i].size(2) == x.T &&
                     g[i].size(3) == TT_ATTN_HEAD_DIM,
-                what, ": gradients must be bf16 [B, heads, T, 64] tensors on the same device");
+                "qkv_norm_rope backward: gradients must be bf16 [B, heads, T, 64] tensors on the same device");
     g[i] = aligned_contiguous(g[i]);
     gp[i] = g[i].data_ptr();
     for (int d = 0; d < 4; ++d) gs[i][d] = g[i].stride(d);
   }
   auto dx = new_cuda(qkv.sizes(), at::kBFloat16, x.x.device());
-  std::optional<torch::Tensor> dqw, dkw;
-  torch::Tensor ws;
+  torch::Tensor dqw, dkw, ws;
   const size_t ws_bytes = tt_attn_qkv_norm_rope_backward_workspace_size();
-  if (w.q.defined()) {
-    dqw = new_cuda({TT_ATTN_HEAD_DIM}, w.q.scalar_type(), x.x.device());
-    dkw = new_cuda({TT_ATTN_HEAD_DIM}, w.q.scalar_type(), x.x.device());
+  if (c.w.q.defined()) {
+    dqw = new_cuda({TT_ATTN_HEAD_DIM}, c.w.q.scalar_type(), x.x.device());
+    dkw = new_cuda({TT_ATTN_HEAD_DIM}, c.w.q.scalar_type(), x.x.device());
     ws = new_cuda({static_cast<int64_t>(ws_bytes)}, at::kByte, x.x.device());
   }
   auto stream = c10::cuda::getCurrentCUDAStream(x.x.get_device());
   const tt_attn_status st = tt_attn_qkv_norm_rope_backward_bf16(
-      x.x.data_ptr(), x.strides, x.B, x.T, x.Hq, x.Hkv, w.qp(), w.kp(), w.f32, cos.data_ptr<float>(),
-      sin.data_ptr<float>(), cos.size(0), pos.host, pos.dev, pos.sb, pos.st, eps, gp[0], gs[0], gp[1], gs[1],
-      gp[2], gs[2], dx.data_ptr(), dqw ? dqw->data_ptr() : nullptr, dkw ? dkw->data_ptr() : nullptr,
-      ws.defined() ? ws.data_ptr() : nullptr, ws_bytes, static_cast<void*>(stream.stream()));
+      x.x.data_ptr(), x.strides, x.B, x.T, x.Hq, x.Hkv, c.w.qp(), c.w.kp(), c.w.f32, cos.data_ptr<float>(),
+      sin.data_ptr<float>(), cos.size(0), c.pos.host, c.pos.dev, c.pos.sb, c.pos.st, eps, gp[0], gs[0], gp[1],
+      gs[1], gp[2], gs[2], dx.data_ptr(), dqw.defined() ? dqw.data_ptr() : nullptr,
+      dkw.defined() ? dkw.data_ptr() : nullptr, ws.defined() ? ws.data_ptr() : nullptr, ws_bytes,
+      static_cast<void*>(stream.stream()));
   TORCH_CHECK(st == TT_ATTN_OK, "tt_attn_qkv_norm_rope_backward_bf16 failed: ", tt_attn_status_string(st), ": ",
               tt_attn_last_error());
   return {dx, dqw, dkw};
+}
+
+// Outputs of a backward pass that has none of its own: differentiating them is an error (what once_differentiable does in
+// Python).
+torch::autograd::variable_list once_differentiable(torch::autograd::variable_list out) {
+  if (!at::GradMode::is_enabled()) return out;
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      "qkv_norm_rope's gradients have no backward", static_cast<int>(out.size()));
+  for (torch::Tensor& x : out)
+    if (x.defined()) x = x.detach().requires_grad_();
+  return (*error)(std::move(out));
+}
+
+// Norm and rotation with gradients, as a native autograd node: called from Python its host time was twice the kernels' of
+// a short step. v is a view of qkv, so that its gradient goes into the one dqkv that the backward kernel writes.
+class QkvNormRope : public torch::autograd::Function<QkvNormRope> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& qkv,
+                                                const std::optional<torch::Tensor>& q_weight,
+                                                const std::optional<torch::Tensor>& k_weight,
+                                                const torch::Tensor& cos, const torch::Tensor& sin,
+                                                const std::optional<torch::Tensor>& position, int64_t host,
+                                                double eps, int64_t kv_heads) {
+    const NormRopeCall c = call(qkv, q_weight, k_weight, cos, sin, position, host, kv_heads, "qkv_norm_rope");
+    auto [q, k] = norm_rope_forward(c, cos, sin, eps);
+    ctx->save_for_backward({qkv, q_weight.value_or(torch::Tensor()), k_weight.value_or(torch::Tensor()), cos, sin,
+                            position.value_or(torch::Tensor())});
+    ctx->saved_data["host"] = host;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["kv_heads"] = kv_heads;
+    ctx->set_materialize_grads(false);
+    return {q, k, value_heads(qkv, c.x.Hkv)};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    torch::autograd::variable_list out(9);
+    if (!grads[0].defined() && !grads[1].defined() && !grads[2].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const torch::Tensor& qkv = saved[0];
+    const c10::cuda::CUDAGuard device_guard(qkv.device());
+    {
+      const at::NoGradGuard no_grad;
+      auto optional = [](const torch::Tensor& x) {
+        return x.defined() ? std::optional<torch::Tensor>(x) : std::nullopt;
+      };
+      const NormRopeCall c =
+          call(qkv, optional(saved[1]), optional(saved[2]), saved[3], saved[4], optional(saved[5]),
+               ctx->saved_data["host"].toInt(), ctx->saved_data["kv_heads"].toInt(), "qkv_norm_rope backward");
+      auto [dqkv, dqw, dkw] = norm_rope_backward(c, qkv, saved[3], saved[4], ctx->saved_data["eps"].toDouble(),
+                                                 grads[0], grads[1], grads[2]);
+      if (ctx->needs_input_grad(0)) out[0] = dqkv;
+      if (saved[1].defined() && ctx->needs_input_grad(1)) out[1] = dqw;
+      if (saved[2].defined() && ctx->needs_input_grad(2)) out[2] = dkw;
+    }
+    return once_differentiable(std::move(out));
+  }
+
+ private:
+  static NormRopeCall call(const torch::Tensor& qkv, const std::optional<torch::Tensor>& q_weight,
+                           const std::optional<torch::Tensor>& k_weight, const torch::Tensor& cos,
+                           const torch::Tensor& sin, const std::optional<torch::Tensor>& position, int64_t host,
+                           int64_t kv_heads, const char* what) {
+    Position pos;
+    pos.host = host;
+    const int64_t B = qkv.size(0), T = qkv.size(1);
+    if (position.has_value()) pos = position_tensor(*position, qkv, B, T, true, what);
+    return norm_rope_call(qkv, q_weight, k_weight, cos, sin, pos,
+                          kv_heads >= 0 ? std::optional<int64_t>(kv_heads) : std::nullopt, what);
+  }
+};
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> qkv_norm_rope(
+    const torch::Tensor& qkv, std::optional<torch::Tensor> q_weight, std::optional<torch::Tensor> k_weight,
+    const torch::Tensor& cos, const torch::Tensor& sin, const pybind11::object& position, double eps,
+    std::optional<int64_t> kv_heads) {
+  const char* what = "qkv_norm_rope";
+  TORCH_CHECK(qkv.defined() && qkv.is_cuda(), what, ": all tensors must be CUDA tensors");
+  TORCH_CHECK(!at::autocast::is_autocast_enabled(at::kCUDA), what, " does not support AMP/autocast yet");
+  TORCH_CHECK(qkv.dim() >= 2, what, ": qkv must be [B, T, 3, H, 64] or [B, T, q_heads + 2 * kv_heads, 64]");
+  TORCH_CHECK(!kv_heads.has_value() || *kv_heads > 0, what, ": q heads must be a positive multiple of the K/V heads");
+  const c10::cuda::CUDAGuard device_guard(qkv.device());
+  const Position pos = position_argument(position, qkv, qkv.size(0), qkv.size(1), true, what);
+  const auto wants = [](const std::optional<torch::Tensor>& x) { return x.has_value() && x->requires_grad(); };
+  if (at::GradMode::is_enabled()) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!cos.requires_grad() && !sin.requires_grad(), what,
+                                " has no gradient for the cos/sin tables");
+    if (qkv.requires_grad() || wants(q_weight) || wants(k_weight)) {
+      const std::optional<torch::Tensor> on_device = pos.t.defined() ? std::make_optional(pos.t) : std::nullopt;
+      auto out = QkvNormRope::apply(qkv, q_weight, k_weight, cos, sin, on_device, pos.host, eps,
+                                    kv_heads.value_or(-1));
+      return {out[0], out[1], out[2]};
+    }
+  }
+  const NormRopeCall c = norm_rope_call(qkv, q_weight, k_weight, cos, sin, pos, kv_heads, what);
+  auto [q, k] = norm_rope_forward(c, cos, sin, eps);
+  return {q, k, value_heads(qkv, c.x.Hkv)};
 }
 
 struct Cache4 {
@@ -922,14 +1032,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("tree_v"), pybind11::arg("path"), pybind11::arg("counts"),
         pybind11::arg("cache_lens"));
   m.def("qkv_norm_rope", &qkv_norm_rope,
-        "RMS norm and rotation of the query and key heads of a fused projection; returns q and k",
+        "RMS norm and rotation of the query and key heads of a fused projection; returns q, k and v, differentiable",
         pybind11::arg("qkv"), pybind11::arg("q_weight"), pybind11::arg("k_weight"), pybind11::arg("cos"),
         pybind11::arg("sin"), pybind11::arg("position"), pybind11::arg("eps"), pybind11::arg("kv_heads"));
-  m.def("qkv_norm_rope_backward", &qkv_norm_rope_backward,
-        "Gradients of qkv_norm_rope; returns dqkv and the norm weights' gradients",
-        pybind11::arg("qkv"), pybind11::arg("q_weight"), pybind11::arg("k_weight"), pybind11::arg("cos"),
-        pybind11::arg("sin"), pybind11::arg("position"), pybind11::arg("eps"), pybind11::arg("kv_heads"),
-        pybind11::arg("dq"), pybind11::arg("dk"), pybind11::arg("dv"));
   m.def("cache4_append", &cache4_append,
         "Norm, rotation and quantised append of a fused projection to a 4-bit cache; returns q",
         pybind11::arg("qkv"), pybind11::arg("cos"), pybind11::arg("sin"), pybind11::arg("position"),
