@@ -196,41 +196,38 @@ def test_format_constants_agree():
     assert oracle.SCALES[byte] == 10240 and len(oracle.SCALES) == byte + 1
 
 
-def test_entry_points_forward_and_guard():
+def test_entry_points_forward_to_the_native_module():
     from tiny_transformer_b200.operators import cache4, fused
-    t = [Mock(is_cuda=True, requires_grad=False) for _ in range(7)]
-    ext, o, lse = Mock(), object(), object()
-    ext.cache4_attention.return_value = (o, lse)
+    t = [object() for _ in range(7)]
+    ext = Mock()
     with patch.object(cache4, "load_attention_extension", return_value=ext):
-        assert cache4.attention(*t[:3], 5) is o
-        ext.cache4_attention.assert_called_with(*t[:3], 5, False)
-        assert cache4.attention_with_lse(*t[:3]) == (o, lse)
-        ext.cache4_attention.assert_called_with(*t[:3], None, True)
+        assert cache4.attention(*t[:3], 5) is ext.cache4_attention.return_value
+        ext.cache4_attention.assert_called_with(*t[:3], 5)
+        assert cache4.attention_with_lse(*t[:3]) is ext.cache4_attention_with_lse.return_value
+        ext.cache4_attention_with_lse.assert_called_with(*t[:3], None)
         cache4.append(t[0], t[1], t[2], 9, t[3], t[4], t[5], t[6], eps=1e-5)
         ext.cache4_append.assert_called_with(t[0], t[1], t[2], 9, t[3], t[4], t[5], t[6], 1e-5)
         cache4.read(t[3], t[4], 2, 3)
         ext.cache4_read.assert_called_with(t[3], t[4], 2, 3)
-        calls = [lambda: cache4.attention(*t[:3]), lambda: cache4.attention_with_lse(*t[:3]),
-                 lambda: cache4.read(t[1], t[2], 0, 1), lambda: cache4.append(*t[:3], 0, *t[1:3], *t[:2])]
-        for call in calls:
-            with patch.object(torch, "is_autocast_enabled", return_value=True), \
-                    pytest.raises(RuntimeError, match="AMP"):
-                call()
-            t[1].requires_grad = True
-            with pytest.raises(NotImplementedError, match="no backward"):
-                call()
-            t[1].requires_grad = False
-            t[1].is_cuda = False
-            with pytest.raises(RuntimeError, match="CUDA"):
-                call()
-            t[1].is_cuda = True
-    with pytest.raises(RuntimeError, match="CUDA"):
-        table = torch.zeros(4, 32)
-        fused.qkv_norm_rope(torch.zeros(1, 1, 3, 1, 64), None, None, table, table)
+    with patch.object(fused, "load_attention_extension", return_value=ext):
+        fused.qkv_norm_rope(*t[:5], kv_heads=4)
+        ext.qkv_norm_rope.assert_called_with(*t[:5], 0, 1e-6, 4)
+
+
+def test_cpu_tensors_are_refused():
+    from tiny_transformer_b200.operators import cache4, fused
+    cache = cache4.new_cache(2, 3, 33, device="cpu")
+    assert cache.shape == (2, 3, 3, 576)
+    x, table, q = torch.zeros(2, 1, 3, 3, 64), torch.zeros(4, 32), torch.zeros(2, 3, 1, 64)
+    for call in (lambda: cache4.attention(q, cache, cache), lambda: cache4.attention_with_lse(q, cache, cache),
+                 lambda: cache4.read(cache, cache, 0, 1),
+                 lambda: cache4.append(x, table, table, 0, cache, cache),
+                 lambda: fused.qkv_norm_rope(x, None, None, table, table)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
     for bad in ((0, 1, 1), (1, 0, 1), (1, 1, 0)):
         with pytest.raises(ValueError, match="positive"):
             cache4.new_cache(*bad, device="cpu")
-    assert cache4.new_cache(2, 3, 33, device="cpu").shape == (2, 3, 3, 576)
 
 
 def test_oracle_quantiser_is_nearest_and_round_trips():

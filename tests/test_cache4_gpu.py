@@ -516,6 +516,7 @@ def test_attention_layouts(c4):
     (lambda q, k, v: (q, k, v, torch.zeros(3, dtype=torch.int32, device="cuda")), "shape"),
     (lambda q, k, v: (q, k, v, torch.zeros(2, device="cuda")), "int32 or int64"),
     (lambda q, k, v: (q, k, v, torch.zeros(2, dtype=torch.int32)), "same device"),
+    (lambda q, k, v: (q, k.cpu(), v), "CUDA"),
     (lambda q, k, v: (q, k.view(-1)[:0].view(2, 2, 0, 576), v.view(-1)[:0].view(2, 2, 0, 576)), "positive"),
 ])
 def test_attention_refusals(c4, bad, match):
@@ -540,6 +541,7 @@ def test_attention_refusals(c4, bad, match):
     (dict(position=lambda x: torch.zeros(2, 3, dtype=torch.long, device="cuda")), "one element"),
     (dict(position=lambda x: torch.zeros(1, dtype=torch.int32, device="cuda")), "int64"),
     (dict(position=lambda x: torch.zeros(1, dtype=torch.long)), "int64 CUDA"),
+    (dict(cos=lambda x: x.cpu()), "CUDA"),
     (dict(position=lambda x: 1.5), "int or an int64"),
     (dict(cache_k=lambda x: x[:, :1]), "multiple|same shape"),
     (dict(cache_k=lambda x: x.to(torch.int8)), "uint8"),
@@ -557,6 +559,25 @@ def test_append_refusals(c4, change, match):
         args[key] = f(args[key])
     with pytest.raises(RuntimeError, match=match):
         c4.append(**args)
+
+
+def test_inference_only(c4):
+    qkv, qw, kw = (x.cuda() for x in _projection(2, 3, 4, 2, 1))
+    cos, sin = (t.cuda() for t in _tables(64))
+    q, k, v = _queries(2, 4, 1, 1).cuda(), c4.new_cache(2, 2, 32), c4.new_cache(2, 2, 32)
+    calls = [(lambda: c4.append(qkv, cos, sin, 0, k, v, qw, kw, EPS), (qkv, cos, qw, kw)),
+             (lambda: c4.attention(q, k, v), (q,)), (lambda: c4.attention_with_lse(q, k, v), (q,)),
+             (lambda: c4.read(k, v, 0, 1), ())]
+    for call, tensors in calls:
+        with torch.autocast("cuda", torch.bfloat16), pytest.raises(RuntimeError, match="AMP"):
+            call()
+        for t in tensors:
+            t.requires_grad_()
+            with pytest.raises(NotImplementedError, match="no backward"):
+                call()
+            with torch.no_grad():
+                call()
+            t.requires_grad_(False)
 
 
 def test_offsets_past_32_bits(c4):

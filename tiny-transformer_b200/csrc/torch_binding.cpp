@@ -890,6 +890,17 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> qkv_norm_rope(
   return {q, k, value_heads(qkv, c.x.Hkv)};
 }
 
+// What the entry points of the 4-bit cache refuse alike (checked here: in Python it took as long as a launch).
+void inference_only(std::initializer_list<const torch::Tensor*> tensors, const char* what) {
+  const bool grad = at::GradMode::is_enabled();
+  for (const torch::Tensor* t : tensors) {
+    TORCH_CHECK(t->defined() && t->is_cuda(), what, " requires CUDA tensors");
+    TORCH_CHECK_NOT_IMPLEMENTED(!(grad && t->requires_grad()), what,
+                                " has no backward; call it under torch.no_grad()");
+  }
+  TORCH_CHECK(!at::autocast::is_autocast_enabled(at::kCUDA), what, " does not support AMP/autocast yet");
+}
+
 struct Cache4 {
   int64_t B, H, blocks;
   int64_t s[4];
@@ -910,7 +921,9 @@ torch::Tensor cache4_append(const torch::Tensor& qkv, const torch::Tensor& cos, 
                             const torch::Tensor& cache_v, std::optional<torch::Tensor> q_weight,
                             std::optional<torch::Tensor> k_weight, double eps) {
   const char* what = "cache4.append";
-  TORCH_CHECK(qkv.defined() && qkv.is_cuda(), what, ": all tensors must be CUDA tensors");
+  inference_only({&qkv, &cos, &sin, &cache_k, &cache_v}, what);
+  if (q_weight.has_value()) inference_only({&*q_weight}, what);
+  if (k_weight.has_value()) inference_only({&*k_weight}, what);
   const Cache4 ck = cache4_tensor(cache_k, qkv, what), cv = cache4_tensor(cache_v, qkv, what);
   const c10::cuda::CUDAGuard device_guard(qkv.device());
   const Projection x = projection(qkv, ck.H, what);
@@ -935,7 +948,7 @@ torch::Tensor cache4_append(const torch::Tensor& qkv, const torch::Tensor& cos, 
 std::tuple<torch::Tensor, torch::Tensor> cache4_read(const torch::Tensor& cache_k, const torch::Tensor& cache_v,
                                                      const pybind11::object& start, int64_t rows) {
   const char* what = "cache4.read";
-  TORCH_CHECK(cache_k.defined() && cache_k.is_cuda(), what, ": all tensors must be CUDA tensors");
+  inference_only({&cache_k, &cache_v}, what);
   const Cache4 ck = cache4_tensor(cache_k, cache_k, what), cv = cache4_tensor(cache_v, cache_k, what);
   TORCH_CHECK(cache_v.sizes() == cache_k.sizes(), what, ": the caches must have the same shape");
   TORCH_CHECK(rows > 0, what, ": the number of rows must be positive");
@@ -956,11 +969,12 @@ std::tuple<torch::Tensor, torch::Tensor> cache4_read(const torch::Tensor& cache_
 }
 
 // Attention over a 4-bit cache (tt_attn_cache4_forward_bf16).
-std::tuple<torch::Tensor, torch::Tensor> cache4_attention(torch::Tensor q, const torch::Tensor& cache_k,
-                                                          const torch::Tensor& cache_v,
-                                                          std::optional<torch::Tensor> kv_lens, bool with_lse) {
+std::tuple<torch::Tensor, torch::Tensor> cache4_attention_impl(torch::Tensor q, const torch::Tensor& cache_k,
+                                                               const torch::Tensor& cache_v,
+                                                               std::optional<torch::Tensor> kv_lens,
+                                                               bool with_lse) {
   const char* what = "cache4.attention";
-  TORCH_CHECK(q.defined() && q.is_cuda(), what, ": all tensors must be CUDA tensors");
+  inference_only({&q, &cache_k, &cache_v}, what);
   TORCH_CHECK(q.scalar_type() == at::kBFloat16 && q.layout() == at::kStrided && q.dim() == 4, what,
               ": q must be a strided 4D bf16 tensor");
   TORCH_CHECK(q.size(3) == TT_ATTN_HEAD_DIM, what, " currently supports only head_dim=64");
@@ -995,6 +1009,17 @@ std::tuple<torch::Tensor, torch::Tensor> cache4_attention(torch::Tensor q, const
   TORCH_CHECK(st == TT_ATTN_OK, "tt_attn_cache4_forward_bf16 failed: ", tt_attn_status_string(st), ": ",
               tt_attn_last_error());
   return {o, lse};
+}
+
+torch::Tensor cache4_attention(torch::Tensor q, const torch::Tensor& cache_k, const torch::Tensor& cache_v,
+                               std::optional<torch::Tensor> kv_lens) {
+  return std::get<0>(cache4_attention_impl(std::move(q), cache_k, cache_v, std::move(kv_lens), false));
+}
+
+std::tuple<torch::Tensor, torch::Tensor> cache4_attention_with_lse(torch::Tensor q, const torch::Tensor& cache_k,
+                                                                   const torch::Tensor& cache_v,
+                                                                   std::optional<torch::Tensor> kv_lens) {
+  return cache4_attention_impl(std::move(q), cache_k, cache_v, std::move(kv_lens), true);
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1042,10 +1067,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("k_weight"), pybind11::arg("eps"));
   m.def("cache4_read", &cache4_read, "Rows of a 4-bit cache as bf16; returns K and V",
         pybind11::arg("cache_k"), pybind11::arg("cache_v"), pybind11::arg("start"), pybind11::arg("rows"));
-  m.def("cache4_attention", &cache4_attention,
-        "Attention over a 4-bit KV cache; returns O and (with_lse) LSE", pybind11::arg("q"),
-        pybind11::arg("cache_k"), pybind11::arg("cache_v"), pybind11::arg("kv_lens") = pybind11::none(),
-        pybind11::arg("with_lse") = true);
+  m.def("cache4_attention", &cache4_attention, "Attention over a 4-bit KV cache; returns O",
+        pybind11::arg("q"), pybind11::arg("cache_k"), pybind11::arg("cache_v"),
+        pybind11::arg("kv_lens") = pybind11::none());
+  m.def("cache4_attention_with_lse", &cache4_attention_with_lse,
+        "Attention over a 4-bit KV cache; returns O and LSE", pybind11::arg("q"), pybind11::arg("cache_k"),
+        pybind11::arg("cache_v"), pybind11::arg("kv_lens") = pybind11::none());
   m.attr("HEAD_DIM") = TT_ATTN_HEAD_DIM;
   m.attr("ABI_VERSION") = TT_ATTN_ABI_VERSION;
 }

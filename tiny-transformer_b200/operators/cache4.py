@@ -20,19 +20,6 @@ BLOCK_BYTES = 576
 MAX_QUERIES = 16
 
 
-def _guard(name, tensors):
-    grad = torch.is_grad_enabled()
-    for x in tensors:
-        if x is None:
-            continue
-        if not x.is_cuda:
-            raise RuntimeError(f"{name} requires CUDA tensors")
-        if grad and x.requires_grad:
-            raise NotImplementedError(f"{name} has no backward; call it under torch.no_grad()")
-    if torch.is_autocast_enabled("cuda"):
-        raise RuntimeError(f"{name} does not support AMP/autocast yet")
-
-
 def new_cache(batch, kv_heads, capacity, device="cuda"):
     """A zeroed cache for ``capacity`` rows (rounded up to whole blocks of 16)."""
     if batch <= 0 or kv_heads <= 0 or capacity <= 0:
@@ -52,7 +39,6 @@ def append(qkv, cos, sin, position, cache_k, cache_v, q_weight=None, k_weight=No
     Rows outside the cache or the tables are not written, their q is zero, and the range bit of the device
     status is set (``tt_attn_device_status``). Runs on the current CUDA stream; inference only.
     """
-    _guard("cache4.append", (qkv, cos, sin, cache_k, cache_v, q_weight, k_weight))
     return load_attention_extension().cache4_append(qkv, cos, sin, position, cache_k, cache_v, q_weight,
                                                     k_weight, eps)
 
@@ -63,7 +49,6 @@ def read(cache_k, cache_v, start, rows):
     ``start`` is an int, or an int64 CUDA tensor with one element or one for each sequence; rows outside the cache
     then read as zero and set the range bit of the device status.
     """
-    _guard("cache4.read", (cache_k, cache_v))
     return load_attention_extension().cache4_read(cache_k, cache_v, start, rows)
 
 
@@ -78,13 +63,10 @@ def attention(q, cache_k, cache_v, kv_lens=None):
     they hold. Longer prompts read their rows back (:func:`read`) for ``student.attention``.
     Runs on the current CUDA stream; inference only.
     """
-    _guard("cache4.attention", (q, cache_k, cache_v))
-    output, _ = load_attention_extension().cache4_attention(q, cache_k, cache_v, kv_lens, False)
-    return output
+    return load_attention_extension().cache4_attention(q, cache_k, cache_v, kv_lens)
 
 
 def attention_with_lse(q, cache_k, cache_v, kv_lens=None):
     """Like :func:`attention` but returns ``(O, LSE)``; LSE is FP32 ``[B, Hq, T]``, natural log (-inf for a query
     that sees no row)."""
-    _guard("cache4.attention_with_lse", (q, cache_k, cache_v))
-    return load_attention_extension().cache4_attention(q, cache_k, cache_v, kv_lens, True)
+    return load_attention_extension().cache4_attention_with_lse(q, cache_k, cache_v, kv_lens)
