@@ -137,8 +137,13 @@ struct Cache4Plan {
   int64_t flat_ctas = 0;  // the flat kernel's CTAs; 0: the cluster kernel
 };
 
-// From here on equal shares of all tiles beat a cluster for each unit.
-constexpr int64_t kCache4FlatTiles = 16384;
+// Measured (B200, us; cluster x parts, lengths half to all of the capacity, one query token):
+//   flat / cluster: 768 units x 128 tiles 46 / 58; 512 x 64 30.6 / 30.6; 384 x 64 21.0 / 21.2; 128 x 64 14.4 / 10.7.
+//   A unit's cluster, 96 units x 128 tiles: 1 to 8 CTAs 21, 15.8, 14.6, 12.3 (4), 13.7 (6), 14.1 (8); 256 x 64: 19.1, 17.3,
+//   21.5, 20.3 (4): three CTAs to an SM are best, and two CTAs a unit where that leaves one.
+//   Few units, parts without a cluster / clusters of 8 in one part or several: 12 x 64 tiles 4.7 / 4.1; 24 x 64 5.6 / 4.9;
+//   4 x 256 5.8 / 7.0; 12 x 512 8.0 / 9.0; 8 x 512 7.8 / 8.4; 2 x 2048 11.3 / 10.2; 32 x 128 8.4 / 7.7.
+constexpr int64_t kCache4FlatTiles = 24576;
 
 Cache4Plan cache4_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t blocks) {
   namespace at = tt::cache4::attn;
@@ -153,12 +158,17 @@ Cache4Plan cache4_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t
     pl.flat_ctas = kPlanSms;
     return pl;
   }
-  // CTAs of a unit: enough to fill three to an SM, each warp with a tile at least; for long caches CTAs of about 64
-  // tiles whatever their number, so that uneven lengths leave short ends.
-  const int64_t most = (tiles + at::WARPS - 1) / at::WARPS;
-  const int64_t want = std::min(most, std::max<int64_t>(3 * kPlanSms / units, std::min<int64_t>(4, tiles / 64)));
-  pl.cluster = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, at::MAX_CLUSTER)));
-  pl.parts = std::max<int64_t>(1, want / at::MAX_CLUSTER);
+  const int64_t most = (tiles + at::WARPS - 1) / at::WARPS;   // each warp with a tile at least
+  const int64_t fill = std::max<int64_t>(3 * kPlanSms / units, units <= 2 * kPlanSms ? 2 : 1);
+  if (units >= 32 || most <= 3 * at::MAX_CLUSTER) {
+    pl.cluster = static_cast<int>(std::min<int64_t>({fill, most, at::MAX_CLUSTER}));
+    return pl;
+  }
+  pl.parts = std::min<int64_t>({2 * kPlanSms / units, 32, most});
+  if (most > 4 * pl.parts && 2 * kPlanSms / units > 32) {   // a long cache of a few heads
+    pl.cluster = at::MAX_CLUSTER;
+    pl.parts = 2 * kPlanSms / units / at::MAX_CLUSTER;
+  }
   return pl;
 }
 

@@ -617,16 +617,34 @@ __device__ __forceinline__ float part_weight(float e, float ref) {
 struct Sum {
   float e = NEG_INF, l = 0.0f, v0 = 0.0f, v1 = 0.0f;
 
-  __device__ __forceinline__ void add(float2 el, float2 v) {
-    const float top = fmaxf(e, el.x);
-    const float f = part_weight(e, top), h = part_weight(el.x, top);
+  // Up to N records from rec on, `step` floats apart, loaded together: one maximum, then all weights side by side.
+  template <int N>
+  __device__ __forceinline__ void add(const float* rec, int64_t step, int count, int lane) {
+    float2 el[N], v[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float* at = rec + (j < count ? j * step : 0);
+      el[j] = *reinterpret_cast<const float2*>(at + HD);
+      v[j] = *reinterpret_cast<const float2*>(at + 2 * lane);
+    }
+    float top = e;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (j >= count) el[j].x = NEG_INF;
+      top = fmaxf(top, el[j].x);
+    }
+    const float f = part_weight(e, top);
     e = top;
-    l = l * f + el.y * h;
-    v0 = v0 * f + v.x * h;
-    v1 = v1 * f + v.y * h;
-  }
-  __device__ __forceinline__ void add(const float* rec, int d) {
-    add(*reinterpret_cast<const float2*>(rec + HD), *reinterpret_cast<const float2*>(rec + d));
+    l *= f;
+    v0 *= f;
+    v1 *= f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float h = part_weight(el[j].x, top);
+      l += j < count ? el[j].y * h : 0.0f;    // (a part that is not counted may hold anything)
+      v0 += j < count ? v[j].x * h : 0.0f;
+      v1 += j < count ? v[j].y * h : 0.0f;
+    }
   }
   __device__ __forceinline__ void store(float* rec, int lane) const {
     *reinterpret_cast<float2*>(rec + 2 * lane) = make_float2(v0, v1);
@@ -708,8 +726,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? MIN_CTAS : 3)
   if (p.cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   for (int r = warp; r < rows; r += WARPS) {
     Sum sum;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) sum.add(sm.warp[w].own[r], 2 * lane);
+    sum.add<WARPS>(sm.warp[0].own[r], sizeof(sm.warp[0]) / sizeof(float), WARPS, lane);
     if (p.cluster > 1) {
       const uint32_t dst = map_to_rank(smem_u32(sm.from[r / p.cluster * p.cluster + rank]),
                                        static_cast<uint32_t>(r % p.cluster));
@@ -726,7 +743,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? MIN_CTAS : 3)
   cluster_sync();
   for (int r = rank + p.cluster * warp; r < rows; r += p.cluster * WARPS) {
     Sum sum;
-    for (int c = 0; c < p.cluster; ++c) sum.add(sm.from[r / p.cluster * p.cluster + c], 2 * lane);
+    sum.add<MAX_CLUSTER>(sm.from[r / p.cluster * p.cluster], REC, p.cluster, lane);
     if (p.parts > 1)
       sum.store(p.records + (static_cast<int64_t>(pc) * ROWS + r) * REC, lane);
     else
@@ -737,6 +754,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? MIN_CTAS : 3)
 // ------------------------------------------------------------------------------- merging records
 
 constexpr int COMBINE_WARPS = 8;
+constexpr int COMBINE_LOADS = 4;   // records of a warp in flight
 
 // Merges the parts' records: one CTA a row, each warp every eighth part.
 __global__ void __launch_bounds__(COMBINE_WARPS * 32)
@@ -749,15 +767,15 @@ __global__ void __launch_bounds__(COMBINE_WARPS * 32)
   wait_for_previous_kernel();
   const float* src = p.records + (unit * p.parts * tile_rows + gr % tile_rows) * REC;
   Sum sum;
-#pragma unroll 4
-  for (int c = warp; c < p.parts; c += COMBINE_WARPS)
-    sum.add(src + static_cast<int64_t>(c) * tile_rows * REC, 2 * lane);
+  const int64_t step = static_cast<int64_t>(tile_rows) * REC * COMBINE_WARPS;
+  src += warp * (step / COMBINE_WARPS);
+  for (int c = warp; c < p.parts; c += COMBINE_WARPS * COMBINE_LOADS, src += COMBINE_LOADS * step)
+    sum.add<COMBINE_LOADS>(src, step, (p.parts - c + COMBINE_WARPS - 1) / COMBINE_WARPS, lane);
   sum.store(rec[warp], lane);
   __syncthreads();
   if (warp != 0) return;
   Sum all;
-#pragma unroll
-  for (int w = 0; w < COMBINE_WARPS; ++w) all.add(rec[w], 2 * lane);
+  all.add<COMBINE_WARPS>(rec[0], REC, COMBINE_WARPS, lane);
   all.finish(p, blockIdx.x, lane);
 }
 
@@ -938,18 +956,8 @@ __global__ void __launch_bounds__(FLAT_COMBINE_WARPS * 32, 8)
   wait_for_previous_kernel();
   if (!valid) return;   // whole warps
   Sum sum;
-  for (int i = 0; i < count; i += FLAT_COMBINE_LOADS, src += FLAT_COMBINE_LOADS * step) {
-    float2 el[FLAT_COMBINE_LOADS], v[FLAT_COMBINE_LOADS];
-#pragma unroll
-    for (int j = 0; j < FLAT_COMBINE_LOADS; ++j) {
-      const float* rec = src + (i + j < count ? j * step : 0);
-      el[j] = *reinterpret_cast<const float2*>(rec + HD);
-      v[j] = *reinterpret_cast<const float2*>(rec + 2 * lane);
-    }
-#pragma unroll
-    for (int j = 0; j < FLAT_COMBINE_LOADS; ++j)
-      if (i + j < count) sum.add(el[j], v[j]);
-  }
+  for (int i = 0; i < count; i += FLAT_COMBINE_LOADS, src += FLAT_COMBINE_LOADS * step)
+    sum.add<FLAT_COMBINE_LOADS>(src, step, count - i, lane);
   sum.finish(p, at, lane);
 }
 
