@@ -234,6 +234,10 @@ def test_append_outside_the_cache_or_table_is_skipped(c4):
     cos, sin = (t.cuda() for t in _tables(40))
     caches = [c4.new_cache(B, H, 32).fill_(7) for _ in range(2)]
     _status()
+    for far in (2**63 - 1, -2**63, 2**31, 2**32 + 3):
+        before = [c.clone() for c in caches]
+        q = c4.append(qkv, cos, sin, torch.tensor([far], device="cuda"), *caches, qw, kw, EPS)
+        assert _status() == 2 and (q == 0).all() and all(map(torch.equal, before, caches))
     at = torch.tensor([-2, 30, 2**62, 5], device="cuda")
     q = c4.append(qkv, cos, sin, at, *caches, qw, kw, EPS)
     assert _status() == 2
@@ -293,6 +297,16 @@ def test_read_outside_the_cache_is_zero(c4):
     all_k = c4.read(k, v, 0, 32)[0]
     assert (got[0][0, 0, 0] == 0).all() and torch.equal(got[0][0, 0, 1:], all_k[0, 0, :2])
     assert (got[0][1, 0, 2] == 0).all() and torch.equal(got[0][1, 0, :2], all_k[1, 0, 30:])
+    for far in (2**63 - 1, 2**63 - 2, -2**63, 2**31, 2**32 + 5, -2**32 + 1):
+        got = c4.read(k, v, torch.tensor([far, 0], device="cuda"), 20)
+        assert _status() == 2
+        assert (got[0][0] == 0).all() and (got[1][0] == 0).all() and torch.equal(got[0][1], all_k[1, :, :20])
+    for start in range(-20, 33):          # every way to lie across the ends, and across blocks
+        got = c4.read(k, v, torch.tensor([start], device="cuda"), 21)
+        for i in range(21):
+            want = all_k[:, :, start + i] if 0 <= start + i < 32 else torch.zeros_like(all_k[:, :, 0])
+            assert torch.equal(got[0][:, :, i], want)
+    _status()
     for bad in (-1, 30):
         with pytest.raises(RuntimeError, match="capacity"):
             c4.read(k, v, bad, 3)

@@ -403,7 +403,9 @@ TT_ATTN_API tt_attn_status tt_attn_cache4_read_bf16(
   p.start = start;
   p.start_dev = start_dev;
   p.start_sb = start_sb;
-  const int64_t items = 2 * batch * kv_heads * ((rows + c4::READ_ROWS - 1) / c4::READ_ROWS);
+  p.chunks.set(static_cast<uint32_t>((rows + c4::READ_ROWS - 1) / c4::READ_ROWS));
+  p.heads.set(static_cast<uint32_t>(kv_heads));
+  const int64_t items = 2 * batch * kv_heads * p.chunks.d;
   const Launch launch(dim3(static_cast<unsigned>((items + c4::READ_WARPS - 1) / c4::READ_WARPS)),
                       c4::READ_WARPS * 32, 0, 1, static_cast<cudaStream_t>(stream));
   return check_launch("cache4_read launch", cudaLaunchKernelEx(&launch.cfg, c4::read_kernel, p));

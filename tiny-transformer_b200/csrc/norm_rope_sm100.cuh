@@ -73,6 +73,7 @@ struct Common {
 __device__ __forceinline__ int64_t position_of(const Common& p, int b, int t) {
   if (p.position_dev == nullptr) return p.position + t;
   const int64_t at = p.position_dev[b * p.pos_sb + t * p.pos_st];
+  if (at < 0 || at > (int64_t(1) << 40)) return at < 0 && p.pos_st == 0 ? max(at, -(int64_t(1) << 40)) + t : -1;
   return p.pos_st != 0 ? at : at + t;
 }
 
