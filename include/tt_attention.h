@@ -98,7 +98,8 @@ TT_ATTN_API int tt_attn_device_supported(void);
 
 /* Reads (and, when clear != 0, resets) the current device's kernel status bits:
  * bit 0 = a bounded wait inside a kernel ran out (returns TT_ATTN_TIMEOUT);
- * bit 1 = tt_rope_append_bf16 met a device-held position outside the cache or the table, or
+ * bit 1 = tt_rope_append_bf16, tt_attn_cache4_append_bf16, tt_attn_cache4_read_bf16 or
+ * tt_attn_qkv_norm_rope_bf16 met a device-held position outside the cache or the table, or
  * tt_attn_tree_commit_bf16 a row or path entry outside its buffer, and skipped those rows
  * (returns TT_ATTN_BAD_ARG). Synchronises the device. */
 TT_ATTN_API tt_attn_status tt_attn_device_status(unsigned* flags, int clear);
@@ -407,7 +408,7 @@ TT_ATTN_API size_t tt_attn_qkv_norm_rope_backward_workspace_size(void);
 /*
  * tt_attn_qkv_norm_rope_bf16's pass with the cache append in it: q goes to q_out, the keys (as bf16, correctly
  * rounded) and the values are quantised into rows position + t of the caches. Other rows are left as they are.
- * position_dev[b * position_sb] + t with a device-held position. Rows outside the cache or the table are not
+ * position_dev[b * position_sb] + t with a device-held position; the two caches must not overlap. Rows outside the cache or the table are not
  * written, their q is zero, and status bit 1 is set.
  */
 TT_ATTN_API tt_attn_status tt_attn_cache4_append_bf16(

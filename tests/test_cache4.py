@@ -104,6 +104,7 @@ def _cache(n=7, H=2):
     (dict(n=2**30), BAD_ARG, "fit int32"),
     (dict(pos=100, L=1000, n=6), BAD_ARG, "cache capacity"),
     (dict(ck=24), UNSUPPORTED, "caches need"),
+    (dict(ck=32), BAD_ARG, "caches of their own"),
     (dict(cs=_s(2 * 7 * 576, 7 * 576, 584, 1)), UNSUPPORTED, "caches need"),
     (dict(cs=_s(2 * 7 * 576, 7 * 576, 576, 2)), UNSUPPORTED, "caches need"),
 ])
@@ -111,7 +112,7 @@ def test_append_rejects_before_cuda(lib, kwargs, status, fragment):
     kwargs = dict(kwargs)
     q, ck, n = kwargs.pop("q", 16), kwargs.pop("ck", 16), kwargs.pop("n", 7)
     cs = kwargs.pop("cs", _cache())
-    assert lib.tt_attn_cache4_append_bf16(*_projection(**kwargs), 1e-6, q, ck, cs, 16, _cache(), n,
+    assert lib.tt_attn_cache4_append_bf16(*_projection(**kwargs), 1e-6, q, ck, cs, 32, _cache(), n,
                                           None) == status
     assert fragment in _err(lib)
 
@@ -176,7 +177,7 @@ def test_workspace_sizes(lib):
     n = lib.tt_attn_cache4_workspace_size(1, 16, 2, 1, 8192)               # few sequences, a long cache
     assert n > 0 and n % (2 * 8 * 66 * 4) == 0
     n = lib.tt_attn_cache4_workspace_size(64, 12, 12, 1, 512)              # many sequences
-    assert n % (8 * 66 * 4) == 0 and n // (8 * 66 * 4) == 64 * 12 + 148 * 16
+    assert n == 64 * 12 * 8 + (64 * 12 + 148 * 16) * 8 * 66 * 4            # a table of the units, records
     for bad in ((0, 1, 1, 1, 1), (1, 3, 2, 1, 1), (1, 1, 1, 17, 1), (1, 1, 1, 1, 0), (2**40, 1, 1, 1, 1)):
         assert lib.tt_attn_cache4_workspace_size(*bad) == 0
     assert lib.tt_attn_qkv_norm_rope_backward_workspace_size() % (64 * 4) == 0

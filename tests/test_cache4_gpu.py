@@ -139,6 +139,34 @@ def test_append_matches_oracle(c4, B, T, Hq, Hkv, C, position, weights):
     _check_append(c4, B, T, Hq, Hkv, C, position, weights)
 
 
+@pytest.mark.parametrize("kind", ["weights", "table", "large", "small", "no eps"])
+def test_append_where_fp32_cannot_decide(c4, kind):
+    """Rows for which the FP32 bound says little or FP32 leaves its range: codes as from 64 bits all the same."""
+    B, T, H, C = 2, 40, 3, 64
+    qkv, qw, kw = _projection(B, T, H, H, 77, "f32")
+    cos, sin = _tables(C)
+    eps = EPS
+    if kind == "weights":        # coefficients of a pair far apart, features the other way round: sums that cancel
+        big = torch.arange(64) % 2 == 0
+        kw = torch.where(big, kw * 2.0 ** 12, kw * 2.0 ** -12)
+        qkv[:, :, H:2 * H] = torch.where(big, qkv[:, :, H:2 * H] * 2.0 ** -12, qkv[:, :, H:2 * H] * 2.0 ** 12)
+    elif kind == "table":        # not a rotation: every first element of a pair nearly cancels
+        cos, sin = torch.ones(C, 32), torch.ones(C, 32)
+        qkv[..., 1::2] = qkv[..., 0::2]
+        kw = torch.ones(64)
+        kw[1::2] += 2.0 ** -20
+    elif kind == "large":
+        qkv = (qkv.float() * 2.0 ** 70).to(torch.bfloat16)
+    else:
+        qkv = (qkv.float() * 2.0 ** -80).to(torch.bfloat16)
+        eps = 0.0 if kind == "no eps" else 1e-30
+    caches = [c4.new_cache(B, H, C) for _ in range(2)]
+    c4.append(qkv.cuda(), cos.cuda(), sin.cuda(), 5, *caches, qw.cuda(), kw.cuda(), eps)
+    at = np.broadcast_to(5 + np.arange(T), (B, T))
+    k, _ = oracle.norm_rope(_np(qkv[:, :, H:2 * H]), _np(kw), _np(cos)[at], _np(sin)[at], eps)
+    _check_rows(caches[0].cpu().numpy(), torch.from_numpy(k).to(torch.bfloat16).double().numpy(), at)
+
+
 def test_append_layouts_give_the_same_bytes(c4):
     """A 5-D projection, strided and unaligned views, transposed caches, views of larger caches."""
     B, T, H, C = 2, 9, 3, 48
@@ -559,6 +587,7 @@ def test_attention_refusals(c4, bad, match):
     (dict(position=lambda x: 1.5), "int or an int64"),
     (dict(cache_k=lambda x: x[:, :1]), "multiple|same shape"),
     (dict(cache_k=lambda x: x.to(torch.int8)), "uint8"),
+    (dict(cache_k=lambda x: x, cache_v="cache_k"), "caches of their own"),
     (dict(q_weight=lambda x: None), "both norm weights"),
     (dict(q_weight=lambda x: x.float()), "both be"),
     (dict(k_weight=lambda x: x[:32]), "shape"),
@@ -570,7 +599,7 @@ def test_append_refusals(c4, change, match):
     args = dict(qkv=qkv, cos=cos, sin=sin, position=0, cache_k=c4.new_cache(2, 2, 32),
                 cache_v=c4.new_cache(2, 2, 32), q_weight=qw, k_weight=kw, eps=EPS)
     for key, f in change.items():
-        args[key] = f(args[key])
+        args[key] = args[f] if isinstance(f, str) else f(args[key])
     with pytest.raises(RuntimeError, match=match):
         c4.append(**args)
 

@@ -176,6 +176,11 @@ int64_t cache4_flat_warps(const Cache4Plan& pl) {
   return pl.nt == 1 ? tt::cache4::attn::Flat<1>::WARPS : tt::cache4::attn::Flat<2>::WARPS;
 }
 
+// The flat kernel's table of units, in front of the records.
+size_t cache4_table_bytes(const Cache4Plan& pl, int64_t units) {
+  return pl.flat_ctas > 0 ? (static_cast<size_t>(units) * sizeof(int2) + 255) & ~size_t(255) : 0;
+}
+
 bool cache4_shape_ok(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t blocks) {
   constexpr int64_t kMax = INT32_MAX / (tt::cache4::MAX_QUERIES * tt::cache4::attn::MAX_CLUSTER);
   return batch > 0 && q_heads > 0 && kv_heads > 0 && q_len > 0 && blocks > 0 && q_heads % kv_heads == 0 &&
@@ -194,8 +199,7 @@ cudaError_t launch_cache4(const Cache4Plan& pl, const tt::cache4::attn::Params& 
     const int64_t rows = static_cast<int64_t>(p.B) * p.Hkv * p.G * p.T;
     const Launch merge(dim3(static_cast<unsigned>((rows + at::FLAT_COMBINE_WARPS - 1) / at::FLAT_COMBINE_WARPS)),
                        at::FLAT_COMBINE_WARPS * 32, 0, 1, stream);
-    return cudaLaunchKernelEx(&merge.cfg, at::flat_combine_kernel, p, 8 * NT,
-                              static_cast<int>(pl.flat_ctas) * at::Flat<NT>::WARPS);
+    return cudaLaunchKernelEx(&merge.cfg, at::flat_combine_kernel, p, 8 * NT);
   }
   const int64_t grid = static_cast<int64_t>(p.B) * p.Hkv * pl.row_tiles * pl.parts * pl.cluster;
   const Launch launch(dim3(static_cast<unsigned>(grid)), at::THREADS, sizeof(at::Smem<NT>), pl.cluster, stream);
@@ -355,6 +359,8 @@ TT_ATTN_API tt_attn_status tt_attn_cache4_append_bf16(
   if (!cache4_view(cache_k, ck_strides, batch, kv_heads, blocks, &p.cache[0]) ||
       !cache4_view(cache_v, cv_strides, batch, kv_heads, blocks, &p.cache[1]))
     return fail(TT_ATTN_UNSUPPORTED, std::string("cache4_append") + kCache4Layout);
+  if (cache_k == cache_v)
+    return fail(TT_ATTN_BAD_ARG, "cache4_append: the keys and the values need caches of their own");
   p.capacity = blocks * c4::BLOCK_ROWS;
   if (position_dev == nullptr && position > p.capacity - q_len)
     return fail(TT_ATTN_BAD_ARG, "cache4_append: position + q_len exceeds the cache capacity");
@@ -418,7 +424,7 @@ TT_ATTN_API size_t tt_attn_cache4_workspace_size(int64_t batch, int64_t q_heads,
   const int64_t units = batch * kv_heads * pl.row_tiles;
   if (pl.flat_ctas == 0 && pl.parts == 1) return 0;
   const int64_t slots = pl.flat_ctas > 0 ? units + pl.flat_ctas * cache4_flat_warps(pl) : units * pl.parts;
-  return static_cast<size_t>(slots) * 8 * pl.nt *
+  return cache4_table_bytes(pl, units) + static_cast<size_t>(slots) * 8 * pl.nt *
          tt::cache4::attn::REC * sizeof(float);
 }
 
@@ -476,7 +482,9 @@ TT_ATTN_API tt_attn_status tt_attn_cache4_forward_bf16(
   p.parts = static_cast<int>(pl.parts);
   p.o = static_cast<__nv_bfloat16*>(out);
   p.lse = lse;
-  p.records = static_cast<float*>(workspace);
+  p.parts_of = static_cast<int2*>(workspace);
+  p.records = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
+                                       cache4_table_bytes(pl, batch * kv_heads * pl.row_tiles));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return check_launch("cache4_attention launch",
                       pl.nt == 2                  ? launch_cache4<2, false>(pl, p, s)

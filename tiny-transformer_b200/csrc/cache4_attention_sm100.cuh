@@ -65,6 +65,7 @@ struct Params {
   int cluster, parts;       // CTAs of a cluster, clusters of a unit (cluster kernel)
   __nv_bfloat16* o;         // [B, Hq, T, 64]
   float* lse;               // optional [B, Hq, T]
+  int2* parts_of;           // flat kernel: of each unit that has tiles, its first worker and their number
   float* records;           // [slot, 8 NT rows, REC]; cluster kernel: slot = unit * parts + part
 };
 
@@ -869,7 +870,7 @@ __global__ void __maxnreg__(NT == 1 ? 112 : 152)
   const uint32_t ring = smem_u32(smem_raw) + warp * STAGES * STAGE_BYTES;
   const int worker = static_cast<int>(blockIdx.x) * W + warp;
   wait_for_previous_kernel();
-  // The merge's launch and its own look at the lengths run under this kernel.
+  // The merge's launch runs under this kernel.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const bool dense = p.cache[0].sn == BLOCK_BYTES && p.cache[1].sn == BLOCK_BYTES;
   int total = 0;
@@ -912,6 +913,10 @@ __global__ void __maxnreg__(NT == 1 ? 112 : 152)
     const int unit = (now.u.b * p.Hkv + now.u.hk) * p.row_tiles + now.u.rt;
     q.end(reinterpret_cast<float(*)[REC]>(p.records) + (static_cast<int64_t>(worker) + unit) * ROWS,
           min(p.G * p.T - now.u.rt * ROWS, ROWS), lane);
+    if (lane == 0 && now.tile + 1 == now.u.tiles) {
+      const int from = shares.owner(first + i - 1 - now.tile);
+      p.parts_of[unit] = make_int2(from, worker - from + 1);
+    }
     if (i == count) break;
     now.step(p);
     raw = q.fetch(p, now.u, lane);
@@ -924,37 +929,20 @@ constexpr int FLAT_COMBINE_LOADS = 4;   // records in flight
 
 // One warp a query row: the records of the shares that hold tiles of its unit.
 __global__ void __launch_bounds__(FLAT_COMBINE_WARPS * 32, 8)
-    flat_combine_kernel(const __grid_constant__ Params p, int tile_rows, int workers) {
+    flat_combine_kernel(const __grid_constant__ Params p, int tile_rows) {
   const int lane = threadIdx.x & 31;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * FLAT_COMBINE_WARPS + (threadIdx.x >> 5);
-  const int per_head = p.G * p.T, heads = p.Hkv * p.row_tiles;
+  const int per_head = p.G * p.T;
   const bool valid = at < static_cast<int64_t>(p.B) * p.Hkv * per_head;
   const int bh = valid ? static_cast<int>(at / per_head) : 0, gr = valid ? static_cast<int>(at % per_head) : 0;
-  const int b = bh / p.Hkv, unit = bh * p.row_tiles + gr / tile_rows;
-  // The lengths were written before the flat kernel started (it lets this one start after its own wait); the records
-  // are read after it has ended.
-  int total = 0, before = 0;
-#pragma unroll 4
-  for (int i = lane; i < p.B; i += 32) {
-    const int n = unit_tiles(p, i);
-    total += n;
-    before += i < b ? n : 0;
-  }
-  const int tiles = unit_tiles(p, b);
-  total = __reduce_add_sync(0xffffffffu, total) * heads;
-  before = __reduce_add_sync(0xffffffffu, before) * heads;
-  int w0 = 0, count = 0;
-  if (tiles > 0) {
-    const int first = before + (unit - b * heads) * tiles;
-    Shares shares;
-    shares.set(total, workers);
-    w0 = shares.owner(first);
-    count = shares.owner(first + tiles - 1) - w0 + 1;
-  }
-  const int64_t step = static_cast<int64_t>(tile_rows) * REC;
-  const float* src = p.records + (static_cast<int64_t>(w0) + unit) * step + gr % tile_rows * REC;
+  const int unit = bh * p.row_tiles + gr / tile_rows, b = bh / p.Hkv;
   wait_for_previous_kernel();
   if (!valid) return;   // whole warps
+  const int len = visible_rows(p, b);
+  const int2 parts = p.parts_of[unit];   // (not written for a unit without tiles)
+  const int w0 = len > 0 ? parts.x : 0, count = len > 0 ? parts.y : 0;
+  const int64_t step = static_cast<int64_t>(tile_rows) * REC;
+  const float* src = p.records + (static_cast<int64_t>(w0) + unit) * step + gr % tile_rows * REC;
   Sum sum;
   for (int i = 0; i < count; i += FLAT_COMBINE_LOADS, src += FLAT_COMBINE_LOADS * step)
     sum.add<FLAT_COMBINE_LOADS>(src, step, count - i, lane);

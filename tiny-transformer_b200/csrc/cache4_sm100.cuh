@@ -145,13 +145,15 @@ struct AppendParams {
 };
 
 // The bf16 values of a key row from FP32, `up` those from above; they differ where FP32 cannot tell how a value is
-// rounded. `most` is the largest coefficient of each pair, times 2^-20.
+// rounded. False for a row whose mean square leaves FP32's safe range. `most` is the largest coefficient of each
+// pair, times 2^-20.
 template <bool NORM>
-__device__ __forceinline__ void key_row(const uint4& v, const norm_rope::Coefficients& k, const uint64_t (&most)[2],
+__device__ __forceinline__ bool key_row(const uint4& v, const norm_rope::Coefficients& k, const uint64_t (&most)[2],
                                         float eps, uint4& out, uint4& up) {
   norm_rope::Pairs x;
   x.unpack(v);
-  if (NORM) x.scale(norm_rope::inverse_rms(x, eps));
+  const float r = NORM ? norm_rope::inverse_rms(x, eps) : 1.0f;
+  if (NORM) x.scale(r);
   const norm_rope::Pairs y = k.turn(x);
   norm_rope::Pairs lo, hi;
 #pragma unroll
@@ -170,6 +172,7 @@ __device__ __forceinline__ void key_row(const uint4& v, const norm_rope::Coeffic
   }
   out = lo.pack();
   up = hi.pack();
+  return r > 1e-15f && r < 1e15f;
 }
 
 __device__ __forceinline__ uint32_t min_u16x2(uint32_t a, uint32_t b) {
@@ -178,16 +181,17 @@ __device__ __forceinline__ uint32_t min_u16x2(uint32_t a, uint32_t b) {
   return d;
 }
 
-// Two candidates for each value to the smaller and the larger magnitudes. The true row lies between these in every
-// place, and scales and codes grow with magnitudes: where both have the same, it has them too. (Candidates of different
-// signs keep the first one's; next to zero both codes are zero.)
+// Two candidates for each value to the smaller and the larger magnitudes (zero below candidates of different signs). The
+// true row lies between these in every place, and scales and codes grow with magnitudes: where both have the same, it
+// has them too (but for the sign of a zero).
 __device__ __forceinline__ void order(uint4& a, uint4& b) {
   uint32_t* x[4] = {&a.x, &a.y, &a.z, &a.w};
   uint32_t* y[4] = {&b.x, &b.y, &b.z, &b.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t sign = *x[i] & 0x80008000u, p = *x[i] & 0x7fff7fffu, q = *y[i] & 0x7fff7fffu;
-    *x[i] = min_u16x2(p, q) | sign;
+    const uint32_t crossed = (((*x[i] ^ *y[i]) >> 15) & 0x00010001u) * 0xffffu;
+    *x[i] = (min_u16x2(p, q) & ~crossed) | sign;
     *y[i] = max_u16x2(p, q) | sign;
   }
 }
@@ -301,15 +305,15 @@ __global__ void __launch_bounds__(norm_rope::THREADS, 7)
     for (int j = 0; j < nr::SMALL_BATCH; ++j, ++h, head += ap.cache[0].sh) {
       if (j >= in.left) break;
       uint4 y, up;
-      key_row<NORM>(in.now[j], k, most, eps, y, up);
+      const bool safe = key_row<NORM>(in.now[j], k, most, eps, y, up);
       uint32_t codes, byte;
-      const bool sure = ((y.x ^ up.x) | (y.y ^ up.y) | (y.z ^ up.z) | (y.w ^ up.w)) == 0;
+      const bool sure = safe && ((y.x ^ up.x) | (y.y ^ up.y) | (y.z ^ up.z) | (y.w ^ up.w)) == 0;
       if (__any_sync(0xffffffffu, !sure)) {
         order(y, up);
         uint32_t above;
         const uint32_t byte_above = quantise8(up, above);
         byte = quantise8(y, codes);
-        if (__any_sync(0xffffffffu, codes != above || byte != byte_above)) unsure |= 1u << h;
+        if (__any_sync(0xffffffffu, !safe || codes != above || byte != byte_above)) unsure |= 1u << h;
       } else {
         byte = quantise8(y, codes);
       }
