@@ -20,7 +20,10 @@
 // than its error bound. Of the others (one in 2^10) both neighbours are quantised, and where that gives different
 // codes the row is computed again in FP64.
 //
-// Both kernels are bound by memory (append: 128 bytes a head in, 128 or 36 out; read: 36 in, 128 out).
+// Memory: append 128 bytes a head in, 128 or 36 out; read 36 in, 128 out. Measured (B200, 4 x 4096 tokens of 12 + 12 + 12
+// heads): append 31 us (115 MB, 3.7 TB/s; its integer and conversion instructions bound it, 200 a head of four
+// rows; 43.7 us with keys, values and queries mixed in a CTA and every doubtful row in FP64), read back 14 us
+// (4.6 TB/s, conversions again). A decode step of 64 sequences: append and read back of its rows 4.3 us.
 #pragma once
 
 #include <cuda_bf16.h>

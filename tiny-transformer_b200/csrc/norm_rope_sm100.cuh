@@ -13,7 +13,12 @@
 // lanes hold a row, 16 bytes each, so a warp's loads and stores are 4 whole rows; the pairs of the rotation stay
 // inside a lane and the norm's sums take three shuffles. A warp's item is four tokens of up to sixteen heads of one
 // kind (query, key or value): the tokens' rows of q and k are adjacent in the [B, H, T, 64] outputs, the weights are
-// multiplied into the table rows once, and the next heads are loaded while these are computed.
+// multiplied into the table rows once, and the next heads are loaded while these are computed. Arithmetic is on packed FP32
+// pairs.
+//
+// Measured (B200, 4 x 4096 tokens of 12 + 12 + 12 heads): forward 16.4 us (100 MB, 6.1 TB/s), backward 37 us (201 MB, 5.4
+// TB/s; it waits for loads: 20 warps an SM, and with registers for 24 it spilled and took 58), the weights' sums 4 us.
+// With items of 4 or 6 heads the step took 62 and 59 us against 57.
 #pragma once
 
 #include <cuda_bf16.h>
