@@ -820,6 +820,16 @@ struct Shares {
   }
 };
 
+// Sum of v over the lanes up to this one.
+__device__ __forceinline__ int lanes_up_to(int v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int x = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v += x;
+  }
+  return v;
+}
+
 // A place in the row of tiles.
 struct Cursor {
   Unit u;
@@ -841,17 +851,12 @@ struct Cursor {
     }
     u.set(p, b, hk, rt, len);
   }
-  // To tile `at` of the row.
-  __device__ __forceinline__ void seek(const Params& p, int at, int lane) {
+  // To tile `at` behind the first one of sequence b0.
+  __device__ __forceinline__ void seek(const Params& p, int b0, int at, int lane) {
     const int heads = p.Hkv * p.row_tiles;
-    for (int b0 = 0;; b0 += 32) {
+    for (;; b0 += 32) {
       const int n = b0 + lane < p.B ? unit_tiles(p, b0 + lane) * heads : 0;
-      int up = n;   // tiles up to this lane's sequence
-#pragma unroll
-      for (int d = 1; d < 32; d *= 2) {
-        const int x = __shfl_up_sync(0xffffffffu, up, d);
-        if (lane >= d) up += x;
-      }
+      const int up = lanes_up_to(n, lane);   // tiles up to this lane's sequence
       const unsigned here = __ballot_sync(0xffffffffu, up > at);
       if (here == 0 && b0 + 32 < p.B) {
         at -= __shfl_sync(0xffffffffu, up, 31);
@@ -880,16 +885,20 @@ __global__ void __maxnreg__(NT == 1 ? 112 : 152)
   // The merge's launch runs under this kernel.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const bool dense = p.cache[0].sn == BLOCK_BYTES && p.cache[1].sn == BLOCK_BYTES;
-  int total = 0;
+  // Each lane counts a thirty-second of the sequences; one scan then finds the lane, and another the sequence.
+  const int chunk = (p.B + 31) / 32;
+  int mine = 0;
 #pragma unroll 4
-  for (int b = lane; b < p.B; b += 32) total += unit_tiles(p, b);
-  total = __reduce_add_sync(0xffffffffu, total) * p.Hkv * p.row_tiles;
+  for (int b = lane * chunk; b < min(p.B, (lane + 1) * chunk); ++b) mine += unit_tiles(p, b);
+  mine *= p.Hkv * p.row_tiles;
+  const int up = lanes_up_to(mine, lane);
   Shares shares;
-  shares.set(total, static_cast<int>(gridDim.x) * W);
-  if (worker >= shares.workers || total == 0) return;
+  shares.set(__shfl_sync(0xffffffffu, up, 31), static_cast<int>(gridDim.x) * W);
+  if (worker >= shares.workers || shares.each == 0) return;
   const int first = shares.first(worker), count = shares.first(worker + 1) - first;
+  const int l = __ffs(static_cast<int>(__ballot_sync(0xffffffffu, up > first))) - 1;
   Cursor now, ahead;
-  now.seek(p, first, lane);
+  now.seek(p, l * chunk, first - __shfl_sync(0xffffffffu, up - mine, l), lane);
   ahead = now;
   Rows<NT, ONE> q;
   auto raw = q.fetch(p, now.u, lane);
