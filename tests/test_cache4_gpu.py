@@ -427,6 +427,41 @@ def test_attention_many_sequences(c4, B, Hq, Hkv, T):
     assert (o == 0).all() and torch.isneginf(lse).all()
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,T", [(513, 1, 1, 1), (513, 4, 2, 3), (1700, 2, 1, 1), (5000, 1, 1, 1)])
+def test_attention_thousands_of_sequences(c4, B, Hq, Hkv, T):
+    """More sequences than a count of 32 or of a CTA's threads, runs of empty ones longer than both, and sequences of
+    several tiles on either side of each multiple of 32."""
+    rows, blocks = 160, 4 * (24576 // (B * Hkv) + 2)
+    rs = np.random.RandomState(B + T)
+    kb, kv = _random_cache(B, Hkv, rows, 81)
+    vb, vv = _random_cache(B, Hkv, rows, 82)
+    full = [torch.full((B, Hkv, blocks, 576), 0xFF, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    for dst, src in zip(full, (kb, vb)):
+        dst[:, :, :rows // 16] = torch.from_numpy(src).cuda()
+    q = _queries(B, Hq, T, 83)
+    S = np.abs(vv).sum(2, keepdims=True).repeat(Hq // Hkv, axis=1)
+    for kind in range(4):
+        lens = rs.randint(0, 20, B)
+        lens[::32] = 160
+        lens[31::64] = 65
+        if kind == 1:
+            lens[:500] = 0                    # a share begins far behind the first sequence
+        if kind == 2:
+            lens[7:-3] = 0                    # nearly nothing between the two ends
+        if kind == 3:
+            lens[5:] = 0
+        args = (q.cuda(), *full, torch.from_numpy(lens).cuda())
+        o, lse = c4.attention_with_lse(*args)
+        ref, ref_lse, A = oracle.attention(_np(q), kv, vv, lens)
+        got, got_lse = _np(o), _np(lse)
+        empty = np.isneginf(ref_lse)
+        assert (got[empty] == 0).all() and np.isneginf(got_lse[empty]).all()
+        assert (np.abs(got - ref) <= 2.0 ** -8 * np.abs(ref) + 2.0 ** -9 * A + 2.0 ** -32 * S).all()
+        lerr = np.abs(got_lse[~empty] - ref_lse[~empty])
+        assert (lerr <= 2.0 ** -12 + 2.0 ** -20 * np.abs(ref_lse[~empty])).all()
+        assert torch.equal(o, c4.attention(*args))
+
+
 def test_attention_weights_reach_every_row(c4):
     """One row at a time has all the weight: a wrong row, feature or scale shows."""
     C, H = 400, 1

@@ -139,6 +139,7 @@ struct Cache4Plan {
 
 // Measured (B200, us; cluster x parts, lengths half to all of the capacity, one query token):
 //   flat / cluster: 768 units x 128 tiles 46 / 58; 512 x 64 30.6 / 30.6; 384 x 64 21.0 / 21.2; 128 x 64 14.4 / 10.7.
+//   One K/V head, full lengths: 4096 x 32 tiles 66 / 70, 16384 x 32 235 / 256; eight heads, 4096 sequences x 1 tile 69 / 164.
 //   A unit's cluster, 96 units x 128 tiles: 1 to 8 CTAs 21, 15.8, 14.6, 12.3 (4), 13.7 (6), 14.1 (8); 256 x 64: 19.1, 17.3,
 //   21.5, 20.3 (4): three CTAs to an SM are best, and two CTAs a unit where that leaves one.
 //   Few units, parts without a cluster / clusters of 8 in one part or several: 12 x 64 tiles 4.7 / 4.1; 24 x 64 5.6 / 4.9;

@@ -885,20 +885,24 @@ __global__ void __maxnreg__(NT == 1 ? 112 : 152)
   // The merge's launch runs under this kernel.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const bool dense = p.cache[0].sn == BLOCK_BYTES && p.cache[1].sn == BLOCK_BYTES;
-  // Each lane counts a thirty-second of the sequences; one scan then finds the lane, and another the sequence.
-  const int chunk = (p.B + 31) / 32;
+  // Each warp counts the tiles of a range of sequences; the ranges' sums tell where this warp's share begins. (A range for
+  // each lane made 4096 sequences take 32 us longer: its loads lie apart.)
+  __shared__ int range_tiles[W];
+  const int range = (p.B + W * 32 - 1) / (W * 32) * 32;
   int mine = 0;
 #pragma unroll 4
-  for (int b = lane * chunk; b < min(p.B, (lane + 1) * chunk); ++b) mine += unit_tiles(p, b);
-  mine *= p.Hkv * p.row_tiles;
-  const int up = lanes_up_to(mine, lane);
+  for (int b = warp * range + lane; b < min(p.B, (warp + 1) * range); b += 32) mine += unit_tiles(p, b);
+  mine = __reduce_add_sync(0xffffffffu, mine) * p.Hkv * p.row_tiles;
+  if (lane == 0) range_tiles[warp] = mine;
+  __syncthreads();
+  const int up = lanes_up_to(lane < W ? range_tiles[lane] : 0, lane);
   Shares shares;
   shares.set(__shfl_sync(0xffffffffu, up, 31), static_cast<int>(gridDim.x) * W);
   if (worker >= shares.workers || shares.each == 0) return;
   const int first = shares.first(worker), count = shares.first(worker + 1) - first;
   const int l = __ffs(static_cast<int>(__ballot_sync(0xffffffffu, up > first))) - 1;
   Cursor now, ahead;
-  now.seek(p, l * chunk, first - __shfl_sync(0xffffffffu, up - mine, l), lane);
+  now.seek(p, l * range, first - (l > 0 ? __shfl_sync(0xffffffffu, up, l - 1) : 0), lane);
   ahead = now;
   Rows<NT, ONE> q;
   auto raw = q.fetch(p, now.u, lane);
