@@ -392,8 +392,8 @@ TT_ATTN_API size_t tt_attn_qkv_norm_rope_backward_workspace_size(void);
  * attended to without ever being expanded in memory. No counterpart in the reference, whose cache has the model's
  * type (tiny_transformer/model.py:11-43).
  *
- * A cache is [batch, kv_heads, blocks, 576] bytes, byte strides c*_strides[4] (last 1, others multiples of 16),
- * 16-byte aligned (TT_ATTN_UNSUPPORTED otherwise); its capacity is 16 * blocks rows. A block holds 16 rows:
+ * A cache is [batch, kv_heads, blocks, 576] bytes, byte strides c*_strides[4] (last 1, others multiples of 16, at least
+ * 576), 16-byte aligned (TT_ATTN_UNSUPPORTED otherwise); its capacity is 16 * blocks rows. A block holds 16 rows:
  *   bytes 0-511    codes, row r at 32 r: feature 2i in the low half of byte i, 2i + 1 in the high half; a code is e2m1
  *                  (bit 3 the sign, then 0 0.5 1 1.5 2 3 4 6)
  *   bytes 512-575  scales, row r at 512 + 4 r, one for 16 features: the upper byte of a half without its sign (5

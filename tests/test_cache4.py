@@ -107,6 +107,8 @@ def _cache(n=7, H=2):
     (dict(ck=32), BAD_ARG, "caches of their own"),
     (dict(cs=_s(2 * 7 * 576, 7 * 576, 584, 1)), UNSUPPORTED, "caches need"),
     (dict(cs=_s(2 * 7 * 576, 7 * 576, 576, 2)), UNSUPPORTED, "caches need"),
+    (dict(cs=_s(2 * 7 * 576, 7 * 576, 560, 1)), UNSUPPORTED, "at least 576"),   # blocks over one another
+    (dict(cs=_s(2 * 7 * 576, 0, 576, 1)), UNSUPPORTED, "at least 576"),
 ])
 def test_append_rejects_before_cuda(lib, kwargs, status, fragment):
     kwargs = dict(kwargs)

@@ -109,7 +109,7 @@ bool cache4_view(void* base, const int64_t* st, int64_t batch, int64_t kv_heads,
   int64_t s[3] = {st[0], st[1], st[2]};
   for (int d = 0; d < 3; ++d) {
     if (size[d] == 1) s[d] = row;
-    if (s[d] <= 0 || s[d] % 16 != 0) return false;
+    if (s[d] < row || s[d] % 16 != 0) return false;   // (blocks that overlap would be written twice)
   }
   if (st[3] != 1) return false;
   *v = {static_cast<uint8_t*>(base), s[0], s[1], s[2]};
@@ -117,7 +117,7 @@ bool cache4_view(void* base, const int64_t* st, int64_t batch, int64_t kv_heads,
 }
 
 const char* const kCache4Layout =
-    ": the caches need a unit last stride, other strides in multiples of 16 bytes and 16-byte aligned bases";
+    ": the caches need a unit last stride, others of at least 576 in multiples of 16 bytes and 16-byte aligned bases";
 
 tt_attn_status cache4_sizes(const std::string& what, int64_t batch, int64_t kv_heads, int64_t blocks) {
   if (batch <= 0 || kv_heads <= 0 || blocks <= 0)
