@@ -292,6 +292,39 @@ def test_captured_training_step(op):
         assert all(map(torch.equal, got, step()))
 
 
+def test_capture_beside_an_eager_graph(op):
+    """A living graph of the same leaves: from the default stream the capture is refused, from another one it works."""
+    B, T, H = 1, 9, 2
+    cos, sin = (t.cuda() for t in _tables())
+    qkv, w, g = _inputs(B, T, H, H, torch.bfloat16, 19)
+    g = [x.cuda() for x in g]
+    leaves = [x.cuda().requires_grad_() for x in (qkv, *w)]
+
+    def step():
+        return torch.autograd.grad(op(*leaves, cos, sin, 3, EPS, H), leaves, g)
+
+    held = op(*leaves, cos, sin, 3, EPS, H)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    want = torch.autograd.grad(held, leaves, g)     # the eager graph is as it was
+    del held
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        held = op(*leaves, cos, sin, 3, EPS, H)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for x in got:
+        x.zero_()
+    graph.replay()
+    assert all(map(torch.equal, got, want))
+    assert all(map(torch.equal, torch.autograd.grad(held, leaves, g), want))
+
+
 @pytest.mark.parametrize("change,match", [
     (dict(qkv=lambda x: x.float()), "bf16"),
     (dict(qkv=lambda x: x[..., :32]), "head_dim=64"),

@@ -11,9 +11,11 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <cstdint>
 #include <limits>
@@ -863,6 +865,21 @@ class QkvNormRope : public torch::autograd::Function<QkvNormRope> {
   }
 };
 
+// A leaf's gradient node keeps the stream of the graph that made it for as long as such a graph lives. If that is the
+// default stream, a captured backward pass would make that stream wait for the capture, which CUDA does not allow, and the
+// process ends inside the backward pass: refused here, while the step's forward is captured.
+void leaves_off_the_default_stream(std::initializer_list<const torch::Tensor*> tensors, const char* what) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  for (const torch::Tensor* t : tensors) {
+    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = node != nullptr ? node->stream() : std::nullopt;
+    TORCH_CHECK(!stream.has_value() || *stream != c10::cuda::getDefaultCUDAStream(t->get_device()).unwrap(), what,
+                ": a graph of the same leaves from the default stream is still alive; release its outputs before "
+                "a training step is captured, or run it on another stream");
+  }
+}
+
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> qkv_norm_rope(
     const torch::Tensor& qkv, std::optional<torch::Tensor> q_weight, std::optional<torch::Tensor> k_weight,
     const torch::Tensor& cos, const torch::Tensor& sin, const pybind11::object& position, double eps,
@@ -879,6 +896,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> qkv_norm_rope(
     TORCH_CHECK_NOT_IMPLEMENTED(!cos.requires_grad() && !sin.requires_grad(), what,
                                 " has no gradient for the cos/sin tables");
     if (qkv.requires_grad() || wants(q_weight) || wants(k_weight)) {
+      const torch::Tensor none;
+      leaves_off_the_default_stream({&qkv, q_weight ? &*q_weight : &none, k_weight ? &*k_weight : &none}, what);
       const std::optional<torch::Tensor> on_device = pos.t.defined() ? std::make_optional(pos.t) : std::nullopt;
       auto out = QkvNormRope::apply(qkv, q_weight, k_weight, cos, sin, on_device, pos.host, eps,
                                     kv_heads.value_or(-1));
