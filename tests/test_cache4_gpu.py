@@ -748,3 +748,70 @@ def test_streams_and_captured_steps(c4):
     torch.cuda.synchronize()
     assert all(map(torch.equal, caches, eager))
     assert _status() == 0
+
+
+def _uneven_cache(q, lens, H, C, seed, share, size, kind):
+    """Keys with one row a head that takes about `share` of a single query's weight (0: none), and values of about `size`:
+    kind "heavy": the heavy row's value is zero; "small": 2^-6 of the others'; "mixed": rows and groups of sizes from
+    2^-8 to 1 of it; "large": a row of no weight has values near 10^4."""
+    rs = np.random.RandomState(seed)
+    B = len(lens)
+    kb, kv = _random_cache(B, H, C, seed)
+    codes, scales = oracle.unpack(kb)
+    vcodes = rs.randint(0, 16, codes.shape)
+    log = np.log2(size / 3) + 0.5 * rs.randn(*scales.shape)
+    if kind == "mixed":
+        log -= 8 * rs.rand(*scales.shape)
+    vscales = np.round(8 * (15 + log))
+    for b, n in enumerate(lens):
+        for h in range(H):
+            x = q[b, h, 0]
+            others = np.exp(kv[b, h, :n] @ x / 8).sum()
+            heavy, light = rs.choice(n, 2, replace=False)
+            codes[b, h, heavy] = np.where(x < 0, 10, 2)      # its key points where the query does
+            if share > 0:
+                s = np.log(share / (1 - share) * others) / (np.abs(x).sum() / 8)
+                scales[b, h, heavy] = oracle.nearest(s, oracle.SCALES)
+                if kind == "heavy":
+                    vscales[b, h, heavy] = 0
+                elif kind == "small":
+                    vscales[b, h, heavy] -= 48
+            if kind == "large":
+                codes[b, h, light] = np.where(x < 0, 2, 10)  # away from it
+                scales[b, h, light] = oracle.nearest(12 / (np.abs(x).sum() / 8), oracle.SCALES)
+                vscales[b, h, light] = 0xDA
+    vscales = np.clip(vscales, 0, 0xE2).astype(np.uint8)
+    return (oracle.pack(codes, scales), oracle.pack(vcodes, vscales), oracle.values(codes, scales),
+            oracle.values(vcodes, vscales))
+
+
+SMALL_VALUES = [(0.9, 1.0, "heavy"), (0.9, 0.1, "small"), (0.9, 0.01, "heavy"), (0.9, 1e-3, "small"), (0.5, 1e-2, "heavy"),
+                (0.5, 1e-3, "small"), (0.5, 1e-4, "heavy"), (0.999, 0.03, "heavy"), (0, 1e-3, "mixed"), (0, 1e-4, ""),
+                (0.9, 0.1, "mixed"), (0, 1e-3, "large"), (0.5, 1.0, "large")]
+
+
+@pytest.mark.parametrize("B,H,C,flat,share,size,kind", [
+    (B, H, C, False, *case) for B, H, C in ((1, 3, 512), (2, 2, 4096), (1, 1, 9000)) for case in SMALL_VALUES
+] + [(B, H, C, True, *case) for B, H, C in ((20, 12, 2048), (1800, 1, 100)) for case in SMALL_VALUES[2::3]])
+def test_attention_small_values_beside_a_heavy_row(c4, B, H, C, flat, share, size, kind):
+    """One query row over values of any size, where one row has most of the weight, in the cluster kernel and the flat
+    one; the same token as the second of two queries."""
+    lens = [C - 7 * (b % 9) for b in range(B)]
+    q = _queries(B, H, 1, C + B)
+    kb, vb, kv, vv = _uneven_cache(_np(q), lens, H, C, 7 * C + B, share, size, kind)
+    if flat:   # capacity enough for the flat kernel's share of all tiles
+        blocks = 4 * (24576 // (B * H) + 2)
+        wide = [np.full((B, H, blocks, 576), 0xFF, np.uint8) for _ in range(2)]
+        for dst, src in zip(wide, (kb, vb)):
+            dst[:, :, :src.shape[2]] = src
+        kb, vb = wide
+    k, v = torch.from_numpy(kb).cuda(), torch.from_numpy(vb).cuda()
+    dev = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    o, lse = c4.attention_with_lse(q.cuda(), k, v, dev)
+    ref, ref_lse, A = oracle.attention(_np(q), kv, vv, lens)
+    S = np.abs(vv).sum(2, keepdims=True)
+    bound = 2.0 ** -8 * np.abs(ref) + 2.0 ** -9 * A + 2.0 ** -32 * S
+    assert (np.abs(_np(o) - ref) <= bound).all(), (np.abs(_np(o) - ref) / bound).max()
+    assert (np.abs(_np(lse) - ref_lse) <= 2.0 ** -12 + 2.0 ** -20 * np.abs(ref_lse)).all()
+    two = c4.attention(torch.cat((_queries(B, H, 1, 3), q), 2).cuda(), k, v, dev)
+    assert (np.abs(_np(two[:, :, 1:]) - _np(o)) <= 2 * bound).all()

@@ -16,8 +16,9 @@
 //      selects for 16 values) before they are converted, not the halves after.
 // Q is scaled by a power of two per row, its largest element to [2^14, 2^15), and held in half precision: 11
 // significant bits over 2^28 against bf16's 8, so nothing is lost that is not 2^-36 of the row's largest element. P is
-// rounded to half precision too: its rows are held below 2^15 by the running maximum, so that a weight is rounded by
-// 2^-11 of itself down to 2^-29 of the largest one. Sums, maxima and the accumulators are FP32.
+// rounded to half precision too: its largest weight is held between 2^7 and 2^15 by the running maximum, so that a weight is
+// rounded by 2^-11 of itself down to 2^-21 of the largest one, and is off by 2^-32 of the largest at most below that. V is
+// scaled exactly and has no part in this. Sums, maxima and the accumulators are FP32.
 //
 // Work. A warp takes tiles of 64 rows of one (sequence, K/V head, row tile), each by asynchronous copies into its own
 // ring of shared memory (two stages: a third took shared memory from other CTAs, 49.1 against 46.5 us on the case below),
@@ -26,11 +27,11 @@
 // distributed shared memory; for few units and long caches several clusters or CTAs write records that a second
 // kernel merges), and for many tiles the flat kernel below.
 //
-// Measured (B200, us in a CUDA graph): 64 sequences of 1024-8192 rows, 12 heads 47.5 (5.4 TB/s; 512 sequences 6.4 TB/s,
+// Measured (B200, us in a CUDA graph): 64 sequences of 1024-8192 rows, 12 heads 49.7 (5.1 TB/s; 512 sequences 6.4 TB/s,
 // the copy rate); 32 x 8 K/V heads, 32 query heads, 1024-4096 rows 18.2 (2.6 TB/s); 2 K/V heads of 131072 rows 10.6;
 // 12 heads of 512 rows 3.8. Long runs are bound by DRAM with one query row and by instruction issue with more (per 16 rows
-// about 100 and 160 instructions: 32 conversions, 32 multiplications by scales where there is more than one
-// row, 8 products), short ones by start, merge and launch.
+// about 100 and 160 instructions: 32 conversions, 32 multiplications by scales, 16 with one
+// query row, 8 products), short ones by start, merge and launch.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -235,8 +236,8 @@ __device__ __forceinline__ void clear_tail(uint32_t ks, int first, int lane) {
 }
 
 // V's A fragments of a block: values of tokens (t4, 4 + t4) and (8 + t4, 12 + t4) in half 0 and 1; features 8 g + 2 i
-// at i, + 1 at 4 + i. The codes of two rows are interleaved, then converted.
-__device__ __forceinline__ void value_codes(uint32_t codes, uint32_t (&a)[2][8]) {
+// at i, + 1 at 4 + i. The codes of two rows are interleaved, then converted and scaled.
+__device__ __forceinline__ void value_fragments(uint32_t codes, uint32_t scales, uint32_t (&a)[2][8]) {
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const uint32_t w0 = lds_u32(codes + half * 8 * (HD / 2)), w1 = lds_u32(codes + (half * 8 + 4) * (HD / 2));
@@ -245,17 +246,15 @@ __device__ __forceinline__ void value_codes(uint32_t codes, uint32_t (&a)[2][8])
     uint32_t x[4], y[4];
     decode8(even, x);
     decode8(odd, y);
+    // The scales of the two tokens as a half pair.
+    const uint32_t from = scales + half * 8 * GROUPS;
+    const uint32_t scale = (lds_u8(from) << 7) + (lds_u8(from + 4 * GROUPS) << 23);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      a[half][i] = x[i];
-      a[half][4 + i] = y[i];
+      a[half][i] = mul_half2(x[i], scale);
+      a[half][4 + i] = mul_half2(y[i], scale);
     }
   }
-}
-
-// Scales of two tokens, four rows apart, as a half pair.
-__device__ __forceinline__ uint32_t value_scales(uint32_t scales) {
-  return (lds_u8(scales) << 7) + (lds_u8(scales + 4 * GROUPS) << 23);
 }
 
 // A warp's query rows of one unit and the softmax over the tiles it has seen.
@@ -427,13 +426,7 @@ struct Rows {
 #pragma unroll
     for (int j = 0; j < TILE_BLOCKS; ++j) {
       uint32_t a[2][8];
-      value_codes(vcodes + j * BLOCK_BYTES, a);
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t scale = value_scales(vscales + j * BLOCK_BYTES + half * 8 * GROUPS);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a[half][i] = mul_half2(a[half][i], scale);
-      }
+      value_fragments(vcodes + j * BLOCK_BYTES, vscales + j * BLOCK_BYTES, a);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -482,15 +475,14 @@ struct Rows {
 // no scaling.
 //   S: column n of B is q where a lane's features belong to group n % 4 and zero elsewhere; a row's four sums times
 //      their scales are added in FP32.
-//   O: column n of B is p x scale of group n % 4 (half precision), and a feature takes the column of its group.
-// 32 multiplications a block of 16 rows less (64 sequences x 12 heads, 1024-8192 rows: 60 -> 55.7 us at the time).
+//   O: as with more rows, all columns alike. (Scales in B, p x scale in half precision, would spare the multiplications
+//   of V too, but leave half precision's range: rows behind a heavy one, or with small values, were lost.)
+// 16 multiplications a block of 16 rows less.
 template <>
 struct Rows<1, true> {
-  // p x scale stays below 2^2 x 10240 as a half.
-  static constexpr float SLACK1 = 4.0f, RAISE1 = -2.0f;
   uint32_t qf[8];
   float factor, mx, ref, total;
-  float acc[4][4];   // features 8 g + 2 i (+ 1 in 2, 3), groups (2 t4) % 4, + 1
+  float acc[4][4];   // features 8 g + 2 i (+ 1 in 2, 3)
 
   __device__ __forceinline__ RawQuery fetch(const Params& p, const Unit& u, int lane) const {
     RawQuery raw;
@@ -563,14 +555,14 @@ struct Rows<1, true> {
 #pragma unroll
     for (int j = 1; j < TILE_BLOCKS; ++j) top = fmax3(top, s[j][0], s[j][1]);
     top *= factor;
-    if (__any_sync(0xffffffffu, top > mx + SLACK1)) {
+    if (__any_sync(0xffffffffu, top > mx + SLACK)) {
       float m = fmaxf(top, mx);
 #pragma unroll
       for (int d = 4; d < 32; d *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
       const float old = ref;
       const bool empty = mx == NEG_INF;
       mx = m;
-      ref = m == NEG_INF ? 0.0f : m - RAISE1;
+      ref = m == NEG_INF ? 0.0f : m - RAISE;
       const float f = empty ? 1.0f : ex2_approx(old - ref);   // empty: the sums are zero, or NaN
       total *= f;
 #pragma unroll
@@ -587,16 +579,14 @@ struct Rows<1, true> {
         total += e;
         pf[j][half] = transpose8x8(pack_half2(e, e));
       }
-    const uint32_t vcodes = vs + t4 * (HD / 2) + g * 4, vscales = vs + CODE_BYTES + t4 * GROUPS + (g & 3);
+    const uint32_t vcodes = vs + t4 * (HD / 2) + g * 4, vscales = vs + CODE_BYTES + t4 * GROUPS + (g >> 1);
 #pragma unroll
     for (int j = 0; j < TILE_BLOCKS; ++j) {
-      uint32_t a[2][8], b[2];
-      value_codes(vcodes + j * BLOCK_BYTES, a);
+      uint32_t a[2][8];
+      value_fragments(vcodes + j * BLOCK_BYTES, vscales + j * BLOCK_BYTES, a);
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
-        b[half] = mul_half2(pf[j][half], value_scales(vscales + j * BLOCK_BYTES + half * 8 * GROUPS));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) mma_f16(acc[i], a[0][i], a[0][4 + i], a[1][i], a[1][4 + i], b[0], b[1]);
+      for (int i = 0; i < 4; ++i)
+        mma_f16(acc[i], a[0][i], a[0][4 + i], a[1][i], a[1][4 + i], pf[j][0], pf[j][1]);
     }
   }
 
@@ -605,11 +595,10 @@ struct Rows<1, true> {
     float sum = total;
 #pragma unroll
     for (int d = 4; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (t4 == g >> 2) {   // the columns of the features' group
+    if (t4 == 0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<float2*>(rec[0] + 8 * g + 2 * i) =
-            (g >> 1) & 1 ? make_float2(acc[i][1], acc[i][3]) : make_float2(acc[i][0], acc[i][2]);
+        *reinterpret_cast<float2*>(rec[0] + 8 * g + 2 * i) = make_float2(acc[i][0], acc[i][2]);
     }
     if (lane == 0)
       *reinterpret_cast<float2*>(rec[0] + HD) = make_float2(mx == NEG_INF && sum == 0.0f ? NEG_INF : ref, sum);
