@@ -815,3 +815,48 @@ def test_attention_small_values_beside_a_heavy_row(c4, B, H, C, flat, share, siz
     assert (np.abs(_np(lse) - ref_lse) <= 2.0 ** -12 + 2.0 ** -20 * np.abs(ref_lse)).all()
     two = c4.attention(torch.cat((_queries(B, H, 1, 3), q), 2).cuda(), k, v, dev)
     assert (np.abs(_np(two[:, :, 1:]) - _np(o)) <= 2 * bound).all()
+
+
+@pytest.mark.parametrize("B,H,C,flat", [(3, 2, 300, False), (1, 1, 9000, False), (160, 1, 200, True)])
+def test_attention_of_one_query_sees_keys_that_are_not_numbers(c4, B, H, C, flat):
+    """A key group of NaN in a row that a single query sees makes its O and LSE NaN, whatever the query's signs; behind the
+    length it changes nothing."""
+    kb, _ = _random_cache(B, H, C, 91)
+    vb, _ = _random_cache(B, H, C, 92)
+    if flat:
+        more = ((0, 0), (0, 0), (0, 4 * (24576 // (B * H) + 2) - kb.shape[2]), (0, 0))
+        kb, vb = np.pad(kb, more), np.pad(vb, more)
+    lens = [C - 1 - b % 5 for b in range(B)]
+    v, dev = torch.from_numpy(vb).cuda(), torch.tensor(lens, device="cuda")
+    q = _queries(B, H, 1, 93).cuda()
+    want = c4.attention_with_lse(q, torch.from_numpy(kb).cuda(), v, dev)
+    codes, scales = oracle.unpack(kb)
+    for b, n in enumerate(lens):
+        scales[b, :, n:] = 0xFF
+    behind = c4.attention_with_lse(q, torch.from_numpy(oracle.pack(codes, scales)).cuda(), v, dev)
+    assert all(map(torch.equal, want, behind))
+    for group, row in ((0, 0), (1, 77), (2, C // 2), (3, lens[0] - 1)):
+        bad = scales.copy()
+        bad[0, 0, row, group] = 0xFF
+        for sign in (1, -1):
+            signed = c4.attention_with_lse(sign * q, torch.from_numpy(kb).cuda(), v, dev)
+            for x, y in zip(c4.attention_with_lse(sign * q, torch.from_numpy(oracle.pack(codes, bad)).cuda(), v, dev),
+                            signed):
+                assert x[0, 0].isnan().all()
+                keep = torch.ones(B, H, dtype=torch.bool)
+                keep[0, 0] = False
+                assert torch.equal(x[keep], y[keep])
+
+
+def test_append_then_attention_of_a_key_that_is_not_a_number(c4):
+    """A NaN that append meets in a projection reaches the output of one query and of two."""
+    B, T, H = 1, 5, 2
+    qkv, qw, kw = (x.cuda() for x in _projection(B, T, H, H, 5))
+    qkv[0, 2, H, 9] = float("nan")                # the first head's key of token 2
+    cos, sin = (t.cuda() for t in _tables(32))
+    caches = [c4.new_cache(B, H, 32) for _ in range(2)]
+    q = c4.append(qkv, cos, sin, 0, *caches, qw, kw, EPS)
+    lens = torch.tensor([T], device="cuda")
+    for tokens in (1, 2):
+        o = c4.attention(q[:, :, -tokens:], *caches, lens)
+        assert o[0, 0].isnan().all() and o[0, 1].isfinite().all()
