@@ -408,8 +408,11 @@ TT_ATTN_API size_t tt_attn_qkv_norm_rope_backward_workspace_size(void);
 /*
  * tt_attn_qkv_norm_rope_bf16's pass with the cache append in it: q goes to q_out, the keys (as bf16, correctly
  * rounded) and the values are quantised into rows position + t of the caches. Other rows are left as they are.
- * position_dev[b * position_sb] + t with a device-held position; the two caches must not overlap. Rows outside the cache or the table are not
+ * position_dev[b * position_sb] + t with a device-held position. Rows outside the cache or the table are not
  * written, their q is zero, and status bit 1 is set.
+ * No two blocks may overlap: sorted by stride, each dimension of a cache has to reach past those inside it
+ * (TT_ATTN_UNSUPPORTED otherwise), and the two caches must not overlap (TT_ATTN_BAD_ARG); with equal strides one may lie
+ * in the other's gaps, as the two halves of [batch, 2, kv_heads, blocks, 576] do.
  */
 TT_ATTN_API tt_attn_status tt_attn_cache4_append_bf16(
     const void* qkv, const int64_t* qkv_strides, int64_t batch, int64_t q_len, int64_t q_heads,

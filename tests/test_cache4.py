@@ -270,3 +270,33 @@ def test_oracle_gradient_against_differences():
         d = np.zeros_like(w)
         d[i] = h
         assert abs((loss(x, w + d) - loss(x, w - d)) / (2 * h) - dw[i]) < 1e-7
+
+
+ROW = 576
+
+
+@pytest.mark.parametrize("ks,vs,apart,status,fragment", [
+    ((ROW, ROW, ROW), None, 1 << 20, UNSUPPORTED, "overlap"),                      # all blocks of all heads in one row
+    ((14 * ROW, 6 * ROW, ROW), None, 1 << 20, UNSUPPORTED, "overlap"),             # a head's last block, the next one's first
+    ((14 * ROW - 16, 7 * ROW, ROW), None, 1 << 20, UNSUPPORTED, "overlap"),
+    ((7 * ROW, 8 * ROW, ROW), None, 1 << 20, UNSUPPORTED, "overlap"),              # heads outside, sequences too close
+    ((2**62, 2**61, 2**60), None, 1 << 20, UNSUPPORTED, "overlap"),                # no such memory
+    (None, (ROW, ROW, ROW), 1 << 20, UNSUPPORTED, "overlap"),
+    (None, None, ROW, BAD_ARG, "caches of their own"),                             # values one block behind the keys
+    (None, None, 7 * ROW, BAD_ARG, "caches of their own"),
+    (None, None, 28 * ROW - 16, BAD_ARG, "caches of their own"),
+    (None, None, 16, BAD_ARG, "caches of their own"),
+    ((28 * ROW, 14 * ROW, 2 * ROW), None, 28 * ROW, BAD_ARG, "caches of their own"),
+    ((28 * ROW, 14 * ROW, 2 * ROW), (28 * ROW, 14 * ROW, 2 * ROW), 16, BAD_ARG, "caches of their own"),
+])
+@pytest.mark.parametrize("first", ["keys", "values"])
+def test_append_refuses_caches_over_one_another(lib, ks, vs, apart, status, fragment, first):
+    """Blocks that share bytes would be written by different warps in no order."""
+    strides = [_s(*(x or (14 * ROW, 7 * ROW, ROW)), 1) for x in (ks, vs)]
+    base = [1 << 30, (1 << 30) + apart]
+    if first == "values":
+        strides.reverse()
+        base.reverse()
+    assert lib.tt_attn_cache4_append_bf16(*_projection(), 1e-6, 16, base[0], strides[0], base[1], strides[1], 7,
+                                          None) == status
+    assert fragment in _err(lib)

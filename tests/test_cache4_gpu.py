@@ -860,3 +860,32 @@ def test_append_then_attention_of_a_key_that_is_not_a_number(c4):
     for tokens in (1, 2):
         o = c4.attention(q[:, :, -tokens:], *caches, lens)
         assert o[0, 0].isnan().all() and o[0, 1].isfinite().all()
+
+
+def test_append_to_caches_beside_one_another(c4):
+    """Keys and values in the gaps of one another's layout; views that overlap are refused and write nothing."""
+    B, T, H, n = 2, 9, 3, 3
+    qkv, qw, kw = (x.cuda() for x in _projection(B, T, H, H, 5))
+    cos, sin = (t.cuda() for t in _tables(16 * n))
+
+    def run(*caches):
+        return c4.append(qkv, cos, sin, 11, *caches, qw, kw, EPS)
+
+    want = [c4.new_cache(B, H, 16 * n) for _ in range(2)]
+    q = run(*want)
+    for shape, dim in (((2, B, H, n, 576), 0), ((B, 2, H, n, 576), 1), ((B, H, 2, n, 576), 2), ((B, H, n, 2, 576), 3),
+                       ((B, H, n, 576 * 2), None)):
+        both = torch.zeros(shape, dtype=torch.uint8, device="cuda")
+        got = both.unbind(dim) if dim is not None else (both[..., 576:], both[..., :576])
+        assert torch.equal(run(*got), q) and all(map(torch.equal, got, want))
+    row = torch.zeros(4 * B * H * n * 576, dtype=torch.uint8, device="cuda")
+    over = row.as_strided((B, H, n, 576), (576, 576, 576, 1))
+    heads = row.as_strided((B, H, n, 576), (H * n * 576, (n - 1) * 576, 576, 1))
+    plain = row[:B * H * n * 576].view(B, H, n, 576)
+    behind = row[576:][:B * H * n * 576].view(B, H, n, 576)
+    other = c4.new_cache(B, H, 16 * n)
+    for caches, match in (((over, other), "overlap"), ((other, heads), "overlap"),
+                          ((plain, behind), "caches of their own"), ((behind, plain), "caches of their own")):
+        with pytest.raises(RuntimeError, match=match):
+            run(*caches)
+    assert (row == 0).all() and (other == 0).all()

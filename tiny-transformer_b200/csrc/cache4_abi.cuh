@@ -109,7 +109,7 @@ bool cache4_view(void* base, const int64_t* st, int64_t batch, int64_t kv_heads,
   int64_t s[3] = {st[0], st[1], st[2]};
   for (int d = 0; d < 3; ++d) {
     if (size[d] == 1) s[d] = row;
-    if (s[d] < row || s[d] % 16 != 0) return false;   // (blocks that overlap would be written twice)
+    if (s[d] < row || s[d] % 16 != 0) return false;
   }
   if (st[3] != 1) return false;
   *v = {static_cast<uint8_t*>(base), s[0], s[1], s[2]};
@@ -118,6 +118,44 @@ bool cache4_view(void* base, const int64_t* st, int64_t batch, int64_t kv_heads,
 
 const char* const kCache4Layout =
     ": the caches need a unit last stride, others of at least 576 in multiples of 16 bytes and 16-byte aligned bases";
+
+struct Cache4Dim {
+  int64_t stride, size;
+};
+
+// Bytes from the first block to the end of the last one, or 0 where blocks might overlap: sorted by stride, each dimension
+// has to step over all that lies inside it (as every layout does that slicing and transposing make).
+template <size_t N>
+int64_t cache4_extent(Cache4Dim (&&dims)[N]) {
+  std::sort(dims, dims + N, [](const Cache4Dim& a, const Cache4Dim& b) { return a.stride < b.stride; });
+  int64_t extent = tt::cache4::BLOCK_BYTES;
+  for (const auto& [stride, size] : dims) {
+    if (size == 1) continue;
+    if (stride < extent || size - 1 > (INT64_MAX - extent) / stride) return 0;
+    extent += (size - 1) * stride;
+  }
+  return extent;
+}
+
+// Caches that are written: no two blocks of the two may share a byte, as different warps write them. K and V may lie in one
+// another's gaps where they have the same strides: their distance is one more dimension then.
+tt_attn_status cache4_apart(const std::string& what, const tt::cache4::View (&c)[2], int64_t batch, int64_t kv_heads,
+                            int64_t blocks) {
+  int64_t extent[2];
+  for (int i = 0; i < 2; ++i) {
+    extent[i] = cache4_extent({{c[i].sb, batch}, {c[i].sh, kv_heads}, {c[i].sn, blocks}});
+    if (extent[i] == 0)
+      return fail(TT_ATTN_UNSUPPORTED, what + ": a cache's blocks must not overlap; each stride has to reach past the "
+                                              "dimensions inside it");
+  }
+  const int first = c[0].p < c[1].p ? 0 : 1;
+  const int64_t apart = c[1 - first].p - c[first].p;
+  const bool alike = c[0].sb == c[1].sb && c[0].sh == c[1].sh && c[0].sn == c[1].sn;
+  if (apart >= extent[first] ||
+      (alike && cache4_extent({{apart, 2}, {c[0].sb, batch}, {c[0].sh, kv_heads}, {c[0].sn, blocks}}) != 0))
+    return TT_ATTN_OK;
+  return fail(TT_ATTN_BAD_ARG, what + ": the keys and the values need caches of their own, not over one another");
+}
 
 tt_attn_status cache4_sizes(const std::string& what, int64_t batch, int64_t kv_heads, int64_t blocks) {
   if (batch <= 0 || kv_heads <= 0 || blocks <= 0)
@@ -364,11 +402,10 @@ TT_ATTN_API tt_attn_status tt_attn_cache4_append_bf16(
   if (!cache4_view(cache_k, ck_strides, batch, kv_heads, blocks, &p.cache[0]) ||
       !cache4_view(cache_v, cv_strides, batch, kv_heads, blocks, &p.cache[1]))
     return fail(TT_ATTN_UNSUPPORTED, std::string("cache4_append") + kCache4Layout);
-  if (cache_k == cache_v)
-    return fail(TT_ATTN_BAD_ARG, "cache4_append: the keys and the values need caches of their own");
   p.capacity = blocks * c4::BLOCK_ROWS;
   if (position_dev == nullptr && position > p.capacity - q_len)
     return fail(TT_ATTN_BAD_ARG, "cache4_append: position + q_len exceeds the cache capacity");
+  if ((st = cache4_apart("cache4_append", p.cache, batch, kv_heads, blocks)) != TT_ATTN_OK) return st;
   int dev = 0;
   if ((st = prepare_device(&dev)) != TT_ATTN_OK) return st;
   p.q_out = static_cast<__nv_bfloat16*>(q_out);

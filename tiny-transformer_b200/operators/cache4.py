@@ -37,7 +37,9 @@ def append(qkv, cos, sin, position, cache_k, cache_v, q_weight=None, k_weight=No
     device (a captured step, sequences of different lengths). The keys are quantised from their correctly
     rounded BF16 values, so the bytes do not depend on the order of a sum; other rows stay as they are.
     Rows outside the cache or the tables are not written, their q is zero, and the range bit of the device
-    status is set (``tt_attn_device_status``). Runs on the current CUDA stream; inference only.
+    status is set (``tt_attn_device_status``). Views whose blocks overlap, in one cache or between the two, are
+    refused; the halves of one ``[B, 2, Hkv, blocks, 576]`` tensor are fine. Runs on the current CUDA stream; inference
+    only.
     """
     return load_attention_extension().cache4_append(qkv, cos, sin, position, cache_k, cache_v, q_weight,
                                                     k_weight, eps)
