@@ -889,3 +889,21 @@ def test_append_to_caches_beside_one_another(c4):
         with pytest.raises(RuntimeError, match=match):
             run(*caches)
     assert (row == 0).all() and (other == 0).all()
+
+
+def test_forward_mode_derivatives_are_refused(c4):
+    import torch.autograd.forward_ad as forward_ad
+    qkv, qw, kw = (x.cuda() for x in _projection(2, 3, 4, 2, 1))
+    cos, sin = (t.cuda() for t in _tables(64))
+    q, k, v = _queries(2, 4, 1, 1).cuda(), c4.new_cache(2, 2, 32), c4.new_cache(2, 2, 32)
+    with forward_ad.dual_level():
+        for i in range(5):
+            x = [qkv, cos, sin, qw, kw]
+            x[i] = forward_ad.make_dual(x[i], torch.ones_like(x[i]))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                c4.append(*x[:3], 0, k, v, *x[3:], EPS)
+        assert (k == 0).all() and (v == 0).all()
+        dual = forward_ad.make_dual(q, q)
+        for call in (c4.attention, c4.attention_with_lse):
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call(dual, k, v)

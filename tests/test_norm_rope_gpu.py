@@ -378,3 +378,38 @@ def test_autocast_is_refused(op):
     cos, sin = (t.cuda() for t in _tables())
     with torch.autocast("cuda", torch.bfloat16), pytest.raises(RuntimeError, match="AMP"):
         op(qkv.cuda(), *[x.cuda() for x in w], cos, sin, 0, EPS, 1)
+
+
+@pytest.mark.parametrize("which", range(5))
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_are_refused(op, which, grad):
+    """A tangent would reach v, a view, and be lost from q and k."""
+    import torch.autograd.forward_ad as forward_ad
+    qkv, w, _ = _inputs(1, 3, 2, 2, torch.bfloat16, 1)
+    inputs = [qkv.cuda(), *(x.cuda() for x in w), *(t.cuda() for t in _tables())]
+    want = op(*inputs, 0, EPS, 2)
+    if grad:
+        inputs[0].requires_grad_()
+    with forward_ad.dual_level():
+        dual = list(inputs)
+        dual[which] = forward_ad.make_dual(inputs[which], torch.ones_like(inputs[which]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            op(*dual, 0, EPS, 2)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+            op(*dual, 0, EPS, 2)
+        assert all(map(torch.equal, op(*inputs, 0, EPS, 2), want))
+        plain = [forward_ad.unpack_dual(x).primal for x in dual]
+        assert all(map(torch.equal, op(*plain, 0, EPS, 2), want))
+
+
+def test_forward_mode_derivatives_of_the_gradients_are_refused(op):
+    import torch.autograd.forward_ad as forward_ad
+    qkv, w, g = _inputs(1, 3, 2, 2, torch.bfloat16, 1)
+    cos, sin = (t.cuda() for t in _tables())
+    leaves = [x.cuda().requires_grad_() for x in (qkv, *w)]
+    g = [x.cuda() for x in g]
+    out = op(*leaves, cos, sin, 0, EPS, 2)
+    for i in range(2):
+        with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(out[i], leaves, forward_ad.make_dual(g[i], g[i]), retain_graph=True, allow_unused=True)
+    assert torch.autograd.grad(out, leaves, g)[0].isfinite().all()

@@ -10,6 +10,7 @@
 #include <ATen/autocast_mode.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -795,6 +796,14 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> norm_rope_backward(
   return {dx, dqw, dkw};
 }
 
+// Forward-mode derivatives (dual tensors, whatever the grad mode): a tangent would be lost without a word.
+void no_tangents(std::initializer_list<const torch::Tensor*> tensors, const char* what) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const torch::Tensor* t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what,
+                                " has no forward-mode derivative");
+}
+
 // Outputs of a backward pass that has none of its own: differentiating them is an error (what once_differentiable does in
 // Python).
 torch::autograd::variable_list once_differentiable(torch::autograd::variable_list out) {
@@ -831,6 +840,7 @@ class QkvNormRope : public torch::autograd::Function<QkvNormRope> {
                                                  torch::autograd::variable_list grads) {
     torch::autograd::variable_list out(9);
     if (!grads[0].defined() && !grads[1].defined() && !grads[2].defined()) return out;
+    no_tangents({&grads[0], &grads[1], &grads[2]}, "qkv_norm_rope backward");
     const auto saved = ctx->get_saved_variables();
     const torch::Tensor& qkv = saved[0];
     const c10::cuda::CUDAGuard device_guard(qkv.device());
@@ -892,12 +902,14 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> qkv_norm_rope(
   const c10::cuda::CUDAGuard device_guard(qkv.device());
   const Position pos = position_argument(position, qkv, qkv.size(0), qkv.size(1), true, what);
   const auto wants = [](const std::optional<torch::Tensor>& x) { return x.has_value() && x->requires_grad(); };
+  const torch::Tensor none;
+  const torch::Tensor *qw = q_weight ? &*q_weight : &none, *kw = k_weight ? &*k_weight : &none;
+  no_tangents({&qkv, qw, kw, &cos, &sin}, what);
   if (at::GradMode::is_enabled()) {
     TORCH_CHECK_NOT_IMPLEMENTED(!cos.requires_grad() && !sin.requires_grad(), what,
                                 " has no gradient for the cos/sin tables");
     if (qkv.requires_grad() || wants(q_weight) || wants(k_weight)) {
-      const torch::Tensor none;
-      leaves_off_the_default_stream({&qkv, q_weight ? &*q_weight : &none, k_weight ? &*k_weight : &none}, what);
+      leaves_off_the_default_stream({&qkv, qw, kw}, what);
       const std::optional<torch::Tensor> on_device = pos.t.defined() ? std::make_optional(pos.t) : std::nullopt;
       auto out = QkvNormRope::apply(qkv, q_weight, k_weight, cos, sin, on_device, pos.host, eps,
                                     kv_heads.value_or(-1));
@@ -917,6 +929,7 @@ void inference_only(std::initializer_list<const torch::Tensor*> tensors, const c
     TORCH_CHECK_NOT_IMPLEMENTED(!(grad && t->requires_grad()), what,
                                 " has no backward; call it under torch.no_grad()");
   }
+  no_tangents(tensors, what);
   TORCH_CHECK(!at::autocast::is_autocast_enabled(at::kCUDA), what, " does not support AMP/autocast yet");
 }
 

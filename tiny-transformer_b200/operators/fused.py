@@ -45,7 +45,8 @@ def qkv_norm_rope(qkv, q_weight, k_weight, cos, sin, position=0, eps=1e-6, kv_he
     device status (``tt_attn_device_status``).
 
     Differentiable in ``qkv`` and the weights: the backward reads q's, k's and v's gradients and writes ``qkv``'s
-    whole, in one kernel; the weights' gradients are summed in a fixed order. Forward and backward can be captured
+    whole, in one kernel; the weights' gradients are summed in a fixed order. There is no second derivative and no
+    forward-mode one (``NotImplementedError``). Forward and backward can be captured
     together in a CUDA graph; while an autograd graph of the same leaves from the default stream lives, that is refused.
     The reference has no such norm (its blocks norm the hidden state only, model.py:46-76).
     """
