@@ -413,3 +413,30 @@ def test_forward_mode_derivatives_of_the_gradients_are_refused(op):
         with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad(out[i], leaves, forward_ad.make_dual(g[i], g[i]), retain_graph=True, allow_unused=True)
     assert torch.autograd.grad(out, leaves, g)[0].isfinite().all()
+
+
+def test_shared_heads_in_front_of_the_attention(op):
+    """Shared K/V heads are repeated for student.attention, which wants as many K/V as query heads: values and gradients as
+    from a projection that holds the repeated heads."""
+    from tiny_transformer_b200.operators import student
+    B, T, Hq, Hkv = 2, 70, 6, 2
+    qkv, w, _ = _inputs(B, T, Hq, Hkv, torch.bfloat16, 31)
+    cos, sin = (t.cuda() for t in _tables())
+    do = torch.randn(B, Hq, T, 64, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+    leaves = [x.cuda().requires_grad_() for x in (qkv, *w)]
+    q, k, v = op(*leaves, cos, sin, 0, EPS, Hkv)
+    with pytest.raises(RuntimeError, match="second dimension"):
+        student.attention(q, k, v)
+    k, v = (x.repeat_interleave(Hq // Hkv, 1) for x in (k, v))
+    o = student.attention(q, k, v)
+    got = torch.autograd.grad(o, leaves, do)
+    wide = torch.cat([qkv[:, :, :Hq], *(x.repeat_interleave(Hq // Hkv, 2) for x in qkv[:, :, Hq:].split(Hkv, 2))], 2)
+    wide = [x.cuda().requires_grad_() for x in (wide, *w)]
+    want_o = student.attention(*op(*wide, cos, sin, 0, EPS, Hq))
+    want = torch.autograd.grad(want_o, wide, do)
+    assert torch.equal(o, want_o)
+    k_v = want[0][:, :, Hq:].double().unflatten(2, (2 * Hkv, -1)).sum(3)
+    dx = torch.cat([want[0][:, :, :Hq].double(), k_v], 2)
+    # Both round the same sums of bf16 gradients once or twice more: three roundings of terms of the whole.
+    for a, b in zip(got, (dx, *want[1:])):
+        assert (a.double() - b.double()).norm() <= 3 * 2.0 ** -8 * b.double().norm()

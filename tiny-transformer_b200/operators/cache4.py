@@ -4,7 +4,8 @@ A cache is a uint8 CUDA tensor ``[B, Hkv, blocks, 576]``, one for the keys and o
 capacity is ``16 * blocks`` rows (tokens). A block holds 16 rows of 64 features as 512 bytes of e2m1 codes and 64
 bytes of scales, one for 16 features (36 bytes a row against 128 in BF16; the exact layout is in
 ``include/tt_attention.h``). A value is its code times its scale. Rows are quantised as they are written:
-the scale is the group's largest magnitude over 6, rounded to 4 significant bits (2^-17 to 10240), codes go to the
+the scale is the group's largest magnitude over 6, rounded to 4 significant bits (2^-14 to 10240; fewer bits down to
+2^-17, that is for groups whose largest value is below 3.7e-4, and zero below 2.3e-5), codes go to the
 nearest value, of two to the one with the even code. A group with a NaN reads back as NaN; larger values saturate.
 
 The reference has no counterpart: its cache has the model's type (tiny_transformer/model.py:11-43).
@@ -34,8 +35,9 @@ def append(qkv, cos, sin, position, cache_k, cache_v, q_weight=None, k_weight=No
     ``qkv``, ``cos`` / ``sin``, the weights and ``eps`` as in :func:`fused.qkv_norm_rope` (weights None: no norm), with
     as many K/V heads as the caches have. Token t of sequence b goes to row ``position + t`` of the caches:
     ``position`` is an int, or an int64 CUDA tensor with one element or one for each sequence, read on the
-    device (a captured step, sequences of different lengths). The keys are quantised from their correctly
-    rounded BF16 values, so the bytes do not depend on the order of a sum; other rows stay as they are.
+    device (a captured step, sequences of different lengths). The keys are quantised from their BF16 values as
+    64 bits give them (rounded by way of FP32), so the bytes do not depend on the order of a sum; other rows stay as
+    they are.
     Rows outside the cache or the tables are not written, their q is zero, and the range bit of the device
     status is set (``tt_attn_device_status``). Views whose blocks overlap, in one cache or between the two, are
     refused; the halves of one ``[B, 2, Hkv, blocks, 576]`` tensor are fine. Runs on the current CUDA stream; inference
@@ -62,7 +64,8 @@ def attention(q, cache_k, cache_v, kv_lens=None):
     the T tokens' own rows: query t sees rows ``j < kv_lens[b] - (T - 1 - t)``. Scale 1/8, FP32 softmax, its weights
     rounded to half precision for the product with V; the codes are used as they are, never expanded in
     memory. A query that sees no row gets O = 0. Rows that a query does not see never change its output, whatever
-    they hold. Longer prompts read their rows back (:func:`read`) for ``student.attention``.
+    they hold. Longer prompts read their rows back (:func:`read`) for ``student.attention``, which wants as many K/V as
+    query heads (``repeat_interleave`` of shared ones).
     Runs on the current CUDA stream; inference only.
     """
     return load_attention_extension().cache4_attention(q, cache_k, cache_v, kv_lens)

@@ -31,13 +31,14 @@ def qkv_rope_append(hidden, w_qkv, cos, sin, position, cache_k, cache_v):
 
 def qkv_norm_rope(qkv, q_weight, k_weight, cos, sin, position=0, eps=1e-6, kv_heads=None):
     """RMS norm of every query and key head of a fused projection, and the position rotation, in one pass;
-    returns ``(q, k, v)`` as ``student.attention`` takes them.
+    returns ``(q, k, v)`` as ``student.attention`` takes them (with as many K/V as query heads: shared ones go there
+    after ``repeat_interleave(Hq // Hkv, 1)``).
 
     ``qkv`` is BF16 ``[B, T, 3, H, 64]``, or ``[B, T, Hq + 2 Hkv, 64]`` (query, key, value heads) with
     ``kv_heads=Hkv``; ``q_weight`` / ``k_weight`` ``[64]``, BF16 or FP32 (both None: the rotation alone);
     ``cos`` / ``sin`` FP32 ``[L, 32]`` tables, a row per position. ``position`` is the first position (an int),
     or an int64 CUDA tensor read on the device: one element, ``[B]`` (a first position for each sequence) or
-    ``[B, T]`` (one for each token: packed documents).
+    ``[B, T]`` (one for each token: packed documents; ``student.attention`` has no mask between them).
 
     A head x becomes ``n = x * rsqrt(mean(x^2) + eps) * weight``, its adjacent pairs turned by the table row; FP32
     throughout, rounded once. ``q`` ``[B, Hq, T, 64]`` and ``k`` ``[B, Hkv, T, 64]`` are contiguous, ``v`` is a view of
