@@ -399,15 +399,16 @@ TT_ATTN_API size_t tt_attn_qkv_norm_rope_backward_workspace_size(void);
  *   bytes 512-575  scales, row r at 512 + 4 r, one for 16 features: the upper byte of a half without its sign (5
  *                  bits of exponent, 3 of mantissa), at most 0xE2 = 10240, or 0xFF = NaN
  * A value is code x scale. 16 values are quantised with scale = max|x| / 6 rounded to nearest even (at most
- * 10240), codes rounded to nearest, ties to the even code, saturating. A group with a NaN gets the scale NaN.
+ * 10240), codes rounded to nearest, ties to the even code, saturating. A group with a NaN gets the scale NaN. Scales have 4
+ * significant bits from 2^-14 (max|x| 3.7e-4) to 10240 and fewer down to 2^-17; smaller groups become zero.
  */
 #define TT_ATTN_CACHE4_BLOCK_ROWS 16
 #define TT_ATTN_CACHE4_BLOCK_BYTES 576
 #define TT_ATTN_CACHE4_MAX_QUERIES 16
 
 /*
- * tt_attn_qkv_norm_rope_bf16's pass with the cache append in it: q goes to q_out, the keys (as bf16, correctly
- * rounded) and the values are quantised into rows position + t of the caches. Other rows are left as they are.
+ * tt_attn_qkv_norm_rope_bf16's pass with the cache append in it: q goes to q_out, the keys (as bf16, rounded from FP64
+ * by way of FP32) and the values are quantised into rows position + t of the caches. Other rows are left as they are.
  * position_dev[b * position_sb] + t with a device-held position. Rows outside the cache or the table are not
  * written, their q is zero, and status bit 1 is set.
  * No two blocks may overlap: sorted by stride, each dimension of a cache has to reach past those inside it

@@ -176,15 +176,15 @@ struct Cache4Plan {
 };
 
 // Measured (B200, us; cluster x parts, lengths half to all of the capacity, one query token):
-//   flat / cluster: 768 units x 128 tiles 46 / 58; 512 x 64 30.6 / 30.6; 384 x 64 21.0 / 21.2; 128 x 64 14.4 / 10.7.
-//   One K/V head, full lengths: 4096 x 32 tiles 66 / 70, 16384 x 32 235 / 256; eight heads, 4096 sequences x 1 tile 69 / 164.
-//   More units than resident CTAs, whose starts then add up: 12000 x 1 29 / 59; 2400 x 1 12.2 / 14.1; 2000 x 2 15.9 / 15.0;
-//   1560 x 8 14.9 / 14.7; 1200 x 4 10.8 / 9.5. Sixteen-row tiles: 384 x 64 29.9 / 31.3; 1000 x 16 24.5 / 26.5; 256 x 32
-//   18.8 / 20.2; 192 x 32 19.1 / 14.1; 256 x 16 17.0 / 15.9.
-//   A unit's cluster, 96 units x 128 tiles: 1 to 8 CTAs 21, 15.8, 14.6, 12.3 (4), 13.7 (6), 14.1 (8); 256 x 64: 19.1, 17.3,
-//   21.5, 20.3 (4): three CTAs to an SM are best, and two CTAs a unit where that leaves one.
-//   Few units, parts without a cluster / clusters of 8 in one part or several: 12 x 64 tiles 4.7 / 4.1; 24 x 64 5.6 / 4.9;
-//   4 x 256 5.8 / 7.0; 12 x 512 8.0 / 9.0; 8 x 512 7.8 / 8.4; 2 x 2048 11.3 / 10.2; 32 x 128 8.4 / 7.7.
+//   flat / cluster: 768 units x 128 tiles 63 / 73; 512 x 64 27.9 / 28.7; 384 x 64 23.4 / 23.1; 128 x 64 14.1 / 10.2.
+//   One K/V head, full lengths (near the copy rate): 4096 x 32 tiles 105 / 103, 16384 x 32 399 / 397; eight heads, 4096
+//   sequences x 1 tile 62 / 144. More units than resident CTAs, whose starts then add up (one tile: full lengths): 12000 x 1
+//   34 / 55; 2400 x 1 11.7 / 11.5; 2000 x 2 11.4 / 13.1; 1560 x 8 16.9 / 16.7; 1200 x 4 11.1 / 10.1. Sixteen-row tiles:
+//   384 x 64 29.9 / 31.3; 1000 x 16 24.5 / 26.5; 256 x 32 18.8 / 20.2; 192 x 32 19.1 / 14.1; 256 x 16 17.0 / 15.9.
+//   A unit's cluster, 96 units x 128 tiles: 1 to 8 CTAs 23.7, 16.7, 15.6, 13.2 (4), 14.5 (6), 14.7 (8); 256 x 64: 18.0,
+//   17.0, 19.8, 19.2 (4): three CTAs to an SM are best, and two CTAs a unit where that leaves one.
+//   Few units, parts without a cluster / clusters of 8 in one part or several: 12 x 64 tiles 5.0 / 4.1; 24 x 64 5.9 / 4.9;
+//   4 x 256 5.3 / 5.9; 12 x 512 8.1 / 10.5; 8 x 512 7.1 / 8.6; 2 x 2048 12.1 / 8.1; 32 x 128 7.7 / 6.7.
 constexpr int64_t kCache4FlatTiles = 24576, kCache4FlatTiles16 = 8000, kCache4FlatUnits = 12 * kPlanSms;
 
 Cache4Plan cache4_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t blocks) {

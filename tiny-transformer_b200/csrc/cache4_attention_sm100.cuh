@@ -27,11 +27,11 @@
 // distributed shared memory; for few units and long caches several clusters or CTAs write records that a second
 // kernel merges), and for many tiles the flat kernel below.
 //
-// Measured (B200, us in a CUDA graph): 64 sequences of 1024-8192 rows, 12 heads 49.7 (5.1 TB/s; 512 sequences 6.4 TB/s,
-// the copy rate); 32 x 8 K/V heads, 32 query heads, 1024-4096 rows 18.2 (2.6 TB/s); 2 K/V heads of 131072 rows 10.6;
-// 12 heads of 512 rows 3.8. Long runs are bound by DRAM with one query row and by instruction issue with more (per 16 rows
-// about 100 and 160 instructions: 32 conversions, 32 multiplications by scales, 16 with one
-// query row, 8 products), short ones by start, merge and launch.
+// Measured (B200, us in a CUDA graph): 64 sequences of 1024-8192 rows, 12 heads 49.7 (5.1 TB/s; 512 sequences 334,
+// 6.1 TB/s); 32 x 8 K/V heads, 32 query heads, 1024-4096 rows 18.2 (2.6 TB/s); 2 K/V heads of 131072 rows 10.6;
+// 12 heads of 512 rows 3.8. Long runs are bound by instruction issue (per 16 rows about 140 instructions with one query row,
+// 160 with more: 32 conversions, 16 or 32 multiplications by scales, 8 products; 2.6 a cycle and SM), hundreds of long
+// sequences with one query row by DRAM, short runs by start, merge and launch.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -5,8 +5,9 @@
 // (row r at 32 r, feature 2i in the low half of byte i), then 64 bytes of scales (row r at 512 + 4 r, one for 16
 // features). A code is e2m1 (sign, 0 0.5 1 1.5 2 3 4 6). A scale is the upper byte of a half without its sign: 5
 // bits of exponent and 3 of mantissa, 2^-17 to 10240 here. A value is code x scale, exact in half precision
-// and in bf16 (2 + 4 significant bits). The five exponent bits make a scale for the whole tensor unnecessary
-// (with 4, a group whose largest value is below 0.09 would lose bits), and a scale becomes a half by a shift.
+// and in bf16 (2 + 4 significant bits). The five exponent bits make a scale for the whole tensor unnecessary:
+// scales have four significant bits from 2^-14 on, for groups whose largest value is at least 3.7e-4 (with 4 exponent bits:
+// 0.09), lose them one by one below that, and groups below 2.3e-5 become zero. A scale becomes a half by a shift.
 //
 // Quantising 16 values x: scale = max|x| / 6 rounded to nearest even (to 10240 at most), code = x / scale rounded to
 // nearest, ties to the even code, saturating at 6. Values are bf16, so borders are exact numbers: a tie x =
@@ -15,8 +16,8 @@
 // In the same way max|x| times 1/6 is off by 2^-23, a tie of the scale has 5 significant bits, and rounding to 20 bits
 // first restores it. A group with a NaN gets the scale NaN; infinities saturate.
 //
-// Append: key rows are quantised from the bf16 values of the rotation, correctly rounded: an error of the last bit
-// next to a border would be a whole step of a code. FP32 decides wherever a value is farther from a bf16 border
+// Append: key rows are quantised from the bf16 values of the rotation, rounded from 64 bits by way of FP32 (as double goes to
+// bf16 in two conversions): an error of the last bit next to a border would be a whole step of a code. FP32 decides wherever a value is farther from a bf16 border
 // than its error bound. Of the others (one in 2^10) both neighbours are quantised, and where that gives different
 // codes the row is computed again in FP64.
 //
@@ -199,7 +200,7 @@ __device__ __forceinline__ void order(uint4& a, uint4& b) {
   }
 }
 
-// The same from FP64: correctly rounded but for FP64's own errors.
+// The same from FP64, rounded to FP32 and then to bf16 (two roundings: within 2^-25 of a bf16 tie the second is a tie).
 template <bool NORM>
 __device__ __forceinline__ uint4 key_row_exact(const norm_rope::Common& p, const uint4& v, int64_t pos, int lane8) {
   constexpr int E = norm_rope::E;
